@@ -60,7 +60,12 @@ enum qmm_dtype {
   QMM_Q8 = 4     /* planar Q8_1: int8 codes [rows, K], then at byte rows*K f32 (f16-rounded d, code sum) per 32 */
 };
 enum qmm_gemm_mode { QMM_GEMM_STORE = 0, QMM_GEMM_ACC = 1, QMM_GEMM_SWIGLU = 2 };
-enum qmm_act { QMM_ACT_SILU = 0, QMM_ACT_SWIGLU_OAI = 1 };
+/* The expert activations (QMM_ACT_SILU, QMM_ACT_SWIGLU_OAI) and those of qmm_linear and qmm_ffn_gate_up. QMM_ACT_GELU is
+ * the tanh form, QMM_ACT_GELU_ERF v Phi(v). */
+enum qmm_act {
+  QMM_ACT_SILU = 0, QMM_ACT_SWIGLU_OAI = 1, QMM_ACT_NONE = 2, QMM_ACT_RELU = 3, QMM_ACT_GELU = 4, QMM_ACT_GELU_ERF = 5,
+  QMM_ACT_SIGMOID = 6
+};
 enum qmm_moe_flags { QMM_MOE_Q8 = 1 /* the decode chain on Q8_1 activations (the reference's MOE_Q8) */ };
 
 /* Library version (major*10000 + minor*100 + patch) and the text of a status code. */
@@ -171,6 +176,75 @@ int qmm_gemm(int fmt, int mode, int64_t rows, int64_t k, int64_t n, const void *
 int qmm_gemm_mxfp4(int fmt, int mode, int64_t rows, int64_t k, int64_t n, const void *x, const void *x_scales,
                    const void *w, const void *ws, const void *w2, const void *ws2, void *y, int y_dtype,
                    qmm_stream_t stream);
+
+/* Root-mean-square norm with the residual's addition, written as the operand of the product that follows (no single
+ * reference kernel: its norm writes f32 rows that a quantizer reads):
+ *   h = x + residual (x without one);   y[t, c] = h[t, c] / sqrt(mean_c(h[t]^2) + eps) * weight[c]
+ * x: [rows, k] f32 or bf16; residual: [rows, k] f32 or bf16, or NULL; weight: [k] f32 or bf16; h: NULL, or [rows, k] of the
+ * residual's type (rounded to nearest even), which may be x or residual itself where the types agree. The norm is that of
+ * the f32 sum, before h is rounded. out by out_dtype:
+ *   QMM_F32 / QMM_BF16  y [rows, k]
+ *   QMM_F16             the qmm_gemm operand: x16 [rows, k], out_scales f32 [rows, 2], as qmm_row_scale_f16 of y
+ *   QMM_Q8              the int8 matvecs' planar Q8_1 buffer, as qmm_quant_q8 of y (k % 32 == 0)
+ *   QMM_MXFP8           the qmm_gemm_mxfp4 operand: E4M3 codes [rows, k], out_scales E8M0 [rows, k/32], as
+ *                       qmm_quant_mxfp8 of y (k % 32 == 0)
+ * each bit for bit what the quantizer gives for the f32 y. 1 <= k <= 32768, rows <= 2^24, eps >= 0; x, weight, residual, h
+ * and out 16-byte aligned for QMM_Q8 / QMM_MXFP8, else to their elements. Sums of squares are f32. */
+int qmm_rms_norm(int64_t rows, int64_t k, const void *x, int x_dtype, const void *residual, int res_dtype,
+                 const void *weight, int w_dtype, float eps, void *h, int out_dtype, void *out, void *out_scales,
+                 qmm_stream_t stream);
+
+/* Product with a bias, an activation and a residual in its epilogue (the reference adds them in kernels of their own):
+ *   y[t, r] = act(sum_k x[t, k] W[r, k] + bias[r]) + residual[t, r]
+ * act: QMM_ACT_NONE, RELU, SILU, SIGMOID, GELU or GELU_ERF. bias f32 [n] or NULL; residual [tokens, n] f32 or bf16 or NULL,
+ * may be y itself where the types agree; y [tokens, n] of y_dtype (QMM_F32, or QMM_BF16 rounded to nearest even, the only
+ * rounding after the f32 sum). x by x_dtype takes the matching product, with its formats, shapes, alignment, K sums and
+ * limits, and the sum has its bits:
+ *   QMM_F32 / QMM_BF16  qmm_mv (rows [tokens, k]; x_scales unused)
+ *   QMM_Q8              qmm_mv_q8 on the planar Q8_1 buffer, or qmm_mv_mxfp4s_q8 (fmt QMM_MXFP4S)
+ *   QMM_F16             qmm_gemm, x_scales f32 [tokens, 2] or NULL (64-row tiles of padding rows are not written)
+ *   QMM_MXFP8           qmm_gemm_mxfp4, x_scales E8M0 [tokens, k/32]
+ * ws: the weights' scale plane for QMM_MXFP4S / QMM_MXFP4T, else NULL. */
+int qmm_linear(int fmt, int act, int64_t tokens, int64_t k, int64_t n, const void *x, int x_dtype, const void *x_scales,
+               const void *w, const void *ws, const float *bias, const void *residual, int res_dtype, void *y, int y_dtype,
+               qmm_stream_t stream);
+
+/* The gated feed-forward block's first half in one kernel: both projections, their biases, the activation, the product
+ *   y[t, r] = act(g) u,   g = sum_k x[t, k] W[r, k] + bias[r],   u = sum_k x[t, k] W2[r, k] + bias2[r]
+ * act: any of enum qmm_act (QMM_ACT_SWIGLU_OAI as the experts': min(g, 7) sigmoid(1.702 min(g, 7)) (clamp(u, -7, 7) + 1)).
+ * Operands as qmm_linear, each with the formats and limits of its two-matrix product: QMM_F32 / QMM_BF16 the GGUF formats
+ * and QMM_MXFP4S, QMM_Q8 those of qmm_mv_swiglu_q8 and QMM_MXFP4S, QMM_F16 qmm_gemm's swiglu formats (one format for both
+ * matrices), QMM_MXFP8 qmm_gemm_mxfp4's. bias, bias2: f32 [n] or NULL. y [tokens, n] f32 or bf16. */
+int qmm_ffn_gate_up(int fmt, int act, int64_t tokens, int64_t k, int64_t n, const void *x, int x_dtype,
+                    const void *x_scales, const void *w, const void *ws, const void *w2, const void *ws2,
+                    const float *bias, const float *bias2, void *y, int y_dtype, qmm_stream_t stream);
+
+/* The backward pass of qmm_ffn_gate_up with frozen weights, first half: the gradients of the two projections' outputs,
+ *   dgu[t, 0, r] = dy[t, r] d(act(g) u)/dg,   dgu[t, 1, r] = dy[t, r] d(act(g) u)/du
+ * with g and u computed again from x as the QMM_F16 call computes them (fmt QMM_Q4_K, QMM_Q4_KT, QMM_Q6_K or QMM_Q4_0). dy:
+ * [tokens, n] f32 or bf16; dgu: bf16 [tokens, 2, n], rounded once (bf16 keeps a gradient's range; what trains beside the
+ * projections reads these rows). relu's slope at 0 is 0, a clamp's at its limit 1. Rows of a padding tile are not written. */
+int qmm_ffn_gate_up_grad(int fmt, int act, int64_t tokens, int64_t k, int64_t n, const void *x, const float *x_scales,
+                         const void *w, const void *w2, const float *bias, const float *bias2, const void *dy, int dy_dtype,
+                         void *dgu, qmm_stream_t stream);
+
+/* The operand of qmm_gemm_t from gradient rows x [rows, parts, n] (f32 or bf16; parts 1 or 2): x16 f16 [rows, parts, N] with
+ * N = n rounded up to a multiple of 64 (the added columns zero), scales f32 [rows, 2] = (2^-e, 2^e) with the row's largest
+ * magnitude times 2^-e in [2^13, 2^14), -126 <= e <= 100 (e = 0 for rows of zeros, subnormals, and with infinities or
+ * NaN). */
+int qmm_grad_operand(int64_t rows, int parts, int64_t n, const void *x, int x_dtype, void *x16, float *scales,
+                     qmm_stream_t stream);
+
+/* The transposed product, a projection's gradient with respect to its input (no reference counterpart: it does not train):
+ *   y[t, c] = sum_r x[t, 0, r] W[r, c] (+ sum_r x[t, 1, r] W2[r, c]),   c < k
+ * x, scales: the operand of qmm_grad_operand, one part without w2 and two with it. W, W2: n rows of k values, fmt QMM_Q4_K,
+ * QMM_Q4_KT, QMM_Q6_K or QMM_Q4_0, staged to f16 as qmm_gemm stages them; k % 256 == 0 (QMM_Q4_KT: n % 16 == 0,
+ * k % 512 == 0). y: [rows, k] f32 or bf16. fp32 accumulation in an order that follows from the shape. workspace: at least
+ * qmm_gemm_t_workspace_size bytes, 16-byte aligned (NULL where that is 0); calls that overlap need one each. */
+int qmm_gemm_t(int fmt, int64_t rows, int64_t k, int64_t n, const void *x, const float *scales, const void *w,
+               const void *w2, void *y, int y_dtype, void *workspace, int64_t workspace_bytes, qmm_stream_t stream);
+/* Workspace bytes of qmm_gemm_t (two: with w2), or -1 for a call it refuses. */
+int64_t qmm_gemm_t_workspace_size(int fmt, int64_t rows, int64_t k, int64_t n, int two);
 
 /* MoE router top-k from logits, g_moe_route / g_moe_route_tr after the router matvec
  * (S/gen_moe.py:116-252, :255-500; llama.cpp gating: 1 softmax, 2 sigmoid, 3 softmax over the picked logits):

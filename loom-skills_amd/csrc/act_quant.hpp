@@ -1,0 +1,54 @@
+// Activation rows in 8-value chunks and their Q8_1 groups: shared by the quantizer and the int8 matvecs that quantize
+// rows while staging them (gemv_q8.hip) and by the norm that writes Q8_1 (rms_norm.hip), so that all give the same bits.
+#pragma once
+
+#include "common.hpp"
+
+namespace qmm {
+
+typedef __attribute__((ext_vector_type(4))) u32 v4u;
+typedef __attribute__((ext_vector_type(2))) u32 v2u;
+
+// 8 activations of the lane as f32: from 16 bytes of bf16 or 32 bytes of f32 at element offset e
+__device__ __forceinline__ void load8_act(const void *x, bool bf, int64_t e, float (&v)[8]) {
+  if (bf) {
+    const v4u q = *reinterpret_cast<const v4u *>(static_cast<const u16 *>(x) + e);
+    const u32 d[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[2 * j] = bf16_to_f32(d[j] & 0xFFFFu); v[2 * j + 1] = bf16_to_f32(d[j] >> 16); }
+  } else {
+    const v4u a = *reinterpret_cast<const v4u *>(static_cast<const float *>(x) + e);
+    const v4u b = *reinterpret_cast<const v4u *>(static_cast<const float *>(x) + e + 4);
+    const u32 d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = u32_as_f32(d[j]);
+  }
+}
+
+// One 32-value group held by four consecutive lanes of a wave (8 values each, the group's first lane a multiple of
+// 4): the lane's 8 codes as two dwords, and the group's f16-rounded d and code sum.
+__device__ __forceinline__ void q8_group4(const float (&v)[8], u32 &c0, u32 &c1, float &d16, float &sum) {
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
+  amax = fmaxf(amax, __shfl_xor(amax, 1, 64));
+  amax = fmaxf(amax, __shfl_xor(amax, 2, 64));
+  const float d = amax / 127.f;
+  int s = 0;
+  u32 c[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = d > 0.f ? v[i] / d : 0.f;
+    const int q = (int)copysignf(floorf(fabsf(t) + 0.5f), t);
+    s += q;
+    c[i >> 2] |= ((u32)q & 0xFFu) << (8 * (i & 3));
+  }
+  s += __shfl_xor(s, 1, 64);
+  s += __shfl_xor(s, 2, 64);
+  c0 = c[0];
+  c1 = c[1];
+  d16 = (float)(_Float16)d;
+  sum = (float)s;
+}
+
+}  // namespace qmm

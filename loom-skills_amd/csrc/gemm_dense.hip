@@ -38,6 +38,7 @@
 // 2048 (p % 2) + 32 (sb % 2) + 16 (p / 2) (codes) or (sb / 2) 4608 + 16 (sb % 2) (header), is the same for every lane.
 #include "common.hpp"
 #include "deq_f16.hpp"
+#include "epilogue.hpp"
 
 #include <type_traits>
 
@@ -79,8 +80,8 @@ __device__ __forceinline__ void header_pairs(const uint4 &hd, u32 (&out)[8]) {
   }
 }
 
-template <bool ACC, bool BF16OUT, bool TL>
-__global__ __launch_bounds__(kWaves * 64, 1) void q4k_dense_kernel(DArgs a) {
+template <bool ACC, bool BF16OUT, bool TL, class EP = NoEpi>
+__global__ __launch_bounds__(kWaves * 64, 1) void q4k_dense_kernel(DArgs a, EP ep) {
   __shared__ __align__(16) u8 abuf[kWaves][2][kAbuf];   // also the K-part reduction area at the end
   __shared__ __align__(16) u32 stab[kWaves][2][kSlot];
   __shared__ int src_row[kBM];
@@ -372,7 +373,18 @@ __global__ __launch_bounds__(kWaves * 64, 1) void q4k_dense_kernel(DArgs a) {
       for (int e = 0; e < 4; ++e) v[4 * q + e] = (x0[e] + x1[e]) * inv;
     }
     const int64_t o = (int64_t)row * N + col;
-    if (vec && col + 8 <= N) {
+    if constexpr (kEpi<EP>) {   // eight columns of a row: their bias and residual values, then the stores
+      float b[8], r[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = col + e < N;
+        b[e] = in ? epi_bias(ep.bias, col + e) : 0.f;
+        r[e] = in && ep.res ? load_val(ep.res, ep.res_bf16, o + e) : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < N) epi_put(ep, o + e, v[e] + b[e], r[e]);
+    } else if (vec && col + 8 <= N) {
       if constexpr (BF16OUT) {
         typedef __attribute__((ext_vector_type(2))) __bf16 bf2;
         u16 *yb = static_cast<u16 *>(a.y) + o;
@@ -415,11 +427,11 @@ __global__ __launch_bounds__(kWaves * 64, 1) void q4k_dense_kernel(DArgs a) {
   }
 }
 
-template <bool ACC, bool BF16OUT>
-int launch_dense(const DArgs &a, bool tiled, hipStream_t s) {
+template <bool ACC, bool BF16OUT, class EP = NoEpi>
+int launch_dense(const DArgs &a, bool tiled, hipStream_t s, EP ep = {}) {
   const dim3 grid((unsigned)(8 * ((a.tiles_total + 7) / 8)));
-  if (tiled) q4k_dense_kernel<ACC, BF16OUT, true><<<grid, kWaves * 64, 0, s>>>(a);
-  else q4k_dense_kernel<ACC, BF16OUT, false><<<grid, kWaves * 64, 0, s>>>(a);
+  if (tiled) q4k_dense_kernel<ACC, BF16OUT, true, EP><<<grid, kWaves * 64, 0, s>>>(a, ep);
+  else q4k_dense_kernel<ACC, BF16OUT, false, EP><<<grid, kWaves * 64, 0, s>>>(a, ep);
   return launch_status();
 }
 
@@ -428,13 +440,14 @@ int launch_dense(const DArgs &a, bool tiled, hipStream_t s) {
 // The Q4_K store / acc path of qmm_gemm (gemm_q4k.hip validates the arguments): GGUF Q4_K weights or (tiled) the
 // QMM_Q4_KT layout, f16 rows.
 int qmm_gemm_q4k_dense(int acc, int tiled, int64_t rows, int64_t k, int64_t n, const void *x, const float *scales,
-                       const void *w, void *y, int y_bf16, hipStream_t s) {
+                       const void *w, void *y, int y_bf16, hipStream_t s, const Epi *ep) {
   DArgs a{};
   a.M = (int)rows; a.N = (int)n; a.K = (int)k;
   a.x16 = static_cast<const _Float16 *>(x); a.scales = scales;
   a.w = static_cast<const u8 *>(w); a.y = y;
   a.tiles_m = (int)((rows + kBM - 1) / kBM);
   a.tiles_total = a.tiles_m * (int)((n + kBN - 1) / kBN);
+  if (ep) return launch_dense<false, false, Epi>(a, tiled, s, *ep);
   if (acc && y_bf16) return launch_dense<true, true>(a, tiled, s);
   if (acc) return launch_dense<true, false>(a, tiled, s);
   if (y_bf16) return launch_dense<false, true>(a, tiled, s);

@@ -469,7 +469,29 @@ int fmt_align(int fmt) { return fmt == QMM_Q4_K || fmt == QMM_Q4_KT ? 16 : fmt =
 
 // the dense Q4_K GEMM (gemm_dense.hip): store / acc modes, GGUF or tiled weights
 int qmm_gemm_q4k_dense(int acc, int tiled, int64_t rows, int64_t k, int64_t n, const void *x, const float *scales,
-                       const void *w, void *y, int y_bf16, hipStream_t s);
+                       const void *w, void *y, int y_bf16, hipStream_t s, const Epi *ep);
+
+// The GEMMs with an epilogue over GGUF-block or tiled Q4_K weights: kind kTLinear, kTGlu or kTGluGrad (gemm_tile.hpp).
+int qmm_gemm_epi(int fmt, int kind, int64_t rows, int64_t k, int64_t n, const void *x, const float *scales, const void *w,
+                 const void *w2, const void *dy, int dy_bf16, hipStream_t s, const Epi &ep) {
+  const bool tiled = fmt == QMM_Q4_KT, two = kind != kTLinear;
+  if (!gguf_gemm_fmt(fmt) && !tiled) return QMM_ERR_FORMAT;
+  if (!x || !w || (two && !w2) || (kind == kTGluGrad && !dy)) return QMM_ERR_NULL;
+  if (rows <= 0 || n <= 0 || k <= 0 || k % 256 || rows > (1 << 24) || n > (1 << 24) || k > (1 << 20)) return QMM_ERR_SHAPE;
+  if (tiled && (n % 16 || k % 512)) return QMM_ERR_SHAPE;   // whole 16-row blocks of whole 512-value units
+  const int wal = fmt_align(fmt);
+  if (!aligned(x, 16) || !aligned(scales, 4) || !aligned(w, wal) || !aligned(w2, wal)) return QMM_ERR_ALIGN;
+  // activation rows and weight rows are addressed by 32-bit buffer offsets
+  if (rows * k * 2 >= (1ll << 31) || n * fmt_row_bytes(fmt, k) >= (1ll << 31)) return QMM_ERR_SHAPE;
+  const int shape = tile_shape(two, fmt == QMM_Q4_K || tiled, rows, n, k);
+  if (shape == kDenseKernel) return qmm_gemm_q4k_dense(0, tiled, rows, k, n, x, scales, w, nullptr, 0, s, &ep);
+  TileArgs t{};
+  t.M = (int)rows; t.N = (int)n; t.K = (int)k;
+  t.x16 = static_cast<const _Float16 *>(x); t.scales = scales; t.x_rows = (int)rows;
+  t.w = static_cast<const u8 *>(w); t.w2 = static_cast<const u8 *>(w2);
+  t.ep = ep; t.dy = dy; t.dy_bf16 = dy_bf16;
+  return tile_gemm(fmt, kind, shape, t, s);
+}
 
 extern "C" int qmm_gemm(int fmt, int mode, int64_t rows, int64_t k, int64_t n, const void *x, int x_dtype,
                         const float *scales, const void *w, const void *w2, void *y, int y_dtype,
@@ -506,7 +528,7 @@ extern "C" int qmm_gemm(int fmt, int mode, int64_t rows, int64_t k, int64_t n, c
     return bf ? launch_mixed<kSwiglu, true>(fmt, fu, a, s) : launch_mixed<kSwiglu, false>(fmt, fu, a, s);
   }
   const int shape = tile_shape(mode == QMM_GEMM_SWIGLU, fmt == QMM_Q4_K || tiled, rows, n, k);
-  if (shape == kDenseKernel) return qmm_gemm_q4k_dense(acc, tiled, rows, k, n, x, scales, w, y, bf, s);
+  if (shape == kDenseKernel) return qmm_gemm_q4k_dense(acc, tiled, rows, k, n, x, scales, w, y, bf, s, nullptr);
   TileArgs t{};
   t.M = (int)rows; t.N = (int)n; t.K = (int)k;
   t.x16 = static_cast<const _Float16 *>(x); t.scales = scales; t.x_rows = (int)rows;

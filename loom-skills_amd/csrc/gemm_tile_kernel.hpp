@@ -6,6 +6,9 @@
 //   swiglu  Y[r, c]   = silu(inv[r] sum_k X16[r, k] Wg[c, k]) (inv[r] sum_k X16[r, k] Wu[c, k])
 //   gu      act[r, c] = act_fn(inv[t] sum_k X16[t, k] Wg[e][c, k] + bg[e, c], inv[t] sum_k X16[t, k] Wu[e][c, k]
 //                       + bu[e, c]),  t = rowmap[r] / KU  (rows gathered from the token rows)
+//   linear  Y[r, c]   = act(inv[r] sum_k X16[r, k] W[c, k] + b[c]) + res[r, c]                          (qmm_linear)
+//   glu     Y[r, c]   = act(g) u, g = inv[r] sum_k X16[r, k] Wg[c, k] + bg[c], u likewise          (qmm_ffn_gate_up)
+//   grad    D[r, 0, c] = dy[r, c] u act'(g), D[r, 1, c] = dy[r, c] act(g)                     (qmm_ffn_gate_up_grad)
 //   dn      ys[r, c]  = inv[r] sum_k A16[r, k] Wd[e][c, k] + bd[e, c]            (rows already sorted)
 //
 // X16 / A16 are the row-scaled f16 operands of g_row_scale_f16[_tiles] (S/gen_llm.py:1843-1915, S/gen_moe.py:503-527),
@@ -77,6 +80,8 @@ struct Raw<kQ40> {   // two blocks' 16 code bytes and d
   u32 d[2];
 };
 
+constexpr bool two_matrices(int kind) { return kind == kTGU || kind == kTSwiglu || kind == kTGlu || kind == kTGluGrad; }
+constexpr bool dense_rows(int kind) { return kind != kTGU && kind != kTDN; }
 constexpr int raw_of(int wf) { return wf == kQ4KT ? kQ4K : wf; }
 constexpr int64_t row_bytes_of(int wf, int64_t k) {
   return wf == kQ40 ? k / 32 * 18 : k / 256 * (wf == kQ6K ? 210 : 144);
@@ -281,8 +286,7 @@ __device__ __forceinline__ u32 dequant2(const Raw<raw_of(WF)> &r, u32 pr, int jh
 template <int WF, int KIND, int BM, int NW, int KS>
 __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) {
   constexpr int NI = BM / 32;
-  constexpr bool kTwoW = KIND == kTGU || KIND == kTSwiglu;
-  constexpr bool kDenseRows = KIND == kTDense || KIND == kTSwiglu;
+  constexpr bool kTwoW = two_matrices(KIND), kDenseRows = dense_rows(KIND);
   constexpr int BN = (kTwoW ? 32 : 64) * NW;   // output columns
   constexpr int kPart = BM * 256;              // LDS bytes of a K-part's staged step
   static_assert(BM <= 64 * NW * KS && BM % (4 * NW) == 0 && 16 % KS == 0, "prologue and staging maps");
@@ -376,7 +380,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
   Stream<WF> st;
   {
     const u8 *mg = a.w, *mu = a.w;
-    if constexpr (KIND == kTSwiglu) mu = a.w2;
+    if constexpr (kDenseRows && kTwoW) mu = a.w2;
     if constexpr (!kDenseRows) mg = mu = a.w + (int64_t)expert * a.ebytes;
     if constexpr (KIND == kTGU) mu = a.w2 ? a.w2 + (int64_t)expert * a.ebytes2 : mg + a.up_off;
     const int64_t nb = (int64_t)n0 * RB;   // n0 is a multiple of 16: tiled columns too
@@ -543,6 +547,64 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
   }
 
   // ---- epilogue: accumulator register r of a block is row 8 (r / 4) + 4 h + r % 4, column lc
+  if constexpr (KIND == kTLinear || KIND == kTGlu || KIND == kTGluGrad) {
+    // The values a 32-row block reads (residual, dy) are loaded before its first store: the compiler cannot move a load
+    // over a store that might alias it, and a round trip a value would cost more than the tile's MFMAs
+    constexpr int NC = kTwoW ? 1 : 2;
+    float b1[NC], b2 = 0.f;
+    int col[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      col[j] = n0 + (kTwoW ? 32 * wn : 64 * wn + 32 * j) + lc;
+      b1[j] = epi_bias(a.ep.bias, min(col[j], N - 1));
+    }
+    if constexpr (kTwoW) b2 = epi_bias(a.ep.bias2, min(col[0], N - 1));
+    const void *in = KIND == kTGluGrad ? a.dy : a.ep.res;
+    const int in_bf16 = KIND == kTGluGrad ? a.dy_bf16 : a.ep.res_bf16;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      float add[NC][RK];
+      if (KIND != kTGlu && in) {
+#pragma unroll
+        for (int r = 0; r < RK; ++r) {
+          const int rr = kp * RK + r;
+          const int lr = 32 * i + 8 * (rr >> 2) + 4 * h + (rr & 3);
+          const bool live = src_row[lr] >= 0;
+#pragma unroll
+          for (int j = 0; j < NC; ++j)
+            add[j][r] = live && col[j] < N ? load_val(in, in_bf16, (int64_t)(m0 + lr) * N + col[j]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < RK; ++r) {
+        const int rr = kp * RK + r;
+        const int lr = 32 * i + 8 * (rr >> 2) + 4 * h + (rr & 3);
+        if (src_row[lr] < 0) continue;
+        const float inv = rinv[lr];
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          if (col[j] >= N) continue;
+          const int64_t o = (int64_t)(m0 + lr) * N + col[j];
+          const float v = __builtin_fmaf(out[i][j][r], inv, b1[j]);
+          if constexpr (KIND == kTLinear) {
+            epi_put(a.ep, o, v, add[j][r]);
+          } else {
+            const float u = __builtin_fmaf(out[i][1][r], inv, b2);
+            if constexpr (KIND == kTGlu) {
+              store_val(a.ep.y, a.ep.y_bf16, o, act2(a.ep.act, v, u));
+            } else {
+              float dg, du;
+              act2_grad(a.ep.act, v, u, add[0][r], dg, du);
+              const int64_t od = 2 * (int64_t)(m0 + lr) * N + col[j];
+              store_val(a.ep.y, 1, od, dg);
+              store_val(a.ep.y, 1, od + N, du);
+            }
+          }
+        }
+      }
+    }
+    return;
+  }
   float *yf = static_cast<float *>(a.y);
   u16 *yb = static_cast<u16 *>(a.y);
 #pragma unroll
@@ -580,8 +642,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
 
 template <int WF, int KIND, int BM, int NW, int KS>
 int launch(TileArgs a, hipStream_t s) {
-  constexpr bool kTwoW = KIND == kTGU || KIND == kTSwiglu;
-  constexpr bool kDenseRows = KIND == kTDense || KIND == kTSwiglu;
+  constexpr bool kTwoW = two_matrices(KIND), kDenseRows = dense_rows(KIND);
   constexpr int BN = (kTwoW ? 32 : 64) * NW;
   constexpr int kLds = 2 * KS * BM * 256 + NW * KS * xpose_bytes(WF);
   if constexpr (kDenseRows) a.tiles_m = (a.M + BM - 1) / BM;   // grouped: the caller's 64-row expert tiles
@@ -595,20 +656,25 @@ int launch(TileArgs a, hipStream_t s) {
   return launch_status();
 }
 
+template <int WF, int KIND>
+int dispatch_dense(int shape, const TileArgs &a, hipStream_t s) {
+  if (shape == kT128x4x1) return launch<WF, KIND, 128, 4, 1>(a, s);
+  if (shape == kT128x4x2) return launch<WF, KIND, 128, 4, 2>(a, s);
+  if (shape == kT64x4x1) return launch<WF, KIND, 64, 4, 1>(a, s);
+  return launch<WF, KIND, 64, 2, 4>(a, s);
+}
+
 template <int WF>
 int dispatch(int kind, int shape, const TileArgs &a, hipStream_t s) {
-  if (kind == kTGU) return launch<WF, kTGU, 64, 4, 1>(a, s);
-  if (kind == kTDN) return launch<WF, kTDN, 64, 4, 1>(a, s);
-  if (kind == kTSwiglu) {
-    if (shape == kT128x4x1) return launch<WF, kTSwiglu, 128, 4, 1>(a, s);
-    if (shape == kT128x4x2) return launch<WF, kTSwiglu, 128, 4, 2>(a, s);
-    if (shape == kT64x4x1) return launch<WF, kTSwiglu, 64, 4, 1>(a, s);
-    return launch<WF, kTSwiglu, 64, 2, 4>(a, s);
+  switch (kind) {
+    case kTGU: return launch<WF, kTGU, 64, 4, 1>(a, s);
+    case kTDN: return launch<WF, kTDN, 64, 4, 1>(a, s);
+    case kTSwiglu: return dispatch_dense<WF, kTSwiglu>(shape, a, s);
+    case kTLinear: return dispatch_dense<WF, kTLinear>(shape, a, s);
+    case kTGlu: return dispatch_dense<WF, kTGlu>(shape, a, s);
+    case kTGluGrad: return dispatch_dense<WF, kTGluGrad>(shape, a, s);
+    default: return dispatch_dense<WF, kTDense>(shape, a, s);
   }
-  if (shape == kT128x4x1) return launch<WF, kTDense, 128, 4, 1>(a, s);
-  if (shape == kT128x4x2) return launch<WF, kTDense, 128, 4, 2>(a, s);
-  if (shape == kT64x4x1) return launch<WF, kTDense, 64, 4, 1>(a, s);
-  return launch<WF, kTDense, 64, 2, 4>(a, s);
 }
 
 }  // namespace tile

@@ -11,6 +11,7 @@
 // token does not depend on how many tokens the call carries (multi-token == one-token, bit for bit).
 #include <type_traits>
 
+#include "epilogue.hpp"
 #include "rowdot.hpp"
 #include "topk.hpp"
 
@@ -34,11 +35,11 @@ __device__ __forceinline__ void reduce_all(float (&acc)[RW][TG]) {
     for (int t = 0; t < TG; ++t) acc[r][t] = wave_sum(acc[r][t]);
 }
 
-template <class P, int TG, int RW>
+template <class P, int TG, int RW, class EP = NoEpi>
 __global__ __launch_bounds__(256) void mv_kernel(int64_t n, int64_t tokens, int64_t k, int accumulate,
                                                  const u8 *__restrict__ x, int64_t x_row_bytes,
                                                  const u8 *__restrict__ w, const u8 *__restrict__ ws, int64_t rb,
-                                                 int64_t srb, float *__restrict__ y) {
+                                                 int64_t srb, float *__restrict__ y, EP ep) {
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int64_t t0 = (int64_t)blockIdx.x * TG;
@@ -73,8 +74,12 @@ __global__ __launch_bounds__(256) void mv_kernel(int64_t n, int64_t tokens, int6
     for (int t = 0; t < TG; ++t) {
       const int64_t row = row0 + r, tok = t0 + t;
       if (lane == r * TG + t && row < n && tok < tokens) {
-        float *p = y + tok * n + row;
-        *p = accumulate ? *p + acc[r][t] : acc[r][t];
+        if constexpr (kEpi<EP>) {
+          epi_store(ep, tok * n + row, row, acc[r][t]);
+        } else {
+          float *p = y + tok * n + row;
+          *p = accumulate ? *p + acc[r][t] : acc[r][t];
+        }
       }
     }
 }
@@ -84,7 +89,7 @@ __global__ __launch_bounds__(256) void mv_kernel(int64_t n, int64_t tokens, int6
 // rg, rg + 64 / LPR, ... of the wave's RW, and a row's LPR lanes meet in the butterfly of wave_sum restricted to
 // their group. With one item a lane up to LPR items, the lanes a full-wave butterfly would add past the group hold
 // zeros, so the row sums are the same for every LPR.
-template <class P, int RW, bool GU, int NS = 0, int LPR = 64>
+template <class P, int RW, bool GU, int NS = 0, int LPR = 64, class EP = NoEpi>
 __global__ __launch_bounds__(256) void expert_mv_kernel(int64_t n, int64_t assignments, int KU, int E, int64_t k,
                                                         const int32_t *__restrict__ ids, const u8 *__restrict__ x,
                                                         int64_t x_row_bytes, const u8 *__restrict__ w,
@@ -92,7 +97,7 @@ __global__ __launch_bounds__(256) void expert_mv_kernel(int64_t n, int64_t assig
                                                         const u8 *__restrict__ ws2, int64_t rb, int64_t srb,
                                                         int64_t ebytes, int64_t esbytes, const float *__restrict__ bias,
                                                         const float *__restrict__ bias2, int act, int accumulate,
-                                                        float *__restrict__ y, RouteArgs route = {}) {
+                                                        float *__restrict__ y, RouteArgs route = {}, EP ep = {}) {
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int64_t a = blockIdx.x;
@@ -161,7 +166,9 @@ __global__ __launch_bounds__(256) void expert_mv_kernel(int64_t n, int64_t assig
 #pragma unroll
   for (int r = 0; r < RL; ++r) {
     const int64_t row = row0 + rg + G * r;
-    if (sub == 0 && row < n) {
+    if constexpr (kEpi<EP>) {   // the dense gate/up matvec with an epilogue: one expert, token a
+      if (sub == 0 && row < n) epi_store2(ep, a * n + row, row, ag[r], au[r]);
+    } else if (sub == 0 && row < n) {
       float g = ag[r];
       if (bias) g += bias[e * n + row];
       float v = g;
@@ -318,26 +325,30 @@ __global__ __launch_bounds__(512) void expert_mv_combine_kernel(int64_t n, int K
 
 template <class P, int TG>
 int launch_mv(int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, int64_t x_row_bytes,
-              const void *w, const void *ws, int64_t rb, int64_t srb, float *y, hipStream_t s) {
+              const void *w, const void *ws, int64_t rb, int64_t srb, float *y, hipStream_t s, const Epi *ep) {
   const dim3 grid((unsigned)((tokens + TG - 1) / TG), (unsigned)((n + kWavesPerBlock * kRW - 1) / (kWavesPerBlock * kRW)));
-  mv_kernel<P, TG, kRW><<<grid, 256, 0, s>>>(n, tokens, k, accumulate, static_cast<const u8 *>(x), x_row_bytes,
-                                            static_cast<const u8 *>(w), static_cast<const u8 *>(ws), rb, srb, y);
-  return launch_status();
+  auto go = [&](auto e) {
+    mv_kernel<P, TG, kRW, decltype(e)><<<grid, 256, 0, s>>>(n, tokens, k, accumulate, static_cast<const u8 *>(x), x_row_bytes,
+                                                            static_cast<const u8 *>(w), static_cast<const u8 *>(ws), rb,
+                                                            srb, y, e);
+    return launch_status();
+  };
+  return ep ? go(*ep) : go(NoEpi{});
 }
 
 // token group: 4 (bf16 activations) or 2 (f32 activations) tokens share every weight load
 template <template <bool> class P>
 int dispatch_mv(bool bf, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, const void *w,
-                const void *ws, int64_t rb, int64_t srb, float *y, hipStream_t s) {
+                const void *ws, int64_t rb, int64_t srb, float *y, hipStream_t s, const Epi *ep) {
   if (bf) {
     const int64_t xb = k * 2;
-    if (tokens >= 4) return launch_mv<P<true>, 4>(k, n, tokens, accumulate, x, xb, w, ws, rb, srb, y, s);
-    if (tokens >= 2) return launch_mv<P<true>, 2>(k, n, tokens, accumulate, x, xb, w, ws, rb, srb, y, s);
-    return launch_mv<P<true>, 1>(k, n, tokens, accumulate, x, xb, w, ws, rb, srb, y, s);
+    if (tokens >= 4) return launch_mv<P<true>, 4>(k, n, tokens, accumulate, x, xb, w, ws, rb, srb, y, s, ep);
+    if (tokens >= 2) return launch_mv<P<true>, 2>(k, n, tokens, accumulate, x, xb, w, ws, rb, srb, y, s, ep);
+    return launch_mv<P<true>, 1>(k, n, tokens, accumulate, x, xb, w, ws, rb, srb, y, s, ep);
   }
   const int64_t xb = k * 4;
-  if (tokens >= 2) return launch_mv<P<false>, 2>(k, n, tokens, accumulate, x, xb, w, ws, rb, srb, y, s);
-  return launch_mv<P<false>, 1>(k, n, tokens, accumulate, x, xb, w, ws, rb, srb, y, s);
+  if (tokens >= 2) return launch_mv<P<false>, 2>(k, n, tokens, accumulate, x, xb, w, ws, rb, srb, y, s, ep);
+  return launch_mv<P<false>, 1>(k, n, tokens, accumulate, x, xb, w, ws, rb, srb, y, s, ep);
 }
 
 template <bool B> using MXG = MXFP4<B, false>;
@@ -359,7 +370,7 @@ int check_weights(int fmt, int64_t k, const void *w, const void *ws) {
 }  // namespace
 
 int qmm_mv_q4k_fast(int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, const void *w, float *y,
-                    hipStream_t s);
+                    hipStream_t s, const Epi *ep);
 int qmm_topk_expert_mv_tiled(const RouteArgs &r, int E, int KU, int64_t tokens, int fused, int act, int64_t k,
                              int64_t n, const void *x, int x_dtype, const void *w, const void *ws, const void *w2,
                              const void *ws2, const float *bias, const float *bias2, float *y, hipStream_t s);
@@ -368,39 +379,43 @@ int qmm_expert_mv_combine_tiled(int64_t k, int64_t n, int E, int KU, int64_t tok
                                 const float *bias, int accumulate, const float *sg, float *y, hipStream_t s);
 
 int qmm_mv_q40t_f32(int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, int x_dtype, const void *w,
-                    float *y, hipStream_t s);
+                    float *y, hipStream_t s, const Epi *ep);
 
-extern "C" int qmm_mv(int fmt, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, int x_dtype,
-                      const void *w, const void *ws, float *y, qmm_stream_t stream) {
+int qmm_mv_impl(int fmt, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, int x_dtype, const void *w,
+                const void *ws, float *y, hipStream_t s, const Epi *ep) {
   if (fmt == QMM_Q4_0T) {   // the tiled Q4_0 units of qmm_tile_q40 (gemv_q4kt.hip)
-    if (!x || !w || !y) return QMM_ERR_NULL;
+    if (!x || !w || (!y && !ep)) return QMM_ERR_NULL;
     if (x_dtype != QMM_F32 && x_dtype != QMM_BF16) return QMM_ERR_DTYPE;
     if (n <= 0 || tokens <= 0 || k <= 0 || n > (1ll << 30) || k > (1ll << 20)) return QMM_ERR_SHAPE;
     if (!aligned(x, 16) || !aligned(w, 16) || !aligned(y, 4)) return QMM_ERR_ALIGN;
-    return qmm_mv_q40t_f32(k, n, tokens, accumulate, x, x_dtype, w, y, reinterpret_cast<hipStream_t>(stream));
+    return qmm_mv_q40t_f32(k, n, tokens, accumulate, x, x_dtype, w, y, s, ep);
   }
   if (!valid_fmt(fmt)) return QMM_ERR_FORMAT;
-  if (!x || !y) return QMM_ERR_NULL;
+  if (!x || (!y && !ep)) return QMM_ERR_NULL;
   if (n <= 0 || tokens <= 0 || row_bytes(fmt, k) == 0) return QMM_ERR_SHAPE;
   if (n > (1ll << 30) || tokens > (1ll << 20) || k > (1ll << 24)) return QMM_ERR_SHAPE;
   if (x_dtype != QMM_F32 && x_dtype != QMM_BF16) return QMM_ERR_DTYPE;
   if (int st = check_weights(fmt, k, w, ws)) return st;
   if (!aligned(x, 16) || !aligned(y, 4)) return QMM_ERR_ALIGN;
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool bf = x_dtype == QMM_BF16;
   const int64_t rb = row_bytes(fmt, k), srb = fmt == QMM_MXFP4S ? k / 32 : 0;
   switch (fmt) {
     case QMM_Q4_K:
       if (bf) {
-        const int st = qmm_mv_q4k_fast(k, n, tokens, accumulate, x, w, y, s);
+        const int st = qmm_mv_q4k_fast(k, n, tokens, accumulate, x, w, y, s, ep);
         if (st != 1) return st;
       }
-      return dispatch_mv<Q4K>(bf, k, n, tokens, accumulate, x, w, w, rb, 0, y, s);
-    case QMM_Q4_0: return dispatch_mv<Q40>(bf, k, n, tokens, accumulate, x, w, w, rb, 0, y, s);
-    case QMM_Q6_K: return dispatch_mv<Q6K>(bf, k, n, tokens, accumulate, x, w, w, rb, 0, y, s);
-    case QMM_MXFP4: return dispatch_mv<MXG>(bf, k, n, tokens, accumulate, x, w, w, rb, 0, y, s);
-    default: return dispatch_mv<MXS>(bf, k, n, tokens, accumulate, x, w, ws, rb, srb, y, s);
+      return dispatch_mv<Q4K>(bf, k, n, tokens, accumulate, x, w, w, rb, 0, y, s, ep);
+    case QMM_Q4_0: return dispatch_mv<Q40>(bf, k, n, tokens, accumulate, x, w, w, rb, 0, y, s, ep);
+    case QMM_Q6_K: return dispatch_mv<Q6K>(bf, k, n, tokens, accumulate, x, w, w, rb, 0, y, s, ep);
+    case QMM_MXFP4: return dispatch_mv<MXG>(bf, k, n, tokens, accumulate, x, w, w, rb, 0, y, s, ep);
+    default: return dispatch_mv<MXS>(bf, k, n, tokens, accumulate, x, w, ws, rb, srb, y, s, ep);
   }
+}
+
+extern "C" int qmm_mv(int fmt, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, int x_dtype,
+                      const void *w, const void *ws, float *y, qmm_stream_t stream) {
+  return qmm_mv_impl(fmt, k, n, tokens, accumulate, x, x_dtype, w, ws, y, reinterpret_cast<hipStream_t>(stream), nullptr);
 }
 
 namespace {
@@ -481,6 +496,21 @@ int launch_swiglu(bool bf, int64_t k, int64_t n, int64_t tokens, int accumulate,
                                         nullptr, QMM_ACT_SILU, y, s, accumulate);
   return launch_expert<P<false>, true>(k, n, 1, 1, tokens, nullptr, x, xb, w, w, w2, w2, rb, 0, rb * n, 0, nullptr,
                                        nullptr, QMM_ACT_SILU, y, s, accumulate);
+}
+
+// The same with the epilogue of qmm_ffn_gate_up.
+template <class P>
+int launch_gate_up(int64_t k, int64_t n, int64_t tokens, const void *x, int64_t x_row_bytes, const void *w, const void *ws,
+                   const void *w2, const void *ws2, int64_t rb, int64_t srb, hipStream_t s, const Epi &ep) {
+  constexpr int RW = expert_rw<true>();
+  const dim3 grid((unsigned)tokens, (unsigned)((n + kWavesPerBlock * RW - 1) / (kWavesPerBlock * RW)));
+  return with_lpr<RW>(expert_lpr(P::items(k), RW), [&](auto lc) {
+    expert_mv_kernel<P, RW, true, 0, decltype(lc)::value, Epi><<<grid, 256, 0, s>>>(
+        n, tokens, 1, 1, k, nullptr, static_cast<const u8 *>(x), x_row_bytes, static_cast<const u8 *>(w),
+        static_cast<const u8 *>(ws), static_cast<const u8 *>(w2), static_cast<const u8 *>(ws2), rb, srb, 0, 0, nullptr,
+        nullptr, 0, 0, nullptr, RouteArgs{}, ep);
+    return launch_status();
+  });
 }
 
 template <template <bool> class P>
@@ -633,6 +663,32 @@ static int expert_mv_impl(int fmt, int mode, int fused, int act, int64_t k, int6
     case QMM_MXFP4: return dispatch_expert<MXG>(gu, bf, k, n, E, KU, assignments, ids, x, w, wsg, wu, wsu, rb, srb, ebytes, esbytes, bias, bias2, act, y, s);
     case QMM_Q6_K: return dispatch_expert<Q6K>(gu, bf, k, n, E, KU, assignments, ids, x, w, wsg, wu, wsu, rb, srb, ebytes, esbytes, bias, bias2, act, y, s);
     default: return dispatch_expert<MXS>(gu, bf, k, n, E, KU, assignments, ids, x, w, wsg, wu, wsu, rb, srb, ebytes, esbytes, bias, bias2, act, y, s);
+  }
+}
+
+int qmm_mv_gate_up_impl(int fmt, int64_t k, int64_t n, int64_t tokens, const void *x, int x_dtype, const void *w,
+                        const void *ws, const void *w2, const void *ws2, hipStream_t s, const Epi &ep) {
+  if (!valid_fmt(fmt)) return QMM_ERR_FORMAT;
+  if (!x) return QMM_ERR_NULL;
+  if (n <= 0 || tokens <= 0 || row_bytes(fmt, k) == 0) return QMM_ERR_SHAPE;
+  if (tokens > (1 << 24) || k > (1 << 24) || n > 65535ll * kWavesPerBlock * expert_rw<true>()) return QMM_ERR_SHAPE;   // the grid
+  if (x_dtype != QMM_F32 && x_dtype != QMM_BF16) return QMM_ERR_DTYPE;
+  if (int st = check_weights(fmt, k, w, ws)) return st;
+  if (int st = check_weights(fmt, k, w2, ws2)) return st;
+  if (!aligned(x, 16)) return QMM_ERR_ALIGN;
+  const bool bf = x_dtype == QMM_BF16;
+  const int64_t rb = row_bytes(fmt, k), srb = fmt == QMM_MXFP4S ? k / 32 : 0, xb = k * (bf ? 2 : 4);
+  if (!srb) { ws = w; ws2 = w2; }
+  auto go = [&](auto pb, auto pf) {
+    return bf ? launch_gate_up<decltype(pb)>(k, n, tokens, x, xb, w, ws, w2, ws2, rb, srb, s, ep)
+              : launch_gate_up<decltype(pf)>(k, n, tokens, x, xb, w, ws, w2, ws2, rb, srb, s, ep);
+  };
+  switch (fmt) {
+    case QMM_Q4_K: return go(Q4K<true>{}, Q4K<false>{});
+    case QMM_Q4_0: return go(Q40<true>{}, Q40<false>{});
+    case QMM_Q6_K: return go(Q6K<true>{}, Q6K<false>{});
+    case QMM_MXFP4: return go(MXG<true>{}, MXG<false>{});
+    default: return go(MXS<true>{}, MXS<false>{});
   }
 }
 

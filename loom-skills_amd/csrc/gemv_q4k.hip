@@ -19,6 +19,7 @@
 // Rows are summed with a transposed butterfly, the same tree for every token count, and a token's arithmetic does
 // not depend on the other tokens of its group: results are identical whatever the number of tokens in the call.
 #include "bfly.hpp"
+#include "epilogue.hpp"
 
 using namespace qmm;
 
@@ -40,10 +41,10 @@ constexpr int kWaves = QMM_Q4K_WAVES;
 constexpr int kThreads = kWaves * 64;
 constexpr int kSlots = QMM_Q4K_SLOTS;
 
-template <int TG, int KB>
+template <int TG, int KB, class EP = NoEpi>
 __global__ __launch_bounds__(kThreads) void mv_q4k_kernel(int64_t n, int64_t tokens, int accumulate,
                                                           const u16 *__restrict__ x, const u8 *__restrict__ w,
-                                                          float *__restrict__ y) {
+                                                          float *__restrict__ y, EP ep) {
   constexpr int K = KB * 4096;
   constexpr int L = 32 * KB;            // lanes per row
   constexpr int RPP = 64 / L;           // rows per wave and slot
@@ -214,28 +215,36 @@ __global__ __launch_bounds__(kThreads) void mv_q4k_kernel(int64_t n, int64_t tok
     const int64_t row = wrow0 + s * RPP + rp, tok = t0 + t;
     if (row < n && tok < tokens) {
       const float v = ldexpf(tot, eexp[t]);
-      float *py = y + tok * n + row;
-      *py = accumulate ? *py + v : v;
+      if constexpr (kEpi<EP>) {
+        epi_store(ep, tok * n + row, row, v);
+      } else {
+        float *py = y + tok * n + row;
+        *py = accumulate ? *py + v : v;
+      }
     }
   }
 }
 
 template <int TG, int KB>
-int launch(int64_t n, int64_t tokens, int accumulate, const void *x, const void *w, float *y, hipStream_t s) {
+int launch(int64_t n, int64_t tokens, int accumulate, const void *x, const void *w, float *y, hipStream_t s,
+           const Epi *ep) {
   constexpr int WG_ROWS = kWaves * kSlots * (2 / KB);
   const dim3 grid((unsigned)((n + WG_ROWS - 1) / WG_ROWS), (unsigned)((tokens + TG - 1) / TG));
-  mv_q4k_kernel<TG, KB><<<grid, kThreads, 0, s>>>(n, tokens, accumulate, static_cast<const u16 *>(x),
-                                                  static_cast<const u8 *>(w), y);
-  return launch_status();
+  auto go = [&](auto e) {
+    mv_q4k_kernel<TG, KB, decltype(e)><<<grid, kThreads, 0, s>>>(n, tokens, accumulate, static_cast<const u16 *>(x),
+                                                                 static_cast<const u8 *>(w), y, e);
+    return launch_status();
+  };
+  return ep ? go(*ep) : go(NoEpi{});
 }
 
 }  // namespace
 
 // Fast path of qmm_mv: Q4_K, bf16 activations, K = 4096 or 8192 (returns 1 when the shape is not covered).
 int qmm_mv_q4k_fast(int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, const void *w, float *y,
-                    hipStream_t s) {
+                    hipStream_t s, const Epi *ep) {
   if (tokens > 65535ll * 2) return 1;
-  if (k == 4096) return tokens >= 2 ? launch<2, 1>(n, tokens, accumulate, x, w, y, s) : launch<1, 1>(n, tokens, accumulate, x, w, y, s);
-  if (k == 8192) return tokens >= 2 ? launch<2, 2>(n, tokens, accumulate, x, w, y, s) : launch<1, 2>(n, tokens, accumulate, x, w, y, s);
+  if (k == 4096) return tokens >= 2 ? launch<2, 1>(n, tokens, accumulate, x, w, y, s, ep) : launch<1, 1>(n, tokens, accumulate, x, w, y, s, ep);
+  if (k == 8192) return tokens >= 2 ? launch<2, 2>(n, tokens, accumulate, x, w, y, s, ep) : launch<1, 2>(n, tokens, accumulate, x, w, y, s, ep);
   return 1;
 }

@@ -31,6 +31,7 @@
 #include <type_traits>
 
 #include "bfly.hpp"
+#include "epilogue.hpp"
 
 using namespace qmm;
 
@@ -89,11 +90,12 @@ __device__ __forceinline__ void q8_group(const float (&v)[8], u32 &c0, u32 &c1, 
   sum = (float)s;
 }
 
-template <int TG, int U, bool STAGEQ, int MODE, int WF>
+template <int TG, int U, bool STAGEQ, int MODE, int WF, class EP = NoEpi>
 __global__ __launch_bounds__(kMaxWaves * 64) void mv_q4kt_q8_kernel(int64_t n, int64_t tokens, int64_t K,
                                                                    int accumulate, const void *__restrict__ x, int bf,
                                                                    const u8 *__restrict__ w, const u8 *__restrict__ w2,
-                                                                   float *__restrict__ y, float *__restrict__ y2) {
+                                                                   float *__restrict__ y, float *__restrict__ y2,
+                                                                   EP ep) {
   constexpr int SLICE = 512 * U, NG = SLICE / 32;   // values / Q8 groups of a wave
   constexpr int NM = MODE == kPlain ? 1 : 2;        // weight matrices streamed
   // the codes of a token's slice, four dwords of padding after every 32 (pidx): the four lane classes (super-block
@@ -326,7 +328,12 @@ __global__ __launch_bounds__(kMaxWaves * 64) void mv_q4kt_q8_kernel(int64_t n, i
       for (int wv = 0; wv < NW; ++wv) tot[m] += red[wv][m][rr][t];
     }
     const int64_t row = 16 * rb + rr, tok = t0 + t;
-    if (tok < tokens) {
+    if constexpr (kEpi<EP>) {
+      if (tok < tokens) {
+        if constexpr (MODE == kSwiglu) epi_store2(ep, tok * n + row, row, tot[0], tot[NM - 1]);
+        else epi_store(ep, tok * n + row, row, tot[0]);
+      }
+    } else if (tok < tokens) {
       float *py = y + tok * n + row;
       if constexpr (MODE == kSwiglu) {
         const float v = tot[0] / (1.0f + expf(-tot[0])) * tot[NM - 1];
@@ -351,10 +358,11 @@ __global__ __launch_bounds__(kMaxWaves * 64) void mv_q4kt_q8_kernel(int64_t n, i
 // then contracts its four blocks (4 h .. 4 h + 3 of span sb of row r) with them, s = sum q x over the block's codes
 // 0..15 as f32 (one fma chain in value order), and adds d (s - 8 sum x): sum d (q - 8) x up to f32 rounding. The row's
 // four lanes meet in a butterfly, the waves in LDS in a fixed order, so a multi-token call equals one-token calls.
-template <int TG, int U, bool BF>
+template <int TG, int U, bool BF, class EP = NoEpi>
 __global__ __launch_bounds__(kMaxWaves * 64) void mv_q40t_f32_kernel(int64_t n, int64_t tokens, int64_t K,
                                                                      int accumulate, const void *__restrict__ x,
-                                                                     const u8 *__restrict__ w, float *__restrict__ y) {
+                                                                     const u8 *__restrict__ w, float *__restrict__ y,
+                                                                     EP ep) {
   constexpr int SLICE = 512 * U, NB = SLICE / 32;
   __shared__ __align__(16) float xs[kMaxWaves][TG][SLICE];
   __shared__ float xsum[kMaxWaves][TG][NB];
@@ -449,22 +457,28 @@ __global__ __launch_bounds__(kMaxWaves * 64) void mv_q40t_f32_kernel(int64_t n, 
     for (int wv = 1; wv < NW; ++wv) tot += red[wv][rr][t];
     const int64_t row = 16 * rb + rr, tok = t0 + t;
     if (row < n && tok < tokens) {
-      float *py = y + tok * n + row;
-      *py = accumulate ? *py + tot : tot;
+      if constexpr (kEpi<EP>) {
+        epi_store(ep, tok * n + row, row, tot);
+      } else {
+        float *py = y + tok * n + row;
+        *py = accumulate ? *py + tot : tot;
+      }
     }
   }
 }
 
 template <int TG, int U>
 int launch_q40t_f32(int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, bool bf, const void *w,
-                    float *y, int nw, hipStream_t s) {
+                    float *y, int nw, hipStream_t s, const Epi *ep) {
   const dim3 grid((unsigned)(n / 16), (unsigned)((tokens + TG - 1) / TG));
-  if (bf)
-    mv_q40t_f32_kernel<TG, U, true><<<grid, nw * 64, 0, s>>>(n, tokens, k, accumulate, x, static_cast<const u8 *>(w), y);
-  else
-    mv_q40t_f32_kernel<TG, U, false><<<grid, nw * 64, 0, s>>>(n, tokens, k, accumulate, x, static_cast<const u8 *>(w),
-                                                              y);
-  return launch_status();
+  const u8 *wp = static_cast<const u8 *>(w);
+  auto go = [&](auto e) {
+    using E = decltype(e);
+    if (bf) mv_q40t_f32_kernel<TG, U, true, E><<<grid, nw * 64, 0, s>>>(n, tokens, k, accumulate, x, wp, y, e);
+    else mv_q40t_f32_kernel<TG, U, false, E><<<grid, nw * 64, 0, s>>>(n, tokens, k, accumulate, x, wp, y, e);
+    return launch_status();
+  };
+  return ep ? go(*ep) : go(NoEpi{});
 }
 
 struct TArgs {
@@ -476,21 +490,24 @@ struct TArgs {
   float *y, *y2;
   int nw;
   int wf;   // TFmt
+  const Epi *ep;
 };
 
 template <int TG, int U, bool STAGEQ, int MODE>
 int launch_tg(const TArgs &a, hipStream_t s) {
   const dim3 grid((unsigned)(a.n / 16), (unsigned)((a.tokens + TG - 1) / TG));
-  if (a.wf == kTQ40) {
-    mv_q4kt_q8_kernel<TG, U, STAGEQ, MODE, kTQ40><<<grid, a.nw * 64, 0, s>>>(
+  auto go = [&](auto wf, auto e) {
+    mv_q4kt_q8_kernel<TG, U, STAGEQ, MODE, decltype(wf)::value, decltype(e)><<<grid, a.nw * 64, 0, s>>>(
         a.n, a.tokens, a.k, a.accumulate, a.x, a.bf, static_cast<const u8 *>(a.w), static_cast<const u8 *>(a.w2), a.y,
-        a.y2);
+        a.y2, e);
     return launch_status();
+  };
+  const std::integral_constant<int, kTQ40> q40;
+  const std::integral_constant<int, kTQ4K> q4k;
+  if constexpr (!STAGEQ && MODE != kPair) {   // an epilogue's operand is the planar buffer
+    if (a.ep) return a.wf == kTQ40 ? go(q40, *a.ep) : go(q4k, *a.ep);
   }
-  mv_q4kt_q8_kernel<TG, U, STAGEQ, MODE, kTQ4K><<<grid, a.nw * 64, 0, s>>>(
-      a.n, a.tokens, a.k, a.accumulate, a.x, a.bf, static_cast<const u8 *>(a.w), static_cast<const u8 *>(a.w2), a.y,
-      a.y2);
-  return launch_status();
+  return a.wf == kTQ40 ? go(q40, NoEpi{}) : go(q4k, NoEpi{});
 }
 
 template <int U, bool STAGEQ, int MODE>
@@ -654,8 +671,8 @@ int launch_mode(TArgs &a, int x_dtype, hipStream_t s) {
 // slices a wave and NW <= 8 waves. mode 0: y = x W^T; 1 (swiglu): y = silu(x W^T) (x W2^T); 2 (pair): y = x W^T and
 // y2 = x W2^T.
 int qmm_mv_q4kt_q8(int fmt, int mode, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x,
-                   int x_dtype, const void *w, const void *w2, float *y, float *y2, hipStream_t s) {
-  TArgs a{n, tokens, k, accumulate, x, 0, w, w2, y, y2, 0, fmt == QMM_Q4_0T ? kTQ40 : kTQ4K};
+                   int x_dtype, const void *w, const void *w2, float *y, float *y2, hipStream_t s, const Epi *ep) {
+  TArgs a{n, tokens, k, accumulate, x, 0, w, w2, y, y2, 0, fmt == QMM_Q4_0T ? kTQ40 : kTQ4K, ep};
   if (mode == kSwiglu) return launch_mode<kSwiglu>(a, x_dtype, s);
   if (mode == kPair) return launch_mode<kPair>(a, x_dtype, s);
   return launch_mode<kPlain>(a, x_dtype, s);
@@ -666,7 +683,7 @@ int qmm_mv_q4kt_q8(int fmt, int mode, int64_t k, int64_t n, int64_t tokens, int 
 // K = 512 U NW with U <= 3 slices a wave (the staged slices fit a workgroup's LDS) and NW <= 8 waves; a workgroup a
 // (row block, token).
 int qmm_mv_q40t_f32(int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, int x_dtype, const void *w,
-                    float *y, hipStream_t s) {
+                    float *y, hipStream_t s, const Epi *ep) {
   if (n % 16 || k % 512 || n / 16 > 2147483647ll || tokens > 65535) return QMM_ERR_SHAPE;
   const int64_t slices = k / 512;
   int U = 1;
@@ -674,9 +691,9 @@ int qmm_mv_q40t_f32(int64_t k, int64_t n, int64_t tokens, int accumulate, const 
   if (U > 3) return QMM_ERR_SHAPE;
   const int nw = (int)(slices / U);
   const bool bf = x_dtype == QMM_BF16;
-  if (U == 1) return launch_q40t_f32<1, 1>(k, n, tokens, accumulate, x, bf, w, y, nw, s);
-  return U == 2 ? launch_q40t_f32<1, 2>(k, n, tokens, accumulate, x, bf, w, y, nw, s)
-                : launch_q40t_f32<1, 3>(k, n, tokens, accumulate, x, bf, w, y, nw, s);
+  if (U == 1) return launch_q40t_f32<1, 1>(k, n, tokens, accumulate, x, bf, w, y, nw, s, ep);
+  return U == 2 ? launch_q40t_f32<1, 2>(k, n, tokens, accumulate, x, bf, w, y, nw, s, ep)
+                : launch_q40t_f32<1, 3>(k, n, tokens, accumulate, x, bf, w, y, nw, s, ep);
 }
 
 int qmm_dequant_q4kt(const void *w, int64_t rows, int64_t k, float *out, hipStream_t s) {

@@ -25,60 +25,17 @@
 //
 //   qmm_moe_expert_mv_q8  the decode expert matvecs on Q8_1 activations, g_moe_{gu|dn}_{fmt}[_fused]_q8_k{K}_r{R}
 //                         (S/gen_moe.py:535-727 with iq; the MOE_Q8 default of S/gen_llm.py:5290-5303)
+#include "act_quant.hpp"
 #include "bfly.hpp"
+#include "epilogue.hpp"
 #include "rowdot.hpp"
 
 using namespace qmm;
 
 namespace {
 
-typedef __attribute__((ext_vector_type(4))) u32 v4u;
-typedef __attribute__((ext_vector_type(2))) u32 v2u;
-
 __device__ __forceinline__ int sdot4(u32 a, u32 b, int c) {
   return __builtin_amdgcn_sdot4((int)a, (int)b, c, false);
-}
-
-// 8 activations of the lane as f32: from 16 bytes of bf16 or 32 bytes of f32 at element offset e
-__device__ __forceinline__ void load8_act(const void *x, bool bf, int64_t e, float (&v)[8]) {
-  if (bf) {
-    const v4u q = *reinterpret_cast<const v4u *>(static_cast<const u16 *>(x) + e);
-    const u32 d[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { v[2 * j] = bf16_to_f32(d[j] & 0xFFFFu); v[2 * j + 1] = bf16_to_f32(d[j] >> 16); }
-  } else {
-    const v4u a = *reinterpret_cast<const v4u *>(static_cast<const float *>(x) + e);
-    const v4u b = *reinterpret_cast<const v4u *>(static_cast<const float *>(x) + e + 4);
-    const u32 d[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = u32_as_f32(d[j]);
-  }
-}
-
-// One 32-value group held by four consecutive lanes of a wave (8 values each, the group's first lane a multiple of
-// 4): the lane's 8 codes as two dwords, and the group's f16-rounded d and code sum.
-__device__ __forceinline__ void q8_group4(const float (&v)[8], u32 &c0, u32 &c1, float &d16, float &sum) {
-  float amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
-  amax = fmaxf(amax, __shfl_xor(amax, 1, 64));
-  amax = fmaxf(amax, __shfl_xor(amax, 2, 64));
-  const float d = amax / 127.f;
-  int s = 0;
-  u32 c[2] = {0u, 0u};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = d > 0.f ? v[i] / d : 0.f;
-    const int q = (int)copysignf(floorf(fabsf(t) + 0.5f), t);
-    s += q;
-    c[i >> 2] |= ((u32)q & 0xFFu) << (8 * (i & 3));
-  }
-  s += __shfl_xor(s, 1, 64);
-  s += __shfl_xor(s, 2, 64);
-  c0 = c[0];
-  c1 = c[1];
-  d16 = (float)(_Float16)d;
-  sum = (float)s;
 }
 
 // --------------------------------------------------------------------------------------------- quantizer
@@ -318,12 +275,12 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f +
 // RW rows per wave (4 for one matrix, 2 when two stream), TG tokens per workgroup sharing every weight load
 // LPR lanes a row (the item count's power of two, at least 64 / RW), the butterfly restricted to the row's lanes:
 // the row sums equal the full-wave butterfly's over one row a pass (the expert matvecs' lane map)
-template <class P, int TG, int MODE, int RW, int LPR = 64>
+template <class P, int TG, int MODE, int RW, int LPR = 64, class EP = NoEpi>
 __global__ __launch_bounds__(256) void mv_q8_kernel(int64_t n, int64_t tokens, int64_t k, int accumulate,
                                                     const u8 *__restrict__ codes, const float *__restrict__ meta,
                                                     const u8 *__restrict__ w, const u8 *__restrict__ w2, int64_t rb,
                                                     const u8 *__restrict__ ws, const u8 *__restrict__ ws2, int64_t sb,
-                                                    float *__restrict__ y, float *__restrict__ y2) {
+                                                    float *__restrict__ y, float *__restrict__ y2, EP ep) {
   constexpr int NM = MODE == kPlain ? 1 : 2;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t t0 = (int64_t)blockIdx.x * TG;
@@ -405,7 +362,12 @@ __global__ __launch_bounds__(256) void mv_q8_kernel(int64_t n, int64_t tokens, i
 #pragma unroll
       for (int t = 0; t < TG; ++t) {
         const int64_t row = row0 + rg + GR * r, tok = t0 + t;
-        if (row < n && tok < tokens) {
+        if constexpr (kEpi<EP>) {
+          if (row < n && tok < tokens) {
+            if constexpr (MODE == kSwiglu) epi_store2(ep, tok * n + row, row, acc[0][r][t], acc[NM - 1][r][t]);
+            else epi_store(ep, tok * n + row, row, acc[0][r][t]);
+          }
+        } else if (row < n && tok < tokens) {
           float *py = y + tok * n + row;
           const float v = MODE == kSwiglu ? silu_mul(acc[0][r][t], acc[NM - 1][r][t]) : acc[0][r][t];
           *py = accumulate ? *py + v : v;
@@ -503,11 +465,12 @@ constexpr int kSWaves = 8;
 #endif
 constexpr int kSSlots = QMM_Q8_SLOTS;   // row groups per wave (they share the lane's activations)
 
-template <int TG, int KB, bool STAGEQ>
+template <int TG, int KB, bool STAGEQ, class EP = NoEpi>
 __global__ __launch_bounds__(kSWaves * 64) void mv_q4k_q8s_kernel(int64_t n, int64_t tokens, int accumulate,
                                                                  const void *__restrict__ x, int bf,
                                                                  const u8 *__restrict__ w1, const u8 *__restrict__ w2,
-                                                                 float *__restrict__ y1, float *__restrict__ y2) {
+                                                                 float *__restrict__ y1, float *__restrict__ y2,
+                                                                 EP ep) {
   constexpr int K = KB * 4096, IPR = 4 * KB, RG = 64 / IPR, RW = RG * kSSlots, SLICE = 512 * KB, NG = SLICE / 32;
   constexpr int64_t RB = (int64_t)K / 256 * 144;
   __shared__ __align__(16) u32 xc[kSWaves][TG][SLICE / 4];
@@ -653,8 +616,12 @@ __global__ __launch_bounds__(kSWaves * 64) void mv_q4k_q8s_kernel(int64_t n, int
     for (int wv = 0; wv < kSWaves; ++wv) tot += red[wv][rr][t];
     const int64_t row = row0 + rr, tok = t0 + t;
     if (row < n && tok < tokens) {
-      float *py = y + tok * n + row;
-      *py = accumulate ? *py + tot : tot;
+      if constexpr (kEpi<EP>) {
+        epi_store(ep, tok * n + row, row, tot);
+      } else {
+        float *py = y + tok * n + row;
+        *py = accumulate ? *py + tot : tot;
+      }
     }
   }
 }
@@ -667,15 +634,19 @@ struct SArgs {
   int bf;
   const void *w, *w2;
   float *y, *y2;
+  const Epi *ep;
 };
 template <int TG, int KB, bool STAGEQ>
 int launch_sliced(const SArgs &a, hipStream_t s) {
   constexpr int RW = 16 / KB * kSSlots;
   const dim3 grid((unsigned)((a.n + RW - 1) / RW), (unsigned)((a.tokens + TG - 1) / TG), a.y2 ? 2u : 1u);
-  mv_q4k_q8s_kernel<TG, KB, STAGEQ><<<grid, kSWaves * 64, 0, s>>>(a.n, a.tokens, a.accumulate, a.x, a.bf,
-                                                                  static_cast<const u8 *>(a.w),
-                                                                  static_cast<const u8 *>(a.w2), a.y, a.y2);
-  return launch_status();
+  auto go = [&](auto ep) {
+    mv_q4k_q8s_kernel<TG, KB, STAGEQ, decltype(ep)><<<grid, kSWaves * 64, 0, s>>>(
+        a.n, a.tokens, a.accumulate, a.x, a.bf, static_cast<const u8 *>(a.w), static_cast<const u8 *>(a.w2), a.y, a.y2, ep);
+    return launch_status();
+  };
+  if constexpr (!STAGEQ) { if (a.ep) return go(*a.ep); }   // an epilogue's operand is the planar buffer
+  return go(NoEpi{});
 }
 
 template <bool STAGEQ>
@@ -699,15 +670,15 @@ extern "C" int qmm_quant_q8(int64_t rows, int64_t k, const void *x, int x_dtype,
 
 bool qmm_mv_q8_mfma_fits(int fmt, int64_t k, int64_t n, int64_t tokens);
 int qmm_mv_q8_mfma(int fmt, int swiglu, int sliced, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *xq,
-                   const void *w, const void *w2, float *y, float *y2, hipStream_t s);
+                   const void *w, const void *w2, float *y, float *y2, hipStream_t s, const Epi *ep);
 int qmm_mv_q4kt_q8(int fmt, int mode, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x,
-                   int x_dtype, const void *w, const void *w2, float *y, float *y2, hipStream_t s);
+                   int x_dtype, const void *w, const void *w2, float *y, float *y2, hipStream_t s, const Epi *ep);
 
 namespace {
 // the generic (GGUF-layout, planar Q8_1) matvec of one format in one mode
 template <class P, int MODE>
 int launch_generic(int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, const void *w, const void *w2,
-                   int64_t rb, float *y, float *y2, hipStream_t s, const void *ws = nullptr,
+                   int64_t rb, float *y, float *y2, hipStream_t s, const Epi *ep, const void *ws = nullptr,
                    const void *ws2 = nullptr) {
   const u8 *codes = static_cast<const u8 *>(x);
   const float *meta = reinterpret_cast<const float *>(codes + tokens * k);
@@ -716,10 +687,14 @@ int launch_generic(int64_t k, int64_t n, int64_t tokens, int accumulate, const v
     constexpr int TG = decltype(tg)::value, RW = decltype(rw)::value;
     const dim3 grid((unsigned)((tokens + TG - 1) / TG), (unsigned)((n + kWaves * RW - 1) / (kWaves * RW)));
     if (grid.x > 2147483647u || grid.y > 65535u) return (int)QMM_ERR_SHAPE;
-    mv_q8_kernel<P, TG, MODE, RW, decltype(lc)::value><<<grid, 256, 0, s>>>(
-        n, tokens, k, accumulate, codes, meta, static_cast<const u8 *>(w), static_cast<const u8 *>(w2), rb,
-        static_cast<const u8 *>(ws), static_cast<const u8 *>(ws2), k / 32, y, y2);
-    return launch_status();
+    auto run = [&](auto e) {
+      mv_q8_kernel<P, TG, MODE, RW, decltype(lc)::value, decltype(e)><<<grid, 256, 0, s>>>(
+          n, tokens, k, accumulate, codes, meta, static_cast<const u8 *>(w), static_cast<const u8 *>(w2), rb,
+          static_cast<const u8 *>(ws), static_cast<const u8 *>(ws2), k / 32, y, y2, e);
+      return launch_status();
+    };
+    if constexpr (MODE != kPair) { if (ep) return run(*ep); }
+    return run(NoEpi{});
   };
   using std::integral_constant;
   if constexpr (P::kAhead > 1) {
@@ -742,16 +717,17 @@ int launch_generic(int64_t k, int64_t n, int64_t tokens, int accumulate, const v
 
 template <int MODE>
 int generic_fmt(int fmt, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, const void *w,
-                const void *w2, float *y, float *y2, hipStream_t s) {
+                const void *w2, float *y, float *y2, hipStream_t s, const Epi *ep) {
   const int64_t rb = row_bytes(fmt, k);
-  if (fmt == QMM_Q4_K) return launch_generic<Q4K8, MODE>(k, n, tokens, accumulate, x, w, w2, rb, y, y2, s);
-  if (fmt == QMM_Q6_K) return launch_generic<Q6K8, MODE>(k, n, tokens, accumulate, x, w, w2, rb, y, y2, s);
-  return launch_generic<Q408, MODE>(k, n, tokens, accumulate, x, w, w2, rb, y, y2, s);
+  if (fmt == QMM_Q4_K) return launch_generic<Q4K8, MODE>(k, n, tokens, accumulate, x, w, w2, rb, y, y2, s, ep);
+  if (fmt == QMM_Q6_K) return launch_generic<Q6K8, MODE>(k, n, tokens, accumulate, x, w, w2, rb, y, y2, s, ep);
+  return launch_generic<Q408, MODE>(k, n, tokens, accumulate, x, w, w2, rb, y, y2, s, ep);
 }
 
 // checks shared by the int8 matvec entry points: formats with integer codes (GGUF Q4_K / Q4_0 / Q6_K, tiled Q4_K / Q4_0)
-int check_q8(int fmt, int64_t k, int64_t n, int64_t tokens, const void *x, int x_dtype, const void *w, const float *y) {
-  if (!x || !w || !y) return QMM_ERR_NULL;
+int check_q8(int fmt, int64_t k, int64_t n, int64_t tokens, const void *x, int x_dtype, const void *w, const float *y,
+             const Epi *ep = nullptr) {
+  if (!x || !w || (!y && !ep)) return QMM_ERR_NULL;
   if (fmt != QMM_Q4_K && fmt != QMM_Q4_0 && fmt != QMM_Q4_KT && fmt != QMM_Q6_K && fmt != QMM_Q4_0T)
     return QMM_ERR_FORMAT;
   if (x_dtype != QMM_Q8 && x_dtype != QMM_F32 && x_dtype != QMM_BF16) return QMM_ERR_DTYPE;
@@ -768,55 +744,64 @@ bool sliced_call(int fmt, int64_t k, int64_t tokens) {
 }
 }  // namespace
 
-extern "C" int qmm_mv_q8(int fmt, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, int x_dtype,
-                         const void *w, float *y, qmm_stream_t stream) {
-  if (int st = check_q8(fmt, k, n, tokens, x, x_dtype, w, y)) return st;
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+int qmm_mv_q8_impl(int fmt, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, int x_dtype,
+                   const void *w, float *y, hipStream_t s, const Epi *ep) {
+  if (int st = check_q8(fmt, k, n, tokens, x, x_dtype, w, y, ep)) return st;
   const bool fast = sliced_call(fmt, k, tokens);
   if (x_dtype == QMM_Q8 && qmm_mv_q8_mfma_fits(fmt, k, n, tokens))
-    return qmm_mv_q8_mfma(fmt, 0, fast, k, n, tokens, accumulate, x, w, nullptr, y, nullptr, s);
+    return qmm_mv_q8_mfma(fmt, 0, fast, k, n, tokens, accumulate, x, w, nullptr, y, nullptr, s, ep);
   if (fmt == QMM_Q4_KT || fmt == QMM_Q4_0T)
-    return qmm_mv_q4kt_q8(fmt, kPlain, k, n, tokens, accumulate, x, x_dtype, w, nullptr, y, nullptr, s);
-  const SArgs a{n, tokens, accumulate, x, x_dtype == QMM_BF16, w, nullptr, y, nullptr};
+    return qmm_mv_q4kt_q8(fmt, kPlain, k, n, tokens, accumulate, x, x_dtype, w, nullptr, y, nullptr, s, ep);
+  const SArgs a{n, tokens, accumulate, x, x_dtype == QMM_BF16, w, nullptr, y, nullptr, ep};
   if (x_dtype != QMM_Q8) {
     // f32 / bf16 rows are quantized while staged; only the fast path stages (others take planar Q8 from
     // qmm_quant_q8)
     return fast ? launch_fast<true>(k, a, s) : QMM_ERR_SHAPE;
   }
   if (fast) return launch_fast<false>(k, a, s);
-  return generic_fmt<kPlain>(fmt, k, n, tokens, accumulate, x, w, nullptr, y, nullptr, s);
+  return generic_fmt<kPlain>(fmt, k, n, tokens, accumulate, x, w, nullptr, y, nullptr, s, ep);
+}
+
+extern "C" int qmm_mv_q8(int fmt, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, int x_dtype,
+                         const void *w, float *y, qmm_stream_t stream) {
+  return qmm_mv_q8_impl(fmt, k, n, tokens, accumulate, x, x_dtype, w, y, reinterpret_cast<hipStream_t>(stream), nullptr);
 }
 
 // The two-matrix int8 matvecs (mode kSwiglu / kPair): the tiled kernel takes planar Q8_1 or f32 / bf16 rows, the
 // GGUF layouts planar Q8_1.
 static int mv2_q8(int mode, int fmt, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, int x_dtype,
-                  const void *w, const void *w2, float *y, float *y2, qmm_stream_t stream) {
-  if (int st = check_q8(fmt, k, n, tokens, x, x_dtype, w, y)) return st;
+                  const void *w, const void *w2, float *y, float *y2, hipStream_t s, const Epi *ep = nullptr) {
+  if (int st = check_q8(fmt, k, n, tokens, x, x_dtype, w, y, ep)) return st;
   if (!w2 || (mode == kPair && !y2)) return QMM_ERR_NULL;
   if (!aligned(w2, fmt == QMM_Q6_K ? 4 : 16) || (y2 && !aligned(y2, 4))) return QMM_ERR_ALIGN;
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (x_dtype == QMM_Q8 && qmm_mv_q8_mfma_fits(fmt, k, n, tokens)) {
-    if (mode == kSwiglu) return qmm_mv_q8_mfma(fmt, 1, 0, k, n, tokens, accumulate, x, w, w2, y, nullptr, s);
-    return qmm_mv_q8_mfma(fmt, 0, sliced_call(fmt, k, tokens), k, n, tokens, accumulate, x, w, w2, y, y2, s);
+    if (mode == kSwiglu) return qmm_mv_q8_mfma(fmt, 1, 0, k, n, tokens, accumulate, x, w, w2, y, nullptr, s, ep);
+    return qmm_mv_q8_mfma(fmt, 0, sliced_call(fmt, k, tokens), k, n, tokens, accumulate, x, w, w2, y, y2, s, nullptr);
   }
   if (fmt == QMM_Q4_KT || fmt == QMM_Q4_0T)
-    return qmm_mv_q4kt_q8(fmt, mode, k, n, tokens, accumulate, x, x_dtype, w, w2, y, y2, s);
+    return qmm_mv_q4kt_q8(fmt, mode, k, n, tokens, accumulate, x, x_dtype, w, w2, y, y2, s, ep);
   if (x_dtype != QMM_Q8) return QMM_ERR_DTYPE;   // GGUF layouts: the planar Q8_1 buffer of qmm_quant_q8
   // a pair takes the one-matrix call's kernel, so that its rows are that call's bit for bit
   if (mode == kPair && sliced_call(fmt, k, tokens) && n <= 65535ll * 8)
-    return launch_fast<false>(k, SArgs{n, tokens, accumulate, x, 0, w, w2, y, y2}, s);
-  return mode == kSwiglu ? generic_fmt<kSwiglu>(fmt, k, n, tokens, accumulate, x, w, w2, y, nullptr, s)
-                         : generic_fmt<kPair>(fmt, k, n, tokens, accumulate, x, w, w2, y, y2, s);
+    return launch_fast<false>(k, SArgs{n, tokens, accumulate, x, 0, w, w2, y, y2, nullptr}, s);
+  return mode == kSwiglu ? generic_fmt<kSwiglu>(fmt, k, n, tokens, accumulate, x, w, w2, y, nullptr, s, ep)
+                         : generic_fmt<kPair>(fmt, k, n, tokens, accumulate, x, w, w2, y, y2, s, nullptr);
+}
+
+int qmm_mv_gate_up_q8_impl(int fmt, int64_t k, int64_t n, int64_t tokens, const void *x, const void *w, const void *w2,
+                           hipStream_t s, const Epi &ep) {
+  return mv2_q8(kSwiglu, fmt, k, n, tokens, 0, x, QMM_Q8, w, w2, nullptr, nullptr, s, &ep);
 }
 
 extern "C" int qmm_mv_swiglu_q8(int fmt, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x,
                                 int x_dtype, const void *w, const void *w2, float *y, qmm_stream_t stream) {
-  return mv2_q8(kSwiglu, fmt, k, n, tokens, accumulate, x, x_dtype, w, w2, y, nullptr, stream);
+  return mv2_q8(kSwiglu, fmt, k, n, tokens, accumulate, x, x_dtype, w, w2, y, nullptr,
+                reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int qmm_mv_pair_q8(int fmt, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x,
                               int x_dtype, const void *w, const void *w2, float *y, float *y2, qmm_stream_t stream) {
-  return mv2_q8(kPair, fmt, k, n, tokens, accumulate, x, x_dtype, w, w2, y, y2, stream);
+  return mv2_q8(kPair, fmt, k, n, tokens, accumulate, x, x_dtype, w, w2, y, y2, reinterpret_cast<hipStream_t>(stream));
 }
 
 namespace {
@@ -884,11 +869,11 @@ extern "C" int qmm_moe_expert_mv_q8(int fmt, int mode, int fused, int act, int64
 // The opt-in int8 decode of MXFP4 split planes (MXFP4S_Q8, S/formats.py:26-28): g_mv_mxfp4s_k{K}[_swiglu|_pair]
 // [_t{TG}]_q8 (S/gen_llm.py:1288-1301 with @g_mxfp4s_icodes, S/gen_mxfp4s.py:1113-1160) and the MOE_Q8 expert
 // matvecs of mxfp4s experts (S/gen_moe.py:535-727), over the generic item walk (MX4S8).
-extern "C" int qmm_mv_mxfp4s_q8(int mode, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x,
-                                int x_dtype, const void *w, const void *ws, const void *w2, const void *ws2, float *y,
-                                float *y2, qmm_stream_t stream) {
+int qmm_mv_mxfp4s_q8_impl(int mode, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x, int x_dtype,
+                          const void *w, const void *ws, const void *w2, const void *ws2, float *y, float *y2,
+                          hipStream_t s, const Epi *ep) {
   if (mode != kPlain && mode != kSwiglu && mode != kPair) return QMM_ERR_RANGE;
-  if (!x || !w || !ws || !y) return QMM_ERR_NULL;
+  if (!x || !w || !ws || (!y && !ep)) return QMM_ERR_NULL;
   if (mode != kPlain && (!w2 || !ws2)) return QMM_ERR_NULL;
   if (mode == kPair && !y2) return QMM_ERR_NULL;
   if (x_dtype != QMM_Q8) return QMM_ERR_DTYPE;   // the planar Q8_1 buffer of qmm_quant_q8
@@ -897,11 +882,17 @@ extern "C" int qmm_mv_mxfp4s_q8(int mode, int64_t k, int64_t n, int64_t tokens, 
   if (!aligned(x, 16) || !aligned(w, 16) || !aligned(ws, 2) || (w2 && !aligned(w2, 16)) || (ws2 && !aligned(ws2, 2)) ||
       !aligned(y, 4) || (y2 && !aligned(y2, 4)))
     return QMM_ERR_ALIGN;
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int64_t rb = k / 2;
-  if (mode == kSwiglu) return launch_generic<MX4S8, kSwiglu>(k, n, tokens, accumulate, x, w, w2, rb, y, nullptr, s, ws, ws2);
-  if (mode == kPair) return launch_generic<MX4S8, kPair>(k, n, tokens, accumulate, x, w, w2, rb, y, y2, s, ws, ws2);
-  return launch_generic<MX4S8, kPlain>(k, n, tokens, accumulate, x, w, nullptr, rb, y, nullptr, s, ws, nullptr);
+  if (mode == kSwiglu) return launch_generic<MX4S8, kSwiglu>(k, n, tokens, accumulate, x, w, w2, rb, y, nullptr, s, ep, ws, ws2);
+  if (mode == kPair) return launch_generic<MX4S8, kPair>(k, n, tokens, accumulate, x, w, w2, rb, y, y2, s, nullptr, ws, ws2);
+  return launch_generic<MX4S8, kPlain>(k, n, tokens, accumulate, x, w, nullptr, rb, y, nullptr, s, ep, ws, nullptr);
+}
+
+extern "C" int qmm_mv_mxfp4s_q8(int mode, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *x,
+                                int x_dtype, const void *w, const void *ws, const void *w2, const void *ws2, float *y,
+                                float *y2, qmm_stream_t stream) {
+  return qmm_mv_mxfp4s_q8_impl(mode, k, n, tokens, accumulate, x, x_dtype, w, ws, w2, ws2, y, y2,
+                               reinterpret_cast<hipStream_t>(stream), nullptr);
 }
 
 extern "C" int qmm_moe_expert_mv_mxfp4s_q8(int mode, int fused, int act, int64_t k, int64_t n, int E, int KU,

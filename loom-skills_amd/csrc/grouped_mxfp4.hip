@@ -48,7 +48,7 @@
 #include <type_traits>
 
 #include "bfly.hpp"
-#include "common.hpp"
+#include "epilogue.hpp"
 
 using namespace qmm;
 
@@ -80,9 +80,10 @@ constexpr int kTileGroup = 12;   // tiles of a range walked together over the co
 
 enum Kind { kGU = 1, kDN = 2, kGU8 = 3 };   // kGU8: gu with its output quantized to MXFP8
 enum Layout { kSplit = 0, kTiled = 1 };
-// where the output goes: the grouped GEMMs' sorted f32 rows, or a dense GEMM's y (f32 / bf16, stored or added to);
+// where the output goes: the grouped GEMMs' sorted f32 rows, or a dense GEMM's y (f32 / bf16, stored or added to, or
+// through the epilogue of qmm_linear / qmm_ffn_gate_up);
 // a dense kGU is the swiglu GEMM silu(X Wg^T) (X Wu^T) over rows 0 .. M - 1 of x
-enum Out { kOutGrouped = 0, kOutF32 = 1, kOutF32Acc = 2, kOutBF16 = 3, kOutBF16Acc = 4 };
+enum Out { kOutGrouped = 0, kOutF32 = 1, kOutF32Acc = 2, kOutBF16 = 3, kOutBF16Acc = 4, kOutEpi = 5 };
 typedef __attribute__((ext_vector_type(4))) u32 v4u;   // a native vector: the register rings stay in VGPRs
 
 struct MArgs {
@@ -100,6 +101,7 @@ struct MArgs {
   float *y;
   u8 *y8, *ys8;                    // kGU8: E4M3 codes [rows, N] and E8M0 scales [rows, N/32] of the activation
   int n_blocks, max_tiles;
+  Epi ep;                          // kOutEpi
 };
 
 // The sigmoid as v_exp_f32 and v_rcp_f32 (each about 1 ulp; exp overflow gives rcp(inf) = 0, as the division would):
@@ -520,6 +522,29 @@ __global__ __launch_bounds__(256, WAVES) void mxfp4_grouped_kernel(MArgs a) {
     for (int cc = 0; cc < CB; ++cc) {
       const int cj = col + 32 * cc;
       if (cj >= N) continue;
+      if constexpr (OUT == kOutEpi) {
+        const float b1 = epi_bias(a.ep.bias, cj), b2 = GU ? epi_bias(a.ep.bias2, cj) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float add[16];   // a block's residual values, all loaded before its first store
+          auto row = [&](int r) { return m0 + 32 * i + 8 * (r >> 2) + 4 * h + (r & 3); };
+          if (!GU && a.ep.res) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              add[r] = row(r) < a.M ? load_val(a.ep.res, a.ep.res_bf16, (int64_t)row(r) * N + cj) : 0.f;
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            if (row(r) >= a.M) continue;
+            const int64_t o = (int64_t)row(r) * N + cj;
+            if constexpr (GU)
+              store_val(a.ep.y, a.ep.y_bf16, o, act2(a.ep.act, acc[i][cc][r] + b1, acc[i][CB + cc][r] + b2));
+            else
+              epi_put(a.ep, o, acc[i][cc][r] + b1, add[r]);
+          }
+        }
+        continue;
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -720,13 +745,13 @@ int qmm_grouped_mxfp4(int tiled, int mode, int fused, int act, int64_t max_tiles
 
 // The dense prefill GEMM on MXFP4 weights (split planes or MFMA-tiled planes): the grouped kernels over dense
 // 64-row tiles of x, one weight matrix (store / acc) or a gate and an up matrix (swiglu).
-extern "C" int qmm_gemm_mxfp4(int fmt, int mode, int64_t rows, int64_t k, int64_t n, const void *x,
-                              const void *x_scales, const void *w, const void *ws, const void *w2, const void *ws2,
-                              void *y, int y_dtype, qmm_stream_t stream) {
+int qmm_gemm_mxfp4_impl(int fmt, int mode, int64_t rows, int64_t k, int64_t n, const void *x, const void *x_scales,
+                        const void *w, const void *ws, const void *w2, const void *ws2, void *y, int y_dtype,
+                        hipStream_t s, const Epi *ep) {
   if (fmt != QMM_MXFP4S && fmt != QMM_MXFP4T) return QMM_ERR_FORMAT;
   if (mode != QMM_GEMM_STORE && mode != QMM_GEMM_ACC && mode != QMM_GEMM_SWIGLU) return QMM_ERR_RANGE;
   if (y_dtype != QMM_F32 && y_dtype != QMM_BF16) return QMM_ERR_DTYPE;
-  if (!x || !x_scales || !w || !ws || !y || (mode == QMM_GEMM_SWIGLU && (!w2 || !ws2))) return QMM_ERR_NULL;
+  if (!x || !x_scales || !w || !ws || (!y && !ep) || (mode == QMM_GEMM_SWIGLU && (!w2 || !ws2))) return QMM_ERR_NULL;
   if (rows <= 0 || k <= 0 || n <= 0 || k % 64 || k > kMaxK || rows > (1 << 24) || n > (1 << 24)) return QMM_ERR_SHAPE;
   const bool tiled = fmt == QMM_MXFP4T;
   if (tiled && n % 32) return QMM_ERR_SHAPE;        // tiled planes hold whole 32-row blocks
@@ -741,7 +766,11 @@ extern "C" int qmm_gemm_mxfp4(int fmt, int mode, int64_t rows, int64_t k, int64_
   a.wn2 = static_cast<const u8 *>(w2); a.wsc2 = static_cast<const u8 *>(ws2);
   a.E = 1; a.KU = 1; a.act = QMM_ACT_SILU; a.y = static_cast<float *>(y);
   a.max_tiles = (int)((rows + BM - 1) / BM);
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (ep) {
+    a.ep = *ep;
+    if (mode == QMM_GEMM_SWIGLU) return tiled ? launch<kGU, kTiled, kOutEpi>(a, s) : launch<kGU, kSplit, kOutEpi>(a, s);
+    return tiled ? launch<kDN, kTiled, kOutEpi>(a, s) : launch<kDN, kSplit, kOutEpi>(a, s);
+  }
   const bool bf = y_dtype == QMM_BF16;
   if (mode == QMM_GEMM_SWIGLU) {
     if (bf) return tiled ? launch<kGU, kTiled, kOutBF16>(a, s) : launch<kGU, kSplit, kOutBF16>(a, s);
@@ -753,6 +782,13 @@ extern "C" int qmm_gemm_mxfp4(int fmt, int mode, int64_t rows, int64_t k, int64_
   }
   if (bf) return tiled ? launch<kDN, kTiled, kOutBF16>(a, s) : launch<kDN, kSplit, kOutBF16>(a, s);
   return tiled ? launch<kDN, kTiled, kOutF32>(a, s) : launch<kDN, kSplit, kOutF32>(a, s);
+}
+
+extern "C" int qmm_gemm_mxfp4(int fmt, int mode, int64_t rows, int64_t k, int64_t n, const void *x,
+                              const void *x_scales, const void *w, const void *ws, const void *w2, const void *ws2,
+                              void *y, int y_dtype, qmm_stream_t stream) {
+  return qmm_gemm_mxfp4_impl(fmt, mode, rows, k, n, x, x_scales, w, ws, w2, ws2, y, y_dtype,
+                             reinterpret_cast<hipStream_t>(stream), nullptr);
 }
 
 extern "C" int qmm_tile_mxfp4(const void *nibbles, const void *scales, int64_t rows, int64_t k, void *nib_t,

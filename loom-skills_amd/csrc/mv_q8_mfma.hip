@@ -38,7 +38,7 @@
 // The sums of 16 tokens x 16 rows lie in four registers: lane (c, q), register i is token 4 q + i, row c, so that a row's
 // scale is one register. The products xs mn of four groups are the four blocks of a v_mfma_f32_16x16x1_4b_f32: lane (c, q)
 // holds row / token c of group q, and register 4 b + i of the result is block b's.
-#include "common.hpp"
+#include "epilogue.hpp"
 
 using namespace qmm;
 
@@ -69,8 +69,8 @@ __device__ __forceinline__ u32x4 page_swap(u32x4 v) {
 __device__ __forceinline__ long pack8(u32 a, u32 b) { return (long)(((uint64_t)b << 32) | a); }
 
 // LONG (kItems): more than 16 super-blocks, so an item lane sums several
-template <bool TL, bool SWIGLU, int ORDER, bool LONG>
-__global__ __launch_bounds__(64 * kWaves, 4) void mv_q8_mfma_kernel(MArgs a) {
+template <bool TL, bool SWIGLU, int ORDER, bool LONG, class EP = NoEpi>
+__global__ __launch_bounds__(64 * kWaves, 4) void mv_q8_mfma_kernel(MArgs a, EP ep) {
   constexpr int NV = ORDER == kItems ? 4 : 2;                             // sums of a super-block: pages, or halves
   // LDS bytes a wave: the codes of 16 tokens, their da and xs [group][token]
   constexpr int kCode = 16 * 256, kMeta = 1024;
@@ -280,10 +280,16 @@ __global__ __launch_bounds__(64 * kWaves, 4) void mv_q8_mfma_kernel(MArgs a) {
     if (tid >= 256) meet[o] = s;
     __syncthreads();
     if (tid < 256 && in) {
-      float *p = a.y + (int64_t)tok * a.n + rw;
-      const float y = act_fn(QMM_ACT_SILU, s, meet[o]);
-      *p = a.accumulate ? *p + y : y;
+      if constexpr (kEpi<EP>) {
+        epi_store2(ep, (int64_t)tok * a.n + rw, rw, s, meet[o]);
+      } else {
+        float *p = a.y + (int64_t)tok * a.n + rw;
+        const float y = act_fn(QMM_ACT_SILU, s, meet[o]);
+        *p = a.accumulate ? *p + y : y;
+      }
     }
+  } else if constexpr (kEpi<EP>) {
+    if (tid < 256 && in) epi_store(ep, (int64_t)tok * a.n + rw, rw, total(meet, o));
   } else if (tid < 256 && in) {
     float *p = (blockIdx.z ? a.y2 : a.y) + (int64_t)tok * a.n + rw;
     const float y = total(meet, o);
@@ -292,11 +298,14 @@ __global__ __launch_bounds__(64 * kWaves, 4) void mv_q8_mfma_kernel(MArgs a) {
 }
 
 template <bool TL, int ORDER, bool LONG>
-int launch(int swiglu, const MArgs &a, hipStream_t s) {
+int launch(int swiglu, const MArgs &a, hipStream_t s, const Epi *ep) {
   const dim3 grid((unsigned)(8 * ((a.tokens + 15) / 16)), (unsigned)((a.n + 127) / 128), a.y2 ? 2u : 1u);
-  if (swiglu) mv_q8_mfma_kernel<TL, true, ORDER, LONG><<<grid, 64 * kWaves, 0, s>>>(a);
-  else mv_q8_mfma_kernel<TL, false, ORDER, LONG><<<grid, 64 * kWaves, 0, s>>>(a);
-  return launch_status();
+  auto go = [&](auto e) {
+    if (swiglu) mv_q8_mfma_kernel<TL, true, ORDER, LONG, decltype(e)><<<grid, 64 * kWaves, 0, s>>>(a, e);
+    else mv_q8_mfma_kernel<TL, false, ORDER, LONG, decltype(e)><<<grid, 64 * kWaves, 0, s>>>(a, e);
+    return launch_status();
+  };
+  return ep ? go(*ep) : go(NoEpi{});
 }
 
 // slices a wave of the tiled matvec kernel: K = 512 U NW, the least U <= 4 with NW <= 8 (qmm_mv_q4kt_q8); 0: none
@@ -324,7 +333,7 @@ bool qmm_mv_q8_mfma_fits(int fmt, int64_t k, int64_t n, int64_t tokens) {
 
 // y2: a pair call (swiglu = 0). sliced: the call's one-token kernel is the K-sliced one (GGUF, K = 4096 or 8192).
 int qmm_mv_q8_mfma(int fmt, int swiglu, int sliced, int64_t k, int64_t n, int64_t tokens, int accumulate, const void *xq,
-                   const void *w, const void *w2, float *y, float *y2, hipStream_t s) {
+                   const void *w, const void *w2, float *y, float *y2, hipStream_t s, const Epi *ep) {
   MArgs a{};
   a.n = (int)n; a.tokens = (int)tokens; a.nsb = (int)(k / 256);
   a.codes = static_cast<const u8 *>(xq);
@@ -333,11 +342,11 @@ int qmm_mv_q8_mfma(int fmt, int swiglu, int sliced, int64_t k, int64_t n, int64_
   a.y = y; a.y2 = y2; a.accumulate = accumulate;
   if (fmt == QMM_Q4_KT) {
     a.chains = 2; a.units = tiled_slices(k);
-    return launch<true, kSlices, false>(swiglu, a, s);
+    return launch<true, kSlices, false>(swiglu, a, s, ep);
   }
   if (sliced) {   // eight slices of 2 (K = 4096) or 4 super-blocks, a chain each
     a.chains = (int)(k / 2048); a.units = 1;
-    return launch<false, kSlices, false>(swiglu, a, s);
+    return launch<false, kSlices, false>(swiglu, a, s, ep);
   }
-  return a.nsb > 2 * kWaves ? launch<false, kItems, true>(swiglu, a, s) : launch<false, kItems, false>(swiglu, a, s);
+  return a.nsb > 2 * kWaves ? launch<false, kItems, true>(swiglu, a, s, ep) : launch<false, kItems, false>(swiglu, a, s, ep);
 }

@@ -19,6 +19,15 @@ SIGNATURES = {
     "qmm_quant_q8": [c_i64, c_i64, c_vp, c_int, c_vp, c_vp],
     "qmm_mv_q8": [c_int, c_i64, c_i64, c_i64, c_int, c_vp, c_int, c_vp, c_vp, c_vp],
     "qmm_gemm": [c_int, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_int, c_vp],
+    "qmm_rms_norm": [c_i64, c_i64, c_vp, c_int, c_vp, c_int, c_vp, c_int, c_float, c_vp, c_int, c_vp, c_vp, c_vp],
+    "qmm_linear": [c_int, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_vp],
+    "qmm_ffn_gate_up": [c_int, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                        c_int, c_vp],
+    "qmm_ffn_gate_up_grad": [c_int, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp,
+                             c_vp],
+    "qmm_grad_operand": [c_i64, c_int, c_i64, c_vp, c_int, c_vp, c_vp, c_vp],
+    "qmm_gemm_t": [c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_i64, c_vp],
+    "qmm_gemm_t_workspace_size": [c_int, c_i64, c_i64, c_i64, c_int],
     "qmm_moe_topk": [c_vp, c_i64, c_int, c_int, c_int, c_int, c_float, c_vp, c_vp, c_vp, c_vp],
     "qmm_moe_topk_operand": [c_vp, c_i64, c_int, c_int, c_int, c_int, c_float, c_vp, c_vp, c_vp, c_i64, c_vp, c_int,
                              c_int, c_vp, c_vp, c_vp],
@@ -69,7 +78,7 @@ SIGNATURES = {
                               c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp],
 }
 RESTYPE = {"qmm_strerror": ctypes.c_char_p, "qmm_row_bytes": c_i64, "qmm_mxfp4t_scale_bytes": c_i64,
-           "qmm_moe_routed_workspace_size": c_i64}
+           "qmm_moe_routed_workspace_size": c_i64, "qmm_gemm_t_workspace_size": c_i64}
 
 
 class QmmError(RuntimeError):

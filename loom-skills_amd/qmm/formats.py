@@ -36,7 +36,9 @@ def gate_format(fmt):
 DTYPE = {"f32": 0, "f16": 1, "bf16": 2, "mxfp8": 3, "q8": 4}    # enum qmm_dtype
 MX_BLOCK = 32                                                   # values per E8M0 scale of an MXFP8 operand
 GEMM_MODE = {"store": 0, "acc": 1, "swiglu": 2}                 # enum qmm_gemm_mode
-ACT = {"silu": 0, "swiglu_oai": 1}                              # enum qmm_act
+ACT = {"silu": 0, "swiglu_oai": 1}                              # enum qmm_act: the experts' activations
+EPILOGUE_ACT = {"none": 2, "relu": 3, "silu": 0, "sigmoid": 6, "gelu": 4, "gelu_erf": 5}   # and those of linear
+GATE_ACT = {**EPILOGUE_ACT, "swiglu_oai": 1}                    # and of ffn_gate_up
 GATING = {"softmax": 1, "sigmoid": 2, "softmax_weight": 3}      # llama.cpp expert_gating_func values
 
 

@@ -27,6 +27,14 @@ S/ = skills/loom-port-llm/starter/):
     row_scale_f16     g_row_scale_f16[_tiles]                 S/gen_llm.py:1843-1915, S/gen_moe.py:503-527
     dequant           the @g_<fmt>_values helpers (bit-exact f32 values)
 
+the rest of a dense feed-forward sub-layer around those products, without counterparts as single reference kernels:
+
+    rms_norm              residual addition and RMS norm, written as the next product's operand
+    linear                with bias, activation, residual, bf16 rows (qmm_linear)
+    ffn_gate_up           act(x Wg^T + bg) (x Wu^T + bu) with any activation and biases
+    ffn_gate_up_backward  its gradients with respect to the projections' outputs and to x (frozen weights)
+    gemm_t                the transposed product x W, a projection's input gradient
+
 plus the gfx950-specific producers ``quant_mxfp8`` (A operand of the scaled MFMA), ``repack_mxfp4`` (GGUF
 MXFP4 blocks to split planes) and ``tile_mxfp4`` (split planes to the MFMA-tiled planes the grouped GEMM streams
 fastest), the last two one-time weight preparations.
@@ -39,7 +47,8 @@ import weakref
 import torch
 
 from . import _lib
-from .formats import ACT, CODE, DTYPE, GEMM_MODE, ICODES, MX_BLOCK, SPLIT, decode_q8, gate_format, row_bytes
+from .formats import (ACT, CODE, DTYPE, EPILOGUE_ACT, GATE_ACT, GEMM_MODE, ICODES, MX_BLOCK, SPLIT, decode_q8,
+                      gate_format, row_bytes)
 
 TILE = 64
 
@@ -730,7 +739,131 @@ GEMM_MIN_TOKENS = 64   # %gemm: epochs of 64+ tokens take the GEMM / grouped cha
 LINEAR_Q8_FORMATS = ("q4_0", "q4_k", "q4_kt", "q6_k", "q4_0t", "mxfp4s")
 
 
-def linear(fmt, x, w, n, k, y=None, mode="store", ws=None, w2=None, ws2=None, q8="auto"):
+def _here(*ts):
+    """_dev, and every tensor on the current device: the kernels are launched on its stream."""
+    _dev(*ts)
+    cur = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.device.index != cur:
+            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{cur}")
+
+
+def _shaped(t, shape, dtypes, what):
+    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype not in dtypes):
+        raise ValueError(f"{what} is {tuple(t.shape)} {t.dtype}, expected {tuple(shape)} "
+                         f"{' or '.join(str(d) for d in dtypes)}")
+
+
+_VALUE = (torch.float32, torch.bfloat16)   # the types of rows that epilogues read and write
+
+
+def _weight_bytes(fmt, w, ws, n, k, what="w"):
+    """The kernels cannot see sizes: a weight tensor too small for [n, k] would be read past its end."""
+    if w is None or w.numel() * w.element_size() < n * row_bytes(fmt, k):
+        raise ValueError(f"{what} is too small for {fmt} [{n}, {k}] ({n * row_bytes(fmt, k)} bytes)")
+    if fmt in SPLIT:
+        need = n * (k // MX_BLOCK) if fmt == "mxfp4s" else -(-n // 32) * ((k + 255) // 256) * 256
+        if ws is None or ws.numel() * ws.element_size() < need:
+            raise ValueError(f"{fmt} weights need their E8M0 scale planes ({need} bytes)")
+    elif ws is not None:
+        raise ValueError(f"{fmt} weights have no scale planes")
+
+
+_F16_GEMM = ("q4_k", "q4_kt", "q6_k", "q4_0")
+
+
+def _product_operand(fmt, x, k, scales, tokens, q8):
+    """(x, its qmm_dtype code, scales) of a product with an epilogue: an operand that rms_norm or a quantizer wrote
+    as it is, or f32 / bf16 rows [tokens, k] brought into the form linear's products take."""
+    if x.dtype == torch.uint8 and fmt in SPLIT and scales is not None:      # E4M3 codes
+        if tokens is not None:
+            raise ValueError("tokens counts the rows of a planar Q8_1 buffer")
+        if x.dim() != 2 or x.shape[1] != k:
+            raise ValueError(f"E4M3 codes are [tokens, {k}], x is {tuple(x.shape)}")
+        _shaped(scales, (x.shape[0], k // MX_BLOCK), (torch.uint8,), "scales")
+        return x, DTYPE["mxfp8"], scales
+    if x.dtype == torch.uint8:
+        if tokens is None or scales is not None:
+            raise ValueError("a planar Q8_1 buffer comes with its token count, E4M3 codes with their scales (MXFP4 planes)")
+        if x.numel() != q8_bytes(tokens, k):
+            raise ValueError(f"the planar Q8_1 buffer holds {x.numel()} bytes, {tokens} rows of K {k} are {q8_bytes(tokens, k)}")
+        return x, DTYPE["q8"], None
+    if tokens is not None:
+        raise ValueError("tokens counts the rows of a planar Q8_1 buffer")
+    if x.dim() != 2 or x.shape[1] != k:
+        raise ValueError(f"x is {tuple(x.shape)}, expected [tokens, {k}]")
+    T = x.shape[0]
+    if x.dtype == torch.float16:
+        _shaped(scales, (T, 2), (torch.float32,), "scales")
+        return x, DTYPE["f16"], scales
+    if scales is not None:
+        raise ValueError("scales come with an f16 or E4M3 operand")
+    if x.dtype not in _VALUE:
+        raise ValueError(f"x is {x.dtype}")
+    if fmt == "mxfp4t" or (T >= GEMM_MIN_TOKENS and fmt == "mxfp4s"):
+        x, scales = quant_mxfp8(x)
+        return x, DTYPE["mxfp8"], scales
+    if T >= GEMM_MIN_TOKENS and fmt in _F16_GEMM:
+        x, scales = row_scale_f16(x)
+        return x, DTYPE["f16"], scales
+    if T >= GEMM_MIN_TOKENS:
+        raise ValueError(f"no prefill GEMM reads {fmt} weights (mxfp4 blocks: repack_mxfp4 once)")
+    iq = decode_q8(fmt) if q8 == "auto" else bool(q8) and fmt in LINEAR_Q8_FORMATS
+    if iq and k // 32 <= 1024:
+        return quant_q8(x), DTYPE["q8"], None
+    return x, _dt(x), None
+
+
+def _act_code(act, table):
+    if act not in table:
+        raise ValueError(f"activation {act!r} is none of {', '.join(table)}")
+    return table[act]
+
+
+def rms_norm(x, weight, eps=1e-6, residual=None, out="bf16", h=None):
+    """h = x + residual and y = h / sqrt(mean(h^2) + eps) * weight in one pass, y in the form the next product reads
+    (qmm_rms_norm). x [rows, k] f32 / bf16, weight f32 / bf16 [k], residual [rows, k] f32 / bf16 or None. Returns
+    (y, scales, h):
+
+        out "bf16" / "f32"  y rows, scales None
+        out "f16"           (x16, scales) of row_scale_f16, for the GGUF prefill GEMMs
+        out "q8"            the planar Q8_1 buffer of quant_q8 (pass tokens=rows with it), scales None
+        out "mxfp8"         (codes, scales) of quant_mxfp8, for the MXFP4 GEMMs
+
+    h has the residual's type (None without one); the h argument takes the output rows, x or residual for an update in
+    place."""
+    _here(x, weight, residual, h)
+    if x.dim() != 2:
+        raise ValueError(f"x is {tuple(x.shape)}, expected [rows, k]")
+    rows, k = x.shape
+    _shaped(x, (rows, k), _VALUE, "x")
+    _shaped(weight, (k,), _VALUE, "weight")
+    _shaped(residual, (rows, k), _VALUE, "residual")
+    if residual is not None:
+        h = torch.empty_like(residual) if h is None else h
+        _shaped(h, (rows, k), (residual.dtype,), "h")
+    elif h is not None:
+        raise ValueError("h is written with a residual")
+    scales = None
+    if out in ("bf16", "f32"):
+        y = torch.empty((rows, k), dtype=torch.bfloat16 if out == "bf16" else torch.float32, device=x.device)
+    elif out == "f16":
+        y = torch.empty((rows, k), dtype=torch.float16, device=x.device)
+        scales = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+    elif out == "q8":
+        y = torch.empty(q8_bytes(rows, k), dtype=torch.uint8, device=x.device)
+    elif out == "mxfp8":
+        y = torch.empty((rows, k), dtype=torch.uint8, device=x.device)
+        scales = torch.empty((rows, k // MX_BLOCK), dtype=torch.uint8, device=x.device)
+    else:
+        raise ValueError(f"out {out!r} is none of bf16, f32, f16, q8, mxfp8")
+    _lib.call("qmm_rms_norm", rows, k, _ptr(x), _dt(x), _ptr(residual), 0 if residual is None else _dt(residual),
+              _ptr(weight), _dt(weight), eps, _ptr(h), DTYPE[out], _ptr(y), _ptr(scales), _stream())
+    return y, scales, h
+
+
+def linear(fmt, x, w, n, k, y=None, mode="store", ws=None, w2=None, ws2=None, q8="auto", bias=None, act="none",
+           residual=None, out_dtype=None, scales=None, tokens=None):
     """Projection y (+)= x W^T, or swiglu y = silu(x W^T) (x W2^T), with the reference's per-epoch choice (linear,
     S/gen_llm.py:4568-4625): the prefill GEMM for 64+ tokens (GGUF q4_k / q6_k / q4_0 on the f16 MFMA, the activation
     row-scaled to f16 first; MXFP4 on the scaled MFMA, the activation quantized to MXFP8 first -- GGUF mxfp4 blocks
@@ -738,7 +871,19 @@ def linear(fmt, x, w, n, k, y=None, mode="store", ws=None, w2=None, ws2=None, q8
     activations where the reference does by default (ACT_Q8, iq = ACT_Q8 and fmt in IQ_FMTS and K / 32 <= 1024,
     S/gen_llm.py:514-519, :4590): Q4_K and Q6_K (and the tiled q4_kt), Q4_0 with the reference's Q4_0_Q8=1 switch,
     MXFP4 split planes with MXFP4S_Q8=1, and the tiled q4_0t always (formats.decode_q8); q8=True also takes it for
-    q4_0 and mxfp4s; q8=False keeps f32 / bf16 activations (ACT_Q8=0). y is f32."""
+    q4_0 and mxfp4s; q8=False keeps f32 / bf16 activations (ACT_Q8=0). y is f32.
+
+    With any of bias (f32 [n]), act (none, relu, silu, sigmoid, gelu: the tanh form, gelu_erf), residual (f32 / bf16
+    [tokens, n], y itself allowed), out_dtype (f32 / bf16), scales or tokens, or a bf16 y, the call is
+    y = act(x W^T + bias) + residual (qmm_linear, mode "store"), the product's own kernel with that epilogue. x may then
+    also be an operand: a planar Q8_1 buffer with tokens, the row-scaled f16 rows or E4M3 codes with their scales; the
+    operand chooses the product whatever the token count. GGUF mxfp4 blocks take up to 63 rows (repack_mxfp4 for more)."""
+    if bias is not None or act != "none" or residual is not None or out_dtype is not None or scales is not None or \
+            tokens is not None or (y is not None and y.dtype == torch.bfloat16):
+        if mode != "store" or w2 is not None or ws2 is not None:
+            raise ValueError("bias, act, residual, out_dtype, scales and tokens go with mode \"store\" (ffn_gate_up for two "
+                             "matrices)")
+        return _linear_epilogue(fmt, x, w, n, k, y, ws, q8, bias, act, residual, out_dtype, scales, tokens)
     if mode not in ("store", "acc", "swiglu"):
         raise ValueError(f"linear mode {mode}")
     if mode == "swiglu" and w2 is None:
@@ -758,6 +903,107 @@ def linear(fmt, x, w, n, k, y=None, mode="store", ws=None, w2=None, ws2=None, q8
     if mode == "swiglu":
         return mv_swiglu(fmt, w, w2, x, n, k, y=y)
     return mv(fmt, w, x, n, k, y=y, accumulate=mode == "acc", ws=ws)
+
+
+def _linear_epilogue(fmt, x, w, n, k, y, ws, q8, bias, act, residual, out_dtype, scales, tokens):
+    _here(x, w, ws, bias, residual, scales, y)
+    code = _act_code(act, EPILOGUE_ACT)
+    _weight_bytes(fmt, w, ws, n, k)
+    T = x.shape[0] if tokens is None else tokens
+    _shaped(bias, (n,), (torch.float32,), "bias")
+    _shaped(residual, (T, n), _VALUE, "residual")
+    y = _rows_out(y, (T, n), out_dtype, x.device)
+    x, xd, scales = _product_operand(fmt, x, k, scales, tokens, q8)
+    _lib.call("qmm_linear", CODE[fmt], code, T, k, n, _ptr(x), xd, _ptr(scales), _ptr(w), _ptr(ws), _ptr(bias),
+              _ptr(residual), 0 if residual is None else _dt(residual), _ptr(y), _dt(y), _stream())
+    return y
+
+
+def _rows_out(y, shape, out_dtype, dev):
+    """The f32 / bf16 output rows: y, or a new tensor of out_dtype (f32 when None)."""
+    if y is None:
+        y = torch.empty(shape, dtype=torch.float32 if out_dtype is None else out_dtype, device=dev)
+    elif out_dtype is not None and y.dtype != out_dtype:
+        raise ValueError(f"y is {y.dtype}, out_dtype {out_dtype}")
+    _shaped(y, shape, _VALUE, "y")
+    return y
+
+
+def ffn_gate_up(fmt, x, w, w2, n, k, y=None, ws=None, ws2=None, q8="auto", bias=None, bias2=None, act="silu",
+                out_dtype=None, scales=None, tokens=None):
+    """The gated feed-forward block's first half, y = act(x W^T + bias) (x W2^T + bias2), in one kernel past the operand's
+    (qmm_ffn_gate_up). x, scales, tokens, q8 as linear; biases f32 [n] or None; act as linear or swiglu_oai (the gpt-oss
+    clamped form); y [tokens, n] f32 or bf16 (out_dtype)."""
+    _here(x, w, ws, w2, ws2, bias, bias2, scales, y)
+    code = _act_code(act, GATE_ACT)
+    _weight_bytes(fmt, w, ws, n, k)
+    _weight_bytes(fmt, w2, ws2, n, k, "w2")
+    T = x.shape[0] if tokens is None else tokens
+    _shaped(bias, (n,), (torch.float32,), "bias")
+    _shaped(bias2, (n,), (torch.float32,), "bias2")
+    y = _rows_out(y, (T, n), out_dtype, x.device)
+    x, xd, scales = _product_operand(fmt, x, k, scales, tokens, q8)
+    _lib.call("qmm_ffn_gate_up", CODE[fmt], code, T, k, n, _ptr(x), xd, _ptr(scales), _ptr(w), _ptr(ws), _ptr(w2), _ptr(ws2),
+              _ptr(bias), _ptr(bias2), _ptr(y), _dt(y), _stream())
+    return y
+
+
+def ffn_gate_up_backward(fmt, x, w, w2, dy, n, k, scales=None, bias=None, bias2=None, act="silu", out_dtype=torch.bfloat16):
+    """The gradients of ffn_gate_up at dy (f32 / bf16 [tokens, n]) with frozen weights: (dx [tokens, k] of out_dtype, dgu bf16
+    [tokens, 2, n]), dgu[:, 0] and dgu[:, 1] the gradients of x W^T + bias and x W2^T + bias2 (what adapters and biases
+    beside the projections train on), dx = dgu[:, 0] W + dgu[:, 1] W2. The projections are computed again from x: f32 / bf16
+    rows, or the f16 operand with its scales as for ffn_gate_up (rows that are all padding have no gradient: pass dy rows of
+    zeros there, their dgu and dx rows are undefined). fmt q4_k, q4_kt, q6_k or q4_0, k % 256 == 0."""
+    _here(x, w, w2, dy, bias, bias2, scales)
+    code = _act_code(act, GATE_ACT)
+    if fmt not in _F16_GEMM:
+        raise ValueError(f"no backward pass reads {fmt} weights")
+    _weight_bytes(fmt, w, None, n, k)
+    _weight_bytes(fmt, w2, None, n, k, "w2")
+    if x.dim() != 2 or x.shape[1] != k:
+        raise ValueError(f"x is {tuple(x.shape)}, expected [tokens, {k}]")
+    T = x.shape[0]
+    _shaped(dy, (T, n), _VALUE, "dy")
+    _shaped(bias, (n,), (torch.float32,), "bias")
+    _shaped(bias2, (n,), (torch.float32,), "bias2")
+    _shaped(scales, (T, 2), (torch.float32,), "scales")
+    if x.dtype != torch.float16:
+        if scales is not None:
+            raise ValueError("scales come with an f16 operand")
+        _shaped(x, (T, k), _VALUE, "x")
+        x, scales = row_scale_f16(x)
+    elif scales is None:
+        raise ValueError("the f16 operand comes with its scales")
+    dgu = torch.empty((T, 2, n), dtype=torch.bfloat16, device=x.device)
+    _lib.call("qmm_ffn_gate_up_grad", CODE[fmt], code, T, k, n, _ptr(x), _ptr(scales), _ptr(w), _ptr(w2), _ptr(bias),
+              _ptr(bias2), _ptr(dy), _dt(dy), _ptr(dgu), _stream())
+    return gemm_t(fmt, dgu, w, n, k, w2=w2, out_dtype=out_dtype), dgu
+
+
+def gemm_t(fmt, x, w, n, k, w2=None, out_dtype=torch.float32, y=None):
+    """The transposed product y = x W [rows, k] of gradient rows x [rows, n], or x[:, 0] W + x[:, 1] W2 of x [rows, 2, n]
+    (f32 / bf16): the input gradient of a projection y = x W^T whose weights stay quantized (qmm_grad_operand, qmm_gemm_t).
+    fmt q4_k, q4_kt, q6_k or q4_0, k % 256 == 0; y f32 or bf16."""
+    _here(x, w, w2, y)
+    if fmt not in _F16_GEMM:
+        raise ValueError(f"no transposed product reads {fmt} weights")
+    _weight_bytes(fmt, w, None, n, k)
+    if w2 is not None:
+        _weight_bytes(fmt, w2, None, n, k, "w2")
+    rows, parts = x.shape[0], 1 if w2 is None else 2
+    _shaped(x, (rows, n) if w2 is None else (rows, 2, n), _VALUE, "x")
+    y = _rows_out(y, (rows, k), None if y is not None else out_dtype, x.device)
+    need = _lib.load().qmm_gemm_t_workspace_size(CODE[fmt], rows, k, n, parts - 1)
+    if need < 0:
+        raise ValueError(f"the transposed product does not take {rows} rows of {fmt} [{n}, {k}]")
+    x16 = torch.empty((rows, parts, -(-n // 64) * 64), dtype=torch.float16, device=x.device)
+    scales = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+    work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    s = _stream()
+    _lib.call("qmm_grad_operand", rows, parts, n, _ptr(x), _dt(x), _ptr(x16), _ptr(scales), s)
+    _lib.call("qmm_gemm_t", CODE[fmt], rows, k, n, _ptr(x16), _ptr(scales), _ptr(w), _ptr(w2), _ptr(y), _dt(y), _ptr(work),
+              need, s)
+    return y
 
 
 def moe_routed(fmt, x, logits, E, KU, H, FE, gating, norm, **kw):
