@@ -72,16 +72,21 @@ __device__ __forceinline__ void epi_store2(const Epi &e, int64_t o, int64_t c, f
 // bias values at column c (0 without one), loaded once where a thread finishes many rows of a column
 __device__ __forceinline__ float epi_bias(const float *b, int64_t c) { return b ? b[c] : 0.f; }
 // v with its bias added, r the residual value
-__device__ __forceinline__ void epi_put(const Epi &e, int64_t o, float v, float r) {
-  v = act1(e.act, v);
+__device__ __forceinline__ void epi_put(const Epi &e, int act, int64_t o, float v, float r) {
+  v = act1(act, v);
   store_val(e.y, e.y_bf16, o, e.res ? v + r : v);
 }
+
+// The gradients leave as bf16, so their sigmoid is v_exp_f32 and v_rcp_f32 (each about 1 ulp, the argument's product with
+// log2 e another |v| half steps of f32): with an IEEE division and a range-reduced expf a value the gradient GEMM's epilogue
+// took a fifth of it
+__device__ __forceinline__ float sigmoid_fast_(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
 
 // act(v) and its slope d act / d v (relu: 0 at 0)
 __device__ __forceinline__ void act1_slope(int act, float v, float &a, float &da) {
   switch (act) {
     case QMM_ACT_SILU: {
-      const float s = sigmoidf_(v);
+      const float s = sigmoid_fast_(v);
       a = v * s;
       da = s * (1.0f + v * (1.0f - s));
       return;
@@ -91,7 +96,7 @@ __device__ __forceinline__ void act1_slope(int act, float v, float &a, float &da
       da = v > 0.f ? 1.f : 0.f;
       return;
     case QMM_ACT_GELU: {   // v s(z): s + v s (1 - s) z'; past the range of v^3 s (1 - s) is 0 and z' infinite
-      const float s = sigmoidf_(gelu_arg(v)), p = s * (1.0f - s);
+      const float s = sigmoid_fast_(gelu_arg(v)), p = s * (1.0f - s);
       a = v * s;
       da = p > 0.f ? s + v * p * 1.5957691216057308f * (1.0f + 0.134145f * v * v) : s;
       return;
@@ -103,7 +108,7 @@ __device__ __forceinline__ void act1_slope(int act, float v, float &a, float &da
       return;
     }
     case QMM_ACT_SIGMOID:
-      a = sigmoidf_(v);
+      a = sigmoid_fast_(v);
       da = a * (1.0f - a);
       return;
     default:
@@ -114,7 +119,7 @@ __device__ __forceinline__ void act1_slope(int act, float v, float &a, float &da
 // the gradients of act2(g, u) at dy. swiglu_oai: those of the clamps are 1 up to and at their limits, 0 past them
 __device__ __forceinline__ void act2_grad(int act, float g, float u, float dy, float &dg, float &du) {
   if (act == QMM_ACT_SWIGLU_OAI) {
-    const float xg = fminf(g, 7.0f), yu = fminf(fmaxf(u, -7.0f), 7.0f), s = sigmoidf_(1.702f * xg);
+    const float xg = fminf(g, 7.0f), yu = fminf(fmaxf(u, -7.0f), 7.0f), s = sigmoid_fast_(1.702f * xg);
     dg = g > 7.0f ? 0.f : dy * (yu + 1.0f) * s * (1.0f + 1.702f * xg * (1.0f - s));
     du = fabsf(u) > 7.0f ? 0.f : dy * xg * s;
     return;

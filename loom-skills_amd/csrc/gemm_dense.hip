@@ -383,7 +383,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void q4k_dense_kernel(DArgs a, EP e
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (col + e < N) epi_put(ep, o + e, v[e] + b[e], r[e]);
+        if (col + e < N) epi_put(ep, ep.act, o + e, v[e] + b[e], r[e]);
     } else if (vec && col + 8 <= N) {
       if constexpr (BF16OUT) {
         typedef __attribute__((ext_vector_type(2))) __bf16 bf2;

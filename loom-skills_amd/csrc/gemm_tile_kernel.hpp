@@ -561,48 +561,63 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
     if constexpr (kTwoW) b2 = epi_bias(a.ep.bias2, min(col[0], N - 1));
     const void *in = KIND == kTGluGrad ? a.dy : a.ep.res;
     const int in_bf16 = KIND == kTGluGrad ? a.dy_bf16 : a.ep.res_bf16;
+    // act, ybf: constants where the activation is the common one, so that a value does not branch on them
+    auto finish = [&](auto act, auto ybf) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      float add[NC][RK];
-      if (KIND != kTGlu && in) {
+      for (int i = 0; i < NI; ++i) {
+        auto row_of = [&](int r) {
+          const int rr = kp * RK + r;
+          return 32 * i + 8 * (rr >> 2) + 4 * h + (rr & 3);
+        };
+        float add[NC][RK];
+        auto load = [&](auto bf) __attribute__((always_inline)) {
+#pragma unroll
+          for (int r = 0; r < RK; ++r)
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+              const bool live = src_row[row_of(r)] >= 0 && col[j] < N;
+              add[j][r] = live ? load_val(in, bf, (int64_t)(m0 + row_of(r)) * N + col[j]) : 0.f;
+            }
+        };
+        if (KIND != kTGlu && in) {
+          if (in_bf16) load(std::integral_constant<int, 1>{});
+          else load(std::integral_constant<int, 0>{});
+        }
 #pragma unroll
         for (int r = 0; r < RK; ++r) {
-          const int rr = kp * RK + r;
-          const int lr = 32 * i + 8 * (rr >> 2) + 4 * h + (rr & 3);
-          const bool live = src_row[lr] >= 0;
+          const int lr = row_of(r);
+          if (src_row[lr] < 0) continue;
+          const float inv = rinv[lr];
 #pragma unroll
-          for (int j = 0; j < NC; ++j)
-            add[j][r] = live && col[j] < N ? load_val(in, in_bf16, (int64_t)(m0 + lr) * N + col[j]) : 0.f;
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < RK; ++r) {
-        const int rr = kp * RK + r;
-        const int lr = 32 * i + 8 * (rr >> 2) + 4 * h + (rr & 3);
-        if (src_row[lr] < 0) continue;
-        const float inv = rinv[lr];
-#pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          if (col[j] >= N) continue;
-          const int64_t o = (int64_t)(m0 + lr) * N + col[j];
-          const float v = __builtin_fmaf(out[i][j][r], inv, b1[j]);
-          if constexpr (KIND == kTLinear) {
-            epi_put(a.ep, o, v, add[j][r]);
-          } else {
-            const float u = __builtin_fmaf(out[i][1][r], inv, b2);
-            if constexpr (KIND == kTGlu) {
-              store_val(a.ep.y, a.ep.y_bf16, o, act2(a.ep.act, v, u));
+          for (int j = 0; j < NC; ++j) {
+            if (col[j] >= N) continue;
+            const int64_t o = (int64_t)(m0 + lr) * N + col[j];
+            const float v = __builtin_fmaf(out[i][j][r], inv, b1[j]);
+            if constexpr (KIND == kTLinear) {
+              const float y = act1(act, v);
+              store_val(a.ep.y, ybf, o, in ? y + add[j][r] : y);
             } else {
-              float dg, du;
-              act2_grad(a.ep.act, v, u, add[0][r], dg, du);
-              const int64_t od = 2 * (int64_t)(m0 + lr) * N + col[j];
-              store_val(a.ep.y, 1, od, dg);
-              store_val(a.ep.y, 1, od + N, du);
+              const float u = __builtin_fmaf(out[i][1][r], inv, b2);
+              if constexpr (KIND == kTGlu) {
+                store_val(a.ep.y, ybf, o, act2(act, v, u));
+              } else {
+                float dg, du;
+                act2_grad(act, v, u, add[0][r], dg, du);
+                const int64_t od = 2 * (int64_t)(m0 + lr) * N + col[j];
+                store_val(a.ep.y, 1, od, dg);
+                store_val(a.ep.y, 1, od + N, du);
+              }
             }
           }
         }
       }
-    }
+    };
+    constexpr std::integral_constant<int, KIND == kTLinear ? QMM_ACT_NONE : QMM_ACT_SILU> usual;
+    constexpr std::integral_constant<int, 0> f32;
+    constexpr std::integral_constant<int, 1> bf16;
+    if (a.ep.act != usual.value) finish(a.ep.act, a.ep.y_bf16);
+    else if (KIND == kTGluGrad || a.ep.y_bf16) finish(usual, bf16);
+    else finish(usual, f32);
     return;
   }
   float *yf = static_cast<float *>(a.y);

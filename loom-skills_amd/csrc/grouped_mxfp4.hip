@@ -540,7 +540,7 @@ __global__ __launch_bounds__(256, WAVES) void mxfp4_grouped_kernel(MArgs a) {
             if constexpr (GU)
               store_val(a.ep.y, a.ep.y_bf16, o, act2(a.ep.act, acc[i][cc][r] + b1, acc[i][CB + cc][r] + b2));
             else
-              epi_put(a.ep, o, acc[i][cc][r] + b1, add[r]);
+              epi_put(a.ep, a.ep.act, o, acc[i][cc][r] + b1, add[r]);
           }
         }
         continue;

@@ -741,15 +741,19 @@ LINEAR_Q8_FORMATS = ("q4_0", "q4_k", "q4_kt", "q6_k", "q4_0t", "mxfp4s")
 
 def _here(*ts):
     """_dev, and every tensor on the current device: the kernels are launched on its stream."""
-    _dev(*ts)
-    cur = torch.cuda.current_device()
+    cur = None
     for t in ts:
-        if t is not None and t.device.index != cur:
-            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{cur}")
+        if t is not None:
+            if not t.is_cuda or not t.is_contiguous():
+                _dev(t)
+            if cur is None:
+                cur = torch.cuda.current_device()
+            if t.get_device() != cur:
+                raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{cur}")
 
 
 def _shaped(t, shape, dtypes, what):
-    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype not in dtypes):
+    if t is not None and (t.shape != shape or t.dtype not in dtypes):
         raise ValueError(f"{what} is {tuple(t.shape)} {t.dtype}, expected {tuple(shape)} "
                          f"{' or '.join(str(d) for d in dtypes)}")
 
