@@ -4,7 +4,7 @@
 //   qmm_ffn_gate_up       y = act(x Wg^T + bg) (x Wu^T + bu)
 //   qmm_ffn_gate_up_grad  dgu[t] = (dy u act'(g), dy act(g)),  g = x Wg^T + bg, u = x Wu^T + bu
 //
-// The kernels are the products' own (gemv.hip, gemv_q4k.hip, gemv_q4kt.hip on f32 / bf16 rows; gemv_q8.hip, gemv_q4kt.hip,
+// A few rows of most formats take mv_mfma.hip. The other kernels are the products' own (gemv.hip, gemv_q4k.hip, gemv_q4kt.hip on f32 / bf16 rows; gemv_q8.hip, gemv_q4kt.hip,
 // mv_q8_mfma.hip on Q8_1; gemm_tile_kernel.hpp, gemm_dense.hip on row-scaled f16; grouped_mxfp4.hip on MXFP8) with the
 // epilogue of epilogue.hpp in place of their plain store, so a product has the bits of the call without one.
 #include "epilogue.hpp"
@@ -14,6 +14,10 @@ using namespace qmm;
 
 int qmm_gemm_epi(int fmt, int kind, int64_t rows, int64_t k, int64_t n, const void *x, const float *scales, const void *w,
                  const void *w2, const void *dy, int dy_bf16, hipStream_t s, const Epi &ep);
+
+bool qmm_mv_mfma_fits(int fmt, int x_dtype, int64_t k, int64_t n, int64_t tokens);
+int qmm_mv_mfma(int fmt, int x_dtype, int64_t k, int64_t n, int64_t tokens, const void *x, const void *w, const void *ws,
+                const void *w2, const void *ws2, hipStream_t s, const Epi &ep);
 
 namespace {
 
@@ -31,6 +35,8 @@ extern "C" int qmm_linear(int fmt, int act, int64_t tokens, int64_t k, int64_t n
   if (!val_aligned(y, y_dtype) || (residual && !val_aligned(residual, res_dtype)) || !aligned(bias, 4)) return QMM_ERR_ALIGN;
   const Epi ep{bias, nullptr, residual, y, act, res_dtype == QMM_BF16, y_dtype == QMM_BF16};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if ((val_dtype(x_dtype) || x_dtype == QMM_Q8) && qmm_mv_mfma_fits(fmt, x_dtype, k, n, tokens))
+    return qmm_mv_mfma(fmt, x_dtype, k, n, tokens, x, w, ws, nullptr, nullptr, s, ep);
   switch (x_dtype) {
     case QMM_F32:
     case QMM_BF16: return qmm_mv_impl(fmt, k, n, tokens, 0, x, x_dtype, w, ws, nullptr, s, &ep);
@@ -56,6 +62,10 @@ extern "C" int qmm_ffn_gate_up(int fmt, int act, int64_t tokens, int64_t k, int6
   if (!val_aligned(y, y_dtype) || !aligned(bias, 4) || !aligned(bias2, 4)) return QMM_ERR_ALIGN;
   const Epi ep{bias, bias2, nullptr, y, act, 0, y_dtype == QMM_BF16};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if ((val_dtype(x_dtype) || x_dtype == QMM_Q8) && qmm_mv_mfma_fits(fmt, x_dtype, k, n, tokens)) {
+    if (!w2) return QMM_ERR_NULL;
+    return qmm_mv_mfma(fmt, x_dtype, k, n, tokens, x, w, ws, w2, ws2, s, ep);
+  }
   switch (x_dtype) {
     case QMM_F32:
     case QMM_BF16: return qmm_mv_gate_up_impl(fmt, k, n, tokens, x, x_dtype, w, ws, w2, ws2, s, ep);

@@ -53,14 +53,14 @@ from .formats import (ACT, CODE, DTYPE, EPILOGUE_ACT, GATE_ACT, GEMM_MODE, ICODE
 TILE = 64
 
 
+_DT = {torch.float32: DTYPE["f32"], torch.bfloat16: DTYPE["bf16"], torch.float16: DTYPE["f16"]}
+
+
 def _dt(t):
-    if t.dtype == torch.float32:
-        return DTYPE["f32"]
-    if t.dtype == torch.bfloat16:
-        return DTYPE["bf16"]
-    if t.dtype == torch.float16:
-        return DTYPE["f16"]
-    raise TypeError(f"unsupported activation dtype {t.dtype}")
+    code = _DT.get(t.dtype)
+    if code is None:
+        raise TypeError(f"unsupported activation dtype {t.dtype}")
+    return code
 
 
 def _ptr(t):
@@ -740,16 +740,21 @@ LINEAR_Q8_FORMATS = ("q4_0", "q4_k", "q4_kt", "q6_k", "q4_0t", "mxfp4s")
 
 
 def _here(*ts):
-    """_dev, and every tensor on the current device: the kernels are launched on its stream."""
-    cur = None
+    """The current stream of the device that holds the tensors (_dev's checks), which must be the current one: the kernels
+    are launched on its stream."""
+    dev = None
     for t in ts:
         if t is not None:
-            if not t.is_cuda or not t.is_contiguous():
+            d = t.get_device()
+            if d < 0 or not t.is_contiguous():
                 _dev(t)
-            if cur is None:
-                cur = torch.cuda.current_device()
-            if t.get_device() != cur:
-                raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{cur}")
+            if dev is None:
+                dev = d
+            elif d != dev:
+                raise ValueError(f"tensors are on cuda:{dev} and cuda:{d}")
+    if dev != torch._C._cuda_getDevice():
+        raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _shaped(t, shape, dtypes, what):
@@ -836,7 +841,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out="bf16", h=None):
 
     h has the residual's type (None without one); the h argument takes the output rows, x or residual for an update in
     place."""
-    _here(x, weight, residual, h)
+    s = _here(x, weight, residual, h)
     if x.dim() != 2:
         raise ValueError(f"x is {tuple(x.shape)}, expected [rows, k]")
     rows, k = x.shape
@@ -850,19 +855,19 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out="bf16", h=None):
         raise ValueError("h is written with a residual")
     scales = None
     if out in ("bf16", "f32"):
-        y = torch.empty((rows, k), dtype=torch.bfloat16 if out == "bf16" else torch.float32, device=x.device)
+        y = x.new_empty((rows, k), dtype=torch.bfloat16 if out == "bf16" else torch.float32)
     elif out == "f16":
-        y = torch.empty((rows, k), dtype=torch.float16, device=x.device)
-        scales = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+        y = x.new_empty((rows, k), dtype=torch.float16)
+        scales = x.new_empty((rows, 2), dtype=torch.float32)
     elif out == "q8":
-        y = torch.empty(q8_bytes(rows, k), dtype=torch.uint8, device=x.device)
+        y = x.new_empty(q8_bytes(rows, k), dtype=torch.uint8)
     elif out == "mxfp8":
-        y = torch.empty((rows, k), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((rows, k // MX_BLOCK), dtype=torch.uint8, device=x.device)
+        y = x.new_empty((rows, k), dtype=torch.uint8)
+        scales = x.new_empty((rows, k // MX_BLOCK), dtype=torch.uint8)
     else:
         raise ValueError(f"out {out!r} is none of bf16, f32, f16, q8, mxfp8")
     _lib.call("qmm_rms_norm", rows, k, _ptr(x), _dt(x), _ptr(residual), 0 if residual is None else _dt(residual),
-              _ptr(weight), _dt(weight), eps, _ptr(h), DTYPE[out], _ptr(y), _ptr(scales), _stream())
+              _ptr(weight), _dt(weight), eps, _ptr(h), DTYPE[out], _ptr(y), _ptr(scales), s)
     return y, scales, h
 
 
@@ -910,24 +915,27 @@ def linear(fmt, x, w, n, k, y=None, mode="store", ws=None, w2=None, ws2=None, q8
 
 
 def _linear_epilogue(fmt, x, w, n, k, y, ws, q8, bias, act, residual, out_dtype, scales, tokens):
-    _here(x, w, ws, bias, residual, scales, y)
+    s = _here(x, w, ws, bias, residual, scales, y)
     code = _act_code(act, EPILOGUE_ACT)
     _weight_bytes(fmt, w, ws, n, k)
     T = x.shape[0] if tokens is None else tokens
     _shaped(bias, (n,), (torch.float32,), "bias")
     _shaped(residual, (T, n), _VALUE, "residual")
-    y = _rows_out(y, (T, n), out_dtype, x.device)
+    y = _rows_out(y, (T, n), out_dtype, x)
     x, xd, scales = _product_operand(fmt, x, k, scales, tokens, q8)
     _lib.call("qmm_linear", CODE[fmt], code, T, k, n, _ptr(x), xd, _ptr(scales), _ptr(w), _ptr(ws), _ptr(bias),
-              _ptr(residual), 0 if residual is None else _dt(residual), _ptr(y), _dt(y), _stream())
+              _ptr(residual), 0 if residual is None else _dt(residual), _ptr(y), _dt(y), s)
     return y
 
 
-def _rows_out(y, shape, out_dtype, dev):
+def _rows_out(y, shape, out_dtype, like):
     """The f32 / bf16 output rows: y, or a new tensor of out_dtype (f32 when None)."""
     if y is None:
-        y = torch.empty(shape, dtype=torch.float32 if out_dtype is None else out_dtype, device=dev)
-    elif out_dtype is not None and y.dtype != out_dtype:
+        y = like.new_empty(shape, dtype=torch.float32 if out_dtype is None else out_dtype)
+        if y.dtype not in _VALUE:
+            raise ValueError(f"out_dtype is float32 or bfloat16, not {out_dtype}")
+        return y
+    if out_dtype is not None and y.dtype != out_dtype:
         raise ValueError(f"y is {y.dtype}, out_dtype {out_dtype}")
     _shaped(y, shape, _VALUE, "y")
     return y
@@ -938,17 +946,17 @@ def ffn_gate_up(fmt, x, w, w2, n, k, y=None, ws=None, ws2=None, q8="auto", bias=
     """The gated feed-forward block's first half, y = act(x W^T + bias) (x W2^T + bias2), in one kernel past the operand's
     (qmm_ffn_gate_up). x, scales, tokens, q8 as linear; biases f32 [n] or None; act as linear or swiglu_oai (the gpt-oss
     clamped form); y [tokens, n] f32 or bf16 (out_dtype)."""
-    _here(x, w, ws, w2, ws2, bias, bias2, scales, y)
+    s = _here(x, w, ws, w2, ws2, bias, bias2, scales, y)
     code = _act_code(act, GATE_ACT)
     _weight_bytes(fmt, w, ws, n, k)
     _weight_bytes(fmt, w2, ws2, n, k, "w2")
     T = x.shape[0] if tokens is None else tokens
     _shaped(bias, (n,), (torch.float32,), "bias")
     _shaped(bias2, (n,), (torch.float32,), "bias2")
-    y = _rows_out(y, (T, n), out_dtype, x.device)
+    y = _rows_out(y, (T, n), out_dtype, x)
     x, xd, scales = _product_operand(fmt, x, k, scales, tokens, q8)
     _lib.call("qmm_ffn_gate_up", CODE[fmt], code, T, k, n, _ptr(x), xd, _ptr(scales), _ptr(w), _ptr(ws), _ptr(w2), _ptr(ws2),
-              _ptr(bias), _ptr(bias2), _ptr(y), _dt(y), _stream())
+              _ptr(bias), _ptr(bias2), _ptr(y), _dt(y), s)
     return y
 
 
@@ -958,7 +966,7 @@ def ffn_gate_up_backward(fmt, x, w, w2, dy, n, k, scales=None, bias=None, bias2=
     beside the projections train on), dx = dgu[:, 0] W + dgu[:, 1] W2. The projections are computed again from x: f32 / bf16
     rows, or the f16 operand with its scales as for ffn_gate_up (rows that are all padding have no gradient: pass dy rows of
     zeros there, their dgu and dx rows are undefined). fmt q4_k, q4_kt, q6_k or q4_0, k % 256 == 0."""
-    _here(x, w, w2, dy, bias, bias2, scales)
+    s = _here(x, w, w2, dy, bias, bias2, scales)
     code = _act_code(act, GATE_ACT)
     if fmt not in _F16_GEMM:
         raise ValueError(f"no backward pass reads {fmt} weights")
@@ -980,7 +988,7 @@ def ffn_gate_up_backward(fmt, x, w, w2, dy, n, k, scales=None, bias=None, bias2=
         raise ValueError("the f16 operand comes with its scales")
     dgu = torch.empty((T, 2, n), dtype=torch.bfloat16, device=x.device)
     _lib.call("qmm_ffn_gate_up_grad", CODE[fmt], code, T, k, n, _ptr(x), _ptr(scales), _ptr(w), _ptr(w2), _ptr(bias),
-              _ptr(bias2), _ptr(dy), _dt(dy), _ptr(dgu), _stream())
+              _ptr(bias2), _ptr(dy), _dt(dy), _ptr(dgu), s)
     return gemm_t(fmt, dgu, w, n, k, w2=w2, out_dtype=out_dtype), dgu
 
 
@@ -988,7 +996,7 @@ def gemm_t(fmt, x, w, n, k, w2=None, out_dtype=torch.float32, y=None):
     """The transposed product y = x W [rows, k] of gradient rows x [rows, n], or x[:, 0] W + x[:, 1] W2 of x [rows, 2, n]
     (f32 / bf16): the input gradient of a projection y = x W^T whose weights stay quantized (qmm_grad_operand, qmm_gemm_t).
     fmt q4_k, q4_kt, q6_k or q4_0, k % 256 == 0; y f32 or bf16."""
-    _here(x, w, w2, y)
+    s = _here(x, w, w2, y)
     if fmt not in _F16_GEMM:
         raise ValueError(f"no transposed product reads {fmt} weights")
     _weight_bytes(fmt, w, None, n, k)
@@ -996,14 +1004,13 @@ def gemm_t(fmt, x, w, n, k, w2=None, out_dtype=torch.float32, y=None):
         _weight_bytes(fmt, w2, None, n, k, "w2")
     rows, parts = x.shape[0], 1 if w2 is None else 2
     _shaped(x, (rows, n) if w2 is None else (rows, 2, n), _VALUE, "x")
-    y = _rows_out(y, (rows, k), None if y is not None else out_dtype, x.device)
+    y = _rows_out(y, (rows, k), None if y is not None else out_dtype, x)
     need = _lib.load().qmm_gemm_t_workspace_size(CODE[fmt], rows, k, n, parts - 1)
     if need < 0:
         raise ValueError(f"the transposed product does not take {rows} rows of {fmt} [{n}, {k}]")
     x16 = torch.empty((rows, parts, -(-n // 64) * 64), dtype=torch.float16, device=x.device)
     scales = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
     work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    s = _stream()
     _lib.call("qmm_grad_operand", rows, parts, n, _ptr(x), _dt(x), _ptr(x16), _ptr(scales), s)
     _lib.call("qmm_gemm_t", CODE[fmt], rows, k, n, _ptr(x16), _ptr(scales), _ptr(w), _ptr(w2), _ptr(y), _dt(y), _ptr(work),
               need, s)
