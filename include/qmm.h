@@ -198,12 +198,15 @@ int qmm_rms_norm(int64_t rows, int64_t k, const void *x, int x_dtype, const void
  *   y[t, r] = act(sum_k x[t, k] W[r, k] + bias[r]) + residual[t, r]
  * act: QMM_ACT_NONE, RELU, SILU, SIGMOID, GELU or GELU_ERF. bias f32 [n] or NULL; residual [tokens, n] f32 or bf16 or NULL,
  * may be y itself where the types agree; y [tokens, n] of y_dtype (QMM_F32, or QMM_BF16 rounded to nearest even, the only
- * rounding after the f32 sum). x by x_dtype takes the matching product, with its formats, shapes, alignment, K sums and
- * limits, and the sum has its bits:
+ * rounding after the f32 sum). x by x_dtype takes the matching product's formats, shapes, alignment and limits:
  *   QMM_F32 / QMM_BF16  qmm_mv (rows [tokens, k]; x_scales unused)
  *   QMM_Q8              qmm_mv_q8 on the planar Q8_1 buffer, or qmm_mv_mxfp4s_q8 (fmt QMM_MXFP4S)
  *   QMM_F16             qmm_gemm, x_scales f32 [tokens, 2] or NULL (64-row tiles of padding rows are not written)
  *   QMM_MXFP8           qmm_gemm_mxfp4, x_scales E8M0 [tokens, k/32]
+ * The sum has that product's bits, except for a few rows (F32, BF16, Q8) of QMM_Q4_0, QMM_Q4_K, QMM_Q6_K, QMM_MXFP4 or
+ * QMM_MXFP4S weights with K % 64 == 0, whose exact products are added in another f32 order (from two rows on; by format and
+ * operand, from one to five). Among those calls a row's bits do not depend on the rows beside it; an f32 row that holds an
+ * infinity gives NaN or infinities.
  * ws: the weights' scale plane for QMM_MXFP4S / QMM_MXFP4T, else NULL. */
 int qmm_linear(int fmt, int act, int64_t tokens, int64_t k, int64_t n, const void *x, int x_dtype, const void *x_scales,
                const void *w, const void *ws, const float *bias, const void *residual, int res_dtype, void *y, int y_dtype,

@@ -161,6 +161,12 @@ __device__ __forceinline__ void copy_to_lds(u8 *dst, const u8 *src, int64_t n, i
   }
 }
 
+// bytes between the scale rows in LDS, sk of them used. kOutEpi: an odd number of dwords, so that the 32 rows a wave
+// reads a byte of fall into 32 banks; at K = 4096 an unpadded row is 32 dwords and they fall into two (4096 x 4096 at
+// 2048 rows 84 -> 53 µs)
+template <int OUT>
+__host__ __device__ constexpr int scale_pitch(int sk) { return OUT == kOutEpi ? 4 * (((sk + 3) / 4) | 1) : sk; }
+
 template <int KIND, int LAYOUT, int DEPTH, int kSub, int OUT, int CB, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void mxfp4_grouped_kernel(MArgs a) {
   constexpr bool DENSE = OUT != kOutGrouped;
@@ -183,7 +189,8 @@ __global__ __launch_bounds__(256, WAVES) void mxfp4_grouped_kernel(MArgs a) {
   // E8M0 scales staged once: the tile's 64 activation rows and, for kSplit, the block's weight columns (gu: 128 gate
   // then 128 up columns; dn: 128 columns), K / 32 bytes each.
   extern __shared__ __align__(16) u8 dyn_lds[];
-  u8 *Asc = dyn_lds, *Wsc = dyn_lds + BM * (a.K / 32);
+  const int ASP = scale_pitch<OUT>(a.K / 32);   // bytes between the activation rows' scales in LDS
+  u8 *Asc = dyn_lds, *Wsc = dyn_lds + BM * ASP;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 
   // ---- which tile and column block: the live tiles [0, L) (L = 1 + the last tile with an expert) in eight
@@ -202,22 +209,36 @@ __global__ __launch_bounds__(256, WAVES) void mxfp4_grouped_kernel(MArgs a) {
     L = live_end;
   }
   const int xcd = (int)(blockIdx.x & 7), xi = (int)(blockIdx.x >> 3);
-  const int t_begin = (int)(((int64_t)xcd * L) >> 3), t_end = (int)(((int64_t)(xcd + 1) * L) >> 3);
-  const int cnt = t_end - t_begin;
-  if (cnt <= 0 || xi >= cnt * a.n_blocks) return;
-  // the range in groups of kTileGroup tiles, each group walked tile-fastest over every column block before the next:
-  // a group's activation rows (12 x 64 rows) are then read by its column blocks while they are still in the XCD's
-  // L2, where one sweep of all the range's tiles per column block lets the weight stream evict them in between
-  // (gpt-oss-20b at T = 4096, HBM reads a launch: gate/up 878 -> 727 MB, down 454 -> 386 MB; times within 2 %)
   int tile, cbk;
-  if (cnt > kTileGroup) {
-    const int per = kTileGroup * a.n_blocks, g = xi / per, r = xi - g * per, gt0 = g * kTileGroup;
-    const int gn = cnt - gt0 < kTileGroup ? cnt - gt0 : kTileGroup;
-    tile = t_begin + gt0 + r % gn;
+  if constexpr (OUT == kOutEpi) {
+    // the call's (tile, column block) pairs, in the order of the groups below, in eight contiguous ranges: a call of
+    // fewer than eight row tiles runs on every XCD, each on its own column blocks (12288 x 4096 at 64 rows 65 -> 29 µs,
+    // at 512 rows 71 -> 68; 22 and 38 with the scale rows' pitch)
+    const int64_t P = (int64_t)L * a.n_blocks, p_begin = (P * xcd) >> 3, p_end = (P * (xcd + 1)) >> 3;
+    if (xi >= p_end - p_begin) return;
+    const int64_t p = p_begin + xi;
+    const int64_t per = (int64_t)kTileGroup * a.n_blocks;
+    const int g = (int)(p / per), r = (int)(p - g * per), gt0 = g * kTileGroup;
+    const int gn = L - gt0 < kTileGroup ? L - gt0 : kTileGroup;
+    tile = gt0 + r % gn;
     cbk = r / gn;
   } else {
-    tile = t_begin + xi % cnt;
-    cbk = xi / cnt;
+    const int t_begin = (int)(((int64_t)xcd * L) >> 3), t_end = (int)(((int64_t)(xcd + 1) * L) >> 3);
+    const int cnt = t_end - t_begin;
+    if (cnt <= 0 || xi >= cnt * a.n_blocks) return;
+    // the range in groups of kTileGroup tiles, each group walked tile-fastest over every column block before the next:
+    // a group's activation rows (12 x 64 rows) are then read by its column blocks while they are still in the XCD's
+    // L2, where one sweep of all the range's tiles per column block lets the weight stream evict them in between
+    // (gpt-oss-20b at T = 4096, HBM reads a launch: gate/up 878 -> 727 MB, down 454 -> 386 MB; times within 2 %)
+    if (cnt > kTileGroup) {
+      const int per = kTileGroup * a.n_blocks, g = xi / per, r = xi - g * per, gt0 = g * kTileGroup;
+      const int gn = cnt - gt0 < kTileGroup ? cnt - gt0 : kTileGroup;
+      tile = t_begin + gt0 + r % gn;
+      cbk = r / gn;
+    } else {
+      tile = t_begin + xi % cnt;
+      cbk = xi / cnt;
+    }
   }
   const int N = a.N, K = a.K, C = K / KC;
   const int n0 = cbk * BN, m0 = tile * BM;
@@ -370,7 +391,7 @@ __global__ __launch_bounds__(256, WAVES) void mxfp4_grouped_kernel(MArgs a) {
     static_assert(BM * 4 == 256, "four threads a scale row");
     const int r = tid >> 2, q0 = tid & 3, n2 = SK / 2;
     const u16 *sp = reinterpret_cast<const u16 *>(a.xs + (int64_t)(src_row[r] >= 0 ? src_row[r] : 0) * SK);
-    u16 *dp = reinterpret_cast<u16 *>(Asc + r * SK);
+    u16 *dp = reinterpret_cast<u16 *>(Asc + r * ASP);
     for (int b = q0; b < n2; b += 32) {
       u16 v[8];
 #pragma unroll
@@ -419,7 +440,7 @@ __global__ __launch_bounds__(256, WAVES) void mxfp4_grouped_kernel(MArgs a) {
         const v4u v0 = *reinterpret_cast<const v4u *>(&As[buf][32 * ii + lc][KC * i + 16 * h]);
         const v4u v1 = *reinterpret_cast<const v4u *>(&As[buf][32 * ii + lc][KC * i + 32 + 16 * h]);
         af = i32x8{(int)v0.x, (int)v0.y, (int)v0.z, (int)v0.w, (int)v1.x, (int)v1.y, (int)v1.z, (int)v1.w};
-        sa = live ? Asc[(32 * ii + lc) * SK + sc_off] : 0;
+        sa = live ? Asc[(32 * ii + lc) * ASP + sc_off] : 0;
       };
       i32x8 bf[NJ];
       int sb[NJ];
@@ -609,16 +630,18 @@ int launch(const MArgs &a0, hipStream_t s) {
   // several weight blocks a wave shorten the super-steps to keep the bytes per barrier
   constexpr int kSub0 = (KIND == kDN ? QMM_MX_SUB_DN : QMM_MX_SUB_GU) / CB;
   constexpr int kSub = kSub0 > 0 ? kSub0 : 1;
-  constexpr int kRows = BM + (LAYOUT == kSplit ? (KIND != kDN ? 256 : 128) : 0);   // scale rows staged in LDS
-  const dim3 grid((unsigned)(8 * a.n_blocks * ((a.max_tiles + 7) / 8)));
-  const size_t dyn = (size_t)kRows * (a.K / 32);
+  constexpr int kWRows = LAYOUT == kSplit ? (KIND != kDN ? 256 : 128) : 0;   // weight scale rows staged in LDS
+  const dim3 grid(OUT == kOutEpi ? (unsigned)(8 * (((int64_t)a.n_blocks * a.max_tiles + 7) / 8))
+                                 : (unsigned)(8 * a.n_blocks * ((a.max_tiles + 7) / 8)));
+  auto scales = [](int k) { return BM * scale_pitch<OUT>(k / 32) + kWRows * (k / 32); };
+  const size_t dyn = (size_t)scales(a.K);
   const void *fn = reinterpret_cast<const void *>(&mxfp4_grouped_kernel<KIND, LAYOUT, kDepth, kSub, OUT, CB, kWaves>);
-  if constexpr ((size_t)kRows * (kMaxK / 32) > 32768) {
+  if constexpr ((size_t)(BM + kWRows) * (kMaxK / 32) > 32768) {
     // beyond the default dynamic LDS limit: raised once per device to the largest K this kernel takes, so the order
     // of calls with different K does not matter
     if (dyn > 32768) {
       static std::atomic<unsigned> raised{0};
-      if (int st = raise_dyn_lds(fn, kRows * (kMaxK / 32), raised)) return st;
+      if (int st = raise_dyn_lds(fn, scales(kMaxK), raised)) return st;
     }
   }
   mxfp4_grouped_kernel<KIND, LAYOUT, kDepth, kSub, OUT, CB, kWaves><<<grid, 256, dyn, s>>>(a);
@@ -633,6 +656,14 @@ int launch(const MArgs &a0, hipStream_t s) {
 // block; down with four blocks 60 / 184 µs at T = 1024 / 4096, with two 67 / 191.)
 constexpr int kWideRows = 64, kWideRowsGU = 128;
 inline bool wide_tiles(int64_t max_tiles, int E, int rows) { return (max_tiles - E) * BM >= (int64_t)rows * E; }
+
+// A dense product with an epilogue: two column blocks a wave once that leaves two workgroups a CU, so that each row of
+// x in LDS meets twice the weights; with fewer, one block keeps more waves on the loads. (Two blocks / one, µs: 2880 x
+// 2880 at 4096 rows, 768 workgroups of two blocks, 50 / 58; 12288 x 4096 at 700, 1024 and 2048 rows, 528 to 1536
+// workgroups, 53 / 58, 61 / 71 and 116 / 131; 4096 x 4096 at 4096 rows 98 / 98; below, 12288 x 4096 at 512 rows, 384
+// workgroups, 47 / 38 and 2880 x 2880 at 2048 rows 42 / 31.) A gated block has two weight blocks a wave with one column
+// block already; with two it takes the registers of a third workgroup a CU (12288 x 4096 at 1024 rows 124 / 101 µs).
+constexpr int64_t kEpiWide = 512;
 
 // MFMA-tiled planes from split planes (a byte permutation): one thread per 16-byte lane slot of a 1 KB tile, and
 // per (row block, chunk group) the 64 lanes' four scale bytes. Chunks past K in the last group get scale 0.
@@ -769,6 +800,7 @@ int qmm_gemm_mxfp4_impl(int fmt, int mode, int64_t rows, int64_t k, int64_t n, c
   if (ep) {
     a.ep = *ep;
     if (mode == QMM_GEMM_SWIGLU) return tiled ? launch<kGU, kTiled, kOutEpi>(a, s) : launch<kGU, kSplit, kOutEpi>(a, s);
+    if (tiled && (n + 255) / 256 * a.max_tiles >= kEpiWide) return launch<kDN, kTiled, kOutEpi, 2>(a, s);
     return tiled ? launch<kDN, kTiled, kOutEpi>(a, s) : launch<kDN, kSplit, kOutEpi>(a, s);
   }
   const bool bf = y_dtype == QMM_BF16;

@@ -4,9 +4,11 @@
 //   qmm_ffn_gate_up       y = act(x Wg^T + bg) (x Wu^T + bu)
 //   qmm_ffn_gate_up_grad  dgu[t] = (dy u act'(g), dy act(g)),  g = x Wg^T + bg, u = x Wu^T + bu
 //
-// A few rows of most formats take mv_mfma.hip. The other kernels are the products' own (gemv.hip, gemv_q4k.hip, gemv_q4kt.hip on f32 / bf16 rows; gemv_q8.hip, gemv_q4kt.hip,
-// mv_q8_mfma.hip on Q8_1; gemm_tile_kernel.hpp, gemm_dense.hip on row-scaled f16; grouped_mxfp4.hip on MXFP8) with the
-// epilogue of epilogue.hpp in place of their plain store, so a product has the bits of the call without one.
+// A few rows of Q4_0, Q4_K, Q6_K and MXFP4 (qmm_mv_mfma_fits) take mv_mfma.hip, which adds the same exact products in an
+// order of its own. The other kernels are the products' own (gemv.hip, gemv_q4k.hip, gemv_q4kt.hip on f32 / bf16 rows;
+// gemv_q8.hip, gemv_q4kt.hip, mv_q8_mfma.hip on Q8_1; gemm_tile_kernel.hpp, gemm_dense.hip on row-scaled f16;
+// grouped_mxfp4.hip on MXFP8) with the epilogue of epilogue.hpp in place of their plain store: their sums have the bits of
+// the call without one.
 #include "epilogue.hpp"
 #include "gemm_tile.hpp"
 
