@@ -140,6 +140,10 @@ def test_mxfp8_rows_have_the_plain_products_bits(dev, fmt, T, n, k):
     buf = torch.full((T * n + 64,), 3.0, device=dev)
     ops.linear(fmt, c, w.w, n, k, ws=w.ws, scales=s, bias=b, residual=res, y=buf[:T * n].view(T, n))
     assert torch.equal(buf[:T * n].view(T, n), (y0 + b) + res.float()) and (buf[T * n:] == 3).all()
+    for at, out in ((1, torch.float32), (2, torch.bfloat16), (8, torch.bfloat16)):   # y rows that are not on 16 bytes, and some that are
+        buf = torch.full((T * n + 64,), 3.0, dtype=out, device=dev)
+        got = ops.linear(fmt, c, w.w, n, k, ws=w.ws, scales=s, bias=b, residual=res, y=buf[at:at + T * n].view(T, n))
+        assert torch.equal(got, ((y0 + b) + res.float()).to(out)) and (buf[:at] == 3).all() and (buf[at + T * n:] == 3).all()
     g = ops.ffn_gate_up(fmt, c, w.w, w.w, n, k, ws=w.ws, ws2=w.ws, scales=s, bias=b, act="gelu", out_dtype=torch.float32)
     pre, up = f64(y0 + b), f64(y0)
     a = glu64("gelu", pre, up)
