@@ -25,21 +25,6 @@ __device__ __forceinline__ void load8_act(const void *x, bool bf, int64_t e, flo
   }
 }
 
-__device__ __forceinline__ u32 bf16_pair(float a, float b) {
-  return (u32)__builtin_bit_cast(u16, (__bf16)a) | ((u32)__builtin_bit_cast(u16, (__bf16)b) << 16);
-}
-// 8 values to element offset e of a bf16 or f32 array
-__device__ __forceinline__ void store8(void *p, int bf, int64_t e, const float (&v)[8]) {
-  if (bf) {
-    *reinterpret_cast<v4u *>(static_cast<u16 *>(p) + e) =
-        v4u{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
-  } else {
-    float *f = static_cast<float *>(p) + e;
-    *reinterpret_cast<v4u *>(f) = v4u{f32_as_u32(v[0]), f32_as_u32(v[1]), f32_as_u32(v[2]), f32_as_u32(v[3])};
-    *reinterpret_cast<v4u *>(f + 4) = v4u{f32_as_u32(v[4]), f32_as_u32(v[5]), f32_as_u32(v[6]), f32_as_u32(v[7])};
-  }
-}
-
 // One 32-value group held by four consecutive lanes of a wave (8 values each, the group's first lane a multiple of
 // 4): the lane's 8 codes as two dwords, and the group's f16-rounded d and code sum.
 __device__ __forceinline__ void q8_group4(const float (&v)[8], u32 &c0, u32 &c1, float &d16, float &sum) {

@@ -55,6 +55,30 @@ __device__ __forceinline__ void store_val(void *p, int bf16, int64_t o, float v)
   else static_cast<float *>(p)[o] = v;
 }
 
+// V (4 or 8) neighbouring values at element offset o, a multiple of V of 16-byte aligned rows
+template <int V>
+__device__ __forceinline__ void load_vals(const void *p, int bf16, int64_t o, float (&v)[V]) {
+  if (bf16) {
+    u32 d[V / 2];
+    __builtin_memcpy(d, __builtin_assume_aligned(static_cast<const u16 *>(p) + o, 2 * V), 2 * V);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) { v[2 * j] = u32_as_f32(d[j] << 16); v[2 * j + 1] = u32_as_f32(d[j] & 0xFFFF0000u); }
+  } else {
+    __builtin_memcpy(v, __builtin_assume_aligned(static_cast<const float *>(p) + o, 16), 4 * V);
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_vals(void *p, int bf16, int64_t o, const float (&v)[V]) {
+  if (bf16) {
+    __bf16 d[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) d[j] = (__bf16)v[j];
+    __builtin_memcpy(__builtin_assume_aligned(static_cast<u16 *>(p) + o, 2 * V), d, 2 * V);
+  } else {
+    __builtin_memcpy(__builtin_assume_aligned(static_cast<float *>(p) + o, 16), v, 4 * V);
+  }
+}
+
 // output o = row n + c of a one-matrix product
 __device__ __forceinline__ void epi_store(const Epi &e, int64_t o, int64_t c, float v) {
   if (e.bias) v += e.bias[c];

@@ -375,6 +375,18 @@ __global__ __launch_bounds__(kWaves * 64, 1) void q4k_dense_kernel(DArgs a, EP e
     const int64_t o = (int64_t)row * N + col;
     if constexpr (kEpi<EP>) {   // eight columns of a row: their bias and residual values, then the stores
       float b[8], r[8];
+      if (N % 8 == 0 && ((reinterpret_cast<uintptr_t>(ep.y) | reinterpret_cast<uintptr_t>(ep.res)) & 15) == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = epi_bias(ep.bias, col + e);
+        if (ep.res) load_vals<8>(ep.res, ep.res_bf16, o, r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = act1(ep.act, v[e] + b[e]);
+          if (ep.res) v[e] += r[e];
+        }
+        store_vals<8>(ep.y, ep.y_bf16, o, v);
+        continue;
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const bool in = col + e < N;

@@ -490,6 +490,7 @@ int qmm_gemm_epi(int fmt, int kind, int64_t rows, int64_t k, int64_t n, const vo
   t.x16 = static_cast<const _Float16 *>(x); t.scales = scales; t.x_rows = (int)rows;
   t.w = static_cast<const u8 *>(w); t.w2 = static_cast<const u8 *>(w2);
   t.ep = ep; t.dy = dy; t.dy_bf16 = dy_bf16;
+  t.wide_rows = n % 8 == 0 && aligned(ep.y, 16) && aligned(ep.res, 16) && aligned(dy, 16);
   return tile_gemm(fmt, kind, shape, t, s);
 }
 

@@ -30,6 +30,7 @@ struct TileArgs {
   Epi ep;                      // kTLinear, kTGlu, kTGluGrad
   const void *dy;              // kTGluGrad: [M, N] f32 or bf16
   int dy_bf16;
+  int wide_rows;               // rows of y and what is read beside it (residual, dy) are 16-byte aligned
 };
 
 int tile_gemm_q4k(int kind, int shape, const TileArgs &a, hipStream_t s);

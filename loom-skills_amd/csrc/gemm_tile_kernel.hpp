@@ -561,6 +561,75 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
     if constexpr (kTwoW) b2 = epi_bias(a.ep.bias2, min(col[0], N - 1));
     const void *in = KIND == kTGluGrad ? a.dy : a.ep.res;
     const int in_bf16 = KIND == kTGluGrad ? a.dy_bf16 : a.ep.res_bf16;
+    constexpr std::integral_constant<int, KIND == kTLinear ? QMM_ACT_NONE : QMM_ACT_SILU> usual;
+    constexpr std::integral_constant<int, 0> f32;
+    constexpr std::integral_constant<int, 1> bf16;
+    if (a.wide_rows) {
+      // Through the wave's own LDS, PR rows of its columns at a time, so that a lane reads and writes V neighbouring values of
+      // a row (the other path below: a column a lane, a load and a store a value). kTGluGrad takes both sums through it.
+      constexpr int WC = 32 * NC, NROW = 32 / KS, PR = 512 / WC < NROW ? 512 / WC : NROW, NP = NROW / PR, V = PR * WC / 64;
+      constexpr int kPlanes = KIND == kTGluGrad ? 2 : 1, PITCH = WC + 8, LR = WC / V;   // LR lanes a row
+      static_assert(NW * KS * kPlanes * PR * PITCH * 4 <= 2 * KS * kPart, "a pass of every wave fits the staged activations");
+      float *T = reinterpret_cast<float *>(smem) + wave * kPlanes * PR * PITCH;
+      if constexpr (KS > 1) __syncthreads();   // the parts' exchange is read
+      const int tr = lane / LR, tc = V * (lane % LR), cw = n0 + WC * wn + tc;
+      auto finish = [&](auto act, auto ybf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int row0 = 32 * i + NROW * kp;
+          auto live = [&](int p) { return src_row[row0 + PR * p + tr] >= 0 && cw < N; };
+          auto at = [&](int p) { return (int64_t)(m0 + row0 + PR * p + tr) * N + cw; };
+          float add[NP][V];
+          if (KIND != kTGlu && in) {
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+              if (live(p)) load_vals<V>(in, in_bf16, at(p), add[p]);
+          }
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+#pragma unroll
+            for (int rr = 0; rr < PR / 2; ++rr) {   // the accumulator registers of the pass's rows
+              const int r = PR / 2 * p + rr, lr = 8 * (rr >> 2) + 4 * h + (rr & 3);
+              const float inv = rinv[row0 + PR * p + lr];
+              float *t = T + lr * PITCH + lc;
+#pragma unroll
+              for (int j = 0; j < NC; ++j) {
+                const float v = __builtin_fmaf(out[i][j][r], inv, b1[j]);
+                if constexpr (KIND == kTLinear) {
+                  t[32 * j] = act1(act, v);
+                } else {
+                  const float u = __builtin_fmaf(out[i][1][r], inv, b2);
+                  t[0] = KIND == kTGlu ? act2(act, v, u) : v;
+                  if constexpr (kPlanes == 2) t[PR * PITCH] = u;
+                }
+              }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            const float *t = T + tr * PITCH + tc;
+            if constexpr (KIND == kTGluGrad) {
+              float dg[V], du[V];
+#pragma unroll
+              for (int q = 0; q < V; ++q) act2_grad(act, t[q], t[PR * PITCH + q], add[p][q], dg[q], du[q]);
+              if (live(p)) {
+                const int64_t od = at(p) + (int64_t)(m0 + row0 + PR * p + tr) * N;
+                store_vals<V>(a.ep.y, ybf, od, dg);
+                store_vals<V>(a.ep.y, ybf, od + N, du);
+              }
+            } else {
+              float v[V];
+#pragma unroll
+              for (int q = 0; q < V; ++q) v[q] = KIND == kTLinear && in ? t[q] + add[p][q] : t[q];
+              if (live(p)) store_vals<V>(a.ep.y, ybf, at(p), v);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          }
+        }
+      };
+      if (a.ep.act != usual.value) finish(a.ep.act, a.ep.y_bf16);
+      else if (KIND == kTGluGrad || a.ep.y_bf16) finish(usual, bf16);
+      else finish(usual, f32);
+      return;
+    }
     // act, ybf: constants where the activation is the common one, so that a value does not branch on them
     auto finish = [&](auto act, auto ybf) __attribute__((always_inline)) {
 #pragma unroll
@@ -612,9 +681,6 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
         }
       }
     };
-    constexpr std::integral_constant<int, KIND == kTLinear ? QMM_ACT_NONE : QMM_ACT_SILU> usual;
-    constexpr std::integral_constant<int, 0> f32;
-    constexpr std::integral_constant<int, 1> bf16;
     if (a.ep.act != usual.value) finish(a.ep.act, a.ep.y_bf16);
     else if (KIND == kTGluGrad || a.ep.y_bf16) finish(usual, bf16);
     else finish(usual, f32);

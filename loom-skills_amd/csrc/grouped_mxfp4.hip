@@ -47,7 +47,6 @@
 // barrier per super-step) and the weights stream straight into registers DEPTH super-steps ahead.
 #include <type_traits>
 
-#include "act_quant.hpp"
 #include "bfly.hpp"
 #include "epilogue.hpp"
 
@@ -85,6 +84,8 @@ enum Layout { kSplit = 0, kTiled = 1 };
 // through the epilogue of qmm_linear / qmm_ffn_gate_up);
 // a dense kGU is the swiglu GEMM silu(X Wg^T) (X Wu^T) over rows 0 .. M - 1 of x
 enum Out { kOutGrouped = 0, kOutF32 = 1, kOutF32Acc = 2, kOutBF16 = 3, kOutBF16Acc = 4, kOutEpi = 5 };
+
+typedef __attribute__((ext_vector_type(4))) u32 v4u;   // a native vector: the register rings stay in VGPRs
 
 struct MArgs {
   int N, K;
@@ -564,7 +565,7 @@ __global__ __launch_bounds__(256, WAVES) void mxfp4_grouped_kernel(MArgs a) {
           if (!GU && a.ep.res) {
 #pragma unroll
             for (int p = 0; p < NP; ++p)
-              if (live(p)) load8_act(a.ep.res, a.ep.res_bf16, at(p), add[p]);
+              if (live(p)) load_vals<8>(a.ep.res, a.ep.res_bf16, at(p), add[p]);
           }
 #pragma unroll
           for (int p = 0; p < NP; ++p) {
@@ -584,7 +585,7 @@ __global__ __launch_bounds__(256, WAVES) void mxfp4_grouped_kernel(MArgs a) {
 #pragma unroll
               for (int q = 0; q < 8; ++q) v[q] += add[p][q];
             }
-            if (live(p)) store8(a.ep.y, a.ep.y_bf16, at(p), v);
+            if (live(p)) store_vals<8>(a.ep.y, a.ep.y_bf16, at(p), v);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
           }
         }

@@ -37,6 +37,21 @@ __device__ __forceinline__ float norm_rate(float sum, int64_t k, float eps) { re
 __device__ __forceinline__ int f16_exponent(float m) { return min(max((int)((f32_as_u32(m) >> 23) & 255u) - 140, 0), 100); }
 __device__ __forceinline__ float pow2(int e) { return u32_as_f32((u32)(127 + e) << 23); }
 
+__device__ __forceinline__ u32 bf16_pair(float a, float b) {
+  return (u32)__builtin_bit_cast(u16, (__bf16)a) | ((u32)__builtin_bit_cast(u16, (__bf16)b) << 16);
+}
+// 8 values to element offset e of a bf16 or f32 array
+__device__ __forceinline__ void store8(void *p, int bf, int64_t e, const float (&v)[8]) {
+  if (bf) {
+    *reinterpret_cast<v4u *>(static_cast<u16 *>(p) + e) =
+        v4u{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
+  } else {
+    float *f = static_cast<float *>(p) + e;
+    *reinterpret_cast<v4u *>(f) = v4u{f32_as_u32(v[0]), f32_as_u32(v[1]), f32_as_u32(v[2]), f32_as_u32(v[3])};
+    *reinterpret_cast<v4u *>(f + 4) = v4u{f32_as_u32(v[4]), f32_as_u32(v[5]), f32_as_u32(v[6]), f32_as_u32(v[7])};
+  }
+}
+
 // v over the row's L lanes (a power of two): a butterfly in the wave, then the waves in order through LDS
 template <int L, bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float *part) {

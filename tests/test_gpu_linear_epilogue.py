@@ -175,3 +175,34 @@ def test_padding_tiles_and_neighbour_rows(dev):
         guard = torch.full((T * n + 64,), 3.0, device=dev)
         ops.linear(fmt, x, w.w, n, k, bias=b, y=guard[:T * n].view(T, n))
         assert (guard[T * n:] == 3).all()
+
+
+@pytest.mark.parametrize("fmt,T,n,k", [("q4_k", 64, 136, 4096), ("q4_k", 333, 4096, 256), ("q4_k", 100, 300, 256), ("q4_kt", 130, 144, 1024),
+                                       ("q6_k", 513, 2104, 256), ("q6_k", 70, 96, 4096), ("q4_0", 200, 264, 512), ("q6_k", 1500, 4104, 256),
+                                       ("q4_k", 1300, 4104, 512)])
+def test_rows_at_any_address(dev, fmt, T, n, k):
+    """Rows of y, the residual and dy that do not start on 16 bytes take the same values as rows that do."""
+    import qmm.ops as ops
+    rng = np.random.default_rng(T + n)
+    w, u, b = Weight(fmt, rng, n, k, dev), Weight(fmt, rng, n, k, dev), vec(rng, n, dev)
+    x, s = ops.row_scale_f16(rows(rng, (T, k), torch.float32, dev))
+
+    def at(off, t):
+        buf = torch.full((T * n + 64,), 3.0, dtype=t.dtype, device=dev)
+        buf[off:off + T * n] = t.reshape(-1)
+        return buf, buf[off:off + T * n].view(T, n)
+
+    for dt in (torch.float32, torch.bfloat16):
+        res, dy = rows(rng, (T, n), dt, dev), rows(rng, (T, n), dt, dev, 1e-3)
+        want = ops.linear(fmt, x, w.w, n, k, scales=s, bias=b, residual=res, act="silu", out_dtype=dt)
+        gated = ops.ffn_gate_up(fmt, x, w.w, u.w, n, k, scales=s, bias=b, act="gelu", out_dtype=dt)
+        grads = ops.ffn_gate_up_backward(fmt, x, w.w, u.w, dy, n, k, scales=s, bias=b)
+        for off in (0, 1, 2, 8):
+            buf, y = at(off, torch.zeros_like(res))
+            ops.linear(fmt, x, w.w, n, k, scales=s, bias=b, residual=at(8 - off, res)[1], act="silu", y=y)
+            assert torch.equal(y, want) and (buf[:off] == 3).all() and (buf[off + T * n:] == 3).all(), off
+            buf, y = at(off, torch.zeros_like(res))
+            ops.ffn_gate_up(fmt, x, w.w, u.w, n, k, scales=s, bias=b, act="gelu", y=y)
+            assert torch.equal(y, gated) and (buf[:off] == 3).all() and (buf[off + T * n:] == 3).all(), off
+            got = ops.ffn_gate_up_backward(fmt, x, w.w, u.w, at(off, dy)[1], n, k, scales=s, bias=b)
+            assert all(torch.equal(p, q) for p, q in zip(got, grads)), off
