@@ -82,6 +82,8 @@ struct Raw<kQ40> {   // two blocks' 16 code bytes and d
 
 constexpr bool two_matrices(int kind) { return kind == kTGU || kind == kTSwiglu || kind == kTGlu || kind == kTGluGrad; }
 constexpr bool dense_rows(int kind) { return kind != kTGU && kind != kTDN; }
+constexpr bool epilogue_kind(int kind) { return kind == kTLinear || kind == kTGlu || kind == kTGluGrad; }
+__host__ __device__ constexpr bool ragged_last(int m, int bm) { return m % bm > 0 && m % bm <= bm / 2; }
 constexpr int raw_of(int wf) { return wf == kQ4KT ? kQ4K : wf; }
 constexpr int64_t row_bytes_of(int wf, int64_t k) {
   return wf == kQ40 ? k / 32 * 18 : k / 256 * (wf == kQ6K ? 210 : 144);
@@ -305,12 +307,24 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
     // XCD-aware order: workgroup b runs on XCD b % 8, which gets a contiguous range of tiles in groups of kGroupM row
     // tiles (rows fastest inside a group), so that the tiles of an XCD at a time share activation rows and weight
     // columns in its L2
-    const int per = (int)(gridDim.x / 8);
-    const int t = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-    if (t >= a.tiles_m * a.tiles_n) return;
-    const int g = t / (kGroupM * a.tiles_n), gm = min(kGroupM, a.tiles_m - g * kGroupM), gt = t - g * kGroupM * a.tiles_n;
-    m0 = (g * kGroupM + gt % gm) * BM;
-    n0 = gt / gm * BN;
+    const int xcd = (int)(blockIdx.x % 8), x = (int)(blockIdx.x / 8);
+    // A last row tile of at most half its rows takes about half the time of the others: with an epilogue its column blocks
+    // run after all of theirs, in a range of their own per XCD, where they fill the last round (12288 x 4096 gate / up of
+    // Q4_K at 700 and 1060 rows 162 and 224 -> 155 and 214 us).
+    const bool ragged = epilogue_kind(KIND) && ragged_last(M, BM);
+    const int fm = a.tiles_m - (ragged ? 1 : 0), full = fm * a.tiles_n, per = (full + 7) / 8;
+    if (x < per) {
+      const int t = xcd * per + x;
+      if (t >= full) return;
+      const int g = t / (kGroupM * a.tiles_n), gm = min(kGroupM, fm - g * kGroupM), gt = t - g * kGroupM * a.tiles_n;
+      m0 = (g * kGroupM + gt % gm) * BM;
+      n0 = gt / gm * BN;
+    } else {
+      const int share = (a.tiles_n + 7) / 8, cb = xcd * share + (x - per);
+      if (!ragged || x - per >= share || cb >= a.tiles_n) return;
+      m0 = fm * BM;
+      n0 = cb * BN;
+    }
   } else {
     // expert tiles dealt to the XCDs round-robin: the bucket writes the live tiles first, so a contiguous range per
     // XCD would leave the XCDs holding the trailing unused tiles idle; a tile's column blocks share one XCD's L2
@@ -547,7 +561,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
   }
 
   // ---- epilogue: accumulator register r of a block is row 8 (r / 4) + 4 h + r % 4, column lc
-  if constexpr (KIND == kTLinear || KIND == kTGlu || KIND == kTGluGrad) {
+  if constexpr (epilogue_kind(KIND)) {
     // The values a 32-row block reads (residual, dy) are loaded before its first store: the compiler cannot move a load
     // over a store that might alias it, and a round trip a value would cost more than the tile's MFMAs
     constexpr int NC = kTwoW ? 1 : 2;
@@ -729,7 +743,8 @@ int launch(TileArgs a, hipStream_t s) {
   if constexpr (kDenseRows) a.tiles_m = (a.M + BM - 1) / BM;   // grouped: the caller's 64-row expert tiles
   a.tiles_n = (a.N + BN - 1) / BN;
   const int64_t tiles = kDenseRows ? (int64_t)a.tiles_m * a.tiles_n : (int64_t)((a.tiles_m + 7) / 8) * 8 * a.tiles_n;
-  const dim3 grid((unsigned)(8 * ((tiles + 7) / 8)));
+  const bool ragged = epilogue_kind(KIND) && ragged_last(a.M, BM);   // two ranges an XCD
+  const dim3 grid((unsigned)(8 * (ragged ? (tiles - a.tiles_n + 7) / 8 + (a.tiles_n + 7) / 8 : (tiles + 7) / 8)));
   static std::atomic<unsigned> raised{0};
   const void *fn = reinterpret_cast<const void *>(&gemm_tile_kernel<WF, KIND, BM, NW, KS>);
   if (int st = raise_dyn_lds(fn, kLds, raised)) return st;

@@ -485,12 +485,17 @@ int launch_t(const MArgs &a, const Epi &ep, hipStream_t s) {
 }
 template <class F, int XT, int NM>
 int launch(const MArgs &a, const Epi &ep, hipStream_t s) {
-  // two row tiles of one matrix share a wave's activations where that leaves two workgroups a CU; two token tiles share its
-  // unpacked weights past 16 tokens
+  // Two row tiles of one matrix share a wave's activations where that leaves two workgroups a CU, or where an XCD's 32 CUs
+  // take them in one round and single tiles in more (f32 and Q8_1 rows, whose operands are made from the loaded values: f32
+  // rows, five tokens, Q4_0 6144 x 2048 8.8 -> 7.4 us, 8192 x 8192 24.9 -> 21.0, Q6_K 40.3 -> 32.9; Q8_1 33 tokens Q4_0
+  // 2720 x 8192 32.1 -> 21.7; bf16 rows 5.7 and 5.6, 13.1 and 13.5, 20.7 and 22.5). Two token tiles share its unpacked
+  // weights past 16 tokens.
   constexpr int kMost = NM == 2 ? 1 : 2, TT = XT == kXF32 ? 1 : 2;
   const bool wide = a.tokens > 16;
   const int tiles = wide ? (a.tokens + 16 * TT - 1) / (16 * TT) : 1;
-  if ((int64_t)((a.n + 31) / 32) * tiles >= 512)
+  auto round = [&](int rows) { return ((a.n + rows - 1) / rows + 7) / 8 * tiles; };   // workgroups of an XCD
+  const bool one_round = XT != kXBF16 && round(16) > 32 && round(32) <= 32;
+  if (one_round || (int64_t)((a.n + 31) / 32) * tiles >= 512)
     return wide ? launch_t<F, XT, kMost, NM, TT>(a, ep, s) : launch_t<F, XT, kMost, NM, 1>(a, ep, s);
   return wide ? launch_t<F, XT, 1, NM, TT>(a, ep, s) : launch_t<F, XT, 1, NM, 1>(a, ep, s);
 }
