@@ -205,8 +205,9 @@ int qmm_rms_norm(int64_t rows, int64_t k, const void *x, int x_dtype, const void
  *   QMM_MXFP8           qmm_gemm_mxfp4, x_scales E8M0 [tokens, k/32]
  * The sum has that product's bits, except for a few rows (F32, BF16, Q8) of QMM_Q4_0, QMM_Q4_K, QMM_Q6_K, QMM_MXFP4 or
  * QMM_MXFP4S weights with K % 64 == 0, whose exact products are added in another f32 order (from two rows on; by format and
- * operand, from one to five). Among those calls a row's bits do not depend on the rows beside it; an f32 row that holds an
- * infinity gives NaN or infinities.
+ * operand, from one to five), and QMM_F16 calls on QMM_Q4_K / QMM_Q4_KT weights that are one round of workgroups, whose K
+ * is cut into other parts. Among the few-row calls a row's bits do not depend on the rows beside it; an f32 row that holds
+ * an infinity gives NaN or infinities.
  * ws: the weights' scale plane for QMM_MXFP4S / QMM_MXFP4T, else NULL. */
 int qmm_linear(int fmt, int act, int64_t tokens, int64_t k, int64_t n, const void *x, int x_dtype, const void *x_scales,
                const void *w, const void *ws, const float *bias, const void *residual, int res_dtype, void *y, int y_dtype,

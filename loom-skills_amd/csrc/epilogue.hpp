@@ -79,6 +79,11 @@ __device__ __forceinline__ void store_vals(void *p, int bf16, int64_t o, const f
   }
 }
 
+// whether the rows of y and the residual start on 16 bytes
+__device__ __forceinline__ bool ep_wide(const Epi &e, int n) {
+  return n % 8 == 0 && ((reinterpret_cast<uintptr_t>(e.y) | reinterpret_cast<uintptr_t>(e.res)) & 15) == 0;
+}
+
 // output o = row n + c of a one-matrix product
 __device__ __forceinline__ void epi_store(const Epi &e, int64_t o, int64_t c, float v) {
   if (e.bias) v += e.bias[c];

@@ -335,6 +335,24 @@ __global__ __launch_bounds__(kWaves * 64, 1) void q4k_dense_kernel(DArgs a, EP e
   auto red_at = [&](int sl, int i, int j, int r) -> float & {
     return red[(sl * kBM + 32 * i + 8 * (r >> 2) + 4 * h + (r & 3)) * kRp + 32 * j + lc];
   };
+  // An epilogue's bias and residual values of the thread's four rows of eight columns are loaded here, all at once, and used
+  // after the exchange (loaded in each of the four passes below they were a round trip each: 4096 x 4096 at 64 rows 28 us,
+  // the plain call 21)
+  float eb[8];
+  u32x4 er[4][2];
+  if constexpr (kEpi<EP>) {
+    const int lc8 = n0 + (tid & 15) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) eb[e] = epi_bias(ep.bias, min(lc8 + e, N - 1));
+    if (ep.res && ep_wide(ep, N)) {
+#pragma unroll
+      for (int pass = 0; pass < 4; ++pass) {
+        const int64_t o = (int64_t)min(m0 + 16 * pass + (tid >> 4), M - 1) * N + min(lc8, N - 8);
+        er[pass][0] = *reinterpret_cast<const u32x4 *>(static_cast<const u8 *>(ep.res) + o * (ep.res_bf16 ? 2 : 4));
+        if (!ep.res_bf16) er[pass][1] = *reinterpret_cast<const u32x4 *>(static_cast<const float *>(ep.res) + o + 4);
+      }
+    }
+  }
   if (wave >= 2) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -374,28 +392,29 @@ __global__ __launch_bounds__(kWaves * 64, 1) void q4k_dense_kernel(DArgs a, EP e
     }
     const int64_t o = (int64_t)row * N + col;
     if constexpr (kEpi<EP>) {   // eight columns of a row: their bias and residual values, then the stores
-      float b[8], r[8];
-      if (N % 8 == 0 && ((reinterpret_cast<uintptr_t>(ep.y) | reinterpret_cast<uintptr_t>(ep.res)) & 15) == 0) {
+      if (ep_wide(ep, N)) {
+        auto act = [&](auto a) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) b[e] = epi_bias(ep.bias, col + e);
-        if (ep.res) load_vals<8>(ep.res, ep.res_bf16, o, r);
+          for (int e = 0; e < 8; ++e) v[e] = act1(a, v[e] + eb[e]);
+        };
+        if (ep.act == QMM_ACT_NONE) act(std::integral_constant<int, QMM_ACT_NONE>{});
+        else act(ep.act);
+        if (ep.res) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] = act1(ep.act, v[e] + b[e]);
-          if (ep.res) v[e] += r[e];
+          for (int e = 0; e < 8; ++e) {
+            const u32 w = er[pass][ep.res_bf16 ? 0 : e >> 2][ep.res_bf16 ? e >> 1 : e & 3];
+            v[e] += u32_as_f32(!ep.res_bf16 ? w : e & 1 ? w & 0xFFFF0000u : w << 16);
+          }
         }
         store_vals<8>(ep.y, ep.y_bf16, o, v);
-        continue;
-      }
+      } else {
+        float r[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool in = col + e < N;
-        b[e] = in ? epi_bias(ep.bias, col + e) : 0.f;
-        r[e] = in && ep.res ? load_val(ep.res, ep.res_bf16, o + e) : 0.f;
-      }
+        for (int e = 0; e < 8; ++e) r[e] = ep.res && col + e < N ? load_val(ep.res, ep.res_bf16, o + e) : 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (col + e < N) epi_put(ep, ep.act, o + e, v[e] + b[e], r[e]);
+        for (int e = 0; e < 8; ++e)
+          if (col + e < N) epi_put(ep, ep.act, o + e, v[e] + eb[e], r[e]);
+      }
     } else if (vec && col + 8 <= N) {
       if constexpr (BF16OUT) {
         typedef __attribute__((ext_vector_type(2))) __bf16 bf2;

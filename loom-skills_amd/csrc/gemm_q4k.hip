@@ -483,7 +483,15 @@ int qmm_gemm_epi(int fmt, int kind, int64_t rows, int64_t k, int64_t n, const vo
   if (!aligned(x, 16) || !aligned(scales, 4) || !aligned(w, wal) || !aligned(w2, wal)) return QMM_ERR_ALIGN;
   // activation rows and weight rows are addressed by 32-bit buffer offsets
   if (rows * k * 2 >= (1ll << 31) || n * fmt_row_bytes(fmt, k) >= (1ll << 31)) return QMM_ERR_SHAPE;
-  const int shape = tile_shape(two, fmt == QMM_Q4_K || tiled, rows, n, k);
+  int shape = tile_shape(two, fmt == QMM_Q4_K || tiled, rows, n, k);
+  // A workgroup of four waves on 64 x 64 outputs where those take the chip once: a wave a SIMD (Q6_K 4096 x 4096 at 64 rows
+  // 28 -> 21 us, 4096 x 12288 75 -> 55, 2 x 768 x 2048 of Q4_0 18.5 -> 13.8; Q4_K, one matrix, against the dense kernel:
+  // 4096 x 4096 at 64 rows 23.0 -> 17.9, 4096 x 12288 55 -> 52, 768 x 2048 16 -> 12). The dense kernel's exchange costs it
+  // one round of a short K (4096 x 1024 at 512 rows 16.8, here 12.3; 768 x 2048 at 2048 rows 19.6, 16.1; 4096 x 4096 at 512
+  // rows 26.6, 29.0).
+  const int64_t m64 = (rows + 63) / 64, cols = two ? 2 * n : n;
+  if (shape == kDenseKernel && k <= 2048 && m64 * ((cols + 127) / 128) <= 256) shape = kT64x2x4;
+  if ((shape == kT64x2x4 || shape == kDenseKernel) && m64 * ((cols + 63) / 64) <= 256) shape = kT64x1x4;
   if (shape == kDenseKernel) return qmm_gemm_q4k_dense(0, tiled, rows, k, n, x, scales, w, nullptr, 0, s, &ep);
   TileArgs t{};
   t.M = (int)rows; t.N = (int)n; t.K = (int)k;

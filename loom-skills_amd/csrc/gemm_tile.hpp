@@ -11,7 +11,7 @@ namespace qmm {
 // bias) (X Wu^T inv + bias2); kTGluGrad: the gradients of that product at dy, bf16 [M, 2, N]
 enum TileKind { kTDense = 0, kTSwiglu = 1, kTGU = 2, kTDN = 3, kTLinear = 4, kTGlu = 5, kTGluGrad = 6 };
 // the workgroup: rows x waves along N x K-parts (a wave holds 64 weight columns)
-enum TileShape { kT128x4x1 = 0, kT128x4x2 = 1, kT64x4x1 = 2, kT64x2x4 = 3 };
+enum TileShape { kT128x4x1 = 0, kT128x4x2 = 1, kT64x4x1 = 2, kT64x2x4 = 3, kT64x1x4 = 4 };
 
 struct TileArgs {
   int M, N, K;                 // dense: rows; grouped: rows of the sorted output (max_tiles * 64)

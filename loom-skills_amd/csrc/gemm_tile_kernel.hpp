@@ -757,6 +757,9 @@ int dispatch_dense(int shape, const TileArgs &a, hipStream_t s) {
   if (shape == kT128x4x1) return launch<WF, KIND, 128, 4, 1>(a, s);
   if (shape == kT128x4x2) return launch<WF, KIND, 128, 4, 2>(a, s);
   if (shape == kT64x4x1) return launch<WF, KIND, 64, 4, 1>(a, s);
+  if constexpr (epilogue_kind(KIND)) {
+    if (shape == kT64x1x4) return launch<WF, KIND, 64, 1, 4>(a, s);
+  }
   return launch<WF, KIND, 64, 2, 4>(a, s);
 }
 

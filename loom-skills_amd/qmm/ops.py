@@ -886,9 +886,8 @@ def linear(fmt, x, w, n, k, y=None, mode="store", ws=None, w2=None, ws2=None, q8
     [tokens, n], y itself allowed), out_dtype (f32 / bf16), scales or tokens, or a bf16 y, the call is
     y = act(x W^T + bias) + residual (qmm_linear, mode "store"). x may then also be an operand: a planar Q8_1 buffer with
     tokens, the row-scaled f16 rows or E4M3 codes with their scales; the operand chooses the product whatever the token
-    count. GGUF mxfp4 blocks take up to 63 rows (repack_mxfp4 for more). The f16 and MXFP8 products, the tiled formats
-    and most single tokens have the plain call's bits before the epilogue; a few rows of Q4_0, Q4_K, Q6_K and MXFP4 add
-    the same exact products in another order (f32 sums)."""
+    count. GGUF mxfp4 blocks take up to 63 rows (repack_mxfp4 for more). The sums are those of the plain call, in some
+    shapes added in another f32 order (qmm_linear). y may be the residual; it may overlap no other argument."""
     if bias is not None or act != "none" or residual is not None or out_dtype is not None or scales is not None or \
             tokens is not None or (y is not None and y.dtype == torch.bfloat16):
         if mode != "store" or w2 is not None or ws2 is not None:
