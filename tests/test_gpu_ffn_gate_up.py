@@ -190,3 +190,20 @@ def test_grad_operand(dev):
         assert torch.equal(x16[..., :n], (x * s[:, :1, None]).half())
         m = (x.abs().amax((1, 2)) * s[:, 0])[1:5]
         assert ((m >= 2.0 ** 13) & (m < 2.0 ** 14)).all() and s[5, 0] == 1
+
+
+@pytest.mark.parametrize("parts,n,dtype", [(2, 12288, torch.bfloat16), (2, 20000, torch.bfloat16), (1, 32768, torch.float32), (2, 40000, torch.bfloat16),
+                                           (2, 264, torch.bfloat16), (2, 2056, torch.float32)])
+def test_grad_operand_of_long_rows(dev, parts, n, dtype):
+    import qmm.ops as ops
+    from qmm import _lib
+    T, N = 3, -(-n // 64) * 64
+    x = rows(np.random.default_rng(n), (T, parts, n), dtype, dev, 1e-3)
+    x[1, parts - 1, n - 1] = 5.0    # a row's largest value is its last
+    x[2, 0, 0] = float("nan")
+    x16 = torch.full((T, parts, N), 9.0, dtype=torch.float16, device=dev)
+    s = torch.empty((T, 2), device=dev)
+    _lib.call("qmm_grad_operand", T, parts, n, x.data_ptr(), ops._dt(x), x16.data_ptr(), s.data_ptr(), ops._stream())
+    assert (x16[..., n:] == 0).all()
+    assert torch.equal(x16[:2, :, :n], (x.float() * s[:, :1, None]).half()[:2])
+    assert x16[2, 0, 0].isnan() and x16[2, :, :n].isnan().sum() == 1 and s[1].tolist() == [2.0 ** 11, 2.0 ** -11]
