@@ -740,18 +740,13 @@ LINEAR_Q8_FORMATS = ("q4_0", "q4_k", "q4_kt", "q6_k", "q4_0t", "mxfp4s")
 
 
 def _here(*ts):
-    """The current stream of the device that holds the tensors (_dev's checks), which must be the current one: the kernels
-    are launched on its stream."""
-    dev = None
+    """The current stream of the device that holds the tensors (_dev's checks; the first is given), which must be the current
+    one: the kernels are launched on its stream."""
+    dev = ts[0].get_device()
     for t in ts:
-        if t is not None:
-            d = t.get_device()
-            if d < 0 or not t.is_contiguous():
-                _dev(t)
-            if dev is None:
-                dev = d
-            elif d != dev:
-                raise ValueError(f"tensors are on cuda:{dev} and cuda:{d}")
+        if t is not None and (t.get_device() != dev or dev < 0 or not t.is_contiguous()):
+            _dev(*ts)
+            raise ValueError(f"tensors are on cuda:{dev} and {t.device}")
     if dev != torch._C._cuda_getDevice():
         raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
     return torch._C._cuda_getCurrentRawStream(dev)
@@ -768,11 +763,11 @@ _VALUE = (torch.float32, torch.bfloat16)   # the types of rows that epilogues re
 
 def _weight_bytes(fmt, w, ws, n, k, what="w"):
     """The kernels cannot see sizes: a weight tensor too small for [n, k] would be read past its end."""
-    if w is None or w.numel() * w.element_size() < n * row_bytes(fmt, k):
+    if w is None or w.nbytes < n * row_bytes(fmt, k):
         raise ValueError(f"{what} is too small for {fmt} [{n}, {k}] ({n * row_bytes(fmt, k)} bytes)")
     if fmt in SPLIT:
         need = n * (k // MX_BLOCK) if fmt == "mxfp4s" else -(-n // 32) * ((k + 255) // 256) * 256
-        if ws is None or ws.numel() * ws.element_size() < need:
+        if ws is None or ws.nbytes < need:
             raise ValueError(f"{fmt} weights need their E8M0 scale planes ({need} bytes)")
     elif ws is not None:
         raise ValueError(f"{fmt} weights have no scale planes")
@@ -844,30 +839,34 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out="bf16", h=None):
     s = _here(x, weight, residual, h)
     if x.dim() != 2:
         raise ValueError(f"x is {tuple(x.shape)}, expected [rows, k]")
-    rows, k = x.shape
-    _shaped(x, (rows, k), _VALUE, "x")
+    rows, k = shape = x.shape
+    _shaped(x, shape, _VALUE, "x")
     _shaped(weight, (k,), _VALUE, "weight")
-    _shaped(residual, (rows, k), _VALUE, "residual")
     if residual is not None:
-        h = torch.empty_like(residual) if h is None else h
-        _shaped(h, (rows, k), (residual.dtype,), "h")
+        _shaped(residual, shape, _VALUE, "residual")
+        if h is None:
+            h = torch.empty_like(residual)
+        else:
+            _shaped(h, shape, (residual.dtype,), "h")
     elif h is not None:
         raise ValueError("h is written with a residual")
     scales = None
     if out in ("bf16", "f32"):
-        y = x.new_empty((rows, k), dtype=torch.bfloat16 if out == "bf16" else torch.float32)
+        dtype = torch.bfloat16 if out == "bf16" else torch.float32
+        y = torch.empty_like(x) if x.dtype == dtype else x.new_empty(shape, dtype=dtype)
     elif out == "f16":
-        y = x.new_empty((rows, k), dtype=torch.float16)
+        y = x.new_empty(shape, dtype=torch.float16)
         scales = x.new_empty((rows, 2), dtype=torch.float32)
     elif out == "q8":
         y = x.new_empty(q8_bytes(rows, k), dtype=torch.uint8)
     elif out == "mxfp8":
-        y = x.new_empty((rows, k), dtype=torch.uint8)
+        y = x.new_empty(shape, dtype=torch.uint8)
         scales = x.new_empty((rows, k // MX_BLOCK), dtype=torch.uint8)
     else:
         raise ValueError(f"out {out!r} is none of bf16, f32, f16, q8, mxfp8")
-    _lib.call("qmm_rms_norm", rows, k, _ptr(x), _dt(x), _ptr(residual), 0 if residual is None else _dt(residual),
-              _ptr(weight), _dt(weight), eps, _ptr(h), DTYPE[out], _ptr(y), _ptr(scales), s)
+    _lib.call("qmm_rms_norm", rows, k, x.data_ptr(), _DT[x.dtype], None if residual is None else residual.data_ptr(),
+              0 if residual is None else _DT[residual.dtype], weight.data_ptr(), _DT[weight.dtype], eps,
+              None if h is None else h.data_ptr(), DTYPE[out], y.data_ptr(), None if scales is None else scales.data_ptr(), s)
     return y, scales, h
 
 
@@ -920,22 +919,26 @@ def _linear_epilogue(fmt, x, w, n, k, y, ws, q8, bias, act, residual, out_dtype,
     code = _act_code(act, EPILOGUE_ACT)
     _weight_bytes(fmt, w, ws, n, k)
     T = x.shape[0] if tokens is None else tokens
-    _shaped(bias, (n,), (torch.float32,), "bias")
-    _shaped(residual, (T, n), _VALUE, "residual")
-    y = _rows_out(y, (T, n), out_dtype, x)
+    if bias is not None:
+        _shaped(bias, (n,), (torch.float32,), "bias")
+    if residual is not None:
+        _shaped(residual, (T, n), _VALUE, "residual")
+    y = _rows_out(y, (T, n), out_dtype, x, residual)
     x, xd, scales = _product_operand(fmt, x, k, scales, tokens, q8)
-    _lib.call("qmm_linear", CODE[fmt], code, T, k, n, _ptr(x), xd, _ptr(scales), _ptr(w), _ptr(ws), _ptr(bias),
-              _ptr(residual), 0 if residual is None else _dt(residual), _ptr(y), _dt(y), s)
+    _lib.call("qmm_linear", CODE[fmt], code, T, k, n, x.data_ptr(), xd, None if scales is None else scales.data_ptr(),
+              w.data_ptr(), None if ws is None else ws.data_ptr(), None if bias is None else bias.data_ptr(),
+              None if residual is None else residual.data_ptr(), 0 if residual is None else _DT[residual.dtype],
+              y.data_ptr(), _DT[y.dtype], s)
     return y
 
 
-def _rows_out(y, shape, out_dtype, like):
-    """The f32 / bf16 output rows: y, or a new tensor of out_dtype (f32 when None)."""
+def _rows_out(y, shape, out_dtype, x, like=None):
+    """The f32 / bf16 output rows: y, or a new tensor of out_dtype (f32 when None); like: a tensor of that shape or None."""
     if y is None:
-        y = like.new_empty(shape, dtype=torch.float32 if out_dtype is None else out_dtype)
-        if y.dtype not in _VALUE:
+        dtype = torch.float32 if out_dtype is None else out_dtype
+        if dtype not in _VALUE:
             raise ValueError(f"out_dtype is float32 or bfloat16, not {out_dtype}")
-        return y
+        return torch.empty_like(like) if like is not None and like.dtype == dtype else x.new_empty(shape, dtype=dtype)
     if out_dtype is not None and y.dtype != out_dtype:
         raise ValueError(f"y is {y.dtype}, out_dtype {out_dtype}")
     _shaped(y, shape, _VALUE, "y")
@@ -952,12 +955,16 @@ def ffn_gate_up(fmt, x, w, w2, n, k, y=None, ws=None, ws2=None, q8="auto", bias=
     _weight_bytes(fmt, w, ws, n, k)
     _weight_bytes(fmt, w2, ws2, n, k, "w2")
     T = x.shape[0] if tokens is None else tokens
-    _shaped(bias, (n,), (torch.float32,), "bias")
-    _shaped(bias2, (n,), (torch.float32,), "bias2")
+    if bias is not None:
+        _shaped(bias, (n,), (torch.float32,), "bias")
+    if bias2 is not None:
+        _shaped(bias2, (n,), (torch.float32,), "bias2")
     y = _rows_out(y, (T, n), out_dtype, x)
     x, xd, scales = _product_operand(fmt, x, k, scales, tokens, q8)
-    _lib.call("qmm_ffn_gate_up", CODE[fmt], code, T, k, n, _ptr(x), xd, _ptr(scales), _ptr(w), _ptr(ws), _ptr(w2), _ptr(ws2),
-              _ptr(bias), _ptr(bias2), _ptr(y), _dt(y), s)
+    _lib.call("qmm_ffn_gate_up", CODE[fmt], code, T, k, n, x.data_ptr(), xd, None if scales is None else scales.data_ptr(),
+              w.data_ptr(), None if ws is None else ws.data_ptr(), w2.data_ptr(), None if ws2 is None else ws2.data_ptr(),
+              None if bias is None else bias.data_ptr(), None if bias2 is None else bias2.data_ptr(), y.data_ptr(),
+              _DT[y.dtype], s)
     return y
 
 
