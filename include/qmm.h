@@ -194,6 +194,19 @@ int qmm_rms_norm(int64_t rows, int64_t k, const void *x, int x_dtype, const void
                  const void *weight, int w_dtype, float eps, void *h, int out_dtype, void *out, void *out_scales,
                  qmm_stream_t stream);
 
+/* The backward pass of qmm_rms_norm at h (its h, or x without a residual) and the gradients dy of y and dh of h (NULL: none):
+ *   dx[t, c] = dh[t, c] + r[t] (weight[c] dy[t, c] - hn[t, c] mean_c(weight dy hn)),   hn = h r,  r = 1 / sqrt(mean(h^2) + eps)
+ *   dweight[c] = sum_t dy[t, c] hn[t, c]
+ * dx is the gradient of x and of residual alike. h, dy, dh, dx: [rows, k], weight [k], each f32 or bf16 (dx rounded once, to
+ * nearest even), aligned to their elements; dx may be dh itself where the types agree, and overlaps nothing else. dweight: f32
+ * [k] or NULL; with it a workspace of qmm_rms_norm_grad_workspace_size bytes, 16-byte aligned, one for each call that
+ * overlaps. Rows and k as qmm_rms_norm. Sums are f32, in an order that follows from the shape and alignment. */
+int qmm_rms_norm_grad(int64_t rows, int64_t k, const void *h, int h_dtype, const void *weight, int w_dtype, float eps,
+                      const void *dy, int dy_dtype, const void *dh, int dh_dtype, void *dx, int dx_dtype, float *dweight,
+                      void *workspace, int64_t workspace_bytes, qmm_stream_t stream);
+/* Workspace bytes of qmm_rms_norm_grad with dweight, or -1 for a shape it refuses. */
+int64_t qmm_rms_norm_grad_workspace_size(int64_t rows, int64_t k);
+
 /* Product with a bias, an activation and a residual in its epilogue (the reference adds them in kernels of their own):
  *   y[t, r] = act(sum_k x[t, k] W[r, k] + bias[r]) + residual[t, r]
  * act: QMM_ACT_NONE, RELU, SILU, SIGMOID, GELU or GELU_ERF. bias f32 [n] or NULL; residual [tokens, n] f32 or bf16 or NULL,

@@ -15,8 +15,18 @@
 // 16, 32 or 64 lanes of a wave (up to 16 rows a workgroup, no barrier), longer ones a workgroup. Four neighbouring lanes
 // hold a 32-value group, so an 8-bit scale is two lane exchanges. 4096 x 4096 bf16 with a residual into f16: 25.6 us for
 // 134 MB, 5.2 TB/s; 65536 x 128 bf16 8.1 us, 4.1 TB/s.
+//
+// The backward pass, with hn = h r the normed row and g = weight dy:
+//
+//   dx = dh + r (g - hn mean_c(g hn));   dweight[c] = sum_rows dy hn
+//
+// the same layout: sum h^2 and sum g h are one exchange, h, dy and dh are read once and dx written once. For dweight a
+// workgroup walks its rows with the column's sum in registers and writes one partial row; a second launch adds the partial
+// rows in a fixed order. HBM is the bound: 4096 x 4096 bf16 rows 26 us for dx (134 MB, 5.2 TB/s), 35 with dweight; 65536 x 128
+// 13.6 and 16.6.
 #include "act_quant.hpp"
 #include "bfly.hpp"
+#include "epilogue.hpp"
 
 using namespace qmm;
 
@@ -239,6 +249,205 @@ int dispatch(const NArgs &a, bool vec, hipStream_t s) {
   return launch<OUT, 1024, 4>(a, s);
 }
 
+// ---- backward
+struct BArgs {
+  int64_t rows, k;
+  const void *h, *weight, *dy, *dh;
+  void *dx;
+  float *part;                 // [workgroups, k] partial dweight rows, or NULL
+  float *rate;                 // rms_norm_grad_long_kernel with part: [rows]
+  float eps;
+  int h_bf16, w_bf16, dy_bf16, dh_bf16, dx_bf16;
+};
+
+// two sums over the row's L lanes
+template <int L>
+__device__ __forceinline__ void row_reduce2(float &u, float &v, float2 *part) {
+  constexpr int W = L < 64 ? L : 64;
+#pragma unroll
+  for (int off = W / 2; off >= 1; off >>= 1) {
+    u += __shfl_xor(u, off, kWave);
+    v += __shfl_xor(v, off, kWave);
+  }
+  if constexpr (L > 64) {
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_float2(u, v);
+    __syncthreads();
+    u = part[0].x;
+    v = part[0].y;
+#pragma unroll
+    for (int i = 1; i < L / 64; ++i) {
+      u += part[i].x;
+      v += part[i].y;
+    }
+  }
+}
+
+// lanes and chunks as rms_norm_kernel; row group g = blockIdx.x, + gridDim.x, ... (DW; without it one group a workgroup)
+template <int L, int J, bool DW>
+__global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_grad_kernel(BArgs a) {
+  constexpr int kRows = L < 256 ? 256 / L : 1;
+  __shared__ float2 part[2][L > 64 ? L / 64 : 1];   // in turn: a wave may still read the last row's
+  const int l = threadIdx.x % L, chunks = (int)(a.k / 8);
+  float w[J][8], acc[DW ? J : 1][8];
+#pragma unroll
+  for (int j = 0; j < J; ++j) load8_act(a.weight, a.w_bf16, 8 * min(l + L * j, chunks - 1), w[j]);
+  if constexpr (DW) {
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[j][i] = 0.f;
+  }
+  const int64_t groups = (a.rows + kRows - 1) / kRows;
+  int turn = 0;
+  for (int64_t g = blockIdx.x; g < groups; g += gridDim.x, turn ^= 1) {
+    const int64_t row_ = g * kRows + threadIdx.x / L;
+    const bool alive = row_ < a.rows;
+    const int64_t r0 = (alive ? row_ : a.rows - 1) * a.k;
+    float h[J][8], d[J][8], e[J][8];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int64_t at = r0 + 8 * min(l + L * j, chunks - 1);
+      load8_act(a.h, a.h_bf16, at, h[j]);
+      load8_act(a.dy, a.dy_bf16, at, d[j]);
+      if (a.dh) load8_act(a.dh, a.dh_bf16, at, e[j]);
+    }
+    float hh = 0.f, gh = 0.f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      float u = 0.f, v = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        u = __builtin_fmaf(h[j][i], h[j][i], u);
+        v = __builtin_fmaf(d[j][i] * w[j][i], h[j][i], v);
+      }
+      hh += l + L * j < chunks ? u : 0.f;
+      gh += l + L * j < chunks ? v : 0.f;
+    }
+    row_reduce2<L>(hh, gh, part[turn]);
+    const float rate = norm_rate(hh, a.k, a.eps), mean = rate * (gh / (float)a.k);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      float o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float hn = h[j][i] * rate;
+        o[i] = rate * __builtin_fmaf(-hn, mean, d[j][i] * w[j][i]);
+        if (a.dh) o[i] += e[j][i];
+        if constexpr (DW) acc[j][i] = alive ? __builtin_fmaf(d[j][i], hn, acc[j][i]) : acc[j][i];
+      }
+      if (alive && l + L * j < chunks) store8(a.dx, a.dx_bf16, r0 + 8 * (l + L * j), o);
+    }
+  }
+  if constexpr (DW) {
+    if constexpr (kRows == 1) {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (l + L * j < chunks) store8(a.part, 0, (int64_t)blockIdx.x * a.k + 8 * (l + L * j), acc[j]);
+    } else {   // the workgroup's rows side by side, added in order
+      static_assert(J == 1, "short rows are one chunk a lane");
+      __shared__ float sums[kRows][8 * L];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sums[threadIdx.x / L][8 * l + i] = acc[0][i];
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.k; c += 256) {
+        float v = sums[0][c];
+#pragma unroll
+        for (int q = 1; q < kRows; ++q) v += sums[q][c];
+        a.part[(int64_t)blockIdx.x * a.k + c] = v;
+      }
+    }
+  }
+}
+
+// Rows of more than 8192 values (V = 8; in registers they spill), any k and alignment (V = 1): a workgroup a row, which is read
+// twice, the second time from L2
+template <int V>
+__global__ __launch_bounds__(512) void rms_norm_grad_long_kernel(BArgs a) {
+  __shared__ float2 part[8];
+  const int64_t r0 = (int64_t)blockIdx.x * a.k;
+  auto load = [](const void *p, int bf, int64_t at, float (&v)[V]) __attribute__((always_inline)) {
+    if constexpr (V == 8) load8_act(p, bf, at, v);
+    else v[0] = load_val(p, bf, at);
+  };
+  float hh = 0.f, gh = 0.f;
+  for (int64_t c = V * threadIdx.x; c < a.k; c += V * 512) {
+    float h[V], d[V], w[V];
+    load(a.h, a.h_bf16, r0 + c, h);
+    load(a.dy, a.dy_bf16, r0 + c, d);
+    load(a.weight, a.w_bf16, c, w);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      hh = __builtin_fmaf(h[i], h[i], hh);
+      gh = __builtin_fmaf(d[i] * w[i], h[i], gh);
+    }
+  }
+  row_reduce2<512>(hh, gh, part);
+  const float rate = norm_rate(hh, a.k, a.eps), mean = rate * (gh / (float)a.k);
+  if (a.part && threadIdx.x == 0) a.rate[blockIdx.x] = rate;
+  for (int64_t c = V * threadIdx.x; c < a.k; c += V * 512) {
+    float h[V], d[V], w[V], e[V];
+    load(a.h, a.h_bf16, r0 + c, h);
+    load(a.dy, a.dy_bf16, r0 + c, d);
+    load(a.weight, a.w_bf16, c, w);
+    if (a.dh) load(a.dh, a.dh_bf16, r0 + c, e);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      d[i] = rate * __builtin_fmaf(-(h[i] * rate), mean, d[i] * w[i]);
+      if (a.dh) d[i] += e[i];
+    }
+    if constexpr (V == 8) store8(a.dx, a.dx_bf16, r0 + c, d);
+    else store_val(a.dx, a.dx_bf16, r0 + c, d[0]);
+  }
+}
+// and its partial dweight rows: 256 columns a workgroup, rows blockIdx.y, + gridDim.y, ...
+__global__ __launch_bounds__(256) void rms_norm_dweight_part_kernel(BArgs a) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.k) return;
+  float v = 0.f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y)
+    v = __builtin_fmaf(load_val(a.dy, a.dy_bf16, row * a.k + c), load_val(a.h, a.h_bf16, row * a.k + c) * a.rate[row], v);
+  a.part[(int64_t)blockIdx.y * a.k + c] = v;
+}
+
+// dweight from n partial rows: 32 columns a workgroup, thread row q adds rows q, q + 32, ...; the 32 sums in order
+__global__ __launch_bounds__(1024) void rms_norm_dweight_kernel(const float *__restrict__ part, int n, int64_t k, float *__restrict__ dw) {
+  __shared__ float sums[32][33];
+  const int x = threadIdx.x & 31, q = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + x;
+  float v = 0.f;
+  if (c < k)
+#pragma unroll 8
+    for (int i = q; i < n; i += 32) v += part[(int64_t)i * k + c];
+  sums[q][x] = v;
+  __syncthreads();
+  if (q == 0 && c < k) {
+#pragma unroll
+    for (int i = 1; i < 32; ++i) v += sums[i][x];
+    dw[c] = v;
+  }
+}
+
+// Partial rows of dweight: enough workgroups to keep their loads in flight, few enough that the partial rows are a small part
+// of the traffic (1024 / 512, us: 16384 x 2048 bf16 55 / 71, 65536 x 128 17 / 19; two chunks a lane 4096 x 4096 36 / 35,
+// 2048 x 8192 44 / 38; long rows 1024 x 12288 64 / 55, 47 with 128)
+constexpr int64_t kParts = 1024, kParts2 = 512, kPartsLong = 128;
+
+template <int L, int J>
+int launch_grad(const BArgs &a, float *dw, hipStream_t s) {
+  constexpr int kRows = L < 256 ? 256 / L : 1, kThreads = L < 256 ? 256 : L;
+  const int64_t groups = (a.rows + kRows - 1) / kRows;
+  if (!dw) {
+    rms_norm_grad_kernel<L, J, false><<<(unsigned)groups, kThreads, 0, s>>>(a);
+    return launch_status();
+  }
+  constexpr int64_t kMost = J == 1 ? kParts : kParts2;
+  const unsigned n = (unsigned)(groups < kMost ? groups : kMost);
+  rms_norm_grad_kernel<L, J, true><<<n, kThreads, 0, s>>>(a);
+  if (int st = launch_status()) return st;
+  rms_norm_dweight_kernel<<<(unsigned)((a.k + 31) / 32), 1024, 0, s>>>(a.part, (int)n, a.k, dw);
+  return launch_status();
+}
+
 }  // namespace
 
 extern "C" int qmm_rms_norm(int64_t rows, int64_t k, const void *x, int x_dtype, const void *residual, int res_dtype,
@@ -267,4 +476,50 @@ extern "C" int qmm_rms_norm(int64_t rows, int64_t k, const void *x, int x_dtype,
     case QMM_Q8: return dispatch<QMM_Q8>(a, vec, s);
     default: return dispatch<QMM_MXFP8>(a, vec, s);
   }
+}
+
+extern "C" int64_t qmm_rms_norm_grad_workspace_size(int64_t rows, int64_t k) {
+  if (rows <= 0 || rows > (1ll << 24) || k <= 0 || k > kMaxK) return -1;
+  return 4 * ((rows < kParts ? rows : kParts) * k + rows);
+}
+
+extern "C" int qmm_rms_norm_grad(int64_t rows, int64_t k, const void *h, int h_dtype, const void *weight, int w_dtype,
+                                 float eps, const void *dy, int dy_dtype, const void *dh, int dh_dtype, void *dx,
+                                 int dx_dtype, float *dweight, void *workspace, int64_t workspace_bytes,
+                                 qmm_stream_t stream) {
+  if (!h || !weight || !dy || !dx) return QMM_ERR_NULL;
+  auto val = [](int d) { return d == QMM_F32 || d == QMM_BF16; };
+  if (!val(h_dtype) || !val(w_dtype) || !val(dy_dtype) || !val(dx_dtype) || (dh && !val(dh_dtype))) return QMM_ERR_DTYPE;
+  if (!(eps >= 0.f)) return QMM_ERR_RANGE;
+  const int64_t need = qmm_rms_norm_grad_workspace_size(rows, k);
+  if (need < 0) return QMM_ERR_SHAPE;
+  auto size = [](int d) { return d == QMM_F32 ? (size_t)4 : (size_t)2; };
+  if (!aligned(h, size(h_dtype)) || !aligned(weight, size(w_dtype)) || !aligned(dy, size(dy_dtype)) ||
+      !aligned(dx, size(dx_dtype)) || (dh && !aligned(dh, size(dh_dtype))) || !aligned(dweight, 4))
+    return QMM_ERR_ALIGN;
+  if (dweight) {
+    if (!workspace || workspace_bytes < need) return QMM_ERR_WORKSPACE;
+    if (!aligned(workspace, 16)) return QMM_ERR_ALIGN;
+  }
+  BArgs a{rows, k, h, weight, dy, dh, dx, dweight ? static_cast<float *>(workspace) : nullptr, nullptr, eps,
+          h_dtype == QMM_BF16, w_dtype == QMM_BF16, dy_dtype == QMM_BF16, dh_dtype == QMM_BF16, dx_dtype == QMM_BF16};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int64_t chunks = k / 8;
+  const bool vec = k % 8 == 0 && aligned(h, 16) && aligned(weight, 16) && aligned(dy, 16) && aligned(dh, 16) && aligned(dx, 16);
+  if (vec && chunks <= 16) return launch_grad<16, 1>(a, dweight, s);
+  if (vec && chunks <= 32) return launch_grad<32, 1>(a, dweight, s);
+  if (vec && chunks <= 64) return launch_grad<64, 1>(a, dweight, s);
+  if (vec && chunks <= 256) return launch_grad<256, 1>(a, dweight, s);
+  if (vec && chunks <= 512) return launch_grad<256, 2>(a, dweight, s);
+  if (vec && chunks <= 1024) return launch_grad<512, 2>(a, dweight, s);
+  const unsigned n = (unsigned)(rows < kPartsLong ? rows : kPartsLong);
+  if (dweight) a.rate = a.part + (int64_t)n * k;
+  if (vec) rms_norm_grad_long_kernel<8><<<(unsigned)rows, 512, 0, s>>>(a);
+  else rms_norm_grad_long_kernel<1><<<(unsigned)rows, 512, 0, s>>>(a);
+  if (int st = launch_status()) return st;
+  if (!dweight) return QMM_OK;
+  rms_norm_dweight_part_kernel<<<dim3((unsigned)((k + 255) / 256), n), 256, 0, s>>>(a);
+  if (int st = launch_status()) return st;
+  rms_norm_dweight_kernel<<<(unsigned)((k + 31) / 32), 1024, 0, s>>>(a.part, (int)n, k, dweight);
+  return launch_status();
 }

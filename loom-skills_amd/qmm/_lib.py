@@ -20,6 +20,9 @@ SIGNATURES = {
     "qmm_mv_q8": [c_int, c_i64, c_i64, c_i64, c_int, c_vp, c_int, c_vp, c_vp, c_vp],
     "qmm_gemm": [c_int, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_int, c_vp],
     "qmm_rms_norm": [c_i64, c_i64, c_vp, c_int, c_vp, c_int, c_vp, c_int, c_float, c_vp, c_int, c_vp, c_vp, c_vp],
+    "qmm_rms_norm_grad": [c_i64, c_i64, c_vp, c_int, c_vp, c_int, c_float, c_vp, c_int, c_vp, c_int, c_vp, c_int, c_vp, c_vp,
+                          c_i64, c_vp],
+    "qmm_rms_norm_grad_workspace_size": [c_i64, c_i64],
     "qmm_linear": [c_int, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_vp],
     "qmm_ffn_gate_up": [c_int, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                         c_int, c_vp],
@@ -78,7 +81,7 @@ SIGNATURES = {
                               c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp],
 }
 RESTYPE = {"qmm_strerror": ctypes.c_char_p, "qmm_row_bytes": c_i64, "qmm_mxfp4t_scale_bytes": c_i64,
-           "qmm_moe_routed_workspace_size": c_i64, "qmm_gemm_t_workspace_size": c_i64}
+           "qmm_moe_routed_workspace_size": c_i64, "qmm_gemm_t_workspace_size": c_i64, "qmm_rms_norm_grad_workspace_size": c_i64}
 
 
 class QmmError(RuntimeError):

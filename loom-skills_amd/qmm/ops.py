@@ -30,6 +30,7 @@ S/ = skills/loom-port-llm/starter/):
 the rest of a dense feed-forward sub-layer around those products, without counterparts as single reference kernels:
 
     rms_norm              residual addition and RMS norm, written as the next product's operand
+    rms_norm_backward     its gradients with respect to x, the residual and the weight
     linear                with bias, activation, residual, bf16 rows (qmm_linear)
     ffn_gate_up           act(x Wg^T + bg) (x Wu^T + bu) with any activation and biases
     ffn_gate_up_backward  its gradients with respect to the projections' outputs and to x (frozen weights)
@@ -868,6 +869,32 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out="bf16", h=None):
               0 if residual is None else _DT[residual.dtype], weight.data_ptr(), _DT[weight.dtype], eps,
               None if h is None else h.data_ptr(), DTYPE[out], y.data_ptr(), None if scales is None else scales.data_ptr(), s)
     return y, scales, h
+
+
+def rms_norm_backward(h, weight, dy, eps=1e-6, dh=None, out_dtype=None, dweight=True, dx=None):
+    """The gradients of rms_norm at its h (x where it had no residual), dy of its normed rows and dh of its h (None: no such
+    gradient): (dx [rows, k], the gradient of x and of the residual; dweight f32 [k], or None with dweight=False)
+    (qmm_rms_norm_grad). h, dy, dh f32 / bf16 [rows, k], weight f32 / bf16 [k]; dx of out_dtype (h's when None), or the
+    caller's rows, dh allowed."""
+    s = _here(h, weight, dy, dh, dx)
+    if h.dim() != 2:
+        raise ValueError(f"h is {tuple(h.shape)}, expected [rows, k]")
+    rows, k = shape = h.shape
+    _shaped(h, shape, _VALUE, "h")
+    _shaped(weight, (k,), _VALUE, "weight")
+    _shaped(dy, shape, _VALUE, "dy")
+    _shaped(dh, shape, _VALUE, "dh")
+    dx = _rows_out(dx, shape, out_dtype if dx is not None or out_dtype is not None else h.dtype, h, h)
+    dw, work, need = None, None, 0
+    if dweight:
+        need = _lib.load().qmm_rms_norm_grad_workspace_size(rows, k)
+        if need < 0:
+            raise ValueError(f"rms_norm does not take {rows} rows of {k} values")
+        dw = torch.empty(k, dtype=torch.float32, device=h.device)
+        work = torch.empty(need, dtype=torch.uint8, device=h.device)
+    _lib.call("qmm_rms_norm_grad", rows, k, _ptr(h), _dt(h), _ptr(weight), _dt(weight), eps, _ptr(dy), _dt(dy), _ptr(dh),
+              0 if dh is None else _dt(dh), _ptr(dx), _dt(dx), _ptr(dw), _ptr(work), need, s)
+    return dx, dw
 
 
 def linear(fmt, x, w, n, k, y=None, mode="store", ws=None, w2=None, ws2=None, q8="auto", bias=None, act="none",

@@ -36,6 +36,29 @@ def test_rms_norm_statuses(lib):   # noqa: F811
         assert call(**bad) == st["QMM_ERR_ALIGN"], bad
 
 
+def test_rms_norm_grad_statuses(lib):   # noqa: F811
+    st = header_enum("qmm_status")
+
+    def call(rows=4, k=64, h=at(), hd=BF16, w=at(), wd=F32, eps=1e-6, dy=at(), yd=BF16, r=None, rd=BF16, o=at(), od=F32, dw=None, ws=None, wb=0):
+        return lib.qmm_rms_norm_grad(rows, k, h, hd, w, wd, ctypes.c_float(eps), dy, yd, r, rd, o, od, dw, ws, wb, None)
+
+    for bad in (dict(h=None), dict(w=None), dict(dy=None), dict(o=None)):
+        assert call(**bad) == st["QMM_ERR_NULL"], bad
+    for bad in (dict(hd=F16), dict(wd=F16), dict(yd=Q8), dict(od=F16), dict(r=at(), rd=F16), dict(od=-1)):
+        assert call(**bad) == st["QMM_ERR_DTYPE"], bad
+    assert call(eps=-1.0) == st["QMM_ERR_RANGE"] and call(eps=float("nan")) == st["QMM_ERR_RANGE"]
+    for bad in (dict(rows=0), dict(rows=(1 << 24) + 1), dict(k=0), dict(k=32769)):
+        assert call(**bad) == st["QMM_ERR_SHAPE"], bad
+        assert lib.qmm_rms_norm_grad_workspace_size(bad.get("rows", 4), bad.get("k", 64)) == -1
+    need = lib.qmm_rms_norm_grad_workspace_size(4, 64)
+    assert need > 0
+    for bad in (dict(h=at(0x10001)), dict(w=at(0x10002)), dict(dy=at(0x10001)), dict(o=at(0x10002)), dict(r=at(0x10001)), dict(dw=at(0x10002), ws=at(), wb=need),
+                dict(dw=at(), ws=at(0x10008), wb=need)):
+        assert call(**bad) == st["QMM_ERR_ALIGN"], bad
+    for bad in (dict(dw=at()), dict(dw=at(), ws=at(), wb=need - 1)):
+        assert call(**bad) == st["QMM_ERR_WORKSPACE"], bad
+
+
 def test_linear_and_gate_up_statuses(lib):   # noqa: F811
     st = header_enum("qmm_status")
 
@@ -134,6 +157,15 @@ def test_rms_norm_errors(ops):
                   ((x, w), dict(residual=x.bfloat16(), h=x)), ((x, w), dict(out="int8")), ((x, w), dict(out=None))):
         with pytest.raises(ValueError):
             ops.rms_norm(*a, **kw)
+
+
+def test_rms_norm_backward_errors(ops):
+    x, w = torch.zeros(4, 64), torch.zeros(64)
+    for a, kw in (((torch.zeros(64), w, x), {}), ((x.half(), w, x), {}), ((x, w[:32], x), {}), ((x, w.half(), x), {}), ((x, w, x[:2]), {}), ((x, w, x.half()), {}),
+                  ((x, w, x), dict(dh=x[:, :32])), ((x, w, x), dict(dh=x.half())), ((x, w, x), dict(out_dtype=torch.float16)), ((x, w, x), dict(dx=x[:2])),
+                  ((x, w, x), dict(dx=x.half())), ((x, w, x), dict(dx=torch.zeros(4, 64), out_dtype=torch.bfloat16))):
+        with pytest.raises(ValueError):
+            ops.rms_norm_backward(*a, **kw)
 
 
 def test_linear_errors(ops):
