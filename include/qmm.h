@@ -226,6 +226,15 @@ int qmm_linear(int fmt, int act, int64_t tokens, int64_t k, int64_t n, const voi
                const void *w, const void *ws, const float *bias, const void *residual, int res_dtype, void *y, int y_dtype,
                qmm_stream_t stream);
 
+/* The backward pass of qmm_linear with frozen weights, first half: the gradient of the activation's argument,
+ *   dpre[t, r] = dy[t, r] act'(sum_k x[t, k] W[r, k] + bias[r])
+ * with the argument computed again from x as the QMM_F16 call computes it (fmt QMM_Q4_K, QMM_Q4_KT, QMM_Q6_K or QMM_Q4_0;
+ * QMM_ACT_NONE needs no call: dpre is dy). dy: [tokens, n] f32 or bf16; dpre: bf16 [tokens, n], rounded once; the residual's
+ * gradient is dy, the bias's the columns' sums of dpre, and x's qmm_gemm_t of dpre. relu's slope at 0 is 0. Rows of a padding
+ * tile are not written. */
+int qmm_linear_grad(int fmt, int act, int64_t tokens, int64_t k, int64_t n, const void *x, const float *x_scales,
+                    const void *w, const float *bias, const void *dy, int dy_dtype, void *dpre, qmm_stream_t stream);
+
 /* The gated feed-forward block's first half in one kernel: both projections, their biases, the activation, the product
  *   y[t, r] = act(g) u,   g = sum_k x[t, k] W[r, k] + bias[r],   u = sum_k x[t, k] W2[r, k] + bias2[r]
  * act: any of enum qmm_act (QMM_ACT_SWIGLU_OAI as the experts': min(g, 7) sigmoid(1.702 min(g, 7)) (clamp(u, -7, 7) + 1)).

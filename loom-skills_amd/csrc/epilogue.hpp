@@ -145,6 +145,12 @@ __device__ __forceinline__ void act1_slope(int act, float v, float &a, float &da
       da = 1.f;
   }
 }
+// the gradient of act1(v) at dy
+__device__ __forceinline__ float act1_grad(int act, float v, float dy) {
+  float a, da;
+  act1_slope(act, v, a, da);
+  return dy * da;
+}
 // the gradients of act2(g, u) at dy. swiglu_oai: those of the clamps are 1 up to and at their limits, 0 past them
 __device__ __forceinline__ void act2_grad(int act, float g, float u, float dy, float &dg, float &du) {
   if (act == QMM_ACT_SWIGLU_OAI) {

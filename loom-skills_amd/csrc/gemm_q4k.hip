@@ -471,19 +471,20 @@ int fmt_align(int fmt) { return fmt == QMM_Q4_K || fmt == QMM_Q4_KT ? 16 : fmt =
 int qmm_gemm_q4k_dense(int acc, int tiled, int64_t rows, int64_t k, int64_t n, const void *x, const float *scales,
                        const void *w, void *y, int y_bf16, hipStream_t s, const Epi *ep);
 
-// The GEMMs with an epilogue over GGUF-block or tiled Q4_K weights: kind kTLinear, kTGlu or kTGluGrad (gemm_tile.hpp).
+// The GEMMs with an epilogue over GGUF-block or tiled Q4_K weights: kind kTLinear, kTGlu, kTGluGrad or kTLinearGrad
+// (gemm_tile.hpp).
 int qmm_gemm_epi(int fmt, int kind, int64_t rows, int64_t k, int64_t n, const void *x, const float *scales, const void *w,
                  const void *w2, const void *dy, int dy_bf16, hipStream_t s, const Epi &ep) {
-  const bool tiled = fmt == QMM_Q4_KT, two = kind != kTLinear;
+  const bool tiled = fmt == QMM_Q4_KT, two = kind == kTGlu || kind == kTGluGrad, grad = kind == kTGluGrad || kind == kTLinearGrad;
   if (!gguf_gemm_fmt(fmt) && !tiled) return QMM_ERR_FORMAT;
-  if (!x || !w || (two && !w2) || (kind == kTGluGrad && !dy)) return QMM_ERR_NULL;
+  if (!x || !w || (two && !w2) || (grad && !dy)) return QMM_ERR_NULL;
   if (rows <= 0 || n <= 0 || k <= 0 || k % 256 || rows > (1 << 24) || n > (1 << 24) || k > (1 << 20)) return QMM_ERR_SHAPE;
   if (tiled && (n % 16 || k % 512)) return QMM_ERR_SHAPE;   // whole 16-row blocks of whole 512-value units
   const int wal = fmt_align(fmt);
   if (!aligned(x, 16) || !aligned(scales, 4) || !aligned(w, wal) || !aligned(w2, wal)) return QMM_ERR_ALIGN;
   // activation rows and weight rows are addressed by 32-bit buffer offsets
   if (rows * k * 2 >= (1ll << 31) || n * fmt_row_bytes(fmt, k) >= (1ll << 31)) return QMM_ERR_SHAPE;
-  int shape = tile_shape(two, fmt == QMM_Q4_K || tiled, rows, n, k);
+  int shape = tile_shape(two, !grad && (fmt == QMM_Q4_K || tiled), rows, n, k);
   // A workgroup of four waves on 64 x 64 outputs where those take the chip once: a wave a SIMD (Q6_K 4096 x 4096 at 64 rows
   // 28 -> 21 us, 4096 x 12288 75 -> 55, 2 x 768 x 2048 of Q4_0 18.5 -> 13.8; Q4_K, one matrix, against the dense kernel:
   // 4096 x 4096 at 64 rows 23.0 -> 17.9, 4096 x 12288 55 -> 52, 768 x 2048 16 -> 12). The dense kernel's exchange costs it

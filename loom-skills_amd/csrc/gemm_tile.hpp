@@ -8,8 +8,10 @@ namespace qmm {
 
 // kTDense: Y (+)= X W^T; kTSwiglu: Y = silu(X Wg^T inv) (X Wu^T inv) over dense rows; kTGU / kTDN: the grouped gate/up
 // and down GEMMs over bucketed 64-row expert tiles; kTLinear: Y = act(X W^T inv + bias) + res; kTGlu: Y = act(X Wg^T inv +
-// bias) (X Wu^T inv + bias2); kTGluGrad: the gradients of that product at dy, bf16 [M, 2, N]
-enum TileKind { kTDense = 0, kTSwiglu = 1, kTGU = 2, kTDN = 3, kTLinear = 4, kTGlu = 5, kTGluGrad = 6 };
+// bias) (X Wu^T inv + bias2); kTGluGrad: the gradients of that product at dy, bf16 [M, 2, N]; kTLinearGrad: dy act'(X W^T inv +
+// bias), bf16 [M, N]
+enum TileKind { kTDense = 0, kTSwiglu = 1, kTGU = 2, kTDN = 3, kTLinear = 4, kTGlu = 5, kTGluGrad = 6,
+                kTLinearGrad = 7 };
 // the workgroup: rows x waves along N x K-parts (a wave holds 64 weight columns)
 enum TileShape { kT128x4x1 = 0, kT128x4x2 = 1, kT64x4x1 = 2, kT64x2x4 = 3, kT64x1x4 = 4 };
 
@@ -27,8 +29,8 @@ struct TileArgs {
   void *y;
   int acc, y_bf16;             // dense: Y += ..., bf16 output rows
   int tiles_m, tiles_n;
-  Epi ep;                      // kTLinear, kTGlu, kTGluGrad
-  const void *dy;              // kTGluGrad: [M, N] f32 or bf16
+  Epi ep;                      // kTLinear, kTGlu, kTGluGrad, kTLinearGrad
+  const void *dy;              // kTGluGrad, kTLinearGrad: [M, N] f32 or bf16
   int dy_bf16;
   int wide_rows;               // rows of y and what is read beside it (residual, dy) are 16-byte aligned
 };

@@ -9,6 +9,7 @@
 //   linear  Y[r, c]   = act(inv[r] sum_k X16[r, k] W[c, k] + b[c]) + res[r, c]                          (qmm_linear)
 //   glu     Y[r, c]   = act(g) u, g = inv[r] sum_k X16[r, k] Wg[c, k] + bg[c], u likewise          (qmm_ffn_gate_up)
 //   grad    D[r, 0, c] = dy[r, c] u act'(g), D[r, 1, c] = dy[r, c] act(g)                     (qmm_ffn_gate_up_grad)
+//           D[r, c] = dy[r, c] act'(inv[r] sum_k X16[r, k] W[c, k] + b[c])                          (qmm_linear_grad)
 //   dn      ys[r, c]  = inv[r] sum_k A16[r, k] Wd[e][c, k] + bd[e, c]            (rows already sorted)
 //
 // X16 / A16 are the row-scaled f16 operands of g_row_scale_f16[_tiles] (S/gen_llm.py:1843-1915, S/gen_moe.py:503-527),
@@ -82,7 +83,8 @@ struct Raw<kQ40> {   // two blocks' 16 code bytes and d
 
 constexpr bool two_matrices(int kind) { return kind == kTGU || kind == kTSwiglu || kind == kTGlu || kind == kTGluGrad; }
 constexpr bool dense_rows(int kind) { return kind != kTGU && kind != kTDN; }
-constexpr bool epilogue_kind(int kind) { return kind == kTLinear || kind == kTGlu || kind == kTGluGrad; }
+constexpr bool grad_kind(int kind) { return kind == kTGluGrad || kind == kTLinearGrad; }
+constexpr bool epilogue_kind(int kind) { return kind == kTLinear || kind == kTGlu || grad_kind(kind); }
 __host__ __device__ constexpr bool ragged_last(int m, int bm) { return m % bm > 0 && m % bm <= bm / 2; }
 constexpr int raw_of(int wf) { return wf == kQ4KT ? kQ4K : wf; }
 constexpr int64_t row_bytes_of(int wf, int64_t k) {
@@ -573,8 +575,8 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
       b1[j] = epi_bias(a.ep.bias, min(col[j], N - 1));
     }
     if constexpr (kTwoW) b2 = epi_bias(a.ep.bias2, min(col[0], N - 1));
-    const void *in = KIND == kTGluGrad ? a.dy : a.ep.res;
-    const int in_bf16 = KIND == kTGluGrad ? a.dy_bf16 : a.ep.res_bf16;
+    const void *in = grad_kind(KIND) ? a.dy : a.ep.res;
+    const int in_bf16 = grad_kind(KIND) ? a.dy_bf16 : a.ep.res_bf16;
     constexpr std::integral_constant<int, KIND == kTLinear ? QMM_ACT_NONE : QMM_ACT_SILU> usual;
     constexpr std::integral_constant<int, 0> f32;
     constexpr std::integral_constant<int, 1> bf16;
@@ -611,6 +613,8 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
                 const float v = __builtin_fmaf(out[i][j][r], inv, b1[j]);
                 if constexpr (KIND == kTLinear) {
                   t[32 * j] = act1(act, v);
+                } else if constexpr (KIND == kTLinearGrad) {
+                  t[32 * j] = v;
                 } else {
                   const float u = __builtin_fmaf(out[i][1][r], inv, b2);
                   t[0] = KIND == kTGlu ? act2(act, v, u) : v;
@@ -632,7 +636,10 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
             } else {
               float v[V];
 #pragma unroll
-              for (int q = 0; q < V; ++q) v[q] = KIND == kTLinear && in ? t[q] + add[p][q] : t[q];
+              for (int q = 0; q < V; ++q) {
+                if constexpr (KIND == kTLinearGrad) v[q] = act1_grad(act, t[q], add[p][q]);
+                else v[q] = KIND == kTLinear && in ? t[q] + add[p][q] : t[q];
+              }
               if (live(p)) store_vals<V>(a.ep.y, ybf, at(p), v);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -640,7 +647,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
         }
       };
       if (a.ep.act != usual.value) finish(a.ep.act, a.ep.y_bf16);
-      else if (KIND == kTGluGrad || a.ep.y_bf16) finish(usual, bf16);
+      else if (grad_kind(KIND) || a.ep.y_bf16) finish(usual, bf16);
       else finish(usual, f32);
       return;
     }
@@ -679,6 +686,8 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
             if constexpr (KIND == kTLinear) {
               const float y = act1(act, v);
               store_val(a.ep.y, ybf, o, in ? y + add[j][r] : y);
+            } else if constexpr (KIND == kTLinearGrad) {
+              store_val(a.ep.y, 1, o, act1_grad(act, v, add[j][r]));
             } else {
               const float u = __builtin_fmaf(out[i][1][r], inv, b2);
               if constexpr (KIND == kTGlu) {
@@ -696,7 +705,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
       }
     };
     if (a.ep.act != usual.value) finish(a.ep.act, a.ep.y_bf16);
-    else if (KIND == kTGluGrad || a.ep.y_bf16) finish(usual, bf16);
+    else if (grad_kind(KIND) || a.ep.y_bf16) finish(usual, bf16);
     else finish(usual, f32);
     return;
   }
@@ -772,6 +781,7 @@ int dispatch(int kind, int shape, const TileArgs &a, hipStream_t s) {
     case kTLinear: return dispatch_dense<WF, kTLinear>(shape, a, s);
     case kTGlu: return dispatch_dense<WF, kTGlu>(shape, a, s);
     case kTGluGrad: return dispatch_dense<WF, kTGluGrad>(shape, a, s);
+    case kTLinearGrad: return dispatch_dense<WF, kTLinearGrad>(shape, a, s);
     default: return dispatch_dense<WF, kTDense>(shape, a, s);
   }
 }

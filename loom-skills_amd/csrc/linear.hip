@@ -1,6 +1,7 @@
 // Products on quantized weights with an epilogue: argument checks and the choice of the kernel by the operand's type.
 //
 //   qmm_linear            y = act(x W^T + bias) + residual
+//   qmm_linear_grad       dpre = dy act'(x W^T + bias)
 //   qmm_ffn_gate_up       y = act(x Wg^T + bg) (x Wu^T + bu)
 //   qmm_ffn_gate_up_grad  dgu[t] = (dy u act'(g), dy act(g)),  g = x Wg^T + bg, u = x Wu^T + bu
 //
@@ -92,5 +93,17 @@ extern "C" int qmm_ffn_gate_up_grad(int fmt, int act, int64_t tokens, int64_t k,
   if (!aligned(dgu, 2) || !val_aligned(dy, dy_dtype) || !aligned(bias, 4) || !aligned(bias2, 4)) return QMM_ERR_ALIGN;
   const Epi ep{bias, bias2, nullptr, dgu, act, 0, 1};
   return qmm_gemm_epi(fmt, kTGluGrad, tokens, k, n, x, x_scales, w, w2, dy, dy_dtype == QMM_BF16,
+                      reinterpret_cast<hipStream_t>(stream), ep);
+}
+
+extern "C" int qmm_linear_grad(int fmt, int act, int64_t tokens, int64_t k, int64_t n, const void *x, const float *x_scales,
+                               const void *w, const float *bias, const void *dy, int dy_dtype, void *dpre,
+                               qmm_stream_t stream) {
+  if (act < QMM_ACT_SILU || act > QMM_ACT_SIGMOID || act == QMM_ACT_SWIGLU_OAI) return QMM_ERR_RANGE;
+  if (!dpre) return QMM_ERR_NULL;
+  if (!val_dtype(dy_dtype)) return QMM_ERR_DTYPE;
+  if (!aligned(dpre, 2) || !val_aligned(dy, dy_dtype) || !aligned(bias, 4)) return QMM_ERR_ALIGN;
+  const Epi ep{bias, nullptr, nullptr, dpre, act, 0, 1};
+  return qmm_gemm_epi(fmt, kTLinearGrad, tokens, k, n, x, x_scales, w, nullptr, dy, dy_dtype == QMM_BF16,
                       reinterpret_cast<hipStream_t>(stream), ep);
 }

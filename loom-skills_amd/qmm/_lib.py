@@ -24,6 +24,7 @@ SIGNATURES = {
                           c_i64, c_vp],
     "qmm_rms_norm_grad_workspace_size": [c_i64, c_i64],
     "qmm_linear": [c_int, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_vp],
+    "qmm_linear_grad": [c_int, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp],
     "qmm_ffn_gate_up": [c_int, c_int, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                         c_int, c_vp],
     "qmm_ffn_gate_up_grad": [c_int, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp,

@@ -32,6 +32,7 @@ the rest of a dense feed-forward sub-layer around those products, without counte
     rms_norm              residual addition and RMS norm, written as the next product's operand
     rms_norm_backward     its gradients with respect to x, the residual and the weight
     linear                with bias, activation, residual, bf16 rows (qmm_linear)
+    linear_backward       its gradients with respect to the activation's argument and to x (frozen weights)
     ffn_gate_up           act(x Wg^T + bg) (x Wu^T + bu) with any activation and biases
     ffn_gate_up_backward  its gradients with respect to the projections' outputs and to x (frozen weights)
     gemm_t                the transposed product x W, a projection's input gradient
@@ -972,6 +973,43 @@ def _rows_out(y, shape, out_dtype, x, like=None):
     return y
 
 
+def linear_backward(fmt, x, w, dy, n, k, scales=None, bias=None, act="none", out_dtype=torch.bfloat16):
+    """The gradients of linear with an epilogue at dy (f32 / bf16 [tokens, n]) with frozen weights: (dx [tokens, k] of
+    out_dtype, dpre), dpre [tokens, n] the gradient of x W^T + bias (bf16; dy itself for act "none"), dx = dpre W. The
+    residual's gradient is dy, the bias's the sum of dpre over the tokens. The argument is computed again from x, whose forms,
+    padding rows and formats are those of ffn_gate_up_backward."""
+    s = _here(x, w, dy, bias, scales)
+    code = _act_code(act, EPILOGUE_ACT)
+    x, scales = _backward_operand(fmt, x, dy, n, k, scales)
+    _weight_bytes(fmt, w, None, n, k)
+    _shaped(bias, (n,), (torch.float32,), "bias")
+    if act == "none":
+        return gemm_t(fmt, dy, w, n, k, out_dtype=out_dtype), dy
+    if x.dtype != torch.float16:
+        x, scales = row_scale_f16(x)
+    dpre = torch.empty((x.shape[0], n), dtype=torch.bfloat16, device=x.device)
+    _lib.call("qmm_linear_grad", CODE[fmt], code, x.shape[0], k, n, _ptr(x), _ptr(scales), _ptr(w), _ptr(bias), _ptr(dy), _dt(dy),
+              _ptr(dpre), s)
+    return gemm_t(fmt, dpre, w, n, k, out_dtype=out_dtype), dpre
+
+
+def _backward_operand(fmt, x, dy, n, k, scales):
+    """Checks of the rows (f32 / bf16, or the f16 operand with its scales) that a backward pass computes from again."""
+    if fmt not in _F16_GEMM:
+        raise ValueError(f"no backward pass reads {fmt} weights")
+    if x.dim() != 2 or x.shape[1] != k:
+        raise ValueError(f"x is {tuple(x.shape)}, expected [tokens, {k}]")
+    _shaped(dy, (x.shape[0], n), _VALUE, "dy")
+    _shaped(scales, (x.shape[0], 2), (torch.float32,), "scales")
+    if x.dtype != torch.float16:
+        if scales is not None:
+            raise ValueError("scales come with an f16 operand")
+        _shaped(x, x.shape, _VALUE, "x")
+    elif scales is None:
+        raise ValueError("the f16 operand comes with its scales")
+    return x, scales
+
+
 def ffn_gate_up(fmt, x, w, w2, n, k, y=None, ws=None, ws2=None, q8="auto", bias=None, bias2=None, act="silu",
                 out_dtype=None, scales=None, tokens=None):
     """The gated feed-forward block's first half, y = act(x W^T + bias) (x W2^T + bias2), in one kernel past the operand's
@@ -1003,24 +1041,14 @@ def ffn_gate_up_backward(fmt, x, w, w2, dy, n, k, scales=None, bias=None, bias2=
     zeros there, their dgu and dx rows are undefined). fmt q4_k, q4_kt, q6_k or q4_0, k % 256 == 0."""
     s = _here(x, w, w2, dy, bias, bias2, scales)
     code = _act_code(act, GATE_ACT)
-    if fmt not in _F16_GEMM:
-        raise ValueError(f"no backward pass reads {fmt} weights")
+    x, scales = _backward_operand(fmt, x, dy, n, k, scales)
     _weight_bytes(fmt, w, None, n, k)
     _weight_bytes(fmt, w2, None, n, k, "w2")
-    if x.dim() != 2 or x.shape[1] != k:
-        raise ValueError(f"x is {tuple(x.shape)}, expected [tokens, {k}]")
     T = x.shape[0]
-    _shaped(dy, (T, n), _VALUE, "dy")
     _shaped(bias, (n,), (torch.float32,), "bias")
     _shaped(bias2, (n,), (torch.float32,), "bias2")
-    _shaped(scales, (T, 2), (torch.float32,), "scales")
     if x.dtype != torch.float16:
-        if scales is not None:
-            raise ValueError("scales come with an f16 operand")
-        _shaped(x, (T, k), _VALUE, "x")
         x, scales = row_scale_f16(x)
-    elif scales is None:
-        raise ValueError("the f16 operand comes with its scales")
     dgu = torch.empty((T, 2, n), dtype=torch.bfloat16, device=x.device)
     _lib.call("qmm_ffn_gate_up_grad", CODE[fmt], code, T, k, n, _ptr(x), _ptr(scales), _ptr(w), _ptr(w2), _ptr(bias),
               _ptr(bias2), _ptr(dy), _dt(dy), _ptr(dgu), s)

@@ -117,6 +117,20 @@ def test_backward_statuses(lib):   # noqa: F811
         assert lib.qmm_gemm_t_workspace_size(bad.get("fmt", 1), bad.get("t", 4), bad.get("k", 512), bad.get("n", 64), 1) == -1
     for bad in (dict(t=0), dict(k=384), dict(n=0), dict(fmt=5, n=24), dict(fmt=5, k=768)):
         assert grad(**bad) == st["QMM_ERR_SHAPE"], bad
+    def lin(fmt=1, act=0, t=4, k=512, n=64, x=at(), s=at(), w=at(), b=None, dy=at(), dd=F32, o=at()):
+        return lib.qmm_linear_grad(fmt, act, t, k, n, x, s, w, b, dy, dd, o, None)
+
+    for bad in (dict(x=None), dict(w=None), dict(dy=None), dict(o=None)):
+        assert lin(**bad) == st["QMM_ERR_NULL"], bad
+    for bad in (dict(act=1), dict(act=7), dict(act=-1)):
+        assert lin(**bad) == st["QMM_ERR_RANGE"], bad
+    for bad in (dict(fmt=2), dict(fmt=4), dict(fmt=7)):
+        assert lin(**bad) == st["QMM_ERR_FORMAT"], bad
+    for bad in (dict(t=0), dict(k=384), dict(n=0), dict(fmt=5, n=24)):
+        assert lin(**bad) == st["QMM_ERR_SHAPE"], bad
+    for bad in (dict(dy=at(0x10002)), dict(dy=at(0x10001), dd=BF16), dict(o=at(0x10001)), dict(b=at(0x10002)), dict(x=at(0x10008)), dict(w=at(0x10008))):
+        assert lin(**bad) == st["QMM_ERR_ALIGN"], bad
+    assert lin(dd=F16) == st["QMM_ERR_DTYPE"]
     for bad in (dict(x=None), dict(s=None), dict(w=None), dict(y=None)):
         assert gemm_t(**bad) == st["QMM_ERR_NULL"], bad
     for bad in (dict(x=None), dict(o=None), dict(s=None)):
@@ -157,6 +171,16 @@ def test_rms_norm_errors(ops):
                   ((x, w), dict(residual=x.bfloat16(), h=x)), ((x, w), dict(out="int8")), ((x, w), dict(out=None))):
         with pytest.raises(ValueError):
             ops.rms_norm(*a, **kw)
+
+
+def test_linear_backward_errors(ops):
+    n, k, T = 32, 512, 4
+    w, x, dy = torch.zeros(n * k // 256 * 144, dtype=torch.uint8), torch.zeros(T, k), torch.zeros(T, n)
+    for fmt, xx, d, kw in (("mxfp4s", x, dy, {}), ("q4_k", x, dy, dict(act="swiglu_oai")), ("q4_k", x[:, :256], dy, {}), ("q4_k", x, dy[:2], {}), ("q4_k", x, dy.half(), {}),
+                           ("q4_k", x, dy, dict(bias=torch.zeros(8))), ("q4_k", x, dy, dict(scales=torch.zeros(T, 2))), ("q4_k", x.half(), dy, {}),
+                           ("q4_k", x.double(), dy, {}), ("q6_k", x, dy, {}), ("q4_k", x.half(), dy, dict(scales=torch.zeros(T, 3)))):
+        with pytest.raises(ValueError):
+            ops.linear_backward(fmt, xx, w, d, n, k, **kw)
 
 
 def test_rms_norm_backward_errors(ops):
