@@ -910,13 +910,13 @@ def linear(fmt, x, w, n, k, y=None, mode="store", ws=None, w2=None, ws2=None, q8
     q4_0 and mxfp4s; q8=False keeps f32 / bf16 activations (ACT_Q8=0). y is f32.
 
     With any of bias (f32 [n]), act (none, relu, silu, sigmoid, gelu: the tanh form, gelu_erf), residual (f32 / bf16
-    [tokens, n], y itself allowed), out_dtype (f32 / bf16), scales or tokens, or a bf16 y, the call is
+    [tokens, n], y itself allowed), out_dtype (f32 / bf16), scales or tokens, or a bf16 y for fewer than 64 rows, the call is
     y = act(x W^T + bias) + residual (qmm_linear, mode "store"). x may then also be an operand: a planar Q8_1 buffer with
     tokens, the row-scaled f16 rows or E4M3 codes with their scales; the operand chooses the product whatever the token
     count. GGUF mxfp4 blocks take up to 63 rows (repack_mxfp4 for more). The sums are those of the plain call, in some
     shapes added in another f32 order (qmm_linear). y may be the residual; it may overlap no other argument."""
     if bias is not None or act != "none" or residual is not None or out_dtype is not None or scales is not None or \
-            tokens is not None or (y is not None and y.dtype == torch.bfloat16):
+            tokens is not None or (y is not None and y.dtype == torch.bfloat16 and mode == "store" and x.shape[0] < GEMM_MIN_TOKENS):
         if mode != "store" or w2 is not None or ws2 is not None:
             raise ValueError("bias, act, residual, out_dtype, scales and tokens go with mode \"store\" (ffn_gate_up for two "
                              "matrices)")

@@ -208,3 +208,23 @@ def test_rows_at_any_address(dev, fmt, T, n, k):
             assert torch.equal(y, gated) and (buf[:off] == 3).all() and (buf[off + T * n:] == 3).all(), off
             got = ops.ffn_gate_up_backward(fmt, x, w.w, u.w, at(off, dy)[1], n, k, scales=s, bias=b)
             assert all(torch.equal(p, q) for p, q in zip(got, grads)), off
+
+
+@pytest.mark.parametrize("fmt", ["q4_k", "q6_k", "q4_0", "mxfp4", "mxfp4t"])
+def test_bf16_y_of_the_prefill_products(dev, fmt):
+    """A bf16 y without any of the epilogue's arguments is the GEMM's own output from 64 rows on, in every mode."""
+    import qmm.ops as ops
+    rng = np.random.default_rng(14)
+    T, n, k = 70, 96, 512
+    w, u, x = Weight(fmt, rng, n, k, dev), Weight(fmt, rng, n, k, dev), rows(rng, (T, k), torch.bfloat16, dev)
+    gfmt, gw, gs, gu, gus = fmt, w.w, w.ws, u.w, u.ws
+    if fmt == "mxfp4":
+        gfmt, (gw, gs), (gu, gus) = "mxfp4s", ops.repack_mxfp4(w.w, n, k), ops.repack_mxfp4(u.w, n, k)
+    for mode in ("store", "acc", "swiglu"):
+        y = rows(rng, (T, n), torch.bfloat16, dev)
+        z, two = y.clone(), mode == "swiglu"
+        ops.linear(fmt, x, w.w, n, k, y=y, mode=mode, ws=w.ws, w2=u.w if two else None, ws2=u.ws if two else None)
+        ops.gemm(gfmt, mode, x, gw, n, k, w2=gu if two else None, y=z, ws=gs, ws2=gus if two else None)
+        assert torch.equal(y, z), mode
+    got = ops.linear(fmt, x[:5], w.w, n, k, y=torch.empty((5, n), dtype=torch.bfloat16, device=dev), ws=w.ws)
+    assert torch.equal(got, ops.linear(fmt, x[:5], w.w, n, k, ws=w.ws, out_dtype=torch.bfloat16))
