@@ -393,12 +393,10 @@ __global__ __launch_bounds__(kWaves * 64, 1) void q4k_dense_kernel(DArgs a, EP e
     const int64_t o = (int64_t)row * N + col;
     if constexpr (kEpi<EP>) {   // eight columns of a row: their bias and residual values, then the stores
       if (ep_wide(ep, N)) {
-        auto act = [&](auto a) __attribute__((always_inline)) {
+        with_act(ep.act, [&](auto a) __attribute__((always_inline)) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = act1(a, v[e] + eb[e]);
-        };
-        if (ep.act == QMM_ACT_NONE) act(std::integral_constant<int, QMM_ACT_NONE>{});
-        else act(ep.act);
+          for (int e = 0; e < 8; ++e) v[e] = act1(a.value, v[e] + eb[e]);
+        });
         if (ep.res) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {

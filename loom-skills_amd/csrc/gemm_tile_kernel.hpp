@@ -577,136 +577,113 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
     if constexpr (kTwoW) b2 = epi_bias(a.ep.bias2, min(col[0], N - 1));
     const void *in = grad_kind(KIND) ? a.dy : a.ep.res;
     const int in_bf16 = grad_kind(KIND) ? a.dy_bf16 : a.ep.res_bf16;
-    constexpr std::integral_constant<int, KIND == kTLinear ? QMM_ACT_NONE : QMM_ACT_SILU> usual;
-    constexpr std::integral_constant<int, 0> f32;
-    constexpr std::integral_constant<int, 1> bf16;
     if (a.wide_rows) {
       // Through the wave's own LDS, PR rows of its columns at a time, so that a lane reads and writes V neighbouring values of
-      // a row (the other path below: a column a lane, a load and a store a value). kTGluGrad takes both sums through it.
+      // a row (the other path below: a column a lane, a load and a store a value). Two matrices take both sums through it.
       constexpr int WC = 32 * NC, NROW = 32 / KS, PR = 512 / WC < NROW ? 512 / WC : NROW, NP = NROW / PR, V = PR * WC / 64;
-      constexpr int kPlanes = KIND == kTGluGrad ? 2 : 1, PITCH = WC + 8, LR = WC / V;   // LR lanes a row
+      constexpr int kPlanes = kTwoW ? 2 : 1, PITCH = WC + 8, LR = WC / V;   // LR lanes a row
       static_assert(NW * KS * kPlanes * PR * PITCH * 4 <= 2 * KS * kPart, "a pass of every wave fits the staged activations");
       float *T = reinterpret_cast<float *>(smem) + wave * kPlanes * PR * PITCH;
       if constexpr (KS > 1) __syncthreads();   // the parts' exchange is read
       const int tr = lane / LR, tc = V * (lane % LR), cw = n0 + WC * wn + tc;
-      auto finish = [&](auto act, auto ybf) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const int row0 = 32 * i + NROW * kp;
-          auto live = [&](int p) { return src_row[row0 + PR * p + tr] >= 0 && cw < N; };
-          auto at = [&](int p) { return (int64_t)(m0 + row0 + PR * p + tr) * N + cw; };
-          float add[NP][V];
-          if (KIND != kTGlu && in) {
-#pragma unroll
-            for (int p = 0; p < NP; ++p)
-              if (live(p)) load_vals<V>(in, in_bf16, at(p), add[p]);
-          }
-#pragma unroll
-          for (int p = 0; p < NP; ++p) {
-#pragma unroll
-            for (int rr = 0; rr < PR / 2; ++rr) {   // the accumulator registers of the pass's rows
-              const int r = PR / 2 * p + rr, lr = 8 * (rr >> 2) + 4 * h + (rr & 3);
-              const float inv = rinv[row0 + PR * p + lr];
-              float *t = T + lr * PITCH + lc;
-#pragma unroll
-              for (int j = 0; j < NC; ++j) {
-                const float v = __builtin_fmaf(out[i][j][r], inv, b1[j]);
-                if constexpr (KIND == kTLinear) {
-                  t[32 * j] = act1(act, v);
-                } else if constexpr (KIND == kTLinearGrad) {
-                  t[32 * j] = v;
-                } else {
-                  const float u = __builtin_fmaf(out[i][1][r], inv, b2);
-                  t[0] = KIND == kTGlu ? act2(act, v, u) : v;
-                  if constexpr (kPlanes == 2) t[PR * PITCH] = u;
-                }
-              }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            const float *t = T + tr * PITCH + tc;
-            if constexpr (KIND == kTGluGrad) {
-              float dg[V], du[V];
-#pragma unroll
-              for (int q = 0; q < V; ++q) act2_grad(act, t[q], t[PR * PITCH + q], add[p][q], dg[q], du[q]);
-              if (live(p)) {
-                const int64_t od = at(p) + (int64_t)(m0 + row0 + PR * p + tr) * N;
-                store_vals<V>(a.ep.y, ybf, od, dg);
-                store_vals<V>(a.ep.y, ybf, od + N, du);
-              }
-            } else {
-              float v[V];
-#pragma unroll
-              for (int q = 0; q < V; ++q) {
-                if constexpr (KIND == kTLinearGrad) v[q] = act1_grad(act, t[q], add[p][q]);
-                else v[q] = KIND == kTLinear && in ? t[q] + add[p][q] : t[q];
-              }
-              if (live(p)) store_vals<V>(a.ep.y, ybf, at(p), v);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          }
-        }
-      };
-      if (a.ep.act != usual.value) finish(a.ep.act, a.ep.y_bf16);
-      else if (grad_kind(KIND) || a.ep.y_bf16) finish(usual, bf16);
-      else finish(usual, f32);
-      return;
-    }
-    // act, ybf: constants where the activation is the common one, so that a value does not branch on them
-    auto finish = [&](auto act, auto ybf) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        auto row_of = [&](int r) {
-          const int rr = kp * RK + r;
-          return 32 * i + 8 * (rr >> 2) + 4 * h + (rr & 3);
-        };
-        float add[NC][RK];
-        auto load = [&](auto bf) __attribute__((always_inline)) {
-#pragma unroll
-          for (int r = 0; r < RK; ++r)
-#pragma unroll
-            for (int j = 0; j < NC; ++j) {
-              const bool live = src_row[row_of(r)] >= 0 && col[j] < N;
-              add[j][r] = live ? load_val(in, bf, (int64_t)(m0 + row_of(r)) * N + col[j]) : 0.f;
-            }
-        };
+        const int row0 = 32 * i + NROW * kp;
+        auto live = [&](int p) { return src_row[row0 + PR * p + tr] >= 0 && cw < N; };
+        auto at = [&](int p) { return (int64_t)(m0 + row0 + PR * p + tr) * N + cw; };
+        float add[NP][V];
         if (KIND != kTGlu && in) {
-          if (in_bf16) load(std::integral_constant<int, 1>{});
-          else load(std::integral_constant<int, 0>{});
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+            if (live(p)) load_vals<V>(in, in_bf16, at(p), add[p]);
         }
 #pragma unroll
-        for (int r = 0; r < RK; ++r) {
-          const int lr = row_of(r);
-          if (src_row[lr] < 0) continue;
-          const float inv = rinv[lr];
+        for (int p = 0; p < NP; ++p) {
+#pragma unroll
+          for (int rr = 0; rr < PR / 2; ++rr) {   // the accumulator registers of the pass's rows
+            const int r = PR / 2 * p + rr, lr = 8 * (rr >> 2) + 4 * h + (rr & 3);
+            const float inv = rinv[row0 + PR * p + lr];
+            float *t = T + lr * PITCH + lc;
+#pragma unroll
+            for (int j = 0; j < NC; ++j) t[32 * j] = __builtin_fmaf(out[i][j][r], inv, b1[j]);
+            if constexpr (kTwoW) t[PR * PITCH] = __builtin_fmaf(out[i][1][r], inv, b2);
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          float *t = T + tr * PITCH + tc;
+          float v[V];
+          if constexpr (KIND == kTGluGrad) {
+            float du[V];
+            act2_grad_rows<V>(a.ep.act, t, t + PR * PITCH, add[p], v, du);
+            if (live(p)) {
+              const int64_t od = at(p) + (int64_t)(m0 + row0 + PR * p + tr) * N;
+              store_vals<V>(a.ep.y, 1, od, v);
+              store_vals<V>(a.ep.y, 1, od + N, du);
+            }
+          } else {
+            if constexpr (KIND == kTGlu) act2_rows<V>(a.ep.act, t, t + PR * PITCH, v);
+            else if constexpr (KIND == kTLinearGrad) act1_grad_rows<V>(a.ep.act, t, add[p], v);
+            else act1_rows<V>(a.ep.act, t, v);
+            if (KIND == kTLinear && in) {
+#pragma unroll
+              for (int q = 0; q < V; ++q) v[q] += add[p][q];
+            }
+            if (live(p)) store_vals<V>(a.ep.y, a.ep.y_bf16, at(p), v);
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      auto row_of = [&](int r) {
+        const int rr = kp * RK + r;
+        return 32 * i + 8 * (rr >> 2) + 4 * h + (rr & 3);
+      };
+      float add[NC][RK];
+      auto load = [&](auto bf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < RK; ++r)
 #pragma unroll
           for (int j = 0; j < NC; ++j) {
-            if (col[j] >= N) continue;
-            const int64_t o = (int64_t)(m0 + lr) * N + col[j];
-            const float v = __builtin_fmaf(out[i][j][r], inv, b1[j]);
-            if constexpr (KIND == kTLinear) {
-              const float y = act1(act, v);
-              store_val(a.ep.y, ybf, o, in ? y + add[j][r] : y);
-            } else if constexpr (KIND == kTLinearGrad) {
-              store_val(a.ep.y, 1, o, act1_grad(act, v, add[j][r]));
+            const bool live = src_row[row_of(r)] >= 0 && col[j] < N;
+            add[j][r] = live ? load_val(in, bf, (int64_t)(m0 + row_of(r)) * N + col[j]) : 0.f;
+          }
+      };
+      if (KIND != kTGlu && in) {
+        if (in_bf16) load(std::integral_constant<int, 1>{});
+        else load(std::integral_constant<int, 0>{});
+      }
+#pragma unroll
+      for (int r = 0; r < RK; ++r) {
+        const int lr = row_of(r);
+        if (src_row[lr] < 0) continue;
+        const float inv = rinv[lr];
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          if (col[j] >= N) continue;
+          const int64_t o = (int64_t)(m0 + lr) * N + col[j];
+          const float v = __builtin_fmaf(out[i][j][r], inv, b1[j]);
+          if constexpr (KIND == kTLinear) {
+            const float y = act1(a.ep.act, v);
+            store_val(a.ep.y, a.ep.y_bf16, o, in ? y + add[j][r] : y);
+          } else if constexpr (KIND == kTLinearGrad) {
+            store_val(a.ep.y, 1, o, act1_grad(a.ep.act, v, add[j][r]));
+          } else {
+            const float u = __builtin_fmaf(out[i][1][r], inv, b2);
+            if constexpr (KIND == kTGlu) {
+              store_val(a.ep.y, a.ep.y_bf16, o, act2(a.ep.act, v, u));
             } else {
-              const float u = __builtin_fmaf(out[i][1][r], inv, b2);
-              if constexpr (KIND == kTGlu) {
-                store_val(a.ep.y, ybf, o, act2(act, v, u));
-              } else {
-                float dg, du;
-                act2_grad(act, v, u, add[0][r], dg, du);
-                const int64_t od = 2 * (int64_t)(m0 + lr) * N + col[j];
-                store_val(a.ep.y, 1, od, dg);
-                store_val(a.ep.y, 1, od + N, du);
-              }
+              float dg, du;
+              act2_grad(a.ep.act, v, u, add[0][r], dg, du);
+              const int64_t od = 2 * (int64_t)(m0 + lr) * N + col[j];
+              store_val(a.ep.y, 1, od, dg);
+              store_val(a.ep.y, 1, od + N, du);
             }
           }
         }
       }
-    };
-    if (a.ep.act != usual.value) finish(a.ep.act, a.ep.y_bf16);
-    else if (grad_kind(KIND) || a.ep.y_bf16) finish(usual, bf16);
-    else finish(usual, f32);
+    }
     return;
   }
   float *yf = static_cast<float *>(a.y);

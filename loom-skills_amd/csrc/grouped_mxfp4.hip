@@ -556,43 +556,41 @@ __global__ __launch_bounds__(256, WAVES) void mxfp4_grouped_kernel(MArgs a) {
         b1[cc] = epi_bias(a.ep.bias, cj);
         b2[cc] = GU ? epi_bias(a.ep.bias2, cj) : 0.f;
       }
-      auto finish = [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float add[NP][8];
-          auto live = [&](int p) { return m0 + 32 * i + PR * p + tr < a.M && cw < N; };
-          auto at = [&](int p) { return (int64_t)(m0 + 32 * i + PR * p + tr) * N + cw; };
-          if (!GU && a.ep.res) {
+      for (int i = 0; i < 2; ++i) {
+        float add[NP][8];
+        auto live = [&](int p) { return m0 + 32 * i + PR * p + tr < a.M && cw < N; };
+        auto at = [&](int p) { return (int64_t)(m0 + 32 * i + PR * p + tr) * N + cw; };
+        if (!GU && a.ep.res) {
 #pragma unroll
-            for (int p = 0; p < NP; ++p)
-              if (live(p)) load_vals<8>(a.ep.res, a.ep.res_bf16, at(p), add[p]);
-          }
+          for (int p = 0; p < NP; ++p)
+            if (live(p)) load_vals<8>(a.ep.res, a.ep.res_bf16, at(p), add[p]);
+        }
 #pragma unroll
-          for (int p = 0; p < NP; ++p) {
+        for (int p = 0; p < NP; ++p) {
+          auto put = [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
             for (int rr = 0; rr < PR / 2; ++rr) {   // the accumulator registers of the pass's rows
               const int r = PR / 2 * p + rr, lr = 8 * (rr >> 2) + 4 * h + (rr & 3);
 #pragma unroll
               for (int cc = 0; cc < CB; ++cc)
                 T[lr * PITCH + 32 * cc + lc] = GU ? act2(act, acc[i][cc][r] + b1[cc], acc[i][NJ - CB + cc][r] + b2[cc])
-                                                  : act1(act, acc[i][cc][r] + b1[cc]);
+                                                  : acc[i][cc][r] + b1[cc];
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            const f32x4 *t = reinterpret_cast<const f32x4 *>(T + tr * PITCH + tc);
-            const f32x4 t0 = t[0], t1 = t[1];
-            float v[8] = {t0[0], t0[1], t0[2], t0[3], t1[0], t1[1], t1[2], t1[3]};
-            if (!GU && a.ep.res) {
+          };
+          if constexpr (GU) with_act(a.ep.act, put);
+          else put(std::integral_constant<int, QMM_ACT_NONE>{});
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          float v[8];
+          act1_rows<8>(GU ? QMM_ACT_NONE : a.ep.act, T + tr * PITCH + tc, v);
+          if (!GU && a.ep.res) {
 #pragma unroll
-              for (int q = 0; q < 8; ++q) v[q] += add[p][q];
-            }
-            if (live(p)) store_vals<8>(a.ep.y, a.ep.y_bf16, at(p), v);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int q = 0; q < 8; ++q) v[q] += add[p][q];
           }
+          if (live(p)) store_vals<8>(a.ep.y, a.ep.y_bf16, at(p), v);
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-      };
-      constexpr std::integral_constant<int, GU ? QMM_ACT_SILU : QMM_ACT_NONE> usual;
-      if (a.ep.act == usual.value) finish(usual);
-      else finish(a.ep.act);
+      }
       return;
     }
   }
