@@ -214,7 +214,7 @@ __device__ __forceinline__ void act2_rows(int act, float *t, const float *t2, fl
     }
   });
 }
-// their gradients at dy
+// its gradient at dy
 template <int V>
 __device__ __forceinline__ void act1_grad_rows(int act, float *t, const float (&dy)[V], float (&d)[V]) {
   if (act == QMM_ACT_GELU_ERF) {
@@ -228,30 +228,6 @@ __device__ __forceinline__ void act1_grad_rows(int act, float *t, const float (&
     if constexpr (a.value != QMM_ACT_GELU_ERF && a.value != QMM_ACT_SWIGLU_OAI) {
 #pragma unroll
       for (int q = 0; q < V; ++q) d[q] = act1_grad(a.value, t[q], dy[q]);
-    }
-  });
-}
-template <int V>
-__device__ __forceinline__ void act2_grad_rows(int act, float *t, float *t2, const float (&dy)[V], float (&dg)[V], float (&du)[V]) {
-  if (act == QMM_ACT_GELU_ERF) {
-#pragma unroll 1
-    for (int q = 0; q < V; ++q) {
-      float a, da;
-      act1_slope(QMM_ACT_GELU_ERF, t[q], a, da);
-      t[q] = t2[q] * da;
-      t2[q] = a;
-    }
-#pragma unroll
-    for (int q = 0; q < V; ++q) {
-      dg[q] = dy[q] * t[q];
-      du[q] = dy[q] * t2[q];
-    }
-    return;
-  }
-  with_act(act, [&](auto a) __attribute__((always_inline)) {
-    if constexpr (a.value != QMM_ACT_GELU_ERF) {
-#pragma unroll
-      for (int q = 0; q < V; ++q) act2_grad(a.value, t[q], t2[q], dy[q], dg[q], du[q]);
     }
   });
 }
