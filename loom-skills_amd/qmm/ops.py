@@ -886,6 +886,8 @@ def rms_norm_backward(h, weight, dy, eps=1e-6, dh=None, out_dtype=None, dweight=
     _shaped(dy, shape, _VALUE, "dy")
     _shaped(dh, shape, _VALUE, "dh")
     dx = _rows_out(dx, shape, out_dtype if dx is not None or out_dtype is not None else h.dtype, h, h)
+    if dx.data_ptr() == dy.data_ptr():
+        raise ValueError("dx overlaps dy")
     dw, work, need = None, None, 0
     if dweight:
         need = _lib.load().qmm_rms_norm_grad_workspace_size(rows, k)
@@ -970,6 +972,8 @@ def _rows_out(y, shape, out_dtype, x, like=None):
     if out_dtype is not None and y.dtype != out_dtype:
         raise ValueError(f"y is {y.dtype}, out_dtype {out_dtype}")
     _shaped(y, shape, _VALUE, "y")
+    if y.data_ptr() == x.data_ptr():
+        raise ValueError("y overlaps the rows it is computed from")
     return y
 
 

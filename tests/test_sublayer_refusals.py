@@ -173,6 +173,15 @@ def test_rms_norm_errors(ops):
             ops.rms_norm(*a, **kw)
 
 
+def test_y_is_not_the_rows_of_x(ops):
+    k = 512
+    w, x = torch.zeros(k * k // 256 * 144, dtype=torch.uint8), torch.zeros(4, k)
+    for call in (lambda: ops.linear("q4_k", x, w, k, k, y=x, act="silu", q8=False), lambda: ops.ffn_gate_up("q4_k", x, w, w, k, k, y=x, q8=False),
+                 lambda: ops.gemm_t("q4_k", x, w, k, k, y=x)):
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
+
+
 def test_linear_backward_errors(ops):
     n, k, T = 32, 512, 4
     w, x, dy = torch.zeros(n * k // 256 * 144, dtype=torch.uint8), torch.zeros(T, k), torch.zeros(T, n)
@@ -187,7 +196,7 @@ def test_rms_norm_backward_errors(ops):
     x, w = torch.zeros(4, 64), torch.zeros(64)
     for a, kw in (((torch.zeros(64), w, x), {}), ((x.half(), w, x), {}), ((x, w[:32], x), {}), ((x, w.half(), x), {}), ((x, w, x[:2]), {}), ((x, w, x.half()), {}),
                   ((x, w, x), dict(dh=x[:, :32])), ((x, w, x), dict(dh=x.half())), ((x, w, x), dict(out_dtype=torch.float16)), ((x, w, x), dict(dx=x[:2])),
-                  ((x, w, x), dict(dx=x.half())), ((x, w, x), dict(dx=torch.zeros(4, 64), out_dtype=torch.bfloat16))):
+                  ((x, w, x), dict(dx=x.half())), ((x, w, torch.zeros(4, 64)), dict(dx=x)), ((torch.zeros(4, 64), w, x), dict(dx=x)), ((x, w, x), dict(dx=torch.zeros(4, 64), out_dtype=torch.bfloat16))):
         with pytest.raises(ValueError):
             ops.rms_norm_backward(*a, **kw)
 
