@@ -113,6 +113,14 @@ inline int launch_status() {
 
 // Raises kernel fn's dynamic-LDS limit to `bytes` (the largest any launch of it asks for) on the current device, once
 // per device: `done` holds one bit per device id (ids >= 32 are raised on every call, which is harmless).
+// A workgroup an item: HIP refuses 2^32 threads along one dimension of a grid, so that items past 2^21 lie along y (1024
+// threads a workgroup at most). item_index() may be past the last item.
+inline dim3 item_grid(int64_t items) {
+  const int64_t x = items < (1 << 21) ? items : 1 << 21;
+  return dim3((unsigned)x, (unsigned)((items + x - 1) / x));
+}
+__device__ __forceinline__ int64_t item_index() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 inline int raise_dyn_lds(const void *fn, int bytes, std::atomic<unsigned> &done) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return QMM_ERR_LAUNCH;

@@ -344,9 +344,10 @@ __device__ __forceinline__ float block_max(float m) {
 // A row's parts x n values into the f16 operand, a workgroup a row. n % 8 == 0, 16-byte aligned rows of at most 8 NT J values:
 // the row is read once, into registers.
 template <int NT, int J>
-__global__ __launch_bounds__(NT) void grad_operand_kernel(int parts, int n, int n64, const void *__restrict__ x, int bf,
+__global__ __launch_bounds__(NT) void grad_operand_kernel(int64_t rows, int parts, int n, int n64, const void *__restrict__ x, int bf,
                                                           _Float16 *__restrict__ x16, float *__restrict__ scales) {
-  const int64_t row = blockIdx.x;
+  const int64_t row = item_index();
+  if (row >= rows) return;
   const int chunks = parts * (n / 8), padded = parts * (n64 / 8);
   float v[J][8], m = 0.f;
 #pragma unroll
@@ -374,9 +375,10 @@ __global__ __launch_bounds__(NT) void grad_operand_kernel(int parts, int n, int 
   }
 }
 // any n and alignment: the row is read twice, the second time from L2 (2048 rows of 2 x 12288 bf16: 77 us, 33 above)
-__global__ __launch_bounds__(256) void grad_operand_any_kernel(int parts, int n, int n64, const void *__restrict__ x, int bf,
+__global__ __launch_bounds__(256) void grad_operand_any_kernel(int64_t rows, int parts, int n, int n64, const void *__restrict__ x, int bf,
                                                                _Float16 *__restrict__ x16, float *__restrict__ scales) {
-  const int64_t row = blockIdx.x, in0 = row * parts * n, out0 = row * parts * n64;
+  const int64_t row = item_index(), in0 = row * parts * n, out0 = row * parts * n64;
+  if (row >= rows) return;
   const int total = parts * n;
   float m = 0.f;
   for (int c = threadIdx.x; c < total; c += 256) m = fmaxf(m, fabsf(load_val(x, bf, in0 + c)));
@@ -456,8 +458,8 @@ extern "C" int qmm_grad_operand(int64_t rows, int parts, int64_t n, const void *
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int64_t chunks = parts * (n / 8);
   auto go = [&](auto *kernel, int threads) {
-    kernel<<<(unsigned)rows, threads, 0, s>>>(parts, (int)n, (int)n64_of(n), x, x_dtype == QMM_BF16,
-                                              static_cast<_Float16 *>(x16), scales);
+    kernel<<<item_grid(rows), threads, 0, s>>>(rows, parts, (int)n, (int)n64_of(n), x, x_dtype == QMM_BF16,
+                                               static_cast<_Float16 *>(x16), scales);
     return launch_status();
   };
   if (n % 8 || !aligned(x, 16) || !aligned(scales, 8) || chunks > 8192) return go(grad_operand_any_kernel, 256);

@@ -671,7 +671,8 @@ int qmm_mv_gate_up_impl(int fmt, int64_t k, int64_t n, int64_t tokens, const voi
   if (!valid_fmt(fmt)) return QMM_ERR_FORMAT;
   if (!x) return QMM_ERR_NULL;
   if (n <= 0 || tokens <= 0 || row_bytes(fmt, k) == 0) return QMM_ERR_SHAPE;
-  if (tokens > (1 << 24) || k > (1 << 24) || n > 65535ll * kWavesPerBlock * expert_rw<true>()) return QMM_ERR_SHAPE;   // the grid
+  if (tokens >= (1 << 24) || k > (1 << 24) || n > 65535ll * kWavesPerBlock * expert_rw<true>()) return QMM_ERR_SHAPE;   // the grid: 256
+                                                                                       // threads a token, fewer than 2^32
   if (x_dtype != QMM_F32 && x_dtype != QMM_BF16) return QMM_ERR_DTYPE;
   if (int st = check_weights(fmt, k, w, ws)) return st;
   if (int st = check_weights(fmt, k, w2, ws2)) return st;

@@ -89,7 +89,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(NArgs a) {
   constexpr int kRows = L < 256 ? 256 / L : 1;
   __shared__ float part[2][L > 64 ? L / 64 : 1];
   const int l = threadIdx.x % L;
-  const int64_t row_ = (int64_t)blockIdx.x * kRows + threadIdx.x / L;
+  const int64_t first = item_index() * kRows, row_ = first + threadIdx.x / L;
+  if (first >= a.rows) return;
   const bool alive = row_ < a.rows;
   const int64_t row = alive ? row_ : a.rows - 1;   // lanes of rows past the last stay for the exchanges and store nothing
   const int chunks = (int)(a.k / 8);
@@ -187,7 +188,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(NArgs a) {
 template <int OUT>
 __global__ __launch_bounds__(256) void rms_norm_any_kernel(NArgs a) {
   __shared__ float part[2][4];
-  const int64_t r0 = (int64_t)blockIdx.x * a.k;
+  const int64_t row = item_index(), r0 = row * a.k;
+  if (row >= a.rows) return;
   auto at = [](const void *p, int bf, int64_t i) {
     return bf ? bf16_to_f32(static_cast<const u16 *>(p)[i]) : static_cast<const float *>(p)[i];
   };
@@ -209,8 +211,8 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(NArgs a) {
     for (int64_t c = threadIdx.x; c < a.k; c += 256) m = fmaxf(m, fabsf(value(c, sum_at(c))));
     e = f16_exponent(row_reduce<256, true>(m, part[1]));
     if (threadIdx.x == 0) {
-      static_cast<float *>(a.scales)[2 * blockIdx.x] = pow2(-e);
-      static_cast<float *>(a.scales)[2 * blockIdx.x + 1] = pow2(e);
+      static_cast<float *>(a.scales)[2 * row] = pow2(-e);
+      static_cast<float *>(a.scales)[2 * row + 1] = pow2(e);
     }
   }
   for (int64_t c = threadIdx.x; c < a.k; c += 256) {
@@ -224,7 +226,7 @@ __global__ __launch_bounds__(256) void rms_norm_any_kernel(NArgs a) {
 template <int OUT, int L, int J>
 int launch(const NArgs &a, hipStream_t s) {
   constexpr int kRows = L < 256 ? 256 / L : 1;
-  rms_norm_kernel<OUT, L, J><<<(unsigned)((a.rows + kRows - 1) / kRows), L < 256 ? 256 : L, 0, s>>>(a);
+  rms_norm_kernel<OUT, L, J><<<item_grid((a.rows + kRows - 1) / kRows), L < 256 ? 256 : L, 0, s>>>(a);
   return launch_status();
 }
 
@@ -232,7 +234,7 @@ template <int OUT>
 int dispatch(const NArgs &a, bool vec, hipStream_t s) {
   if (!vec) {
     if constexpr (OUT == QMM_F32 || OUT == QMM_BF16 || OUT == QMM_F16) {
-      rms_norm_any_kernel<OUT><<<(unsigned)a.rows, 256, 0, s>>>(a);
+      rms_norm_any_kernel<OUT><<<item_grid(a.rows), 256, 0, s>>>(a);
       return launch_status();
     } else {
       return QMM_ERR_ALIGN;
@@ -282,7 +284,8 @@ __device__ __forceinline__ void row_reduce2(float &u, float &v, float2 *part) {
   }
 }
 
-// lanes and chunks as rms_norm_kernel; row group g = blockIdx.x, + gridDim.x, ... (DW; without it one group a workgroup)
+// lanes and chunks as rms_norm_kernel; row group g = blockIdx.x, + gridDim.x, ... (without DW one group a workgroup, up to
+// the most workgroups of a grid)
 template <int L, int J, bool DW>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_grad_kernel(BArgs a) {
   constexpr int kRows = L < 256 ? 256 / L : 1;
@@ -364,7 +367,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_grad_kernel(BArgs 
 template <int V>
 __global__ __launch_bounds__(512) void rms_norm_grad_long_kernel(BArgs a) {
   __shared__ float2 part[8];
-  const int64_t r0 = (int64_t)blockIdx.x * a.k;
+  const int64_t row = item_index(), r0 = row * a.k;
+  if (row >= a.rows) return;
   auto load = [](const void *p, int bf, int64_t at, float (&v)[V]) __attribute__((always_inline)) {
     if constexpr (V == 8) load8_act(p, bf, at, v);
     else v[0] = load_val(p, bf, at);
@@ -383,7 +387,7 @@ __global__ __launch_bounds__(512) void rms_norm_grad_long_kernel(BArgs a) {
   }
   row_reduce2<512>(hh, gh, part);
   const float rate = norm_rate(hh, a.k, a.eps), mean = rate * (gh / (float)a.k);
-  if (a.part && threadIdx.x == 0) a.rate[blockIdx.x] = rate;
+  if (a.part && threadIdx.x == 0) a.rate[row] = rate;
   for (int64_t c = V * threadIdx.x; c < a.k; c += V * 512) {
     float h[V], d[V], w[V], e[V];
     load(a.h, a.h_bf16, r0 + c, h);
@@ -437,7 +441,7 @@ int launch_grad(const BArgs &a, float *dw, hipStream_t s) {
   constexpr int kRows = L < 256 ? 256 / L : 1, kThreads = L < 256 ? 256 : L;
   const int64_t groups = (a.rows + kRows - 1) / kRows;
   if (!dw) {
-    rms_norm_grad_kernel<L, J, false><<<(unsigned)groups, kThreads, 0, s>>>(a);
+    rms_norm_grad_kernel<L, J, false><<<item_grid(groups).x, kThreads, 0, s>>>(a);
     return launch_status();
   }
   constexpr int64_t kMost = J == 1 ? kParts : kParts2;
@@ -514,8 +518,8 @@ extern "C" int qmm_rms_norm_grad(int64_t rows, int64_t k, const void *h, int h_d
   if (vec && chunks <= 1024) return launch_grad<512, 2>(a, dweight, s);
   const unsigned n = (unsigned)(rows < kPartsLong ? rows : kPartsLong);
   if (dweight) a.rate = a.part + (int64_t)n * k;
-  if (vec) rms_norm_grad_long_kernel<8><<<(unsigned)rows, 512, 0, s>>>(a);
-  else rms_norm_grad_long_kernel<1><<<(unsigned)rows, 512, 0, s>>>(a);
+  if (vec) rms_norm_grad_long_kernel<8><<<item_grid(rows), 512, 0, s>>>(a);
+  else rms_norm_grad_long_kernel<1><<<item_grid(rows), 512, 0, s>>>(a);
   if (int st = launch_status()) return st;
   if (!dweight) return QMM_OK;
   rms_norm_dweight_part_kernel<<<dim3((unsigned)((k + 255) / 256), n), 256, 0, s>>>(a);
