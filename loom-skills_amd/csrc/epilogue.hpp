@@ -136,10 +136,12 @@ __device__ __forceinline__ void act1_slope(int act, float v, float &a, float &da
       da = c + 0.3989422804014327f * v * expf(-0.5f * v * v);
       return;
     }
-    case QMM_ACT_SIGMOID:
-      a = sigmoid_fast_(v);
-      da = a * (1.0f - a);
+    case QMM_ACT_SIGMOID: {   // s(v) s(-v) from e = e^-|v|: 1 - s(v) has no bits left for v past 17
+      const float e = __expf(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
+      a = v < 0.f ? e * r : r;
+      da = e * r * r;
       return;
+    }
     default:
       a = v;
       da = 1.f;
