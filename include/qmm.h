@@ -256,7 +256,7 @@ int qmm_ffn_gate_up_grad(int fmt, int act, int64_t tokens, int64_t k, int64_t n,
 
 /* The operand of qmm_gemm_t from gradient rows x [rows, parts, n] (f32 or bf16; parts 1 or 2): x16 f16 [rows, parts, N] with
  * N = n rounded up to a multiple of 64 (the added columns zero), scales f32 [rows, 2] = (2^-e, 2^e) with the row's largest
- * magnitude times 2^-e in [2^13, 2^14), -126 <= e <= 100 (e = 0 for rows of zeros, subnormals, and with infinities;
+ * magnitude times 2^-e in [2^13, 2^14), -126 <= e <= 114 (e = 0 for rows of zeros, subnormals, and with infinities;
  * NaN values are passed over and stay NaN). */
 int qmm_grad_operand(int64_t rows, int parts, int64_t n, const void *x, int x_dtype, void *x16, float *scales,
                      qmm_stream_t stream);

@@ -320,11 +320,11 @@ __global__ __launch_bounds__(256) void gemm_t_join_kernel(int64_t quads, int K, 
   for (int q = 0; q < 4; ++q) store_val(y, y_bf16, 4 * i + q, s[q] * inv);
 }
 
-// 2^-e brings the largest magnitude m into [2^13, 2^14): gradients are small, so e may be negative (the forward operand's is
-// not); a row of zeros or subnormals, or with infinities, takes e = 0 (NaN values are passed over and stay NaN)
+// 2^-e brings the largest magnitude m into [2^13, 2^14), up to the largest floats' 2^127 (e = 114): gradients are small, so e may
+// be negative (the forward operand's is not); a row of zeros or subnormals, or with infinities, takes e = 0 (NaN values are passed over and stay NaN)
 __device__ __forceinline__ int grad_exponent(float m) {
   const int biased = (int)((f32_as_u32(m) >> 23) & 255u);
-  return biased == 0 || biased == 255 ? 0 : min(max(biased - 140, -126), 100);
+  return biased == 0 || biased == 255 ? 0 : max(biased - 140, -126);
 }
 __device__ __forceinline__ float pow2(int e) { return u32_as_f32((u32)(127 + e) << 23); }
 // the row's maximum over a workgroup of NT threads

@@ -25,3 +25,20 @@ def test_sigmoid_slope_keeps_its_bits(dev, n):
     _, dgu = ops.ffn_gate_up_backward("q4_0", x, w.w, w.w, dy, n, 256, scales=s, bias=b, bias2=one, act="sigmoid")
     close(f64(dpre), want.expand(3, n), tol.expand(3, n), "dpre")
     close(f64(dgu[:, 0]), want.expand(3, n), tol.expand(3, n), "dg")
+
+
+@pytest.mark.parametrize("n", [64, 63, 8 * 8193])
+def test_gradient_rows_near_the_largest_floats(dev, n):
+    """The exponent of a row's scale reaches the largest floats': finite rows stay finite, in [2^13, 2^14) for their largest value."""
+    import qmm.ops as ops
+    from qmm import _lib
+    T, N = 5, -(-n // 64) * 64
+    x = torch.from_numpy(np.random.default_rng(2).uniform(-1, 1, (T, 1, n)).astype(np.float32)).to(dev)
+    x[:, 0, 0] = 1
+    x = x * torch.tensor([2.0 ** 113, 2.0 ** 114, 2.0 ** 117, 2.0 ** 126, 2.0 ** 127], device=dev).reshape(-1, 1, 1)
+    x16 = torch.empty((T, 1, N), dtype=torch.float16, device=dev)
+    s = torch.empty((T, 2), device=dev)
+    _lib.call("qmm_grad_operand", T, 1, n, x.data_ptr(), 0, x16.data_ptr(), s.data_ptr(), ops._stream())
+    assert torch.equal(s[:, 1].log2(), torch.tensor([100.0, 101, 104, 113, 114], device=dev)) and (s[:, 0] * s[:, 1] == 1).all()
+    assert torch.equal(x16[..., :n], (x * s[:, :1, None]).half()) and (x16[..., n:] == 0).all()
+    assert (x16.abs().amax((1, 2)) == 2.0 ** 13).all()
