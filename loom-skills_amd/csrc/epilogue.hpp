@@ -43,8 +43,15 @@ __device__ __forceinline__ float act1(int act, float v) {
     default: return v;
   }
 }
+// swiglu_oai's clamps by comparisons, which keep a NaN (fminf and fmaxf return their other argument); other values as act_fn's
+__device__ __forceinline__ float oai_gate(float g) { return g > 7.0f ? 7.0f : g; }
+__device__ __forceinline__ float oai_up(float u) { return u > 7.0f ? 7.0f : u < -7.0f ? -7.0f : u; }
 __device__ __forceinline__ float act2(int act, float g, float u) {
-  return act == QMM_ACT_SILU || act == QMM_ACT_SWIGLU_OAI ? act_fn(act, g, u) : act1(act, g) * u;
+  if (act == QMM_ACT_SWIGLU_OAI) {
+    const float xg = oai_gate(g);
+    return xg / (1.0f + expf(-1.702f * xg)) * (oai_up(u) + 1.0f);
+  }
+  return act == QMM_ACT_SILU ? act_fn(act, g, u) : act1(act, g) * u;
 }
 
 __device__ __forceinline__ float load_val(const void *p, int bf16, int64_t o) {
@@ -156,7 +163,7 @@ __device__ __forceinline__ float act1_grad(int act, float v, float dy) {
 // the gradients of act2(g, u) at dy. swiglu_oai: those of the clamps are 1 up to and at their limits, 0 past them
 __device__ __forceinline__ void act2_grad(int act, float g, float u, float dy, float &dg, float &du) {
   if (act == QMM_ACT_SWIGLU_OAI) {
-    const float xg = fminf(g, 7.0f), yu = fminf(fmaxf(u, -7.0f), 7.0f), s = sigmoid_fast_(1.702f * xg);
+    const float xg = oai_gate(g), yu = oai_up(u), s = sigmoid_fast_(1.702f * xg);
     dg = g > 7.0f ? 0.f : dy * (yu + 1.0f) * s * (1.0f + 1.702f * xg * (1.0f - s));
     du = fabsf(u) > 7.0f ? 0.f : dy * xg * s;
     return;

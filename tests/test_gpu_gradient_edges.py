@@ -42,3 +42,32 @@ def test_gradient_rows_near_the_largest_floats(dev, n):
     assert torch.equal(s[:, 1].log2(), torch.tensor([100.0, 101, 104, 113, 114], device=dev)) and (s[:, 0] * s[:, 1] == 1).all()
     assert torch.equal(x16[..., :n], (x * s[:, :1, None]).half()) and (x16[..., n:] == 0).all()
     assert (x16.abs().amax((1, 2)) == 2.0 ** 13).all()
+
+
+@pytest.mark.parametrize("kind,fmt,T,n,k", [("f16", "q4_k", 70, 96, 256), ("f16", "q6_k", 70, 95, 256), ("f16", "q4_0", 1500, 2104, 256), ("f32", "q4_0", 1, 40, 256),
+                                            ("f32", "q4_0", 9, 40, 256), ("q8", "q4_k", 1, 40, 512), ("q8", "q4_k", 20, 40, 512), ("mxfp8", "mxfp4t", 70, 96, 256),
+                                            ("mxfp8", "mxfp4s", 70, 95, 256)])
+def test_clamped_gate_of_nan_is_nan(dev, kind, fmt, T, n, k):
+    """swiglu_oai's clamps keep a NaN of either projection, and take infinities to their limits."""
+    import qmm.ops as ops
+    from test_gpu_linear_epilogue import _operand
+    rng = np.random.default_rng(n)
+    w = Weight(fmt, rng, n, k, dev)
+    x, kw, _ = _operand(kind, rng, T, k, dev)
+    b, b2 = torch.zeros(n, device=dev), torch.zeros(n, device=dev)
+    call = lambda: ops.ffn_gate_up(fmt, x, w.w, w.w, n, k, ws=w.ws, ws2=w.ws, bias=b, bias2=b2, act="swiglu_oai", out_dtype=torch.float32, **kw)   # noqa: E731
+    clean = call()
+    b[3], b2[5] = float("nan"), float("nan")
+    b[7], b2[8], b2[9] = float("inf"), float("inf"), float("-inf")
+    y = call()
+    assert y[:, [3, 5]].isnan().all() and y[:, [7, 8, 9]].isfinite().all()
+    keep = [i for i in range(n) if i not in (3, 5, 7, 8, 9)]
+    assert torch.equal(y[:, keep], clean[:, keep])
+    if kind != "f16":
+        return
+    dy = torch.ones((T, n), device=dev)
+    _, dgu = ops.ffn_gate_up_backward(fmt, x, w.w, w.w, dy, n, k, bias=b, bias2=b2, act="swiglu_oai", **kw)
+    assert dgu[:, 0, 3].isnan().all()
+    for d in (dgu[:, 1, 3], dgu[:, 0, 5]):   # past a limit its slope is 0 whatever the other's value
+        assert (d.isnan() | (d == 0)).all()
+    assert dgu[:, 0, 5].isnan().any()
