@@ -368,6 +368,19 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
     nlive = (u32)(b >> 32) ? 2 * i + 2 : nlive;
   }
   nlive = __builtin_amdgcn_readfirstlane(nlive);
+  if constexpr (grad_kind(KIND)) {   // padding rows have no gradient: zeros, which sums over the rows may read
+#pragma unroll
+    for (int i = 0; i < BM / 64; ++i) {
+      if (live_rows[i] != 0) continue;
+      for (int e = tid; e < 64 * BN; e += 64 * NW * KS) {
+        const int row = m0 + 64 * i + e / BN, col = n0 + e % BN;
+        if (row >= M || col >= N) continue;
+        u16 *d = static_cast<u16 *>(a.ep.y) + (int64_t)row * (kTwoW ? 2 : 1) * N + col;
+        d[0] = 0;
+        if constexpr (kTwoW) d[N] = 0;
+      }
+    }
+  }
   if (nlive == 0) return;
 
   // ---- the K-part's steps of 128 values

@@ -71,3 +71,38 @@ def test_clamped_gate_of_nan_is_nan(dev, kind, fmt, T, n, k):
     for d in (dgu[:, 1, 3], dgu[:, 0, 5]):   # past a limit its slope is 0 whatever the other's value
         assert (d.isnan() | (d == 0)).all()
     assert dgu[:, 0, 5].isnan().any()
+
+
+@pytest.mark.parametrize("fmt,T,n,k", [("q4_k", 200, 136, 512), ("q6_k", 200, 133, 512), ("q4_0", 77, 768, 256), ("q4_k", 2011, 4104, 256), ("q4_kt", 1000, 2064, 512),
+                                       ("q6_k", 1500, 4099, 256)])
+def test_padding_rows_have_no_gradient(dev, fmt, T, n, k):
+    """64-row tiles of padding rows: zeros in dpre, dgu and dx, so that sums over the rows (a bias's gradient) hold the others' alone."""
+    import qmm.ops as ops
+    from qmm import _lib
+    from qmm.formats import CODE
+    rng = np.random.default_rng(T)
+    w, u = Weight(fmt, rng, n, k, dev), Weight(fmt, rng, n, k, dev)
+    x = torch.from_numpy(rng.standard_normal((T, k)).astype(np.float32)).to(dev)
+    dy = torch.from_numpy(rng.standard_normal((T, n)).astype(np.float32)).to(dev)
+    b = torch.from_numpy(rng.standard_normal(n).astype(np.float32)).to(dev)
+    live = torch.ones(T, dtype=torch.bool, device=dev)
+    live[64:128] = False
+    live[64 * ((T - 1) // 64):] = False   # the last tile, ragged
+    if T > 1000:
+        live[512:1024] = False            # whole tiles of 128 rows and more
+    info = live.int().reshape(-1, 1).expand(T, 4).contiguous()
+    x16, s = ops.row_scale_f16(x, info=info)
+    full, fs = ops.row_scale_f16(x)
+    assert (s[~live, 0] == 0).all() and torch.equal(x16[live], full[live])
+    dpre = torch.full((T, n), float("nan"), dtype=torch.bfloat16, device=dev)
+    dgu = torch.full((T, 2, n), float("nan"), dtype=torch.bfloat16, device=dev)
+    st = ops._stream()
+    _lib.call("qmm_linear_grad", CODE[fmt], 0, T, k, n, x16.data_ptr(), s.data_ptr(), w.w.data_ptr(), b.data_ptr(), dy.data_ptr(), 0, dpre.data_ptr(), st)
+    _lib.call("qmm_ffn_gate_up_grad", CODE[fmt], 0, T, k, n, x16.data_ptr(), s.data_ptr(), w.w.data_ptr(), u.w.data_ptr(), b.data_ptr(), None, dy.data_ptr(), 0,
+              dgu.data_ptr(), st)
+    dx, dp = ops.linear_backward(fmt, x16, w.w, dy, n, k, scales=s, bias=b, act="silu")
+    dx2, dg = ops.ffn_gate_up_backward(fmt, x16, w.w, u.w, dy, n, k, scales=s, bias=b)
+    want = ops.linear_backward(fmt, full, w.w, dy, n, k, scales=fs, bias=b, act="silu")
+    want2 = ops.ffn_gate_up_backward(fmt, full, w.w, u.w, dy, n, k, scales=fs, bias=b)
+    for got, ref in ((dpre, want[1]), (dgu, want2[1]), (dp, want[1]), (dg, want2[1]), (dx, want[0]), (dx2, want2[0])):
+        assert torch.equal(got[live], ref[live]) and (got[~live] == 0).all()
