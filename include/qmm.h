@@ -181,8 +181,8 @@ int qmm_gemm_mxfp4(int fmt, int mode, int64_t rows, int64_t k, int64_t n, const 
  * reference kernel: its norm writes f32 rows that a quantizer reads):
  *   h = x + residual (x without one);   y[t, c] = h[t, c] / sqrt(mean_c(h[t]^2) + eps) * weight[c]
  * x: [rows, k] f32 or bf16; residual: [rows, k] f32 or bf16, or NULL; weight: [k] f32 or bf16; h: NULL, or [rows, k] of the
- * residual's type (rounded to nearest even), which may be x or residual itself where the types agree. The norm is that of
- * the f32 sum, before h is rounded. out by out_dtype:
+ * residual's type (rounded to nearest even), which may be x or residual itself where the types agree and overlaps nothing
+ * else (nor does out). The norm is that of the f32 sum, before h is rounded. out by out_dtype:
  *   QMM_F32 / QMM_BF16  y [rows, k]
  *   QMM_F16             the qmm_gemm operand: x16 [rows, k], out_scales f32 [rows, 2], as qmm_row_scale_f16 of y
  *   QMM_Q8              the int8 matvecs' planar Q8_1 buffer, as qmm_quant_q8 of y (k % 32 == 0)
@@ -210,8 +210,9 @@ int64_t qmm_rms_norm_grad_workspace_size(int64_t rows, int64_t k);
 /* Product with a bias, an activation and a residual in its epilogue (the reference adds them in kernels of their own):
  *   y[t, r] = act(sum_k x[t, k] W[r, k] + bias[r]) + residual[t, r]
  * act: QMM_ACT_NONE, RELU, SILU, SIGMOID, GELU or GELU_ERF. bias f32 [n] or NULL; residual [tokens, n] f32 or bf16 or NULL,
- * may be y itself where the types agree; y [tokens, n] of y_dtype (QMM_F32, or QMM_BF16 rounded to nearest even, the only
- * rounding after the f32 sum). x by x_dtype takes the matching product's formats, shapes, alignment and limits:
+ * may be y itself where the types agree (y overlaps nothing else); y [tokens, n] of y_dtype (QMM_F32, or QMM_BF16 rounded to
+ * nearest even, the only rounding after the f32 sum). x by x_dtype takes the matching product's formats, shapes, alignment
+ * and limits:
  *   QMM_F32 / QMM_BF16  qmm_mv (rows [tokens, k]; x_scales unused)
  *   QMM_Q8              qmm_mv_q8 on the planar Q8_1 buffer, or qmm_mv_mxfp4s_q8 (fmt QMM_MXFP4S)
  *   QMM_F16             qmm_gemm, x_scales f32 [tokens, 2] or NULL (64-row tiles of padding rows are not written)

@@ -760,6 +760,23 @@ def _shaped(t, shape, dtypes, what):
                          f"{' or '.join(str(d) for d in dtypes)}")
 
 
+def _apart(y, what, reads, same=()):
+    """A given output shares no byte with what the kernel reads in other workgroups while it is written, except that it may be
+    one of same itself (each value of those is read by the thread that writes it)."""
+    a = y.data_ptr()
+    b = a + y.nbytes
+    for t in reads:
+        if t is not None:
+            p = t.data_ptr()
+            if p < b and (p >= a or p + t.nbytes > a):
+                raise ValueError(f"{what} overlaps a tensor it is computed from")
+    for t in same:
+        if t is not None and t is not y:
+            p = t.data_ptr()
+            if p < b and (p >= a or p + t.nbytes > a) and (p != a or t.shape != y.shape or t.dtype != y.dtype):
+                raise ValueError(f"{what} overlaps a tensor it is computed from and is not that tensor")
+
+
 _VALUE = (torch.float32, torch.bfloat16)   # the types of rows that epilogues read and write
 
 
@@ -836,8 +853,8 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out="bf16", h=None):
         out "q8"            the planar Q8_1 buffer of quant_q8 (pass tokens=rows with it), scales None
         out "mxfp8"         (codes, scales) of quant_mxfp8, for the MXFP4 GEMMs
 
-    h has the residual's type (None without one); the h argument takes the output rows, x or residual for an update in
-    place."""
+    h has the residual's type (None without one); the h argument takes the output rows, x or residual itself for an update
+    in place; it overlaps nothing else."""
     s = _here(x, weight, residual, h)
     if x.dim() != 2:
         raise ValueError(f"x is {tuple(x.shape)}, expected [rows, k]")
@@ -850,6 +867,7 @@ def rms_norm(x, weight, eps=1e-6, residual=None, out="bf16", h=None):
             h = torch.empty_like(residual)
         else:
             _shaped(h, shape, (residual.dtype,), "h")
+            _apart(h, "h", (weight,), (x, residual))
     elif h is not None:
         raise ValueError("h is written with a residual")
     scales = None
@@ -876,7 +894,7 @@ def rms_norm_backward(h, weight, dy, eps=1e-6, dh=None, out_dtype=None, dweight=
     """The gradients of rms_norm at its h (x where it had no residual), dy of its normed rows and dh of its h (None: no such
     gradient): (dx [rows, k], the gradient of x and of the residual; dweight f32 [k], or None with dweight=False)
     (qmm_rms_norm_grad). h, dy, dh f32 / bf16 [rows, k], weight f32 / bf16 [k]; dx of out_dtype (h's when None), or the
-    caller's rows, dh allowed."""
+    caller's rows, dh itself allowed; it overlaps nothing else."""
     s = _here(h, weight, dy, dh, dx)
     if h.dim() != 2:
         raise ValueError(f"h is {tuple(h.shape)}, expected [rows, k]")
@@ -885,9 +903,7 @@ def rms_norm_backward(h, weight, dy, eps=1e-6, dh=None, out_dtype=None, dweight=
     _shaped(weight, (k,), _VALUE, "weight")
     _shaped(dy, shape, _VALUE, "dy")
     _shaped(dh, shape, _VALUE, "dh")
-    dx = _rows_out(dx, shape, out_dtype if dx is not None or out_dtype is not None else h.dtype, h, h)
-    if dx.data_ptr() == dy.data_ptr():
-        raise ValueError("dx overlaps dy")
+    dx = _rows_out(dx, shape, out_dtype if dx is not None or out_dtype is not None else h.dtype, h, (h, weight, dy), h, dh, "dx")
     dw, work, need = None, None, 0
     if dweight:
         need = _lib.load().qmm_rms_norm_grad_workspace_size(rows, k)
@@ -916,7 +932,7 @@ def linear(fmt, x, w, n, k, y=None, mode="store", ws=None, w2=None, ws2=None, q8
     y = act(x W^T + bias) + residual (qmm_linear, mode "store"). x may then also be an operand: a planar Q8_1 buffer with
     tokens, the row-scaled f16 rows or E4M3 codes with their scales; the operand chooses the product whatever the token
     count. GGUF mxfp4 blocks take up to 63 rows (repack_mxfp4 for more). The sums are those of the plain call, in some
-    shapes added in another f32 order (qmm_linear). y may be the residual; it may overlap no other argument."""
+    shapes added in another f32 order (qmm_linear). y may be the residual itself; it overlaps nothing else."""
     if bias is not None or act != "none" or residual is not None or out_dtype is not None or scales is not None or \
             tokens is not None or (y is not None and y.dtype == torch.bfloat16 and mode == "store" and x.shape[0] < GEMM_MIN_TOKENS):
         if mode != "store" or w2 is not None or ws2 is not None:
@@ -953,7 +969,7 @@ def _linear_epilogue(fmt, x, w, n, k, y, ws, q8, bias, act, residual, out_dtype,
         _shaped(bias, (n,), (torch.float32,), "bias")
     if residual is not None:
         _shaped(residual, (T, n), _VALUE, "residual")
-    y = _rows_out(y, (T, n), out_dtype, x, residual)
+    y = _rows_out(y, (T, n), out_dtype, x, (x, w, ws, bias, scales), residual, residual)
     x, xd, scales = _product_operand(fmt, x, k, scales, tokens, q8)
     _lib.call("qmm_linear", CODE[fmt], code, T, k, n, x.data_ptr(), xd, None if scales is None else scales.data_ptr(),
               w.data_ptr(), None if ws is None else ws.data_ptr(), None if bias is None else bias.data_ptr(),
@@ -962,18 +978,18 @@ def _linear_epilogue(fmt, x, w, n, k, y, ws, q8, bias, act, residual, out_dtype,
     return y
 
 
-def _rows_out(y, shape, out_dtype, x, like=None):
-    """The f32 / bf16 output rows: y, or a new tensor of out_dtype (f32 when None); like: a tensor of that shape or None."""
+def _rows_out(y, shape, out_dtype, x, reads, like=None, same=None, what="y"):
+    """The f32 / bf16 output rows: y, or a new tensor of out_dtype (f32 when None); like: a tensor of that shape or None; reads: what
+    y may not overlap; same: the tensor or None that it may be."""
     if y is None:
         dtype = torch.float32 if out_dtype is None else out_dtype
         if dtype not in _VALUE:
             raise ValueError(f"out_dtype is float32 or bfloat16, not {out_dtype}")
         return torch.empty_like(like) if like is not None and like.dtype == dtype else x.new_empty(shape, dtype=dtype)
     if out_dtype is not None and y.dtype != out_dtype:
-        raise ValueError(f"y is {y.dtype}, out_dtype {out_dtype}")
-    _shaped(y, shape, _VALUE, "y")
-    if y.data_ptr() == x.data_ptr():
-        raise ValueError("y overlaps the rows it is computed from")
+        raise ValueError(f"{what} is {y.dtype}, out_dtype {out_dtype}")
+    _shaped(y, shape, _VALUE, what)
+    _apart(y, what, reads, (same,))
     return y
 
 
@@ -1028,7 +1044,7 @@ def ffn_gate_up(fmt, x, w, w2, n, k, y=None, ws=None, ws2=None, q8="auto", bias=
         _shaped(bias, (n,), (torch.float32,), "bias")
     if bias2 is not None:
         _shaped(bias2, (n,), (torch.float32,), "bias2")
-    y = _rows_out(y, (T, n), out_dtype, x)
+    y = _rows_out(y, (T, n), out_dtype, x, (x, w, ws, w2, ws2, bias, bias2, scales))
     x, xd, scales = _product_operand(fmt, x, k, scales, tokens, q8)
     _lib.call("qmm_ffn_gate_up", CODE[fmt], code, T, k, n, x.data_ptr(), xd, None if scales is None else scales.data_ptr(),
               w.data_ptr(), None if ws is None else ws.data_ptr(), w2.data_ptr(), None if ws2 is None else ws2.data_ptr(),
@@ -1071,7 +1087,7 @@ def gemm_t(fmt, x, w, n, k, w2=None, out_dtype=torch.float32, y=None):
         _weight_bytes(fmt, w2, None, n, k, "w2")
     rows, parts = x.shape[0], 1 if w2 is None else 2
     _shaped(x, (rows, n) if w2 is None else (rows, 2, n), _VALUE, "x")
-    y = _rows_out(y, (rows, k), None if y is not None else out_dtype, x)
+    y = _rows_out(y, (rows, k), None if y is not None else out_dtype, x, (x, w, w2))
     need = _lib.load().qmm_gemm_t_workspace_size(CODE[fmt], rows, k, n, parts - 1)
     if need < 0:
         raise ValueError(f"the transposed product does not take {rows} rows of {fmt} [{n}, {k}]")
