@@ -782,6 +782,8 @@ _VALUE = (torch.float32, torch.bfloat16)   # the types of rows that epilogues re
 
 def _weight_bytes(fmt, w, ws, n, k, what="w"):
     """The kernels cannot see sizes: a weight tensor too small for [n, k] would be read past its end."""
+    if fmt not in CODE:
+        raise ValueError(f"{fmt!r} is not one of the formats {', '.join(CODE)} (both matrices of a gated block are of one)")
     if w is None or w.nbytes < n * row_bytes(fmt, k):
         raise ValueError(f"{what} is too small for {fmt} [{n}, {k}] ({n * row_bytes(fmt, k)} bytes)")
     if fmt in SPLIT:
@@ -1033,8 +1035,8 @@ def _backward_operand(fmt, x, dy, n, k, scales):
 def ffn_gate_up(fmt, x, w, w2, n, k, y=None, ws=None, ws2=None, q8="auto", bias=None, bias2=None, act="silu",
                 out_dtype=None, scales=None, tokens=None):
     """The gated feed-forward block's first half, y = act(x W^T + bias) (x W2^T + bias2), in one kernel past the operand's
-    (qmm_ffn_gate_up). x, scales, tokens, q8 as linear; biases f32 [n] or None; act as linear or swiglu_oai (the gpt-oss
-    clamped form); y [tokens, n] f32 or bf16 (out_dtype)."""
+    (qmm_ffn_gate_up), both matrices of one format. x, scales, tokens, q8 as linear; biases f32 [n] or None; act as linear or
+    swiglu_oai (the gpt-oss clamped form); y [tokens, n] f32 or bf16 (out_dtype)."""
     s = _here(x, w, ws, w2, ws2, bias, bias2, scales, y)
     code = _act_code(act, GATE_ACT)
     _weight_bytes(fmt, w, ws, n, k)
