@@ -16,9 +16,12 @@
 //           parts that are stored, each exact
 //   MXFP4   2^e dot                Q8_1: times the group's da
 //
-// What bounds it: the vector instructions that unpack weights and split activations (30 - 90 a group of 16 rows x 32 values);
-// loads are coalesced (neighbouring lanes on neighbouring bytes, through the wave's own LDS): with every lane reading its own
-// row the address unit took 64 cycles a load and was the bound (12288 x 4096 Q4_0, bf16 rows, two tokens: 32 us).
+// What bounds it: the vector instructions that unpack weights and split activations (30 - 90 a group of 16 rows x 32 values) in
+// large calls (Q6_K 12288 x 4096 at 63 rows: vector pipes 0.67 busy on f32 rows, 0.65 on Q8_1, MFMA 0.32 and 0.19, waves waiting
+// 0.33 and 0.40 of their time); in small ones those and the wait for loads alike (Q4_0 6144 x 2048, five f32 rows: 0.50, waiting
+// 0.42). Gate and up at once: Q4_0 2 x 6144 x 2048 13.4 us at five f32 rows, 18.5 at 33 bf16 rows; Q6_K 2 x 4096 x 4096 21.0 at 17
+// Q8_1 rows. Loads are coalesced (neighbouring lanes on neighbouring bytes, through the wave's own LDS): with every lane reading
+// its own row the address unit took 64 cycles a load and was the bound (12288 x 4096 Q4_0, bf16 rows, two tokens: 32 us).
 //
 // A workgroup: RT tiles of 16 weight rows (of each of NM matrices) x TT tiles of 16 tokens, eight waves. A wave takes whole
 // chunks of 256 values of all its rows (chunk v, v + 8, ...): it brings the rows' bytes into its own LDS, then the tokens' values

@@ -10,11 +10,16 @@
 // h is f32 (the norm does not see the rounding of a bf16 h), its squares are summed in f32 in a fixed tree, and y is rounded
 // once, by the output form; the operand forms have the bits of the quantizer applied to the f32 y.
 //
-// One pass over memory: a row lives in registers (8 J values a lane, L lanes a row) between the sum of its squares and its
-// output, so x and residual are read once and h and y written once, which is what bounds it. Rows of up to 512 values take
-// 16, 32 or 64 lanes of a wave (up to 16 rows a workgroup, no barrier), longer ones a workgroup. Four neighbouring lanes
-// hold a 32-value group, so an 8-bit scale is two lane exchanges. 4096 x 4096 bf16 with a residual into f16: 25.6 us for
-// 134 MB, 5.2 TB/s; 65536 x 128 bf16 8.1 us, 4.1 TB/s.
+// k % 8 == 0 and rows on 16 bytes: one pass over memory, a row lives in registers (8 J values a lane, L lanes a row) between
+// the sum of its squares and its output, so x and residual are read once and h and y written once, which is what bounds it.
+// Rows of up to 512 values take 16, 32 or 64 lanes of a wave (up to 16 rows a workgroup, no barrier), longer ones a workgroup.
+// Four neighbouring lanes hold a 32-value group, so an 8-bit scale is two lane exchanges. 4096 x 4096 bf16 with a residual into
+// f16: 29.6 us for 134 MB, 4.5 TB/s (25.7 where part of the inputs is in the last-level cache); 65536 x 128 bf16 9.0 us, 3.7 TB/s.
+//
+// Other k and addresses (f32, bf16 and f16 outputs): a workgroup of 256 threads a row, a value a load, x and residual read twice
+// (into f16 three times) from memory and then L2. Its instructions bound it (vector pipes 0.90 busy at 65536 x 100), with most
+// lanes idle in short rows: 65536 x 100 bf16 57 us (65536 x 104: 9.0), 4096 x 4095 with a residual 77, into f16 107, 333 x 2881
+// 15 (333 x 2880: 5.0).
 //
 // The backward pass, with hn = h r the normed row and g = weight dy:
 //
@@ -22,8 +27,10 @@
 //
 // the same layout: sum h^2 and sum g h are one exchange, h, dy and dh are read once and dx written once. For dweight a
 // workgroup walks its rows with the column's sum in registers and writes one partial row; a second launch adds the partial
-// rows in a fixed order. HBM is the bound: 4096 x 4096 bf16 rows 26 us for dx (134 MB, 5.2 TB/s), 35 with dweight; 65536 x 128
-// 13.6 and 16.6.
+// rows in a fixed order. Memory bounds it (inputs out of cache): 4096 x 4096 bf16 rows with dh 31 us for dx (134 MB, 4.3 TB/s), 48
+// with dweight (512 workgroups, a row's loads awaited before the next row's); 65536 x 128 15 and 20. Rows of more than 8192
+// values are read twice, with dweight three times: 1024 x 12288 29 and 53. Other k and addresses take that kernel a value a load,
+// 512 threads a row, and a column a thread for dweight: 65536 x 100 169 and 526, 4096 x 4095 97 and 125, 333 x 2881 12 and 20.
 #include "act_quant.hpp"
 #include "bfly.hpp"
 #include "epilogue.hpp"
@@ -432,8 +439,8 @@ __global__ __launch_bounds__(1024) void rms_norm_dweight_kernel(const float *__r
 }
 
 // Partial rows of dweight: enough workgroups to keep their loads in flight, few enough that the partial rows are a small part
-// of the traffic (1024 / 512, us: 16384 x 2048 bf16 55 / 71, 65536 x 128 17 / 19; two chunks a lane 4096 x 4096 36 / 35,
-// 2048 x 8192 44 / 38; long rows 1024 x 12288 64 / 55, 47 with 128)
+// of the traffic (1024 / 512, us in a graph on one set of inputs: 16384 x 2048 bf16 55 / 71, 65536 x 128 17 / 19; two chunks a
+// lane 4096 x 4096 36 / 35, 2048 x 8192 44 / 38; long rows 1024 x 12288 64 / 55, 47 with 128)
 constexpr int64_t kParts = 1024, kParts2 = 512, kPartsLong = 128;
 
 template <int L, int J>

@@ -933,8 +933,14 @@ def linear(fmt, x, w, n, k, y=None, mode="store", ws=None, w2=None, ws2=None, q8
     [tokens, n], y itself allowed), out_dtype (f32 / bf16), scales or tokens, or a bf16 y for fewer than 64 rows, the call is
     y = act(x W^T + bias) + residual (qmm_linear, mode "store"). x may then also be an operand: a planar Q8_1 buffer with
     tokens, the row-scaled f16 rows or E4M3 codes with their scales; the operand chooses the product whatever the token
-    count. GGUF mxfp4 blocks take up to 63 rows (repack_mxfp4 for more). The sums are those of the plain call, in some
-    shapes added in another f32 order (qmm_linear). y may be the residual itself; it overlaps nothing else."""
+    count. GGUF mxfp4 blocks take up to 63 rows (repack_mxfp4 for more). y may be the residual itself; it overlaps nothing else.
+    The y rows of a 64-row tile of padding (row_scale_f16's info) are not written: pass a y where they are read.
+
+    The sums are those of the plain call, in some shapes added in another f32 order (qmm_linear). Few rows of the GGUF formats and
+    mxfp4s then run on the matrix units: Q6_K 12288 x 4096 at 63 f32 rows 105 us, without an epilogue 1442 (Q8_1 rows 56 and
+    227), so out_dtype=torch.float32 alone makes the plain product faster where its order is free. The plain call gives a token
+    the same bits whatever the number of tokens; with an epilogue that holds among calls of one kernel, not between one row and
+    several."""
     if bias is not None or act != "none" or residual is not None or out_dtype is not None or scales is not None or \
             tokens is not None or (y is not None and y.dtype == torch.bfloat16 and mode == "store" and x.shape[0] < GEMM_MIN_TOKENS):
         if mode != "store" or w2 is not None or ws2 is not None:
@@ -1058,9 +1064,10 @@ def ffn_gate_up(fmt, x, w, w2, n, k, y=None, ws=None, ws2=None, q8="auto", bias=
 def ffn_gate_up_backward(fmt, x, w, w2, dy, n, k, scales=None, bias=None, bias2=None, act="silu", out_dtype=torch.bfloat16):
     """The gradients of ffn_gate_up at dy (f32 / bf16 [tokens, n]) with frozen weights: (dx [tokens, k] of out_dtype, dgu bf16
     [tokens, 2, n]), dgu[:, 0] and dgu[:, 1] the gradients of x W^T + bias and x W2^T + bias2 (what adapters and biases
-    beside the projections train on), dx = dgu[:, 0] W + dgu[:, 1] W2. The projections are computed again from x: f32 / bf16
-    rows, or the f16 operand with its scales as for ffn_gate_up: the dgu and dx rows of a 64-row tile of padding rows are zero
-    whatever dy holds there; a padding row beside others is a row of zeros, with dy's zero rows its gradient is zero. fmt q4_k, q4_kt, q6_k or q4_0, k % 256 == 0."""
+    beside the projections train on), dx = dgu[:, 0] W + dgu[:, 1] W2 of those bf16 rows, whatever dy's type and out_dtype.
+    The projections are computed again from x: f32 / bf16 rows, or the f16 operand with its scales as for ffn_gate_up: the
+    dgu and dx rows of a 64-row tile of padding rows are zero whatever dy holds there; a padding row beside others is a row of
+    zeros, with dy's zero rows its gradient is zero. fmt q4_k, q4_kt, q6_k or q4_0, k % 256 == 0."""
     s = _here(x, w, w2, dy, bias, bias2, scales)
     code = _act_code(act, GATE_ACT)
     x, scales = _backward_operand(fmt, x, dy, n, k, scales)
@@ -1080,7 +1087,7 @@ def ffn_gate_up_backward(fmt, x, w, w2, dy, n, k, scales=None, bias=None, bias2=
 def gemm_t(fmt, x, w, n, k, w2=None, out_dtype=torch.float32, y=None):
     """The transposed product y = x W [rows, k] of gradient rows x [rows, n], or x[:, 0] W + x[:, 1] W2 of x [rows, 2, n]
     (f32 / bf16): the input gradient of a projection y = x W^T whose weights stay quantized (qmm_grad_operand, qmm_gemm_t).
-    fmt q4_k, q4_kt, q6_k or q4_0, k % 256 == 0; y f32 or bf16."""
+    fmt q4_k, q4_kt, q6_k or q4_0, k % 256 == 0; y f32 or bf16. Rows times parts times n (rounded up to 64) below 2^30."""
     s = _here(x, w, w2, y)
     if fmt not in _F16_GEMM:
         raise ValueError(f"no transposed product reads {fmt} weights")
