@@ -231,8 +231,8 @@ int qmm_linear(int fmt, int act, int64_t tokens, int64_t k, int64_t n, const voi
  *   dpre[t, r] = dy[t, r] act'(sum_k x[t, k] W[r, k] + bias[r])
  * with the argument computed again from x as the QMM_F16 call computes it (fmt QMM_Q4_K, QMM_Q4_KT, QMM_Q6_K or QMM_Q4_0;
  * QMM_ACT_NONE needs no call: dpre is dy). dy: [tokens, n] f32 or bf16; dpre: bf16 [tokens, n], rounded once; the residual's
- * gradient is dy, the bias's the columns' sums of dpre, and x's qmm_gemm_t of dpre. relu's slope at 0 is 0. The rows of
- * a 64-row tile of padding rows (qmm_gemm) are zero. */
+ * gradient is dy, the bias's the columns' sums of dpre, and x's qmm_gemm_t of dpre. relu's slope at 0 is 0. Padding
+ * rows (x_scales 0, as qmm_row_scale_f16_live writes them) have zeros. */
 int qmm_linear_grad(int fmt, int act, int64_t tokens, int64_t k, int64_t n, const void *x, const float *x_scales,
                     const void *w, const float *bias, const void *dy, int dy_dtype, void *dpre, qmm_stream_t stream);
 
@@ -250,8 +250,8 @@ int qmm_ffn_gate_up(int fmt, int act, int64_t tokens, int64_t k, int64_t n, cons
  *   dgu[t, 0, r] = dy[t, r] d(act(g) u)/dg,   dgu[t, 1, r] = dy[t, r] d(act(g) u)/du
  * with g and u computed again from x as the QMM_F16 call computes them (fmt QMM_Q4_K, QMM_Q4_KT, QMM_Q6_K or QMM_Q4_0). dy:
  * [tokens, n] f32 or bf16; dgu: bf16 [tokens, 2, n], rounded once (bf16 keeps a gradient's range; what trains beside the
- * projections reads these rows). relu's slope at 0 is 0, a clamp's at its limit 1. The rows of a 64-row tile
- * of padding rows (qmm_gemm) are zero. */
+ * projections reads these rows). relu's slope at 0 is 0, a clamp's at its limit 1. Padding rows
+ * (x_scales 0, as qmm_row_scale_f16_live writes them) have zeros. */
 int qmm_ffn_gate_up_grad(int fmt, int act, int64_t tokens, int64_t k, int64_t n, const void *x, const float *x_scales,
                          const void *w, const void *w2, const float *bias, const float *bias2, const void *dy, int dy_dtype,
                          void *dgu, qmm_stream_t stream);

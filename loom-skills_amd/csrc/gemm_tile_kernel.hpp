@@ -368,7 +368,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
     nlive = (u32)(b >> 32) ? 2 * i + 2 : nlive;
   }
   nlive = __builtin_amdgcn_readfirstlane(nlive);
-  if constexpr (grad_kind(KIND)) {   // padding rows have no gradient: zeros, which sums over the rows may read
+  if constexpr (grad_kind(KIND)) {   // padding rows have no gradient: zeros, which sums over the rows may read (here 64 of them)
 #pragma unroll
     for (int i = 0; i < BM / 64; ++i) {
       if (live_rows[i] != 0) continue;
@@ -609,8 +609,13 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
           float add[NP][V];
           if (KIND != kTGlu && in) {
 #pragma unroll
-            for (int p = 0; p < NP; ++p)
+            for (int p = 0; p < NP; ++p) {
               if (live(p)) load_vals<V>(in, in_bf16, at(p), add[p]);
+              if (grad_kind(KIND) && rinv[row0 + PR * p + tr] == 0.f) {   // a padding row among others: as if its dy were 0
+#pragma unroll
+                for (int q = 0; q < V; ++q) add[p][q] = 0.f;
+              }
+            }
           }
 #pragma unroll
           for (int p = 0; p < NP; ++p) {
@@ -666,7 +671,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
           for (int r = 0; r < RK; ++r)
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
-              const bool live = src_row[row_of(r)] >= 0 && col[j] < N;
+              const bool live = src_row[row_of(r)] >= 0 && col[j] < N && !(grad_kind(KIND) && rinv[row_of(r)] == 0.f);
               add[j][r] = live ? load_val(in, bf, (int64_t)(m0 + row_of(r)) * N + col[j]) : 0.f;
             }
         };

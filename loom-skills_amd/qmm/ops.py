@@ -1065,9 +1065,8 @@ def ffn_gate_up_backward(fmt, x, w, w2, dy, n, k, scales=None, bias=None, bias2=
     """The gradients of ffn_gate_up at dy (f32 / bf16 [tokens, n]) with frozen weights: (dx [tokens, k] of out_dtype, dgu bf16
     [tokens, 2, n]), dgu[:, 0] and dgu[:, 1] the gradients of x W^T + bias and x W2^T + bias2 (what adapters and biases
     beside the projections train on), dx = dgu[:, 0] W + dgu[:, 1] W2 of those bf16 rows, whatever dy's type and out_dtype.
-    The projections are computed again from x: f32 / bf16 rows, or the f16 operand with its scales as for ffn_gate_up: the
-    dgu and dx rows of a 64-row tile of padding rows are zero whatever dy holds there; a padding row beside others is a row of
-    zeros, with dy's zero rows its gradient is zero. fmt q4_k, q4_kt, q6_k or q4_0, k % 256 == 0."""
+    The projections are computed again from x: f32 / bf16 rows, or the f16 operand with its scales as for ffn_gate_up; the
+    dgu and dx rows of its padding rows are zero whatever dy holds there. fmt q4_k, q4_kt, q6_k or q4_0, k % 256 == 0."""
     s = _here(x, w, w2, dy, bias, bias2, scales)
     code = _act_code(act, GATE_ACT)
     x, scales = _backward_operand(fmt, x, dy, n, k, scales)

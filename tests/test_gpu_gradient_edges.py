@@ -106,3 +106,26 @@ def test_padding_rows_have_no_gradient(dev, fmt, T, n, k):
     want2 = ops.ffn_gate_up_backward(fmt, full, w.w, u.w, dy, n, k, scales=fs, bias=b)
     for got, ref in ((dpre, want[1]), (dgu, want2[1]), (dp, want[1]), (dg, want2[1]), (dx, want[0]), (dx2, want2[0])):
         assert torch.equal(got[live], ref[live]) and (got[~live] == 0).all()
+
+
+@pytest.mark.parametrize("fmt,T,n,k", [("q4_k", 200, 136, 512), ("q6_k", 200, 133, 512), ("q4_0", 1, 768, 256), ("q4_k", 2011, 4104, 256), ("q4_kt", 1000, 2064, 512),
+                                       ("q6_k", 1500, 4099, 256)])
+def test_padding_rows_among_others_have_no_gradient(dev, fmt, T, n, k):
+    """The same for single padding rows, whose dy holds anything: zero like those of whole tiles, the rows beside them unchanged."""
+    import qmm.ops as ops
+    rng = np.random.default_rng(T + 1)
+    w, u = Weight(fmt, rng, n, k, dev), Weight(fmt, rng, n, k, dev)
+    x = torch.from_numpy(rng.standard_normal((T, k)).astype(np.float32)).to(dev)
+    b = torch.from_numpy(rng.standard_normal(n).astype(np.float32)).to(dev)
+    live = torch.from_numpy(rng.random(T) < 0.7).to(dev) if T > 1 else torch.zeros(T, dtype=torch.bool, device=dev)
+    x16, s = ops.row_scale_f16(x, info=live.int().reshape(-1, 1).expand(T, 4).contiguous())
+    full, fs = ops.row_scale_f16(x)
+    for dt in (torch.float32, torch.bfloat16):
+        clean = torch.from_numpy(rng.standard_normal((T, n)).astype(np.float32)).to(dt).to(dev)
+        dy = torch.where(live[:, None], clean, torch.full_like(clean, float("nan")))
+        got = ops.linear_backward(fmt, x16, w.w, dy, n, k, scales=s, bias=b, act="gelu") + \
+            ops.ffn_gate_up_backward(fmt, x16, w.w, u.w, dy, n, k, scales=s, bias=b, bias2=b)
+        want = ops.linear_backward(fmt, full, w.w, clean, n, k, scales=fs, bias=b, act="gelu") + \
+            ops.ffn_gate_up_backward(fmt, full, w.w, u.w, clean, n, k, scales=fs, bias=b, bias2=b)
+        for g, r in zip(got, want):
+            assert torch.equal(g[live], r[live]) and (g[~live] == 0).all()
