@@ -371,7 +371,7 @@ __global__ __launch_bounds__(64 * NW * KS, 2) void gemm_tile_kernel(TileArgs a) 
   if constexpr (grad_kind(KIND)) {   // padding rows have no gradient: zeros, which sums over the rows may read (here 64 of them)
 #pragma unroll
     for (int i = 0; i < BM / 64; ++i) {
-      if (live_rows[i] != 0) continue;
+      if (live_rows[i] != 0 || m0 + 64 * i >= M) continue;
       for (int e = tid; e < 64 * BN; e += 64 * NW * KS) {
         const int row = m0 + 64 * i + e / BN, col = n0 + e % BN;
         if (row >= M || col >= N) continue;
