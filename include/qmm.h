@@ -274,6 +274,53 @@ int qmm_gemm_t(int fmt, int64_t rows, int64_t k, int64_t n, const void *x, const
 /* Workspace bytes of qmm_gemm_t (two: with w2), or -1 for a call it refuses. */
 int64_t qmm_gemm_t_workspace_size(int fmt, int64_t rows, int64_t k, int64_t n, int two);
 
+/* 4-bit weights with group scales and zero points, W[r, c] = s[r, c / group] (q[r, c] - z[r, c / group]) with codes q and zero
+ * points z of 0 .. 15 and f16 scales s (the form that weight-only quantizers write; no reference counterpart). group: 32, 64,
+ * 128, ... (a power of two), or at least k: one scale a row. k % 32 == 0 (the last group may be short), n any, k and n <= 2^20.
+ * qmm_w4_pack lays them out once: codes u8 [E, n, k] (a byte a code), scales f16 [E, n, ceil(k / group)], zeros u8 of the same
+ * shape or NULL (8: symmetric codes) -> w, E times qmm_w4_bytes(n, k) bytes: tiles of 16 rows x 128 values, 1 KB each
+ * [E][ceil(n / 16)][ceil(k / 128)], lane 16 h + r's word j holding values 32 j + 8 h .. + 7 of row r (byte b: value b in the
+ * low nibble, value 4 + b in the high one); ws, E times qmm_w4_scale_bytes(n, k, group) bytes: words (f16 s, f16 1024 + z)
+ * [E][ceil(n / 16)][groups][16]. Both 16-byte aligned. E <= 1024. */
+int qmm_w4_pack(int E, int64_t n, int64_t k, int64_t group, const uint8_t *codes, const void *scales, const uint8_t *zeros,
+                void *w, void *ws, qmm_stream_t stream);
+/* Bytes of one packed matrix, and of its scale words; -1 for a shape that is not taken. */
+int64_t qmm_w4_bytes(int64_t n, int64_t k);
+int64_t qmm_w4_scale_bytes(int64_t n, int64_t k, int64_t group);
+
+/* The product y[t, r] = sum_c x[t, c] W_e[r, c] on packed 4-bit weights. offsets NULL: one matrix (E = 1) for all rows; else
+ * i32 [E + 1] on the device, expert e's rows being offsets[e] .. offsets[e + 1] - 1, as many as it has (offsets are clamped to
+ * 0 .. rows, an expert whose end is not past its start has none; rows of no expert are not written, and no row belongs to two).
+ *   x_dtype QMM_F32 / QMM_BF16  x [rows, k]: exact products, f32 sums; for few rows an expert (weights are read once for up to
+ *                               64 of them). A row that holds an infinity gives NaN or infinities. x_scales unused.
+ *   x_dtype QMM_F16             the qmm_gemm operand: x16 [rows, k] with x_scales f32 [rows, 2] of qmm_row_scale_f16, or NULL;
+ *                               weights enter as f16(s (q - z)) (one rounding; finite for |s| <= 4366), f32 sums.
+ * y: [rows, n] of y_dtype, QMM_F32 or QMM_BF16 (rounded once). x, w, ws 16-byte aligned; rows <= 2^24. y overlaps nothing. */
+int qmm_w4_mm(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_t *offsets, const void *x, int x_dtype,
+              const float *x_scales, const void *w, const void *ws, void *y, int y_dtype, qmm_stream_t stream);
+
+/* The transposed product y[t, c] = sum_r x[t, r] W_e[r, c], c < k: the input gradient of qmm_w4_mm with frozen weights. x,
+ * scales: the one-part operand of qmm_grad_operand (f16 [rows, n rounded up to 64], padded with zeros). Weights enter as
+ * f16(s (q - z)). Other arguments as qmm_w4_mm. */
+int qmm_w4_mm_t(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_t *offsets, const void *x,
+                const float *scales, const void *w, const void *ws, void *y, int y_dtype, qmm_stream_t stream);
+
+/* Products of rows sorted by expert with 16-bit expert weights W [E, n, k], without padding between the experts (the bucketed
+ * GEMMs of qmm_moe_grouped pad each to 64 rows and take quantized weights), and their gradients:
+ *   qmm_ragged_mm     y[t, r]     = sum_c x[t, c] W_e[r, c]       t of expert e
+ *   qmm_ragged_mm_t   dx[t, c]    = sum_r dy[t, r] W_e[r, c]
+ *   qmm_ragged_mm_dw  dw[e, r, c] = sum_t dy[t, r] x[t, c]        over expert e's rows, zero for an expert without rows
+ * offsets: i32 [E + 1] on the device, as qmm_w4_mm. dtype QMM_BF16 or QMM_F16 for x, W and dy alike; outputs QMM_F32 or that
+ * type (rounded once); f32 sums in an order that follows from the sizes. x [rows, k], dy [rows, n]; n % 8 == 0, k % 8 == 0,
+ * both <= 2^20, rows <= 2^24, E <= 1024; tensors 16-byte aligned. Rows of no expert are neither written (y, dx) nor read into
+ * a sum (dw). Outputs overlap nothing. */
+int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *x, const void *w, int dtype,
+                  void *y, int y_dtype, qmm_stream_t stream);
+int qmm_ragged_mm_t(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy, const void *w, int dtype,
+                    void *dx, int dx_dtype, qmm_stream_t stream);
+int qmm_ragged_mm_dw(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy, const void *x, int dtype,
+                     void *dw, int dw_dtype, qmm_stream_t stream);
+
 /* MoE router top-k from logits, g_moe_route / g_moe_route_tr after the router matvec
  * (S/gen_moe.py:116-252, :255-500; llama.cpp gating: 1 softmax, 2 sigmoid, 3 softmax over the picked logits):
  *   ids i32 [tokens, KU] = the top-KU experts by score (ties to the lower id), wts f32 [tokens, KU].

@@ -1,0 +1,81 @@
+// Products of 16-bit expert weights W [E, n, k] and rows sorted by expert, with their gradients: argument checks and the choice
+// of the kernel. Expert e owns rows offsets[e] .. offsets[e + 1] - 1, as many as it has: no padding between experts.
+//
+//   qmm_ragged_mm     y[t] = W_e x[t]          few rows an expert on few_rows.hpp, else the tiles of tile_mm.hpp
+//   qmm_ragged_mm_t   dx[t] = W_e^T dy[t]
+//   qmm_ragged_mm_dw  dW_e = sum_t dy[t] x[t]^T
+#include "ragged_mm.hpp"
+
+using namespace qmm;
+
+namespace qmm {
+int ragged_few(const few::Args &a, bool f16, hipStream_t s) {
+  return f16 ? few::launch_tt<few::kWF16, false, 4>(a, s) : few::launch_tt<few::kWBF16, false, 4>(a, s);
+}
+}  // namespace qmm
+
+namespace {
+
+constexpr int64_t kMaxSide = 1 << 20, kMaxRows = 1 << 24;
+
+int check(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *p, const void *q, int dtype,
+          const void *out, int out_dtype) {
+  if (dtype != QMM_BF16 && dtype != QMM_F16) return QMM_ERR_DTYPE;
+  if (out_dtype != QMM_F32 && out_dtype != dtype) return QMM_ERR_DTYPE;
+  if (rows < 0 || rows > kMaxRows || k <= 0 || k > kMaxSide || k % 8 || n <= 0 || n > kMaxSide || n % 8) return QMM_ERR_SHAPE;
+  if (E < 1 || E > kMaxRaggedE) return QMM_ERR_RANGE;
+  if (!offsets || !out || (rows && (!p || !q))) return QMM_ERR_NULL;
+  if (!aligned(p, 16) || !aligned(q, 16) || !aligned(offsets, 4) || !aligned(out, 16)) return QMM_ERR_ALIGN;
+  return QMM_OK;
+}
+
+int tiles(int op, tmm::Args &a, int dtype, int out_dtype, void *out, qmm_stream_t stream) {
+  a.y = out;
+  a.y_type = out_dtype;
+  a.wide = 1;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return dtype == QMM_F16 ? ragged_tiles_f16(op, a, s) : ragged_tiles_bf16(op, a, s);
+}
+
+}  // namespace
+
+extern "C" int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *x, const void *w,
+                             int dtype, void *y, int y_dtype, qmm_stream_t stream) {
+
+  if (int st = check(rows, k, n, E, offsets, x, w, dtype, rows ? y : w, y_dtype)) return st;
+  if (rows == 0) return QMM_OK;
+  if (rows <= 16 * (int64_t)E) {
+    const few::Args a{offsets, E, (int)rows, (int)n, (int)k, static_cast<const u8 *>(x), static_cast<const u8 *>(w),
+                      2 * n * k, nullptr, 0, 0, y, y_dtype == QMM_F32 ? 4 : 2};
+    return ragged_few(a, dtype == QMM_F16, reinterpret_cast<hipStream_t>(stream));
+  }
+  tmm::Args a{};
+  a.offsets = offsets, a.E = E, a.rows = (int)rows;
+  a.N = (int)n, a.K = (int)k;
+  a.a = static_cast<const u8 *>(x), a.a_row = 2 * k;
+  a.b = static_cast<const u8 *>(w), a.b_row = 2 * k, a.b_expert = 2 * n * k;
+  return tiles(kRaggedY, a, dtype, y_dtype, y, stream);
+}
+
+extern "C" int qmm_ragged_mm_t(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy, const void *w,
+                               int dtype, void *dx, int dx_dtype, qmm_stream_t stream) {
+  if (int st = check(rows, k, n, E, offsets, dy, w, dtype, rows ? dx : w, dx_dtype)) return st;
+  if (rows == 0) return QMM_OK;
+  tmm::Args a{};
+  a.offsets = offsets, a.E = E, a.rows = (int)rows;
+  a.N = (int)k, a.K = (int)n;
+  a.a = static_cast<const u8 *>(dy), a.a_row = 2 * n;
+  a.b = static_cast<const u8 *>(w), a.b_row = 2 * k, a.b_expert = 2 * n * k;
+  return tiles(kRaggedDX, a, dtype, dx_dtype, dx, stream);
+}
+
+extern "C" int qmm_ragged_mm_dw(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy,
+                                const void *x, int dtype, void *dw, int dw_dtype, qmm_stream_t stream) {
+  if (int st = check(rows, k, n, E, offsets, dy, x, dtype, dw, dw_dtype)) return st;
+  tmm::Args a{};
+  a.offsets = offsets, a.E = E, a.rows = (int)rows;
+  a.M = (int)n, a.N = (int)k;
+  a.a = static_cast<const u8 *>(dy), a.a_row = 2 * n;
+  a.b = static_cast<const u8 *>(x), a.b_row = 2 * k;
+  return tiles(kRaggedDW, a, dtype, dw_dtype, dw, stream);
+}

@@ -1,0 +1,422 @@
+// C = A B over 16-bit operands on v_mfma_f32_32x32x16, one matrix or one an expert over ragged segments of rows:
+//
+//   forward          Y[t, r]   = sum_c X[t, c] W_e[r, c]        t in expert e's segment
+//   input gradient   dX[t, c]  = sum_r dY[t, r] W_e[r, c]
+//   weight gradient  dW_e[r,c] = sum_t dY[t, r] X[t, c]         t over expert e's segment
+//
+// with W_e as 16-bit rows or as 4-bit codes with group scales, dequantized to f16 on their way into LDS: f16(s (q - z)), the
+// one rounding (q - z is exact).
+//
+// A workgroup owns BM x BN outputs, WM x WN waves of (BM / WM) x (BN / WN), and walks the sum 64 values at a time through two
+// LDS buffers. An operand whose memory rows run along the sum (kRow) keeps them: LDS rows of 64 values, 16-byte chunk i at
+// i ^ (row / 2 % 8), so that the 16 rows a fragment read covers at a time lie in all banks. One whose memory rows run along the
+// outputs (kCol) keeps those too, 64 LDS rows of BM or BN values, and is transposed by ds_read_b64_tr_b16 (16 lanes read a
+// 4 x 16 block and get its columns): chunk i of LDS row k at i ^ (4 (k % 4)) ^ (k / 4 % 4), for the reads (four rows x 64 bytes at
+// a time) and the stores of dequantized weights (16 rows of one chunk). 16-bit operands go straight into LDS
+// (buffer_load ... lds), rows past a segment's end and values past a row's end as zeros. The fragments of the next 16 values
+// are read while the MFMAs of these run, and the barrier of a step stands before its last 16 values' MFMAs, so that the next
+// step's first reads run under them.
+#pragma once
+#include <algorithm>
+#include <type_traits>
+
+#include "ragged.hpp"
+
+namespace qmm {
+namespace tmm {
+
+typedef __attribute__((ext_vector_type(4))) u32 u32x4;
+typedef __attribute__((ext_vector_type(2))) u32 u32x2;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(2))) _Float16 h2;
+
+enum Src { kRow = 0, kCol = 1, kW4Row = 2, kW4Col = 3 };
+enum Sum { kSumFixed = 0, kSumRagged = 1 };   // what the segments cut: A's rows (kSumFixed) or the sum (the weight gradient)
+constexpr u32 kPast = 0x80000000u;            // an offset past every resource: the load gives zeros
+constexpr int kGroupM = 8;
+
+struct Args {
+  const int32_t *offsets;      // NULL: one segment of all rows
+  int E, rows;
+  int M, N, K;                 // outputs M x N (kSumFixed: M unused), sum of K values (kSumRagged: K unused)
+  const u8 *a, *b;
+  int64_t a_row, b_row;        // bytes from one memory row to the next (w4: unused)
+  int64_t b_expert;            // bytes from one expert's matrix to the next
+  const u32 *ws;               // w4: (f16 scale, f16 1024 + zero) words [E][ceil(rows of W / 16)][groups][16]
+  int w_blocks, w_tiles;       // w4: 16-row blocks and 128-value tiles of an expert's matrix
+  int groups, gshift;          // w4: group of 32-value step i: min(i >> gshift, groups - 1)
+  const float *scales;         // [rows, 2] or NULL: output row t times scales[t, 1]
+  void *y;
+  int y_type;                  // QMM_F32, QMM_BF16 or QMM_F16
+  int wide;                    // output rows are 16-byte aligned
+  int tiles_n;
+};
+
+template <int DT>
+__device__ __forceinline__ f32x16 mfma(u32x4 x, u32x4 w, f32x16 c) {
+  if constexpr (DT == QMM_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, w), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, w), c, 0, 0, 0);
+}
+
+// 16 bytes a lane from a buffer resource into LDS at lds + 16 lane (wave-uniform lds); lanes past the resource's end write
+// zeros. Written out so that the compiler's wait counting stays with the register loads; the caller waits before the barrier.
+__device__ __forceinline__ void lds_load16(u32x4 rsrc, u32 voff, u32 lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :
+               : "v"(voff), "s"(rsrc), "s"(lds)
+               : "m0", "memory");
+}
+// every load has landed, every LDS access of this wave is done, and the same holds for the workgroup's other waves
+__device__ __forceinline__ void wait_all_barrier() {
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+__device__ __forceinline__ u32x4 resource(const u8 *p, int64_t bytes) {
+  const uint64_t at = (uint64_t)p;
+  const u32 n = (u32)max((int64_t)0, min(bytes, (int64_t)0x7FFFFFF0));
+  return u32x4{(u32)__builtin_amdgcn_readfirstlane((int)(u32)at), (u32)__builtin_amdgcn_readfirstlane((int)((u32)(at >> 32) & 0xFFFFu)),
+               (u32)__builtin_amdgcn_readfirstlane((int)n), 0x00020000u};
+}
+
+__device__ __forceinline__ h2 as_h2(u32 v) { return __builtin_bit_cast(h2, v); }
+// eight weights f16(s (q - z)) from a code word (low nibbles values 0 .. 3, high nibbles 4 .. 7) and a scale word
+__device__ __forceinline__ u32x4 dequant(u32 q, u32 sc) {
+  const u32 lo = q & 0x0F0F0F0Fu, hi = (q >> 4) & 0x0F0F0F0Fu;
+  const h2 v = as_h2(sc), s = {v.x, v.x}, z = {v.y, v.y};
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {   // 0x6400 | q is 1024 + q; the difference is exact
+    const h2 c = as_h2(__builtin_amdgcn_perm(0x64646464u, i < 2 ? lo : hi, i & 1 ? 0x04030402u : 0x04010400u));
+    o[i] = __builtin_bit_cast(u32, (c - z) * s);
+  }
+  return o;
+}
+
+template <int SRC>
+__device__ __forceinline__ int chunk_swizzle(int row) {
+  if constexpr (SRC == kRow || SRC == kW4Row) return (row >> 1) & 7;
+  else return ((row & 3) << 2) ^ ((row >> 2) & 3);
+}
+
+// DT: QMM_BF16 or QMM_F16; SA, SB: the operands' sources; GS: 32-value steps a w4 scale covers (1, 2; 4: more)
+template <int DT, int SA, int SB, int SUM, int BM, int BN, int WM, int WN, int GS>
+__global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
+  constexpr int NW = WM * WN, NT = 64 * NW, NI = BM / WM / 32, NJ = BN / WN / 32;
+  constexpr int kA = BM * 128, kB = BN * 128;             // LDS bytes of a step's operands
+  constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;       // 1 KB loads a wave and step
+  constexpr bool kW4 = SB == kW4Row || SB == kW4Col;
+  static_assert(SA == kRow || BM >= 128, "a transposed operand is at least 128 wide");
+  static_assert((SB == kRow || SB == kW4Row) || BN >= 128, "a transposed operand is at least 128 wide");
+  extern __shared__ __align__(1024) u8 smem[];            // A [2], B [2]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  // ---- the workgroup's tile. Workgroup i runs on XCD i % 8, which takes a contiguous range of tiles in groups of kGroupM row
+  // tiles, rows fastest: the tiles that an XCD works on at a time share operand rows in its L2.
+  int e = 0, lo = 0, hi = a.rows, m0, nt;
+  if constexpr (SUM == kSumFixed) {
+    TileScan sc{(a.rows + BM - 1) / BM, 0, 1};
+    if (a.offsets) sc = scan_tiles<BM>(a.offsets, a.E, a.rows);
+    const int total = sc.total * a.tiles_n, per = (total + 7) >> 3;
+    const int i = (int)(blockIdx.x >> 3), t = (int)(blockIdx.x & 7) * per + i;
+    if (i >= per || t >= total) return;
+    const int g = t / (kGroupM * a.tiles_n), gm = min(kGroupM, sc.total - g * kGroupM), gt = t - g * kGroupM * a.tiles_n;
+    int mt = g * kGroupM + gt % gm;
+    nt = gt / gm;
+    if (a.offsets) find_tile<BM>(a.offsets, a.E, a.rows, sc, mt, e, lo, hi, mt);
+    m0 = mt * BM;
+  } else {
+    const int tiles_m = (a.M + BM - 1) / BM, per_e = tiles_m * a.tiles_n, total = per_e * a.E, per = (total + 7) >> 3;
+    const int i = (int)(blockIdx.x >> 3), t = (int)(blockIdx.x & 7) * per + i;
+    if (i >= per || t >= total) return;
+    e = t / per_e;
+    const int r = t - e * per_e;
+    m0 = (r % tiles_m) * BM;
+    nt = r / tiles_m;
+    lo = clamp_row(__builtin_amdgcn_readfirstlane(a.offsets[e]), a.rows);
+    hi = clamp_row(__builtin_amdgcn_readfirstlane(a.offsets[e + 1]), a.rows);
+  }
+  const int n0 = nt * BN;
+  const int seg = max(hi - lo, 0);                        // the segment's rows
+  const int m_end = SUM == kSumFixed ? seg : a.M;         // outputs m0 .. min(m0 + BM, m_end) - 1
+  const int K = SUM == kSumFixed ? a.K : seg, S = (K + 63) >> 6;
+
+  // ---- straight into LDS: load i of a wave is 1 KB of the step, lane l's 16 bytes a chunk of row (i NW + wave) ROWS + l / CH
+  u32 aoff[LA], boff[LB];
+  int acol[SA == kRow ? LA : 1], bcol[SB == kRow ? LB : 1];   // kRow: first value of the lane's chunk
+  auto place = [&](auto src, int R, int first, int end, int64_t stride, int i, u32 &off, int &col) __attribute__((always_inline)) {
+    constexpr int SRC = decltype(src)::value;
+    const int CH = SRC == kRow ? 8 : R / 8;
+    const int row = (i * NW + wave) * (64 / CH) + lane / CH, ch = (lane & (CH - 1)) ^ chunk_swizzle<SRC>(row);
+    if constexpr (SRC == kRow) {
+      off = (u32)((int64_t)row * stride + 16 * ch);
+      col = 8 * ch;
+    } else {
+      off = first + 8 * ch < end ? (u32)((int64_t)row * stride + 16 * ch) : kPast;
+      col = 0;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < LA; ++i)
+    place(std::integral_constant<int, SA>{}, BM, m0, a.M, a.a_row, i, aoff[i], acol[SA == kRow ? i : 0]);
+  if constexpr (!kW4) {
+#pragma unroll
+    for (int i = 0; i < LB; ++i)
+      place(std::integral_constant<int, SB>{}, BN, n0, a.N, a.b_row, i, boff[i], bcol[SB == kRow ? i : 0]);
+  }
+  // where the tile's operands start, and the bytes from there to the end of what it may read
+  const u8 *ap, *bp = a.b;
+  if constexpr (SUM == kSumFixed) {
+    ap = a.a + (int64_t)(lo + m0) * a.a_row;
+    if constexpr (!kW4) bp += (int64_t)e * a.b_expert + (SB == kRow ? (int64_t)n0 * a.b_row : (int64_t)n0 * 2);
+    else bp += (int64_t)e * a.b_expert;
+  } else {
+    ap = a.a + (int64_t)lo * a.a_row + (int64_t)m0 * 2;
+    bp += (int64_t)lo * a.b_row + (int64_t)n0 * 2;
+  }
+  const u32 lds0 = (u32)(uintptr_t)(__attribute__((address_space(3))) u8 *)smem;
+  auto load_a = [&](int s, int i) __attribute__((always_inline)) {
+    const u32 dst = __builtin_amdgcn_readfirstlane(lds0 + (u32)((s & 1) * kA + (i * NW + wave) * 1024));
+    if constexpr (SA == kRow) {
+      const u32x4 r = resource(ap + (int64_t)s * 128, (int64_t)min(BM, m_end - m0) * a.a_row - (int64_t)s * 128);
+      lds_load16(r, 64 * s + acol[i] < K ? aoff[i] : kPast, dst);
+    } else {
+      const u32x4 r = resource(ap + (int64_t)s * 64 * a.a_row, (int64_t)min(64, K - 64 * s) * a.a_row - (int64_t)m0 * 2);
+      lds_load16(r, aoff[i], dst);
+    }
+  };
+  auto load_b = [&](int s, int i) __attribute__((always_inline)) {
+    const u32 dst = __builtin_amdgcn_readfirstlane(lds0 + (u32)(2 * kA + (s & 1) * kB + (i * NW + wave) * 1024));
+    if constexpr (SB == kRow) {
+      const u32x4 r = resource(bp + (int64_t)s * 128, (int64_t)min(BN, a.N - n0) * a.b_row - (int64_t)s * 128);
+      lds_load16(r, 64 * s + bcol[i] < K ? boff[i] : kPast, dst);
+    } else if constexpr (SB == kCol) {
+      const u32x4 r = resource(bp + (int64_t)s * 64 * a.b_row, (int64_t)min(64, K - 64 * s) * a.b_row - (int64_t)n0 * 2);
+      lds_load16(r, boff[i], dst);
+    }
+  };
+
+  // ---- w4: unit u of a step is a lane's 16 bytes of a 16-row x 128-value tile (kW4Row: the half that the step covers). Rows and
+  // tiles past the end read the last ones: their outputs are not stored, and in the sum A is zero there.
+  constexpr int kAll = SB == kW4Row ? BN * 4 : BN * 2;    // units of a step
+  constexpr int kUnits = (kAll + NT - 1) / NT;
+  constexpr int kWords = SB == kW4Row ? 2 : 4;            // code words of a unit
+  constexpr int kScales = GS >= kWords ? 1 : kWords / GS;
+  u32 cw[kUnits][kWords], cs[kUnits][kScales];
+  auto load_w4 = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int u = i * NT + tid, l = u & 63, b = u >> 6;
+      const int rb = min(SB == kW4Row ? (n0 >> 4) + b : 4 * s + (b & 3), a.w_blocks - 1);
+      const int t = min(SB == kW4Row ? s >> 1 : (n0 >> 7) + (b >> 2), a.w_tiles - 1);
+      const u8 *p = bp + ((int64_t)rb * a.w_tiles + t) * 1024 + 16 * l;
+      if constexpr (SB == kW4Row) {
+        const u32x2 v = *reinterpret_cast<const u32x2 *>(p + 8 * (s & 1));
+        cw[i][0] = v.x;
+        cw[i][1] = v.y;
+      } else {
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) cw[i][j] = v[j];
+      }
+      const u32 *sp = a.ws + ((int64_t)e * a.w_blocks + rb) * a.groups * 16 + (l & 15);
+      const int step = SB == kW4Row ? 2 * s : 4 * t;      // the unit's first 32-value step along W's rows
+#pragma unroll
+      for (int g = 0; g < kScales; ++g) cs[i][g] = sp[min((step + GS * g) >> a.gshift, a.groups - 1) * 16];
+    }
+  };
+  auto store_w4 = [&](int s, int i) __attribute__((always_inline)) {
+    const int u = i * NT + tid, l = u & 63, b = u >> 6;
+    if (kAll % NT && u >= kAll) return;
+    u8 *out = smem + 2 * kA + (s & 1) * kB;
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) {
+      const u32x4 v = dequant(cw[i][j], cs[i][kScales == 1 ? 0 : j / GS]);
+      if constexpr (SB == kW4Row) {
+        const int row = 16 * b + (l & 15), ch = 4 * j + (l >> 4);
+        *reinterpret_cast<u32x4 *>(out + row * 128 + ((ch ^ chunk_swizzle<SB>(row)) * 16)) = v;
+      } else {
+        const int row = 16 * (b & 3) + (l & 15), ch = 16 * (b >> 2) + 4 * j + (l >> 4);
+        *reinterpret_cast<u32x4 *>(out + row * (BN * 2) + ((ch ^ chunk_swizzle<SB>(row)) * 16)) = v;
+      }
+    }
+  };
+
+  // ---- fragments: lane (c, h) = (l % 32, l / 32) holds values 8 h .. + 7 of the 16 of row or column c
+  const int c = lane & 31, h = lane >> 5, p = lane & 15, q = (lane >> 4) & 1;
+  const u32 row_base = (u32)(c * 128 + ((h ^ ((c >> 1) & 7)) * 16));
+  auto read_row = [&](u32 at, int blk, int kk) __attribute__((always_inline)) {   // rows 32 blk .. of the operand at `at`
+    return *reinterpret_cast<const u32x4 *>(smem + ((at + row_base) ^ (u32)(kk * 32)) + blk * 4096);
+  };
+  auto read_col = [&](u32 at, int RS, int blk, int kk) __attribute__((always_inline)) {   // columns 32 blk ..
+    u32x4 v;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int kr = p >> 2, k = 8 * h + 4 * t + kr;
+      const int ch = ((4 * blk) ^ (kr << 2)) + ((2 * q + ((p & 3) >> 1)) ^ (2 * h + t));
+      const u8 *src = smem + at + (16 * kk) * RS + k * RS + ch * 16 + (p & 1) * 8;
+      const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(src));
+      const u32x2 d = __builtin_bit_cast(u32x2, r);
+      v[2 * t] = d.x;
+      v[2 * t + 1] = d.y;
+    }
+    return v;
+  };
+  auto read_a = [&](int s, int i, int kk) __attribute__((always_inline)) {
+    const u32 at = (u32)((s & 1) * kA);
+    if constexpr (SA == kRow) return read_row(at, wm * NI + i, kk);
+    else return read_col(at, BM * 2, wm * NI + i, kk);
+  };
+  auto read_b = [&](int s, int j, int kk) __attribute__((always_inline)) {
+    const u32 at = (u32)(2 * kA + (s & 1) * kB);
+    if constexpr (SB == kRow || SB == kW4Row) return read_row(at, wn * NJ + j, kk);
+    else return read_col(at, BN * 2, wn * NJ + j, kk);
+  };
+
+  f32x16 acc[NI][NJ];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+  auto load = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < LA; ++i) load_a(s, i);
+    if constexpr (!kW4) {
+#pragma unroll
+      for (int i = 0; i < LB; ++i) load_b(s, i);
+    }
+  };
+  u32x4 fa[2][NI], fb[2][NJ];
+  auto read = [&](int set, int s, int kk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) fb[set][j] = read_b(s, j, kk);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) fa[set][i] = read_a(s, i, kk);
+  };
+  auto multiply = [&](int set) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = mfma<DT>(fa[set][i], fb[set][j], acc[i][j]);
+  };
+
+  if (S > 0) {
+    load(0);
+    if constexpr (kW4) {
+      load_w4(0);
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) store_w4(0, i);
+      if (S > 1) load_w4(1);
+    }
+    wait_all_barrier();
+    if (S > 1) load(1);
+    read(0, 0, 0);
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int kk = 0; kk < 3; ++kk) {
+        read((kk + 1) & 1, s, kk + 1);
+        if constexpr (kW4) {   // the next step's weights, whose buffer the last barrier has freed
+#pragma unroll
+          for (int i = kk; i < kUnits; i += 3)
+            if (s + 1 < S) store_w4(s + 1, i);
+        }
+        multiply(kk & 1);
+      }
+      wait_all_barrier();
+      if (s + 2 < S) {
+        load(s + 2);
+        if constexpr (kW4) load_w4(s + 2);
+      }
+      if (s + 1 < S) read(0, s + 1, 0);
+      multiply(1);
+    }
+  }
+
+  // ---- outputs, 32 rows of a wave at a time through its own LDS (every wave is past its last read of the operands): the sums
+  // of a lane are one column of 16 rows, a store covers neighbouring columns
+  constexpr int kPitch = NJ * 32 + 8;   // floats; 4 rows apart is 32 banks apart
+  static_assert(32 * kPitch * 4 * NW <= 2 * (kA + kB), "the staging areas fit the operands' buffers");
+  float *stage = reinterpret_cast<float *>(smem) + wave * 32 * kPitch;
+  const int64_t out0 = SUM == kSumFixed ? (int64_t)lo * a.N : (int64_t)e * a.M * a.N;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) stage[((r & 3) + 8 * (r >> 2) + 4 * h) * kPitch + 32 * j + c] = acc[i][j][r];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    const int mb = m0 + (wm * NI + i) * 32, nb = n0 + wn * NJ * 32;
+    auto row_scale = [&](int m) __attribute__((always_inline)) {
+      return SUM == kSumFixed && a.scales ? a.scales[2 * (int64_t)(lo + m) + 1] : 1.f;
+    };
+    if (a.wide) {
+      constexpr int LR = NJ * 4, RP = 64 / LR;   // lanes a row (8 values each), rows a pass
+#pragma unroll
+      for (int r0 = 0; r0 < 32; r0 += RP) {
+        const int r = r0 + lane / LR, col = (lane % LR) * 8;
+        const int m = mb + r, n = nb + col;
+        if (m < m_end && n < a.N) {
+          const f32x4 v0 = *reinterpret_cast<const f32x4 *>(stage + r * kPitch + col);
+          const f32x4 v1 = *reinterpret_cast<const f32x4 *>(stage + r * kPitch + col + 4);
+          const float sc = row_scale(m);
+          const int64_t at = out0 + (int64_t)m * a.N + n;
+          if (a.y_type == QMM_F32) {
+            f32x4 *o = reinterpret_cast<f32x4 *>(static_cast<float *>(a.y) + at);
+            o[0] = v0 * sc;
+            o[1] = v1 * sc;
+          } else if (a.y_type == QMM_BF16) {
+            bf16x8 b;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) b[x] = (__bf16)((x < 4 ? v0[x] : v1[x - 4]) * sc);
+            *reinterpret_cast<bf16x8 *>(static_cast<__bf16 *>(a.y) + at) = b;
+          } else {
+            f16x8 b;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) b[x] = (_Float16)((x < 4 ? v0[x] : v1[x - 4]) * sc);
+            *reinterpret_cast<f16x8 *>(static_cast<_Float16 *>(a.y) + at) = b;
+          }
+        }
+      }
+    } else {
+      for (int v = lane; v < 32 * 32 * NJ; v += 64) {
+        const int r = v / (32 * NJ), m = mb + r, n = nb + v % (32 * NJ);
+        if (m < m_end && n < a.N) {
+          const float o = stage[r * kPitch + v % (32 * NJ)] * row_scale(m);
+          const int64_t at = out0 + (int64_t)m * a.N + n;
+          if (a.y_type == QMM_F32) static_cast<float *>(a.y)[at] = o;
+          else if (a.y_type == QMM_BF16) static_cast<__bf16 *>(a.y)[at] = (__bf16)o;
+          else static_cast<_Float16 *>(a.y)[at] = (_Float16)o;
+        }
+      }
+    }
+  }
+}
+
+template <int DT, int SA, int SB, int SUM, int BM, int BN, int WM, int WN, int GS>
+int launch(const Args &in, hipStream_t s) {
+  Args a = in;
+  a.tiles_n = (a.N + BN - 1) / BN;
+  // row tiles: at most one ragged tile an expert beside the whole ones
+  const int64_t tiles_m = SUM == kSumRagged ? (int64_t)((a.M + BM - 1) / BM) * a.E
+                          : a.offsets       ? std::min<int64_t>((int64_t)a.rows / BM + a.E, a.rows)
+                                            : (a.rows + BM - 1) / BM;
+  const int64_t tiles = tiles_m * a.tiles_n;
+  if (tiles > (1 << 22)) return QMM_ERR_SHAPE;   // HIP refuses 2^32 threads along a grid's dimension
+  constexpr int lds = 2 * (BM + BN) * 128;
+  auto *fn = tile_mm_kernel<DT, SA, SB, SUM, BM, BN, WM, WN, GS>;
+  static std::atomic<unsigned> raised{0};
+  if (int st = raise_dyn_lds(reinterpret_cast<const void *>(fn), lds, raised)) return st;
+  fn<<<dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * WM * WN), lds, s>>>(a);
+  return launch_status();
+}
+
+}  // namespace tmm
+}  // namespace qmm

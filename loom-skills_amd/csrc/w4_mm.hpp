@@ -1,0 +1,10 @@
+// The 4-bit products' launchers, a translation unit each (w4_few.hip, w4_gemm.hip, w4_gemm_t.hip). Arguments are checked.
+#pragma once
+#include "few_rows.hpp"
+#include "tile_mm.hpp"
+
+namespace qmm {
+int w4_few(const few::Args &a, bool x_f32, int gs, hipStream_t s);
+int w4_gemm(const tmm::Args &a, int gs, hipStream_t s);
+int w4_gemm_t(const tmm::Args &a, int gs, hipStream_t s);
+}  // namespace qmm

@@ -37,6 +37,14 @@ the rest of a dense feed-forward sub-layer around those products, without counte
     ffn_gate_up_backward  its gradients with respect to the projections' outputs and to x (frozen weights)
     gemm_t                the transposed product x W, a projection's input gradient
 
+products on 4-bit weights with group scales and on rows sorted by expert, without counterparts in the reference either:
+
+    w4_pack               codes, scales and zero points laid out once
+    w4_mm                 x W^T, dense or by expert over ragged segments of rows
+    w4_mm_t               its input gradient (frozen weights)
+    ragged_mm             x W_e^T with 16-bit expert weights over ragged segments
+    ragged_mm_backward    its gradients (ragged_mm_t with respect to x, ragged_mm_dw to the weights)
+
 plus the gfx950-specific producers ``quant_mxfp8`` (A operand of the scaled MFMA), ``repack_mxfp4`` (GGUF
 MXFP4 blocks to split planes) and ``tile_mxfp4`` (split planes to the MFMA-tiled planes the grouped GEMM streams
 fastest), the last two one-time weight preparations.
@@ -1106,6 +1114,177 @@ def gemm_t(fmt, x, w, n, k, w2=None, out_dtype=torch.float32, y=None):
     _lib.call("qmm_gemm_t", CODE[fmt], rows, k, n, _ptr(x16), _ptr(scales), _ptr(w), _ptr(w2), _ptr(y), _dt(y), _ptr(work),
               need, s)
     return y
+
+
+# ------------------------------------------------------- 4-bit weights with group scales; rows sorted by expert
+def _w4_sizes(n, k, group):
+    """(bytes of a packed matrix, bytes of its scale words); the library refuses shapes it does not take."""
+    lib = _lib.load()
+    size, words = lib.qmm_w4_bytes(n, k), lib.qmm_w4_scale_bytes(n, k, group)
+    if size < 0 or words < 0:
+        raise ValueError(f"4-bit weights have K % 32 == 0 and groups of 32, 64, 128, ... values or whole rows, not [{n}, {k}] "
+                         f"in groups of {group}")
+    return size, words
+
+
+def w4_pack(codes, scales, zeros=None, group=128):
+    """4-bit weights W[r, c] = scales[r, c // group] (codes[r, c] - zeros[r, c // group]) in the layout that w4_mm reads, made
+    once (qmm_w4_pack): codes u8 [n, k] or [E, n, k] of 0 .. 15, scales f16 [..., n, ceil(k / group)], zeros u8 of 0 .. 15 of that
+    shape, or None for 8. group 32, 64, 128, ... or at least k for one scale a row; k % 32 == 0. Returns (w u8, ws i32)."""
+    s = _here(codes, scales, zeros)
+    if codes.dim() not in (2, 3) or codes.dtype != torch.uint8:
+        raise ValueError(f"codes are u8 [n, k] or [E, n, k], not {codes.dtype} {tuple(codes.shape)}")
+    E = codes.shape[0] if codes.dim() == 3 else 1
+    n, k = codes.shape[-2:]
+    size, words = _w4_sizes(n, k, group)
+    groups = (*codes.shape[:-1], -(-k // group))
+    _shaped(scales, groups, (torch.float16,), "scales")
+    _shaped(zeros, groups, (torch.uint8,), "zeros")
+    w = torch.empty(E * size, dtype=torch.uint8, device=codes.device)
+    ws = torch.empty(E * words // 4, dtype=torch.int32, device=codes.device)
+    _lib.call("qmm_w4_pack", E, n, k, group, _ptr(codes), _ptr(scales), _ptr(zeros), _ptr(w), _ptr(ws), s)
+    return w, ws
+
+
+def _segments(offsets):
+    """The number of experts that offsets [E + 1] separate (None: one matrix for all rows)."""
+    if offsets is None:
+        return 1
+    if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.numel() < 2:
+        raise ValueError(f"offsets are i32 [E + 1], not {offsets.dtype} {tuple(offsets.shape)}")
+    return offsets.numel() - 1
+
+
+def _w4_weights(w, ws, n, k, group, E):
+    size, words = _w4_sizes(n, k, group)
+    if w.nbytes != E * size or ws.nbytes != E * words:
+        raise ValueError(f"{E} packed matrices [{n}, {k}] in groups of {group} are {E * size} and {E * words} bytes, w and ws have "
+                         f"{w.nbytes} and {ws.nbytes}")
+
+
+def _w4_few(rows, E, offsets):
+    """Whether f32 / bf16 rows are multiplied as they are (weights streamed once for up to 64 rows) rather than as f16 tiles."""
+    return rows < GEMM_MIN_TOKENS if offsets is None else rows <= 16 * E
+
+
+def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=None):
+    """y = x W^T on weights of w4_pack (qmm_w4_mm): one matrix, or with offsets (i32 [E + 1] on the device) the matrix of
+    expert e for rows offsets[e] .. offsets[e + 1] - 1; rows of no expert are left as they were in y. x f32 / bf16 [rows, k]: few
+    rows (below 64, or 16 an expert) are multiplied exactly, more go through row_scale_f16 first; or the f16 operand
+    [rows, k] with its scales f32 [rows, 2] (or None). y [rows, n] f32 or bf16 (out_dtype)."""
+    s = _here(x, w, ws, offsets, scales, y)
+    E = _segments(offsets)
+    _w4_weights(w, ws, n, k, group, E)
+    if x.dim() != 2 or x.shape[1] != k:
+        raise ValueError(f"x is {tuple(x.shape)}, expected [rows, {k}]")
+    rows = x.shape[0]
+    y = _rows_out(y, (rows, n), out_dtype, x, (x, w, ws, offsets, scales))
+    if x.dtype == torch.float16:
+        _shaped(scales, (rows, 2), (torch.float32,), "scales")
+    elif scales is not None:
+        raise ValueError("scales come with an f16 operand")
+    elif x.dtype not in _VALUE:
+        raise ValueError(f"x is {x.dtype}")
+    elif not _w4_few(rows, E, offsets):
+        x, scales = row_scale_f16(x)
+    _lib.call("qmm_w4_mm", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), x.data_ptr(), _DT[x.dtype],
+              None if scales is None else scales.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), _DT[y.dtype], s)
+    return y
+
+
+def w4_mm_t(dy, w, ws, n, k, group, offsets=None, y=None, out_dtype=None):
+    """dx = dy W, the input gradient of w4_mm at dy (f32 / bf16 [rows, n]) with frozen weights (qmm_grad_operand, qmm_w4_mm_t);
+    offsets as w4_mm. dx [rows, k] f32 or bf16 (out_dtype, or y)."""
+    s = _here(dy, w, ws, offsets, y)
+    E = _segments(offsets)
+    _w4_weights(w, ws, n, k, group, E)
+    if dy.dim() != 2:
+        raise ValueError(f"dy is {tuple(dy.shape)}, expected [rows, {n}]")
+    rows = dy.shape[0]
+    _shaped(dy, (rows, n), _VALUE, "dy")
+    y = _rows_out(y, (rows, k), out_dtype, dy, (dy, w, ws, offsets))
+    if rows == 0:
+        return y
+    x16 = torch.empty((rows, 1, -(-n // 64) * 64), dtype=torch.float16, device=dy.device)
+    scales = torch.empty((rows, 2), dtype=torch.float32, device=dy.device)
+    _lib.call("qmm_grad_operand", rows, 1, n, dy.data_ptr(), _DT[dy.dtype], x16.data_ptr(), scales.data_ptr(), s)
+    _lib.call("qmm_w4_mm_t", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), x16.data_ptr(),
+              scales.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), _DT[y.dtype], s)
+    return y
+
+
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def _ragged_weights(offsets, w, what="w"):
+    E = _segments(offsets)
+    if w.dim() != 3 or w.shape[0] != E or w.dtype not in _HALF:
+        raise ValueError(f"{what} is {w.dtype} {tuple(w.shape)}, expected bf16 or f16 [{E}, n, k]")
+    return w.shape
+
+
+def _ragged_out(y, shape, out_dtype, x, reads, what):
+    """An output of a ragged product: f32 or the operands' type (that type when neither y nor out_dtype says)."""
+    if y is None:
+        y = torch.empty(shape, dtype=x.dtype if out_dtype is None else out_dtype, device=x.device)
+    elif out_dtype is not None and out_dtype != y.dtype:
+        raise ValueError(f"{what} is {y.dtype}, out_dtype {out_dtype}")
+    _shaped(y, shape, (torch.float32, x.dtype), what)
+    _apart(y, what, reads)
+    return y
+
+
+def ragged_mm(x, offsets, w, y=None, out_dtype=None):
+    """y[t] = W_e x[t] for rows sorted by expert, offsets[e] .. offsets[e + 1] - 1 (i32 [E + 1] on the device) being expert e's
+    (qmm_ragged_mm). x [rows, k] and w [E, n, k] bf16 or f16 alike, n % 8 == 0, k % 8 == 0; y [rows, n] of that type or f32
+    (out_dtype). Rows of no expert are left as they were in y."""
+    s = _here(x, offsets, w, y)
+    E, n, k = _ragged_weights(offsets, w)
+    if x.dim() != 2:
+        raise ValueError(f"x is {tuple(x.shape)}, expected [rows, {k}]")
+    rows = x.shape[0]
+    _shaped(x, (rows, k), (w.dtype,), "x")
+    y = _ragged_out(y, (rows, n), out_dtype, x, (x, offsets, w), "y")
+    _lib.call("qmm_ragged_mm", rows, k, n, E, offsets.data_ptr(), x.data_ptr(), w.data_ptr(), _DT[w.dtype], y.data_ptr(),
+              _DT[y.dtype], s)
+    return y
+
+
+def ragged_mm_t(dy, offsets, w, dx=None, out_dtype=None):
+    """dx[t] = W_e^T dy[t], the gradient of ragged_mm with respect to x (qmm_ragged_mm_t): dy [rows, n] of w's type, dx
+    [rows, k] of that type or f32. Rows of no expert are left as they were in dx."""
+    s = _here(dy, offsets, w, dx)
+    E, n, k = _ragged_weights(offsets, w)
+    if dy.dim() != 2:
+        raise ValueError(f"dy is {tuple(dy.shape)}, expected [rows, {n}]")
+    rows = dy.shape[0]
+    _shaped(dy, (rows, n), (w.dtype,), "dy")
+    dx = _ragged_out(dx, (rows, k), out_dtype, dy, (dy, offsets, w), "dx")
+    _lib.call("qmm_ragged_mm_t", rows, k, n, E, offsets.data_ptr(), dy.data_ptr(), w.data_ptr(), _DT[w.dtype], dx.data_ptr(),
+              _DT[dx.dtype], s)
+    return dx
+
+
+def ragged_mm_dw(dy, x, offsets, dw=None, out_dtype=None):
+    """dw[e] = sum of dy[t] x[t]^T over expert e's rows, the gradient of ragged_mm with respect to the weights
+    (qmm_ragged_mm_dw): dy [rows, n], x [rows, k] of one 16-bit type, dw [E, n, k] of that type or f32, zero for an expert
+    without rows; rows of no expert count nowhere."""
+    s = _here(x, dy, offsets, dw)
+    E = _segments(offsets)
+    if x.dim() != 2 or dy.dim() != 2 or x.dtype not in _HALF:
+        raise ValueError(f"x and dy are bf16 or f16 rows, not {x.dtype} {tuple(x.shape)} and {tuple(dy.shape)}")
+    rows, k = x.shape
+    n = dy.shape[1]
+    _shaped(dy, (rows, n), (x.dtype,), "dy")
+    dw = _ragged_out(dw, (E, n, k), out_dtype, x, (x, dy, offsets), "dw")
+    _lib.call("qmm_ragged_mm_dw", rows, k, n, E, offsets.data_ptr(), dy.data_ptr(), x.data_ptr(), _DT[x.dtype], dw.data_ptr(),
+              _DT[dw.dtype], s)
+    return dw
+
+
+def ragged_mm_backward(dy, x, offsets, w, out_dtype=None, dw_dtype=None):
+    """The gradients of ragged_mm at dy: (dx, dw) of out_dtype and dw_dtype (w's type, or f32)."""
+    return ragged_mm_t(dy, offsets, w, out_dtype=out_dtype), ragged_mm_dw(dy, x, offsets, out_dtype=dw_dtype)
 
 
 def moe_routed(fmt, x, logits, E, KU, H, FE, gating, norm, **kw):

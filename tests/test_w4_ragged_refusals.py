@@ -1,0 +1,150 @@
+"""What the 4-bit and ragged products refuse, without a device: the C entry points' statuses and the errors of the Python
+surface. Nothing is launched."""
+import pytest
+import torch
+
+from test_abi import header_enum, lib  # noqa: F401  (fixture)
+from test_sublayer_refusals import BF16, F16, F32, MXFP8, Q8, at, ops  # noqa: F401  (fixture)
+
+ODD, BYTE = at(0x10008), at(0x10001)
+
+
+def test_w4_sizes(lib):   # noqa: F811
+    assert lib.qmm_w4_bytes(16, 128) == 1024 and lib.qmm_w4_bytes(17, 160) == 4096 and lib.qmm_w4_bytes(1, 32) == 1024
+    assert lib.qmm_w4_scale_bytes(17, 160, 64) == 2 * 3 * 64 and lib.qmm_w4_scale_bytes(16, 4096, 1 << 40) == 64
+    for n, k in ((0, 32), (8, 0), (8, 33), (-1, 32), ((1 << 20) + 1, 32), (8, (1 << 20) + 32)):
+        assert lib.qmm_w4_bytes(n, k) == -1
+    for group in (0, 16, 33, 96, -32):
+        assert lib.qmm_w4_scale_bytes(8, 256, group) == -1
+
+
+def test_w4_pack_statuses(lib):   # noqa: F811
+    st = header_enum("qmm_status")
+
+    def call(E=1, n=8, k=64, group=32, codes=at(), scales=at(), zeros=None, w=at(), ws=at()):
+        return lib.qmm_w4_pack(E, n, k, group, codes, scales, zeros, w, ws, None)
+
+    for bad in (dict(n=0), dict(k=48), dict(k=0), dict(group=48), dict(group=16)):
+        assert call(**bad) == st["QMM_ERR_SHAPE"], bad
+    for bad in (dict(E=0), dict(E=1025)):
+        assert call(**bad) == st["QMM_ERR_RANGE"], bad
+    for bad in (dict(codes=None), dict(scales=None), dict(w=None), dict(ws=None)):
+        assert call(**bad) == st["QMM_ERR_NULL"], bad
+    for bad in (dict(w=ODD), dict(ws=ODD), dict(scales=BYTE)):
+        assert call(**bad) == st["QMM_ERR_ALIGN"], bad
+
+
+def test_w4_mm_statuses(lib):   # noqa: F811
+    st = header_enum("qmm_status")
+
+    def mm(rows=4, k=64, n=8, group=32, E=1, off=None, x=at(), xd=BF16, s=None, w=at(), ws=at(), y=at(), yd=F32):
+        return lib.qmm_w4_mm(rows, k, n, group, E, off, x, xd, s, w, ws, y, yd, None)
+
+    def back(rows=4, k=64, n=8, group=32, E=1, off=None, x=at(), s=at(), w=at(), ws=at(), y=at(), yd=F32):
+        return lib.qmm_w4_mm_t(rows, k, n, group, E, off, x, s, w, ws, y, yd, None)
+
+    for call in (mm, back):
+        for bad in (dict(rows=-1), dict(rows=(1 << 24) + 1), dict(k=40), dict(n=0), dict(group=24), dict(k=(1 << 20) + 32)):
+            assert call(**bad) == st["QMM_ERR_SHAPE"], bad
+        for bad in (dict(E=0), dict(E=2), dict(E=1025, off=at())):
+            assert call(**bad) == st["QMM_ERR_RANGE"], bad
+        for bad in (dict(yd=F16), dict(yd=Q8), dict(yd=-1)):
+            assert call(**bad) == st["QMM_ERR_DTYPE"], bad
+        for bad in (dict(x=None), dict(w=None), dict(ws=None), dict(y=None)):
+            assert call(**bad) == st["QMM_ERR_NULL"], bad
+        for bad in (dict(x=ODD), dict(w=ODD), dict(ws=ODD), dict(y=at(0x10002)), dict(yd=BF16, y=BYTE), dict(off=at(0x10002)), dict(s=at(0x10002))):
+            assert call(**bad) == st["QMM_ERR_ALIGN"], bad
+        assert call(rows=0, x=None, w=None, ws=None, y=None) == 0
+    assert back(s=None) == st["QMM_ERR_NULL"]
+    for xd in (Q8, MXFP8, -1):
+        assert mm(xd=xd) == st["QMM_ERR_DTYPE"]
+
+
+def test_ragged_statuses(lib):   # noqa: F811
+    st = header_enum("qmm_status")
+
+    def of(fn):
+        return lambda rows=4, k=64, n=8, E=2, off=at(), a=at(), b=at(), d=BF16, y=at(), yd=F32: fn(rows, k, n, E, off, a, b, d, y, yd, None)
+
+    for fn in (lib.qmm_ragged_mm, lib.qmm_ragged_mm_t, lib.qmm_ragged_mm_dw):
+        call = of(fn)
+        for bad in (dict(d=F32), dict(d=Q8), dict(yd=F16), dict(d=F16, yd=BF16)):
+            assert call(**bad) == st["QMM_ERR_DTYPE"], bad
+        for bad in (dict(rows=-1), dict(rows=(1 << 24) + 1), dict(k=0), dict(k=60), dict(n=12), dict(n=(1 << 20) + 8)):
+            assert call(**bad) == st["QMM_ERR_SHAPE"], bad
+        for bad in (dict(E=0), dict(E=1025)):
+            assert call(**bad) == st["QMM_ERR_RANGE"], bad
+        for bad in (dict(off=None), dict(a=None), dict(b=None), dict(y=None)):
+            assert call(**bad) == st["QMM_ERR_NULL"], bad
+        for bad in (dict(a=ODD), dict(b=ODD), dict(y=ODD), dict(off=at(0x10002))):
+            assert call(**bad) == st["QMM_ERR_ALIGN"], bad
+    assert of(lib.qmm_ragged_mm)(rows=0, a=None, y=None) == 0
+    assert of(lib.qmm_ragged_mm_t)(rows=0, a=None, y=None) == 0
+
+
+def w4(n=8, k=64, group=32, E=1):
+    blocks, tiles, groups = -(-n // 16), -(-k // 128), -(-k // group)
+    return torch.zeros(E * blocks * tiles * 1024, dtype=torch.uint8), torch.zeros(E * blocks * groups * 16, dtype=torch.int32)
+
+
+def test_w4_surface(ops):   # noqa: F811
+    w, ws = w4()
+    x, dy, off = torch.zeros(4, 64), torch.zeros(4, 8), torch.zeros(2, dtype=torch.int32)
+    half = torch.zeros(4, 64, dtype=torch.float16)
+    wrong = [
+        lambda: ops.w4_pack(torch.zeros(8, 64), torch.zeros(8, 2).half(), group=32),
+        lambda: ops.w4_pack(torch.zeros(8, 64, dtype=torch.uint8), torch.zeros(8, 2), group=32),
+        lambda: ops.w4_pack(torch.zeros(8, 64, dtype=torch.uint8), torch.zeros(8, 1).half(), group=32),
+        lambda: ops.w4_pack(torch.zeros(8, 64, dtype=torch.uint8), torch.zeros(8, 2).half(), torch.zeros(8, 2), group=32),
+        lambda: ops.w4_pack(torch.zeros(8, 48, dtype=torch.uint8), torch.zeros(8, 2).half(), group=32),
+        lambda: ops.w4_pack(torch.zeros(64, dtype=torch.uint8), torch.zeros(2).half(), group=32),
+        lambda: ops.w4_mm(x, w[:-1], ws, 8, 64, 32), lambda: ops.w4_mm(x, w, ws[:-1], 8, 64, 32), lambda: ops.w4_mm(x, w, ws, 8, 64, 64),
+        lambda: ops.w4_mm(x, w, ws, 8, 64, 48), lambda: ops.w4_mm(x, w, ws, 24, 64, 32), lambda: ops.w4_mm(x[:, :32].contiguous(), w, ws, 8, 64, 32),
+        lambda: ops.w4_mm(x[0], w, ws, 8, 64, 32), lambda: ops.w4_mm(x[:, ::2], w, ws, 8, 32, 32), lambda: ops.w4_mm(x.double(), w, ws, 8, 64, 32),
+        lambda: ops.w4_mm(x, w, ws, 8, 64, 32, scales=torch.ones(4, 2)), lambda: ops.w4_mm(half, w, ws, 8, 64, 32, scales=torch.ones(3, 2)),
+        lambda: ops.w4_mm(x, w, ws, 8, 64, 32, offsets=off.long()), lambda: ops.w4_mm(x, w, ws, 8, 64, 32, offsets=off[:1]),
+        lambda: ops.w4_mm(x, w, ws, 8, 64, 32, offsets=torch.zeros(3, dtype=torch.int32)),
+        lambda: ops.w4_mm(x, w, ws, 8, 64, 32, y=torch.zeros(4, 9)), lambda: ops.w4_mm(x, w, ws, 8, 64, 32, out_dtype=torch.float16),
+        lambda: ops.w4_mm(x, w, ws, 8, 64, 32, y=x.view(-1)[8:40].view(4, 8)), lambda: ops.w4_mm(x, w, ws, 8, 64, 32, y=w.view(torch.float32)[:32].view(4, 8)),
+        lambda: ops.w4_mm_t(dy[:, :4].contiguous(), w, ws, 8, 64, 32), lambda: ops.w4_mm_t(dy.half(), w, ws, 8, 64, 32),
+        lambda: ops.w4_mm_t(dy[0], w, ws, 8, 64, 32), lambda: ops.w4_mm_t(dy, w, ws[1:], 8, 64, 32),
+        lambda: ops.w4_mm_t(dy, w, ws, 8, 64, 32, y=w.view(torch.float32).view(4, 64)),
+    ]
+    for i, call in enumerate(wrong):
+        with pytest.raises(ValueError):
+            print("call", i)
+            call()
+
+
+def test_ragged_surface(ops):   # noqa: F811
+    x, dy, w = torch.zeros(4, 64).bfloat16(), torch.zeros(4, 16).bfloat16(), torch.zeros(2, 16, 64).bfloat16()
+    off = torch.zeros(3, dtype=torch.int32)
+    wrong = [
+        lambda: ops.ragged_mm(x, off[:2], w), lambda: ops.ragged_mm(x, off.long(), w), lambda: ops.ragged_mm(x, off, w[0]),
+        lambda: ops.ragged_mm(x.float(), off, w), lambda: ops.ragged_mm(x.half(), off, w), lambda: ops.ragged_mm(x, off, w.float()),
+        lambda: ops.ragged_mm(x[:, :32].contiguous(), off, w), lambda: ops.ragged_mm(x[0], off, w), lambda: ops.ragged_mm(x, off, w.transpose(1, 2)),
+        lambda: ops.ragged_mm(x, off, w, out_dtype=torch.float16), lambda: ops.ragged_mm(x, off, w, y=torch.zeros(4, 8)),
+        lambda: ops.ragged_mm(x, off, w, y=torch.zeros(4, 16), out_dtype=torch.bfloat16), lambda: ops.ragged_mm(x, off, w, y=x.view(-1)[:64].view(4, 16)),
+        lambda: ops.ragged_mm_t(dy[:, :8].contiguous(), off, w), lambda: ops.ragged_mm_t(dy.half(), off, w), lambda: ops.ragged_mm_t(dy, off, w, dx=w[0, :4]),
+        lambda: ops.ragged_mm_t(dy[0], off, w), lambda: ops.ragged_mm_dw(dy[:3], x, off), lambda: ops.ragged_mm_dw(dy.half(), x, off),
+        lambda: ops.ragged_mm_dw(dy.float(), x.float(), off), lambda: ops.ragged_mm_dw(dy[0], x, off), lambda: ops.ragged_mm_dw(dy, x, off, dw=torch.zeros(2, 64, 16)),
+        lambda: ops.ragged_mm_dw(dy, x, off.float()),
+    ]
+    for i, call in enumerate(wrong):
+        with pytest.raises(ValueError):
+            print("call", i)
+            call()
+
+
+def test_good_calls_reach_the_library(ops):   # noqa: F811
+    w, ws = w4()
+    x = torch.zeros(4, 64)
+    off = torch.zeros(3, dtype=torch.int32)
+    w2, ws2 = w4(E=2)
+    r = torch.zeros(2, 16, 64).bfloat16()
+    for call in (lambda: ops.w4_mm(x, w, ws, 8, 64, 32), lambda: ops.w4_mm(x.half(), w, ws, 8, 64, 32, y=torch.zeros(4, 8)),
+                 lambda: ops.w4_mm(x, w2, ws2, 8, 64, 32, offsets=off), lambda: ops.w4_mm_t(torch.zeros(4, 8), w, ws, 8, 64, 32),
+                 lambda: ops.ragged_mm(x.bfloat16(), off, r), lambda: ops.ragged_mm_t(torch.zeros(4, 16).bfloat16(), off, r),
+                 lambda: ops.ragged_mm_dw(torch.zeros(4, 16).bfloat16(), x.bfloat16(), off)):
+        with pytest.raises(AssertionError, match="was reached"):
+            call()
