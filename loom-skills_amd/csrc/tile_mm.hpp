@@ -74,11 +74,11 @@ __device__ __forceinline__ void wait_all_barrier() {
   __builtin_amdgcn_s_waitcnt(0x0070);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
-__device__ __forceinline__ u32x4 resource(const u8 *p, int64_t bytes) {
+// bytes past 0 (every extent here is below 2^31: at most 256 rows of 2^21 bytes)
+__device__ __forceinline__ u32x4 resource(const u8 *p, int bytes) {
   const uint64_t at = (uint64_t)p;
-  const u32 n = (u32)max((int64_t)0, min(bytes, (int64_t)0x7FFFFFF0));
   return u32x4{(u32)__builtin_amdgcn_readfirstlane((int)(u32)at), (u32)__builtin_amdgcn_readfirstlane((int)((u32)(at >> 32) & 0xFFFFu)),
-               (u32)__builtin_amdgcn_readfirstlane((int)n), 0x00020000u};
+               (u32)__builtin_amdgcn_readfirstlane(max(bytes, 0)), 0x00020000u};
 }
 
 __device__ __forceinline__ h2 as_h2(u32 v) { return __builtin_bit_cast(h2, v); }
@@ -129,11 +129,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
     if (a.offsets) find_tile<BM>(a.offsets, a.E, a.rows, sc, mt, e, lo, hi, mt);
     m0 = mt * BM;
   } else {
-    const int tiles_m = (a.M + BM - 1) / BM, per_e = tiles_m * a.tiles_n, total = per_e * a.E, per = (total + 7) >> 3;
-    const int i = (int)(blockIdx.x >> 3), t = (int)(blockIdx.x & 7) * per + i;
-    if (i >= per || t >= total) return;
-    e = t / per_e;
-    const int r = t - e * per_e;
+    // every XCD takes an eighth of every expert's tiles, one expert after the other: experts differ in their rows
+    const int tiles_m = (a.M + BM - 1) / BM, per_e = tiles_m * a.tiles_n, per = (per_e + 7) >> 3;
+    const int i = (int)(blockIdx.x >> 3);
+    e = i / per;
+    const int r = (int)(blockIdx.x & 7) * per + i - e * per;
+    if (e >= a.E || r >= per_e) return;
     m0 = (r % tiles_m) * BM;
     nt = r / tiles_m;
     lo = clamp_row(__builtin_amdgcn_readfirstlane(a.offsets[e]), a.rows);
@@ -178,25 +179,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
     bp += (int64_t)lo * a.b_row + (int64_t)n0 * 2;
   }
   const u32 lds0 = (u32)(uintptr_t)(__attribute__((address_space(3))) u8 *)smem;
+  const int a_row = (int)a.a_row, b_row = (int)a.b_row;
+  const int a_bytes = SA == kRow ? min(BM, m_end - m0) * a_row : 0, b_bytes = SB == kRow ? min(BN, a.N - n0) * b_row : 0;
+  // past the last step (s >= S) the loads give zeros: kRow by the values' check, kCol by the rows left
   auto load_a = [&](int s, int i) __attribute__((always_inline)) {
     const u32 dst = __builtin_amdgcn_readfirstlane(lds0 + (u32)((s & 1) * kA + (i * NW + wave) * 1024));
-    if constexpr (SA == kRow) {
-      const u32x4 r = resource(ap + (int64_t)s * 128, (int64_t)min(BM, m_end - m0) * a.a_row - (int64_t)s * 128);
-      lds_load16(r, 64 * s + acol[i] < K ? aoff[i] : kPast, dst);
-    } else {
-      const u32x4 r = resource(ap + (int64_t)s * 64 * a.a_row, (int64_t)min(64, K - 64 * s) * a.a_row - (int64_t)m0 * 2);
-      lds_load16(r, aoff[i], dst);
-    }
+    if constexpr (SA == kRow)
+      lds_load16(resource(ap + (int64_t)s * 128, a_bytes - s * 128), 64 * s + acol[i] < K ? aoff[i] : kPast, dst);
+    else
+      lds_load16(resource(ap + (int64_t)s * 64 * a_row, min(64, K - 64 * s) * a_row - m0 * 2), aoff[i], dst);
   };
   auto load_b = [&](int s, int i) __attribute__((always_inline)) {
     const u32 dst = __builtin_amdgcn_readfirstlane(lds0 + (u32)(2 * kA + (s & 1) * kB + (i * NW + wave) * 1024));
-    if constexpr (SB == kRow) {
-      const u32x4 r = resource(bp + (int64_t)s * 128, (int64_t)min(BN, a.N - n0) * a.b_row - (int64_t)s * 128);
-      lds_load16(r, 64 * s + bcol[i] < K ? boff[i] : kPast, dst);
-    } else if constexpr (SB == kCol) {
-      const u32x4 r = resource(bp + (int64_t)s * 64 * a.b_row, (int64_t)min(64, K - 64 * s) * a.b_row - (int64_t)n0 * 2);
-      lds_load16(r, boff[i], dst);
-    }
+    if constexpr (SB == kRow)
+      lds_load16(resource(bp + (int64_t)s * 128, b_bytes - s * 128), 64 * s + bcol[i] < K ? boff[i] : kPast, dst);
+    else if constexpr (SB == kCol)
+      lds_load16(resource(bp + (int64_t)s * 64 * b_row, min(64, K - 64 * s) * b_row - n0 * 2), boff[i], dst);
   };
 
   // ---- w4: unit u of a step is a lane's 16 bytes of a 16-row x 128-value tile (kW4Row: the half that the step covers). Rows and
@@ -292,20 +290,57 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
       for (int i = 0; i < LB; ++i) load_b(s, i);
     }
   };
+  constexpr int kLoads = LA + (kW4 ? 0 : LB);
   u32x4 fa[2][NI], fb[2][NJ];
-  auto read = [&](int set, int s, int kk) __attribute__((always_inline)) {
+  // the walk along the sum with the wave's first NA 32-row blocks; every wave meets every barrier
+  auto walk = [&](auto blocks) __attribute__((always_inline)) {
+    constexpr int NA = decltype(blocks)::value;
+    auto read = [&](int set, int s, int kk) __attribute__((always_inline)) {
+      if constexpr (NA > 0) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) fb[set][j] = read_b(s, j, kk);
+        for (int j = 0; j < NJ; ++j) fb[set][j] = read_b(s, j, kk);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) fa[set][i] = read_a(s, i, kk);
-  };
-  auto multiply = [&](int set) __attribute__((always_inline)) {
+        for (int i = 0; i < NA; ++i) fa[set][i] = read_a(s, i, kk);
+      }
+    };
+    auto multiply = [&](int set) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+      for (int i = 0; i < NA; ++i)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[i][j] = mfma<DT>(fa[set][i], fb[set][j], acc[i][j]);
+        for (int j = 0; j < NJ; ++j) acc[i][j] = mfma<DT>(fa[set][i], fb[set][j], acc[i][j]);
+    };
+    read(0, 0, 0);
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int kk = 0; kk < 3; ++kk) {
+        read((kk + 1) & 1, s, kk + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kW4) {   // the next step's weights, whose buffer the last barrier has freed
+#pragma unroll
+          for (int i = kk; i < kUnits; i += 3)
+            if (s + 1 < S) store_w4(s + 1, i);
+        }
+        multiply(kk & 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      wait_all_barrier();
+      read(0, s + 1, 0);   // past the last step: what the buffer holds, not used
+      if constexpr (kW4) load_w4(s + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      // the step after the next one's loads (past the last step: zeros) between these MFMAs
+#pragma unroll
+      for (int m = 0; m < (NA * NJ > kLoads ? NA * NJ : kLoads); ++m) {
+        if (m < LA) load_a(s + 2, m);
+        else if (m < kLoads) load_b(s + 2, m - LA);
+        if (m < NA * NJ) acc[m / NJ][m % NJ] = mfma<DT>(fa[1][m / NJ], fb[1][m % NJ], acc[m / NJ][m % NJ]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    wait_all_barrier();   // the buffers are the outputs' staging areas next
   };
 
+  // blocks of 32 rows of the wave that hold outputs at all (the last tile of a segment is often nearly empty)
+  const int live = n0 + wn * NJ * 32 < a.N ? min(max((m_end - m0 - wm * NI * 32 + 31) >> 5, 0), NI) : 0;
   if (S > 0) {
     load(0);
     if constexpr (kW4) {
@@ -316,26 +351,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
     }
     wait_all_barrier();
     if (S > 1) load(1);
-    read(0, 0, 0);
-    for (int s = 0; s < S; ++s) {
-#pragma unroll
-      for (int kk = 0; kk < 3; ++kk) {
-        read((kk + 1) & 1, s, kk + 1);
-        if constexpr (kW4) {   // the next step's weights, whose buffer the last barrier has freed
-#pragma unroll
-          for (int i = kk; i < kUnits; i += 3)
-            if (s + 1 < S) store_w4(s + 1, i);
-        }
-        multiply(kk & 1);
-      }
-      wait_all_barrier();
-      if (s + 2 < S) {
-        load(s + 2);
-        if constexpr (kW4) load_w4(s + 2);
-      }
-      if (s + 1 < S) read(0, s + 1, 0);
-      multiply(1);
-    }
+    if (live == NI) walk(std::integral_constant<int, NI>{});
+    else if (live == 0) walk(std::integral_constant<int, 0>{});
+    else if (NI > 1 && live == 1) walk(std::integral_constant<int, 1>{});
+    else if (NI > 2 && live == 2) walk(std::integral_constant<int, NI < 2 ? NI : 2>{});
+    else if (NI > 3) walk(std::integral_constant<int, NI < 3 ? NI : 3>{});
   }
 
   // ---- outputs, 32 rows of a wave at a time through its own LDS (every wave is past its last read of the operands): the sums
@@ -346,6 +366,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   const int64_t out0 = SUM == kSumFixed ? (int64_t)lo * a.N : (int64_t)e * a.M * a.N;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
+    if (i >= live) break;
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
@@ -405,10 +426,8 @@ int launch(const Args &in, hipStream_t s) {
   Args a = in;
   a.tiles_n = (a.N + BN - 1) / BN;
   // row tiles: at most one ragged tile an expert beside the whole ones
-  const int64_t tiles_m = SUM == kSumRagged ? (int64_t)((a.M + BM - 1) / BM) * a.E
-                          : a.offsets       ? std::min<int64_t>((int64_t)a.rows / BM + a.E, a.rows)
-                                            : (a.rows + BM - 1) / BM;
-  const int64_t tiles = tiles_m * a.tiles_n;
+  const int64_t tiles_m = a.offsets ? std::min<int64_t>((int64_t)a.rows / BM + a.E, a.rows) : (a.rows + BM - 1) / BM;
+  const int64_t tiles = SUM == kSumRagged ? ((int64_t)((a.M + BM - 1) / BM) * a.tiles_n + 7) / 8 * 8 * a.E : tiles_m * a.tiles_n;
   if (tiles > (1 << 22)) return QMM_ERR_SHAPE;   // HIP refuses 2^32 threads along a grid's dimension
   constexpr int lds = 2 * (BM + BN) * 128;
   auto *fn = tile_mm_kernel<DT, SA, SB, SUM, BM, BN, WM, WN, GS>;
