@@ -290,6 +290,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
       for (int i = 0; i < LB; ++i) load_b(s, i);
     }
   };
+  constexpr int kGap = 32 * kWords * ((kUnits + 1) / 2) / (NI * NJ) + 1;   // vector instructions between two MFMAs
+  static_assert(!kW4 || kUnits <= 2, "a unit a phase");
   constexpr int kLoads = LA + (kW4 ? 0 : LB);
   u32x4 fa[2][NI], fb[2][NJ];
   // the walk along the sum with the wave's first NA 32-row blocks; every wave meets every barrier
@@ -315,12 +317,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
       for (int kk = 0; kk < 3; ++kk) {
         read((kk + 1) & 1, s, kk + 1);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (kW4) {   // the next step's weights, whose buffer the last barrier has freed
-#pragma unroll
-          for (int i = kk; i < kUnits; i += 3)
-            if (s + 1 < S) store_w4(s + 1, i);
+        // the next step's weights, whose buffer the last barrier has freed: late in the step, their loads are one step old then
+        if constexpr (kW4 && kUnits > 1) {
+          if (kk > 0) store_w4(s + 1, kk - 1);
+        } else if constexpr (kW4) {
+          if (kk == 2) store_w4(s + 1, 0);
         }
         multiply(kk & 1);
+        if constexpr (kW4) {
+          if (kk > 0) {
+#pragma unroll
+            for (int m = 0; m < NA * NJ; ++m) {   // an MFMA, then vector instructions of the weights
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, kGap, 0);
+            }
+          }
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
       wait_all_barrier();
