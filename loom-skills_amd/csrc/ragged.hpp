@@ -59,22 +59,19 @@ __device__ __forceinline__ TileScan scan_tiles(const int32_t *offsets, int E, in
   s.before = sum - own;
   return s;
 }
-// Expert and segment of row tile t < s.total, and the tile's number within the segment. Wave-uniform.
+// Expert and segment of row tile t < s.total, and the expert's first tile. Wave-uniform.
 template <int BM>
 __device__ __forceinline__ void find_tile(const int32_t *offsets, int E, int rows, const TileScan &s, int t, int &e, int &lo,
-                                          int &hi, int &nth) {
+                                          int &hi, int &first) {
   const int l = __popcll(__ballot(s.before <= t)) - 1;   // before does not fall along the lanes: the last lane at or below t
-  int left = t - __builtin_amdgcn_readlane(s.before, l);
-  e = s.per * l;
-  for (;;) {
+  first = __builtin_amdgcn_readlane(s.before, l);
+  for (e = min(s.per * l, E - 1);; ++e) {
     lo = clamp_row(__builtin_amdgcn_readfirstlane(offsets[e]), rows);
     hi = clamp_row(__builtin_amdgcn_readfirstlane(offsets[e + 1]), rows);
     const int n = (max(hi - lo, 0) + BM - 1) / BM;
-    if (left < n || e + 1 >= E) break;
-    left -= n;
-    ++e;
+    if (t < first + n || e + 1 >= E) return;
+    first += n;
   }
-  nth = left;
 }
 
 }  // namespace qmm

@@ -114,20 +114,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
-  // ---- the workgroup's tile. Workgroup i runs on XCD i % 8, which takes a contiguous range of tiles in groups of kGroupM row
-  // tiles, rows fastest: the tiles that an XCD works on at a time share operand rows in its L2.
+  // ---- the workgroup's tile. Workgroup i runs on XCD i % 8, which takes a contiguous range of tiles: an expert's in
+  // groups of kGroupM row tiles, rows fastest, so that the tiles that an XCD works on at a time share operands in its L2.
   int e = 0, lo = 0, hi = a.rows, m0, nt;
   if constexpr (SUM == kSumFixed) {
     TileScan sc{(a.rows + BM - 1) / BM, 0, 1};
     if (a.offsets) sc = scan_tiles<BM>(a.offsets, a.E, a.rows);
     const int total = sc.total * a.tiles_n, per = (total + 7) >> 3;
-    const int i = (int)(blockIdx.x >> 3), t = (int)(blockIdx.x & 7) * per + i;
+    const int i = (int)(blockIdx.x >> 3);
+    int t = (int)(blockIdx.x & 7) * per + i, first = 0;
     if (i >= per || t >= total) return;
-    const int g = t / (kGroupM * a.tiles_n), gm = min(kGroupM, sc.total - g * kGroupM), gt = t - g * kGroupM * a.tiles_n;
-    int mt = g * kGroupM + gt % gm;
+    if (a.offsets) find_tile<BM>(a.offsets, a.E, a.rows, sc, t / a.tiles_n, e, lo, hi, first);
+    t -= first * a.tiles_n;
+    const int own = a.offsets ? (max(hi - lo, 1) + BM - 1) / BM : sc.total;   // the expert's row tiles
+    const int g = t / (kGroupM * a.tiles_n), gm = max(1, min(kGroupM, own - g * kGroupM)), gt = t - g * kGroupM * a.tiles_n;
+    m0 = (g * kGroupM + gt % gm) * BM;
     nt = gt / gm;
-    if (a.offsets) find_tile<BM>(a.offsets, a.E, a.rows, sc, mt, e, lo, hi, mt);
-    m0 = mt * BM;
   } else {
     // every XCD takes an eighth of every expert's tiles, one expert after the other: experts differ in their rows
     const int tiles_m = (a.M + BM - 1) / BM, per_e = tiles_m * a.tiles_n, per = (per_e + 7) >> 3;
