@@ -112,7 +112,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   static_assert((SB == kRow || SB == kW4Row) || BN >= 128, "a transposed operand is at least 128 wide");
   extern __shared__ __align__(1024) u8 smem[];            // A [2], B [2]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / WN, wn = wave % WN;
 
   // ---- the workgroup's tile. Workgroup i runs on XCD i % 8, which takes a contiguous range of tiles: an expert's in
   // groups of kGroupM row tiles, rows fastest, so that the tiles that an XCD works on at a time share operands in its L2.
@@ -143,6 +142,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
     hi = clamp_row(__builtin_amdgcn_readfirstlane(a.offsets[e + 1]), a.rows);
   }
   const int n0 = nt * BN;
+  // the wave's blocks of 32 rows rb0 .. rb0 + rows_of - 1 and columns cb0 .. cb0 + NJ - 1. Where a tile has outputs in half or a
+  // quarter of its columns only, twice or four times as many waves share those, with fewer rows each.
+  const int fold = NI >= 4 && WN >= 4 && n0 + BN / 4 >= a.N ? 4 : NI >= 2 && WN >= 2 && n0 + BN / 2 >= a.N ? 2 : 1;
+  const int across = WN / fold, rows_of = NI / fold;
+  const int rb0 = wave / across * rows_of, cb0 = wave % across * NJ;
   const int seg = max(hi - lo, 0);                        // the segment's rows
   const int m_end = SUM == kSumFixed ? seg : a.M;         // outputs m0 .. min(m0 + BM, m_end) - 1
   const int K = SUM == kSumFixed ? a.K : seg, S = (K + 63) >> 6;
@@ -267,13 +271,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   };
   auto read_a = [&](int s, int i, int kk) __attribute__((always_inline)) {
     const u32 at = (u32)((s & 1) * kA);
-    if constexpr (SA == kRow) return read_row(at, wm * NI + i, kk);
-    else return read_col(at, BM * 2, wm * NI + i, kk);
+    if constexpr (SA == kRow) return read_row(at, rb0 + i, kk);
+    else return read_col(at, BM * 2, rb0 + i, kk);
   };
   auto read_b = [&](int s, int j, int kk) __attribute__((always_inline)) {
     const u32 at = (u32)(2 * kA + (s & 1) * kB);
-    if constexpr (SB == kRow || SB == kW4Row) return read_row(at, wn * NJ + j, kk);
-    else return read_col(at, BN * 2, wn * NJ + j, kk);
+    if constexpr (SB == kRow || SB == kW4Row) return read_row(at, cb0 + j, kk);
+    else return read_col(at, BN * 2, cb0 + j, kk);
   };
 
   f32x16 acc[NI][NJ];
@@ -284,17 +288,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  auto load = [&](int s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < LA; ++i) load_a(s, i);
-    if constexpr (!kW4) {
-#pragma unroll
-      for (int i = 0; i < LB; ++i) load_b(s, i);
-    }
-  };
   constexpr int kGap = 32 * kWords * ((kUnits + 1) / 2) / (NI * NJ) + 1;   // vector instructions between two MFMAs
   static_assert(!kW4 || kUnits <= 2, "a unit a phase");
   constexpr int kLoads = LA + (kW4 ? 0 : LB);
+  // of a step's loads, those that go out past the barrier; the rest follow a phase later (w4: none, that phase has the weights)
+  constexpr int kFirst = kW4 ? kLoads : (kLoads + 1) / 2;
+  auto load_one = [&](int s, int l) __attribute__((always_inline)) {
+    if (l < LA) load_a(s, l);
+    else if constexpr (!kW4) load_b(s, l - LA);
+  };
   u32x4 fa[2][NI], fb[2][NJ];
   // the walk along the sum with the wave's first NA 32-row blocks; every wave meets every barrier
   auto walk = [&](auto blocks) __attribute__((always_inline)) {
@@ -313,6 +315,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[i][j] = mfma<DT>(fa[set][i], fb[set][j], acc[i][j]);
     };
+    auto multiply_loading = [&](int set, int s, int first, int end) __attribute__((always_inline)) {   // loads of step s between
+#pragma unroll
+      for (int m = 0; m < (NA * NJ > end - first ? NA * NJ : end - first); ++m) {
+        if (m < end - first) load_one(s, first + m);
+        if (m < NA * NJ) acc[m / NJ][m % NJ] = mfma<DT>(fa[set][m / NJ], fb[set][m % NJ], acc[m / NJ][m % NJ]);
+        if (m < end - first) __builtin_amdgcn_sched_barrier(0);
+      }
+    };
     read(0, 0, 0);
     for (int s = 0; s < S; ++s) {
 #pragma unroll
@@ -325,7 +335,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
         } else if constexpr (kW4) {
           if (kk == 2) store_w4(s + 1, 0);
         }
-        multiply(kk & 1);
+        if (kk == 0) multiply_loading(0, s + 1, kFirst, kLoads);
+        else multiply(kk & 1);
         if constexpr (kW4) {
           if (kk > 0) {
 #pragma unroll
@@ -341,22 +352,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
       read(0, s + 1, 0);   // past the last step: what the buffer holds, not used
       if constexpr (kW4) load_w4(s + 2);
       __builtin_amdgcn_sched_barrier(0);
-      // the step after the next one's loads (past the last step: zeros) between these MFMAs
-#pragma unroll
-      for (int m = 0; m < (NA * NJ > kLoads ? NA * NJ : kLoads); ++m) {
-        if (m < LA) load_a(s + 2, m);
-        else if (m < kLoads) load_b(s + 2, m - LA);
-        if (m < NA * NJ) acc[m / NJ][m % NJ] = mfma<DT>(fa[1][m / NJ], fb[1][m % NJ], acc[m / NJ][m % NJ]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      multiply_loading(1, s + 2, 0, kFirst);   // past the last step: zeros
     }
     wait_all_barrier();   // the buffers are the outputs' staging areas next
   };
 
   // blocks of 32 rows of the wave that hold outputs at all (the last tile of a segment is often nearly empty)
-  const int live = n0 + wn * NJ * 32 < a.N ? min(max((m_end - m0 - wm * NI * 32 + 31) >> 5, 0), NI) : 0;
+  const int live = n0 + cb0 * 32 < a.N ? min(max((m_end - m0 - rb0 * 32 + 31) >> 5, 0), rows_of) : 0;
   if (S > 0) {
-    load(0);
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) load_one(0, l);
     if constexpr (kW4) {
       load_w4(0);
 #pragma unroll
@@ -364,7 +369,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
       if (S > 1) load_w4(1);
     }
     wait_all_barrier();
-    if (S > 1) load(1);
+#pragma unroll
+    for (int l = 0; l < kFirst; ++l) load_one(1, l);
     if (live == NI) walk(std::integral_constant<int, NI>{});
     else if (live == 0) walk(std::integral_constant<int, 0>{});
     else if (NI > 1 && live == 1) walk(std::integral_constant<int, 1>{});
@@ -388,7 +394,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
       for (int r = 0; r < 16; ++r) stage[((r & 3) + 8 * (r >> 2) + 4 * h) * kPitch + 32 * j + c] = acc[i][j][r];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
-    const int mb = m0 + (wm * NI + i) * 32, nb = n0 + wn * NJ * 32;
+    const int mb = m0 + (rb0 + i) * 32, nb = n0 + cb0 * 32;
     auto row_scale = [&](int m) __attribute__((always_inline)) {
       return SUM == kSumFixed && a.scales ? a.scales[2 * (int64_t)(lo + m) + 1] : 1.f;
     };
