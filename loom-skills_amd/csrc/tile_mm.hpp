@@ -457,5 +457,37 @@ int launch(const Args &in, hipStream_t s) {
   return launch_status();
 }
 
+// The tile of a product whose segments cut A's rows, by an estimate of its time: rounds of workgroups over the chip's places
+// times (steps times a step's time + a workgroup's start and end). Measured on full rounds, us a step: 256 x 256 1.65 (one a CU),
+// 256 x 128 1.04 (one), 128 x 128 1.04 (two), 64 x 128 0.95 (three); 6 us a workgroup. It has the measured order of the four at
+// 16384 rows of 32 experts 2880 x 2880 (estimated 321, 422, 370, 441 us; measured 320, 414, 363, 447), 8000 rows of 128 experts
+// 1536 x 2048 (S), 2048 x 4096 x 12288 (256 x 128) and 333 x 12288 x 4096 (256 x 128).
+enum Tile { kT256x256 = 0, kT256x128 = 1, kT128x128 = 2, kT64x128 = 3 };
+inline Tile choose_tile(const Args &a) {
+  static const struct { int bm, bn, slots; float step; } shapes[] = {{256, 256, 256, 1.65f}, {256, 128, 256, 1.04f},
+                                                                     {128, 128, 512, 1.04f}, {64, 128, 768, 0.95f}};
+  const int64_t hit = a.offsets ? std::min(a.E, a.rows) : 1, steps = (a.K + 63) / 64;
+  int best = 0;
+  float least = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const auto &t = shapes[i];
+    // ragged: a segment's last tile is half empty on average, and hardly an expert is without rows
+    const int64_t m = a.offsets ? std::max<int64_t>(a.rows / t.bm + hit / 2, hit - hit / 10) : (a.rows + t.bm - 1) / t.bm;
+    const int64_t tiles = m * ((a.N + t.bn - 1) / t.bn);
+    const float us = (float)((tiles + t.slots - 1) / t.slots) * ((float)steps * t.step + 6.f);
+    if (i == 0 || us < least) best = i, least = us;
+  }
+  return (Tile)best;
+}
+template <int DT, int SA, int SB, int GS>
+int launch_chosen(const Args &a, hipStream_t s) {
+  switch (choose_tile(a)) {
+    case kT256x256: return launch<DT, SA, SB, kSumFixed, 256, 256, 2, 4, GS>(a, s);
+    case kT256x128: return launch<DT, SA, SB, kSumFixed, 256, 128, 4, 2, GS>(a, s);
+    case kT128x128: return launch<DT, SA, SB, kSumFixed, 128, 128, 2, 2, GS>(a, s);
+    default: return launch<DT, SA, SB, kSumFixed, 64, 128, 1, 4, GS>(a, s);
+  }
+}
+
 }  // namespace tmm
 }  // namespace qmm

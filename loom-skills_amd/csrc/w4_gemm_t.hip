@@ -4,16 +4,6 @@
 namespace qmm {
 using namespace tmm;
 
-namespace {
-template <int GS>
-int pick(const Args &a, hipStream_t s) {
-  const int avg = a.offsets ? (a.rows + a.E - 1) / a.E : a.rows;
-  if (avg >= 192) return launch<QMM_F16, kRow, kW4Col, kSumFixed, 256, 256, 2, 4, GS>(a, s);
-  if (avg > 64) return launch<QMM_F16, kRow, kW4Col, kSumFixed, 128, 128, 2, 2, GS>(a, s);
-  return launch<QMM_F16, kRow, kW4Col, kSumFixed, 64, 128, 1, 4, GS>(a, s);
-}
-}  // namespace
-
-int w4_gemm_t(const Args &a, int gs, hipStream_t s) { return gs == 1 ? pick<1>(a, s) : gs == 2 ? pick<2>(a, s) : pick<4>(a, s); }
+int w4_gemm_t(const Args &a, int gs, hipStream_t s) { return gs == 1 ? launch_chosen<QMM_F16, kRow, kW4Col, 1>(a, s) : gs == 2 ? launch_chosen<QMM_F16, kRow, kW4Col, 2>(a, s) : launch_chosen<QMM_F16, kRow, kW4Col, 4>(a, s); }
 
 }  // namespace qmm
