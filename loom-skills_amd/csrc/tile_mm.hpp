@@ -31,7 +31,7 @@ typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(2))) _Float16 h2;
 
-enum Src { kRow = 0, kCol = 1, kW4Row = 2, kW4Col = 3 };
+enum Src { kRow = 0, kCol = 1, kW4Col = 2 };
 enum Sum { kSumFixed = 0, kSumRagged = 1 };   // what the segments cut: A's rows (kSumFixed) or the sum (the weight gradient)
 constexpr u32 kPast = 0x80000000u;            // an offset past every resource: the load gives zeros
 constexpr int kGroupM = 8;
@@ -95,10 +95,93 @@ __device__ __forceinline__ u32x4 dequant(u32 q, u32 sc) {
   return o;
 }
 
+// 32 output rows mb .. of a wave (those below m_end), columns nb .. nb + 32 NJ - 1 (those below N), through its own LDS: the sums
+// of a lane are one column of 16 rows, a store covers neighbouring columns. scales: of the segment's rows, or NULL.
+template <int NJ>
+constexpr int stage_pitch() { return NJ * 32 + 8; }   // floats; 4 rows apart is 32 banks apart
+template <int NJ>
+__device__ __forceinline__ void store_rows(const Args &a, float *stage, const f32x16 (&acc)[NJ], int64_t out0, int mb, int m_end, int nb,
+                                           const float *scales, int lane) {
+  constexpr int kPitch = stage_pitch<NJ>();
+  const int c = lane & 31, h = lane >> 5;
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) stage[((r & 3) + 8 * (r >> 2) + 4 * h) * kPitch + 32 * j + c] = acc[j][r];
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+  auto row_scale = [&](int m) __attribute__((always_inline)) { return scales ? scales[2 * (int64_t)m + 1] : 1.f; };
+  if (a.wide) {
+    constexpr int LR = NJ * 4, RP = 64 / LR;   // lanes a row (8 values each), rows a pass
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += RP) {
+      const int r = r0 + lane / LR, col = (lane % LR) * 8;
+      const int m = mb + r, n = nb + col;
+      if (m < m_end && n < a.N) {
+        const f32x4 v0 = *reinterpret_cast<const f32x4 *>(stage + r * kPitch + col);
+        const f32x4 v1 = *reinterpret_cast<const f32x4 *>(stage + r * kPitch + col + 4);
+        const float sc = row_scale(m);
+        const int64_t at = out0 + (int64_t)m * a.N + n;
+        if (a.y_type == QMM_F32) {
+          f32x4 *o = reinterpret_cast<f32x4 *>(static_cast<float *>(a.y) + at);
+          o[0] = v0 * sc;
+          o[1] = v1 * sc;
+        } else if (a.y_type == QMM_BF16) {
+          bf16x8 b;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) b[x] = (__bf16)((x < 4 ? v0[x] : v1[x - 4]) * sc);
+          *reinterpret_cast<bf16x8 *>(static_cast<__bf16 *>(a.y) + at) = b;
+        } else {
+          f16x8 b;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) b[x] = (_Float16)((x < 4 ? v0[x] : v1[x - 4]) * sc);
+          *reinterpret_cast<f16x8 *>(static_cast<_Float16 *>(a.y) + at) = b;
+        }
+      }
+    }
+  } else {
+    for (int v = lane; v < 32 * 32 * NJ; v += 64) {
+      const int r = v / (32 * NJ), m = mb + r, n = nb + v % (32 * NJ);
+      if (m < m_end && n < a.N) {
+        const float o = stage[r * kPitch + v % (32 * NJ)] * row_scale(m);
+        const int64_t at = out0 + (int64_t)m * a.N + n;
+        if (a.y_type == QMM_F32) static_cast<float *>(a.y)[at] = o;
+        else if (a.y_type == QMM_BF16) static_cast<__bf16 *>(a.y)[at] = (__bf16)o;
+        else static_cast<_Float16 *>(a.y)[at] = (_Float16)o;
+      }
+    }
+  }
+}
+
 template <int SRC>
 __device__ __forceinline__ int chunk_swizzle(int row) {
-  if constexpr (SRC == kRow || SRC == kW4Row) return (row >> 1) & 7;
+  if constexpr (SRC == kRow) return (row >> 1) & 7;
   else return ((row & 3) << 2) ^ ((row >> 2) & 3);
+}
+
+// The workgroup's output tile where the segments cut A's rows: expert, segment, first row in it, column tile; false for a workgroup
+// too many. Workgroup i runs on XCD i % 8, which takes a contiguous range of tiles: an expert's in groups of kGroupM row tiles,
+// rows fastest, so that the tiles that an XCD works on at a time share operands in its L2.
+template <int BM>
+__device__ __forceinline__ bool row_tile(const Args &a, int &e, int &lo, int &hi, int &m0, int &nt) {
+  TileScan sc{(a.rows + BM - 1) / BM, 0, 1};
+  if (a.offsets) sc = scan_tiles<BM>(a.offsets, a.E, a.rows);
+  const int total = sc.total * a.tiles_n, per = (total + 7) >> 3;
+  const int i = (int)(blockIdx.x >> 3);
+  int t = (int)(blockIdx.x & 7) * per + i, first = 0;
+  if (i >= per || t >= total) return false;
+  if (a.offsets) find_tile<BM>(a.offsets, a.E, a.rows, sc, t / a.tiles_n, e, lo, hi, first);
+  t -= first * a.tiles_n;
+  const int own = a.offsets ? (max(hi - lo, 1) + BM - 1) / BM : sc.total;   // the expert's row tiles
+  const int g = t / (kGroupM * a.tiles_n), gm = max(1, min(kGroupM, own - g * kGroupM)), gt = t - g * kGroupM * a.tiles_n;
+  m0 = (g * kGroupM + gt % gm) * BM;
+  nt = gt / gm;
+  return true;
+}
+// row tiles that offsets may give at most
+inline int64_t most_row_tiles(const Args &a, int bm) {
+  return a.offsets ? std::min<int64_t>((int64_t)a.rows / bm + a.E, a.rows) : (a.rows + bm - 1) / bm;
 }
 
 // DT: QMM_BF16 or QMM_F16; SA, SB: the operands' sources; GS: 32-value steps a w4 scale covers (1, 2; 4: more)
@@ -107,28 +190,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   constexpr int NW = WM * WN, NT = 64 * NW, NI = BM / WM / 32, NJ = BN / WN / 32;
   constexpr int kA = BM * 128, kB = BN * 128;             // LDS bytes of a step's operands
   constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;       // 1 KB loads a wave and step
-  constexpr bool kW4 = SB == kW4Row || SB == kW4Col;
+  constexpr bool kW4 = SB == kW4Col;
   static_assert(SA == kRow || BM >= 128, "a transposed operand is at least 128 wide");
-  static_assert((SB == kRow || SB == kW4Row) || BN >= 128, "a transposed operand is at least 128 wide");
+  static_assert(SB == kRow || BN >= 128, "a transposed operand is at least 128 wide");
   extern __shared__ __align__(1024) u8 smem[];            // A [2], B [2]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  // ---- the workgroup's tile. Workgroup i runs on XCD i % 8, which takes a contiguous range of tiles: an expert's in
-  // groups of kGroupM row tiles, rows fastest, so that the tiles that an XCD works on at a time share operands in its L2.
   int e = 0, lo = 0, hi = a.rows, m0, nt;
   if constexpr (SUM == kSumFixed) {
-    TileScan sc{(a.rows + BM - 1) / BM, 0, 1};
-    if (a.offsets) sc = scan_tiles<BM>(a.offsets, a.E, a.rows);
-    const int total = sc.total * a.tiles_n, per = (total + 7) >> 3;
-    const int i = (int)(blockIdx.x >> 3);
-    int t = (int)(blockIdx.x & 7) * per + i, first = 0;
-    if (i >= per || t >= total) return;
-    if (a.offsets) find_tile<BM>(a.offsets, a.E, a.rows, sc, t / a.tiles_n, e, lo, hi, first);
-    t -= first * a.tiles_n;
-    const int own = a.offsets ? (max(hi - lo, 1) + BM - 1) / BM : sc.total;   // the expert's row tiles
-    const int g = t / (kGroupM * a.tiles_n), gm = max(1, min(kGroupM, own - g * kGroupM)), gt = t - g * kGroupM * a.tiles_n;
-    m0 = (g * kGroupM + gt % gm) * BM;
-    nt = gt / gm;
+    if (!row_tile<BM>(a, e, lo, hi, m0, nt)) return;
   } else {
     // every XCD takes an eighth of every expert's tiles, one expert after the other: experts differ in their rows
     const int tiles_m = (a.M + BM - 1) / BM, per_e = tiles_m * a.tiles_n, per = (per_e + 7) >> 3;
@@ -203,33 +273,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
       lds_load16(resource(bp + (int64_t)s * 64 * b_row, min(64, K - 64 * s) * b_row - n0 * 2), boff[i], dst);
   };
 
-  // ---- w4: unit u of a step is a lane's 16 bytes of a 16-row x 128-value tile (kW4Row: the half that the step covers). Rows and
-  // tiles past the end read the last ones: their outputs are not stored, and in the sum A is zero there.
-  constexpr int kAll = SB == kW4Row ? BN * 4 : BN * 2;    // units of a step
-  constexpr int kUnits = (kAll + NT - 1) / NT;
-  constexpr int kWords = SB == kW4Row ? 2 : 4;            // code words of a unit
-  constexpr int kScales = GS >= kWords ? 1 : kWords / GS;
-  u32 cw[kUnits][kWords], cs[kUnits][kScales];
+  // ---- w4: unit u of a step is a lane's 16 bytes of a 16-row x 128-value tile. Rows and tiles past the end read the last ones:
+  // their outputs are not stored, and in the sum A is zero there.
+  constexpr int kAll = BN * 2, kUnits = (kAll + NT - 1) / NT;   // units of a step, of a thread
+  constexpr int kScales = 4 / GS;
+  u32 cw[kUnits][4], cs[kUnits][kScales];
   auto load_w4 = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
       const int u = i * NT + tid, l = u & 63, b = u >> 6;
-      const int rb = min(SB == kW4Row ? (n0 >> 4) + b : 4 * s + (b & 3), a.w_blocks - 1);
-      const int t = min(SB == kW4Row ? s >> 1 : (n0 >> 7) + (b >> 2), a.w_tiles - 1);
-      const u8 *p = bp + ((int64_t)rb * a.w_tiles + t) * 1024 + 16 * l;
-      if constexpr (SB == kW4Row) {
-        const u32x2 v = *reinterpret_cast<const u32x2 *>(p + 8 * (s & 1));
-        cw[i][0] = v.x;
-        cw[i][1] = v.y;
-      } else {
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
+      const int rb = min(4 * s + (b & 3), a.w_blocks - 1), t = min((n0 >> 7) + (b >> 2), a.w_tiles - 1);
+      const u32x4 v = *reinterpret_cast<const u32x4 *>(bp + ((int64_t)rb * a.w_tiles + t) * 1024 + 16 * l);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) cw[i][j] = v[j];
-      }
+      for (int j = 0; j < 4; ++j) cw[i][j] = v[j];
       const u32 *sp = a.ws + ((int64_t)e * a.w_blocks + rb) * a.groups * 16 + (l & 15);
-      const int step = SB == kW4Row ? 2 * s : 4 * t;      // the unit's first 32-value step along W's rows
 #pragma unroll
-      for (int g = 0; g < kScales; ++g) cs[i][g] = sp[min((step + GS * g) >> a.gshift, a.groups - 1) * 16];
+      for (int g = 0; g < kScales; ++g) cs[i][g] = sp[min((4 * t + GS * g) >> a.gshift, a.groups - 1) * 16];
     }
   };
   auto store_w4 = [&](int s, int i) __attribute__((always_inline)) {
@@ -237,15 +296,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
     if (kAll % NT && u >= kAll) return;
     u8 *out = smem + 2 * kA + (s & 1) * kB;
 #pragma unroll
-    for (int j = 0; j < kWords; ++j) {
-      const u32x4 v = dequant(cw[i][j], cs[i][kScales == 1 ? 0 : j / GS]);
-      if constexpr (SB == kW4Row) {
-        const int row = 16 * b + (l & 15), ch = 4 * j + (l >> 4);
-        *reinterpret_cast<u32x4 *>(out + row * 128 + ((ch ^ chunk_swizzle<SB>(row)) * 16)) = v;
-      } else {
-        const int row = 16 * (b & 3) + (l & 15), ch = 16 * (b >> 2) + 4 * j + (l >> 4);
-        *reinterpret_cast<u32x4 *>(out + row * (BN * 2) + ((ch ^ chunk_swizzle<SB>(row)) * 16)) = v;
-      }
+    for (int j = 0; j < 4; ++j) {
+      const int row = 16 * (b & 3) + (l & 15), ch = 16 * (b >> 2) + 4 * j + (l >> 4);
+      *reinterpret_cast<u32x4 *>(out + row * (BN * 2) + ((ch ^ chunk_swizzle<SB>(row)) * 16)) = dequant(cw[i][j], cs[i][j / GS]);
     }
   };
 
@@ -276,7 +329,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   };
   auto read_b = [&](int s, int j, int kk) __attribute__((always_inline)) {
     const u32 at = (u32)(2 * kA + (s & 1) * kB);
-    if constexpr (SB == kRow || SB == kW4Row) return read_row(at, cb0 + j, kk);
+    if constexpr (SB == kRow) return read_row(at, cb0 + j, kk);
     else return read_col(at, BN * 2, cb0 + j, kk);
   };
 
@@ -288,7 +341,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  constexpr int kGap = 32 * kWords * ((kUnits + 1) / 2) / (NI * NJ) + 1;   // vector instructions between two MFMAs
+  constexpr int kGap = 128 * ((kUnits + 1) / 2) / (NI * NJ) + 1;   // vector instructions between two MFMAs
   static_assert(!kW4 || kUnits <= 2, "a unit a phase");
   constexpr int kLoads = LA + (kW4 ? 0 : LB);
   // of a step's loads, those that go out past the barrier; the rest follow a phase later (w4: none, that phase has the weights)
@@ -378,66 +431,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
     else if (NI > 3) walk(std::integral_constant<int, NI < 3 ? NI : 3>{});
   }
 
-  // ---- outputs, 32 rows of a wave at a time through its own LDS (every wave is past its last read of the operands): the sums
-  // of a lane are one column of 16 rows, a store covers neighbouring columns
-  constexpr int kPitch = NJ * 32 + 8;   // floats; 4 rows apart is 32 banks apart
-  static_assert(32 * kPitch * 4 * NW <= 2 * (kA + kB), "the staging areas fit the operands' buffers");
-  float *stage = reinterpret_cast<float *>(smem) + wave * 32 * kPitch;
+  // ---- outputs (every wave is past its last read of the operands)
+  constexpr int kStage = 32 * stage_pitch<NJ>();
+  static_assert(kStage * 4 * NW <= 2 * (kA + kB), "the staging areas fit the operands' buffers");
   const int64_t out0 = SUM == kSumFixed ? (int64_t)lo * a.N : (int64_t)e * a.M * a.N;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     if (i >= live) break;
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) stage[((r & 3) + 8 * (r >> 2) + 4 * h) * kPitch + 32 * j + c] = acc[i][j][r];
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
-    const int mb = m0 + (rb0 + i) * 32, nb = n0 + cb0 * 32;
-    auto row_scale = [&](int m) __attribute__((always_inline)) {
-      return SUM == kSumFixed && a.scales ? a.scales[2 * (int64_t)(lo + m) + 1] : 1.f;
-    };
-    if (a.wide) {
-      constexpr int LR = NJ * 4, RP = 64 / LR;   // lanes a row (8 values each), rows a pass
-#pragma unroll
-      for (int r0 = 0; r0 < 32; r0 += RP) {
-        const int r = r0 + lane / LR, col = (lane % LR) * 8;
-        const int m = mb + r, n = nb + col;
-        if (m < m_end && n < a.N) {
-          const f32x4 v0 = *reinterpret_cast<const f32x4 *>(stage + r * kPitch + col);
-          const f32x4 v1 = *reinterpret_cast<const f32x4 *>(stage + r * kPitch + col + 4);
-          const float sc = row_scale(m);
-          const int64_t at = out0 + (int64_t)m * a.N + n;
-          if (a.y_type == QMM_F32) {
-            f32x4 *o = reinterpret_cast<f32x4 *>(static_cast<float *>(a.y) + at);
-            o[0] = v0 * sc;
-            o[1] = v1 * sc;
-          } else if (a.y_type == QMM_BF16) {
-            bf16x8 b;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) b[x] = (__bf16)((x < 4 ? v0[x] : v1[x - 4]) * sc);
-            *reinterpret_cast<bf16x8 *>(static_cast<__bf16 *>(a.y) + at) = b;
-          } else {
-            f16x8 b;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) b[x] = (_Float16)((x < 4 ? v0[x] : v1[x - 4]) * sc);
-            *reinterpret_cast<f16x8 *>(static_cast<_Float16 *>(a.y) + at) = b;
-          }
-        }
-      }
-    } else {
-      for (int v = lane; v < 32 * 32 * NJ; v += 64) {
-        const int r = v / (32 * NJ), m = mb + r, n = nb + v % (32 * NJ);
-        if (m < m_end && n < a.N) {
-          const float o = stage[r * kPitch + v % (32 * NJ)] * row_scale(m);
-          const int64_t at = out0 + (int64_t)m * a.N + n;
-          if (a.y_type == QMM_F32) static_cast<float *>(a.y)[at] = o;
-          else if (a.y_type == QMM_BF16) static_cast<__bf16 *>(a.y)[at] = (__bf16)o;
-          else static_cast<_Float16 *>(a.y)[at] = (_Float16)o;
-        }
-      }
-    }
+    store_rows<NJ>(a, reinterpret_cast<float *>(smem) + wave * kStage, acc[i], out0, m0 + (rb0 + i) * 32, m_end, n0 + cb0 * 32,
+                   SUM == kSumFixed && a.scales ? a.scales + 2 * (int64_t)lo : nullptr, lane);
   }
 }
 
@@ -445,9 +447,7 @@ template <int DT, int SA, int SB, int SUM, int BM, int BN, int WM, int WN, int G
 int launch(const Args &in, hipStream_t s) {
   Args a = in;
   a.tiles_n = (a.N + BN - 1) / BN;
-  // row tiles: at most one ragged tile an expert beside the whole ones
-  const int64_t tiles_m = a.offsets ? std::min<int64_t>((int64_t)a.rows / BM + a.E, a.rows) : (a.rows + BM - 1) / BM;
-  const int64_t tiles = SUM == kSumRagged ? ((int64_t)((a.M + BM - 1) / BM) * a.tiles_n + 7) / 8 * 8 * a.E : tiles_m * a.tiles_n;
+  const int64_t tiles = SUM == kSumRagged ? ((int64_t)((a.M + BM - 1) / BM) * a.tiles_n + 7) / 8 * 8 * a.E : most_row_tiles(a, BM) * a.tiles_n;
   if (tiles > (1 << 22)) return QMM_ERR_SHAPE;   // HIP refuses 2^32 threads along a grid's dimension
   constexpr int lds = 2 * (BM + BN) * 128;
   auto *fn = tile_mm_kernel<DT, SA, SB, SUM, BM, BN, WM, WN, GS>;
@@ -457,34 +457,37 @@ int launch(const Args &in, hipStream_t s) {
   return launch_status();
 }
 
-// The tile of a product whose segments cut A's rows, by an estimate of its time: rounds of workgroups over the chip's places
-// times (steps times a step's time + a workgroup's start and end). Measured on full rounds, us a step: 256 x 256 1.65 (one a CU),
-// 256 x 128 1.04 (one), 128 x 128 1.04 (two), 64 x 128 0.95 (three); 6 us a workgroup. It has the measured order of the four at
-// 16384 rows of 32 experts 2880 x 2880 (estimated 321, 422, 370, 441 us; measured 320, 414, 363, 447), 8000 rows of 128 experts
-// 1536 x 2048 (S), 2048 x 4096 x 12288 (256 x 128) and 333 x 12288 x 4096 (256 x 128).
-enum Tile { kT256x256 = 0, kT256x128 = 1, kT128x128 = 2, kT64x128 = 3 };
-inline Tile choose_tile(const Args &a) {
-  static const struct { int bm, bn, slots; float step; } shapes[] = {{256, 256, 256, 1.65f}, {256, 128, 256, 1.04f},
-                                                                     {128, 128, 512, 1.04f}, {64, 128, 768, 0.95f}};
-  const int64_t hit = a.offsets ? std::min(a.E, a.rows) : 1, steps = (a.K + 63) / 64;
+// Of several tile shapes the one with the least estimated time: the workgroups that a CU gets times (turns along the sum times a
+// turn's time + a start and end). A shape's figures are measured on launches that fill the chip: us a turn over the workgroups that
+// share a CU.
+struct Shape {
+  int bm, bn;
+  float turn, ends;
+};
+template <int COUNT>
+int least_time(const Args &a, const Shape (&shapes)[COUNT], int64_t turns) {
+  const int64_t hit = a.offsets ? std::min(a.E, a.rows) : 1;
   int best = 0;
   float least = 0.f;
-  for (int i = 0; i < 4; ++i) {
-    const auto &t = shapes[i];
+  for (int i = 0; i < COUNT; ++i) {
+    const Shape &t = shapes[i];
     // ragged: a segment's last tile is half empty on average, and hardly an expert is without rows
     const int64_t m = a.offsets ? std::max<int64_t>(a.rows / t.bm + hit / 2, hit - hit / 10) : (a.rows + t.bm - 1) / t.bm;
     const int64_t tiles = m * ((a.N + t.bn - 1) / t.bn);
-    const float us = (float)((tiles + t.slots - 1) / t.slots) * ((float)steps * t.step + 6.f);
+    const float us = (float)((tiles + 255) / 256) * ((float)turns * t.turn + t.ends);
     if (i == 0 || us < least) best = i, least = us;
   }
-  return (Tile)best;
+  return best;
 }
+// Measured against estimated, us: 16384 rows of 32 experts 2880 x 2880 320, 414, 363, 447 (322, 414, 343, 411 estimated); gradients
+// of 2048 x 4096 x 12288 in 4 bits 318, 248, 269, 338 (323, 205, 206, 248).
 template <int DT, int SA, int SB, int GS>
 int launch_chosen(const Args &a, hipStream_t s) {
-  switch (choose_tile(a)) {
-    case kT256x256: return launch<DT, SA, SB, kSumFixed, 256, 256, 2, 4, GS>(a, s);
-    case kT256x128: return launch<DT, SA, SB, kSumFixed, 256, 128, 4, 2, GS>(a, s);
-    case kT128x128: return launch<DT, SA, SB, kSumFixed, 128, 128, 2, 2, GS>(a, s);
+  static const Shape shapes[] = {{256, 256, 1.65f, 6.f}, {256, 128, 1.04f, 5.f}, {128, 128, 0.52f, 3.f}, {64, 128, 0.32f, 2.f}};
+  switch (least_time(a, shapes, (a.K + 63) / 64)) {
+    case 0: return launch<DT, SA, SB, kSumFixed, 256, 256, 2, 4, GS>(a, s);
+    case 1: return launch<DT, SA, SB, kSumFixed, 256, 128, 4, 2, GS>(a, s);
+    case 2: return launch<DT, SA, SB, kSumFixed, 128, 128, 2, 2, GS>(a, s);
     default: return launch<DT, SA, SB, kSumFixed, 64, 128, 1, 4, GS>(a, s);
   }
 }
