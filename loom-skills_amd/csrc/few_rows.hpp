@@ -10,6 +10,8 @@
 // values (its leading 8 bits, the next 8, the rest: three MFMAs), so every product is exact and every sum f32; the groups' sums
 // of x come from an MFMA with ones.
 #pragma once
+#include <type_traits>
+
 #include "ragged.hpp"
 
 namespace qmm {
@@ -75,17 +77,27 @@ __device__ __forceinline__ Parts split(u32x4 a, u32x4 b) {
 }
 
 // W: the weights; F32: rows x are f32 (w4 only), else 16-bit; GS: 32-value steps a scale covers within a 128-value tile; TT:
-// tiles of 16 tokens at a time. Grid: (16-row blocks of W, experts with rows, token chunks of a dense call).
-template <int W, bool F32, int GS, int TT>
-__global__ __launch_bounds__(64 * kWaves) void few_rows_kernel(Args a) {
+// tiles of 16 tokens at a time; KS: waves that share a 16-row block of W, each with every KS-th 128-value tile (a workgroup has
+// 8 / KS blocks); TL: rows of x a wave keeps in LDS. Grid: (row blocks, experts with rows, token chunks of a dense call).
+//
+// x: up to TL rows are brought into the wave's own LDS, a batch of U tiles at a time and 8 values a lane (f32 rows split into
+// their parts there, once instead of once a lane), rows of U x 16 chunks, chunk i of row t at i ^ t; a fragment read past the last
+// row reads that one again, its outputs are not stored. With one row a load then brings 1 KB where the fragments' own loads would
+// use four lanes. More rows are read as fragments from memory.
+template <int W, bool F32, int GS, int TT, int KS, int TL>
+__global__ __launch_bounds__(64 * kWaves, TT > 1 ? 2 : F32 || TL > 2 || (TL > 1 && W == kW4) ? 4 : 6) void few_rows_kernel(Args a) {
   constexpr int kParts = F32 ? 3 : 1, kLoads = F32 ? 2 : 1, kES = F32 ? 4 : 2;
-  constexpr int U = W == kW4 ? 4 : 2;   // tiles of a wave whose weights are in flight
-  __shared__ __align__(16) float red[kWaves][TT][64][4];
+  constexpr int U = W == kW4 && !F32 ? 4 : 2;   // tiles of a wave whose weights are in flight
+  constexpr int kBlocks = kWaves / KS;
+  static_assert(TL == 0 || (TT == 1 && TL <= 16), "staged rows are one tile of tokens");
+  __shared__ __align__(16) float red[KS > 1 ? kWaves : 1][TT][64][4];
+  __shared__ __align__(16) u8 xs[TL > 0 ? kWaves : 1][TL > 0 ? kParts : 1][TL > 0 ? TL : 1][U * 256];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 15, h = lane >> 4, rb = blockIdx.x;
+  const int c = lane & 15, h = lane >> 4, part = wave % KS;
+  const int KT = (a.k + 127) >> 7, nb = (a.n + 15) >> 4;
+  const int rb0 = (int)blockIdx.x * kBlocks, rb = min(rb0 + wave / KS, nb - 1);
   int e = 0, lo = 0, hi = a.rows;
   if (a.offsets && !nth_segment(a.offsets, a.E, a.rows, blockIdx.y, e, lo, hi)) return;
-  const int KT = (a.k + 127) >> 7, nb = (a.n + 15) >> 4;
   const u8 *w = a.w + (int64_t)e * a.w_expert;
   const u32 *ws = nullptr;
   __amdgpu_buffer_rsrc_t wr;
@@ -98,111 +110,188 @@ __global__ __launch_bounds__(64 * kWaves) void few_rows_kernel(Args a) {
   const u32 one = W == kWF16 ? 0x3C003C00u : 0x3F803F80u;
   const u32x4 ones = {one, one, one, one};
 
-  for (int t0 = lo + (int)blockIdx.z * 16 * TT; t0 < hi; t0 += (int)gridDim.z * 16 * TT) {
-    const __amdgpu_buffer_rsrc_t xr = rsrc(a.x + (int64_t)t0 * a.k * kES, (u32)min(16 * TT, hi - t0) * (u32)a.k * kES);
+  struct Batch {
+    u32x4 q[U][W == kW4 ? 1 : 4];
+    u32 sc[U][4 / GS];
+    u32x4 x[TL > 0 ? TL * U / 4 + (TL * U % 4 != 0) : 1][kLoads];   // 8 values a lane
+  };
+  constexpr int kX = TL * U * 16;   // chunks of 8 values of a batch's staged rows
+
+  constexpr int kRows = TL > 0 ? TL : 16 * TT;   // at a time
+  for (int t0 = lo + (int)blockIdx.z * kRows; t0 < hi; t0 += (int)gridDim.z * kRows) {
+    const int rows = min(kRows, hi - t0);
+    const __amdgpu_buffer_rsrc_t xr = rsrc(a.x + (int64_t)t0 * a.k * kES, (u32)rows * (u32)a.k * kES);
     f32x4 acc[TT];
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) acc[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int tb = wave; tb < KT; tb += kWaves * U) {
-      u32x4 q[U][W == kW4 ? 1 : 4];
-      u32 sc[U][4 / GS];
+
+    constexpr bool kLds = TL > 0;
+    {
+      // batch at tb: tiles tb, tb + KS, ... (past the last: that one again, not used)
+      auto load = [&](int tb, Batch &b) __attribute__((always_inline)) {
+        if constexpr (kLds) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = min(tb + kWaves * u, KT - 1);
-        if constexpr (W == kW4) {
-          q[u][0] = *reinterpret_cast<const u32x4 *>(w + (int64_t)t * 1024 + 16 * lane);
+          for (int i = 0; 64 * i < kX; ++i) {
+            const int at = 64 * i + lane, t = at / (U * 16), u = at / 16 % U, k = 128 * (tb + KS * u) + 8 * (at & 15);
+            const u32 off = k < a.k && t < TL ? ((u32)t * (u32)a.k + (u32)k) * kES : kPast;
 #pragma unroll
-          for (int g = 0; g < 4 / GS; ++g) sc[u][g] = ws[min((4 * t + GS * g) >> a.gshift, a.groups - 1) * 16];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int kk = 128 * t + 32 * j + 8 * h;
-            q[u][j] = ld(wr, kk < a.k ? (u32)(c * a.k + kk) * 2u : kPast);
+            for (int p = 0; p < kLoads; ++p) b.x[i][p] = ld(xr, off + 16 * p);
           }
         }
-      }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = tb + kWaves * u;
-        if (t >= KT) break;
-        u32x4 xv[TT][4][kLoads];
+        for (int u = 0; u < U; ++u) {
+          const int t = min(tb + KS * u, KT - 1);
+          if constexpr (W == kW4) {
+            b.q[u][0] = *reinterpret_cast<const u32x4 *>(w + (int64_t)t * 1024 + 16 * lane);
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
+            for (int g = 0; g < 4 / GS; ++g) b.sc[u][g] = ws[min((4 * t + GS * g) >> a.gshift, a.groups - 1) * 16];
+          } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int p = 0; p < kLoads; ++p) {
+            for (int j = 0; j < 4; ++j) {
               const int kk = 128 * t + 32 * j + 8 * h;
-              xv[tt][j][p] = ld(xr, kk < a.k ? ((u32)(16 * tt + c) * (u32)a.k + (u32)kk) * kES + 16 * p : kPast);
+              b.q[u][j] = ld(wr, kk < a.k ? (u32)(c * a.k + kk) * 2u : kPast);
             }
+          }
+        }
+      };
+      auto use = [&](int tb, const Batch &b) __attribute__((always_inline)) {
+        if constexpr (kLds) {
+          __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int g = 0; g < 4 / GS; ++g) {
-          f32x4 dot[TT], sum[TT];
+          for (int i = 0; 64 * i < kX; ++i) {
+            const int at = 64 * i + lane, t = at / (U * 16), ch = (at % (U * 16)) ^ t;
+            if (kX % 64 == 0 || t < TL) {
+              if constexpr (F32) {
+                const Parts v = split(b.x[i][0], b.x[i][kLoads - 1]);
 #pragma unroll
-          for (int tt = 0; tt < TT; ++tt) dot[tt] = sum[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int jj = 0; jj < GS; ++jj) {
-            const int j = GS * g + jj;
-            u32x4 wf;
-            if constexpr (W == kW4) wf = codes(q[u][0][j]);
-            else wf = q[u][j];
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt) {
-              Parts xp;
-              if constexpr (F32) xp = split(xv[tt][j][0], xv[tt][j][kLoads - 1]);
-              else xp.p[0] = xv[tt][j][0];
-#pragma unroll
-              for (int p = kParts - 1; p >= 0; --p) {
-                if constexpr (W == kW4) {
-                  dot[tt] = mfma<W>(xp.p[p], wf, dot[tt]);
-                  sum[tt] = mfma<W>(xp.p[p], ones, sum[tt]);
-                } else {
-                  acc[tt] = mfma<W>(xp.p[p], wf, acc[tt]);
-                }
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(&xs[wave][p][t][16 * ch]) = v.p[p];
+              } else {
+                *reinterpret_cast<u32x4 *>(&xs[wave][0][t][16 * ch]) = b.x[i][0];
               }
             }
           }
-          if constexpr (W == kW4) {
-            const float s = f16_to_f32(sc[u][g]), z = (float)(sc[u][g] >> 16 & 15u);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_wave_barrier();
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int t = tb + KS * u;
+          if (t >= KT) break;
+          u32x4 xv[TT][4][kLds ? 1 : kLoads];
+          if constexpr (!kLds) {
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) acc[tt][i] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[tt][i], dot[tt][i]), acc[tt][i]);
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int p = 0; p < kLoads; ++p) {
+                  const int kk = 128 * t + 32 * j + 8 * h;
+                  xv[tt][j][p] = ld(xr, kk < a.k ? ((u32)(16 * tt + c) * (u32)a.k + (u32)kk) * kES + 16 * p : kPast);
+                }
+          }
+#pragma unroll
+          for (int g = 0; g < 4 / GS; ++g) {
+            f32x4 dot[TT], sum[TT];
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) dot[tt] = sum[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int jj = 0; jj < GS; ++jj) {
+              const int j = GS * g + jj;
+              u32x4 wf;
+              if constexpr (W == kW4) wf = codes(b.q[u][0][j]);
+              else wf = b.q[u][j];
+#pragma unroll
+              for (int tt = 0; tt < TT; ++tt) {
+                Parts xp;
+                if constexpr (kLds) {
+                  const int row = min(c, rows - 1), ch = (16 * u + 4 * j + h) ^ row;
+#pragma unroll
+                  for (int p = 0; p < kParts; ++p) xp.p[p] = *reinterpret_cast<const u32x4 *>(&xs[wave][p][row][16 * ch]);
+                } else if constexpr (F32) {
+                  xp = split(xv[tt][j][0], xv[tt][j][kLds ? 0 : kLoads - 1]);
+                } else {
+                  xp.p[0] = xv[tt][j][0];
+                }
+#pragma unroll
+                for (int p = kParts - 1; p >= 0; --p) {
+                  if constexpr (W == kW4) {
+                    dot[tt] = mfma<W>(xp.p[p], wf, dot[tt]);
+                    sum[tt] = mfma<W>(xp.p[p], ones, sum[tt]);
+                  } else {
+                    acc[tt] = mfma<W>(xp.p[p], wf, acc[tt]);
+                  }
+                }
+              }
+            }
+            if constexpr (W == kW4) {
+              const float s = f16_to_f32(b.sc[u][g]), z = (float)(b.sc[u][g] >> 16 & 15u);
+#pragma unroll
+              for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[tt][i] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[tt][i], dot[tt][i]), acc[tt][i]);
+            }
           }
         }
+      };
+      Batch b;
+      for (int tb = part; tb < KT; tb += KS * U) {
+        load(tb, b);
+        use(tb, b);
       }
     }
+
+    auto store = [&](int token, int row, float v) __attribute__((always_inline)) {   // token of the chunk
+      if (token < rows && row < a.n) {
+        const int64_t at = (int64_t)(t0 + token) * a.n + row;
+        if (a.y_bytes == 4) static_cast<float *>(a.y)[at] = v;
+        else if constexpr (W == kWF16) static_cast<_Float16 *>(a.y)[at] = (_Float16)v;
+        else static_cast<__bf16 *>(a.y)[at] = (__bf16)v;
+      }
+    };
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) *reinterpret_cast<f32x4 *>(red[wave][tt][lane]) = acc[tt];
     __syncthreads();
-    for (int v = tid; v < 256 * TT; v += 64 * kWaves) {   // output (token v / 16, row v % 16), the waves' sums in order
-      const int token = v >> 4, r = v & 15, l = ((token & 15) >> 2) * 16 + r;
+    // output (block v / (256 TT), token, row v % 16): the block's waves' sums in order
+    for (int v = tid; v < 256 * TT * kBlocks; v += 64 * kWaves) {
+      const int b = v / (256 * TT), token = (v >> 4) % (16 * TT), r = v & 15, l = ((token & 15) >> 2) * 16 + r;
+      if (token >= rows) continue;
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) s += red[i][token >> 4][l][token & 3];
-      if (t0 + token < hi && 16 * rb + r < a.n) {
-        const int64_t at = (int64_t)(t0 + token) * a.n + 16 * rb + r;
-        if (a.y_bytes == 4) static_cast<float *>(a.y)[at] = s;
-        else if constexpr (W == kWF16) static_cast<_Float16 *>(a.y)[at] = (_Float16)s;
-        else static_cast<__bf16 *>(a.y)[at] = (__bf16)s;
-      }
+      for (int i = 0; i < KS; ++i) s += red[b * KS + i][token >> 4][l][token & 3];
+      store(token, 16 * (rb0 + b) + r, s);
     }
     __syncthreads();
   }
 }
 
 // Rows behind the last segment are not written. All extents are checked by the callers.
+template <int W, bool F32, int GS, int TT, int KS, int TL>
+int launch(const Args &a, int slots, hipStream_t s) {
+  constexpr int kRows = TL > 0 ? TL : 16 * TT;
+  const unsigned chunks = a.offsets ? 1u : (unsigned)min((a.rows + kRows - 1) / kRows, 65535);
+  const int per = 16 * kWaves / KS;
+  few_rows_kernel<W, F32, GS, TT, KS, TL><<<dim3((unsigned)((a.n + per - 1) / per), slots, chunks), dim3(64 * kWaves), 0, s>>>(a);
+  return launch_status();
+}
+// us in a graph on inputs out of cache. x in LDS (TL) against fragments from memory: one dense row, w4 12288 x 4096 7.6 against 9.7,
+// 4096 x 12288 8.6 and 12.7, f32 4096 x 4096 6.0 and 8.2; two or four dense rows no difference. By expert with a row each:
+// 16-bit 8 rows 1536 x 2048 11.9 and 13.8; w4 the same 7.2 and 5.9 (two tiles a wave: nothing to save), 104 rows 28 and 30.
+// Two waves a row block instead of eight where the blocks fill the chip: 104 rows of 128 experts w4 1536 x 2048 28 against 47; with
+// more rows a segment (1500) 122 against 105.
 template <int W, bool F32, int GS>
 int launch_tt(const Args &a, hipStream_t s) {
   const int slots = a.offsets ? min(a.E, a.rows) : 1;
-  const int avg = a.offsets ? (a.rows + a.E - 1) / a.E : a.rows;   // tokens at a time: as many as a segment may hold
-  const dim3 blk(64 * kWaves);
-  const unsigned nb = (unsigned)((a.n + 15) / 16);
-  auto chunks = [&](int tt) { return a.offsets ? 1u : (unsigned)min((a.rows + 16 * tt - 1) / (16 * tt), 65535); };
-  if (avg <= 16) few_rows_kernel<W, F32, GS, 1><<<dim3(nb, slots, chunks(1)), blk, 0, s>>>(a);
-  else if (avg <= 32) few_rows_kernel<W, F32, GS, 2><<<dim3(nb, slots, chunks(2)), blk, 0, s>>>(a);
-  else few_rows_kernel<W, F32, GS, 4><<<dim3(nb, slots, chunks(4)), blk, 0, s>>>(a);
-  return launch_status();
+  const int avg = (a.rows + slots - 1) / slots;   // tokens at a time: as many as a segment may hold
+  if (a.rows == 1) return launch<W, F32, GS, 1, 8, 1>(a, slots, s);
+  if (avg == 1) {
+    if constexpr (W == kW4) {
+      if ((int64_t)((a.n + 15) / 16) * slots >= 2048) return launch<W, F32, GS, 1, 2, 4>(a, slots, s);
+    } else {
+      return launch<W, F32, GS, 1, 8, 2>(a, slots, s);
+    }
+  }
+  if (avg <= 16) return launch<W, F32, GS, 1, 8, 0>(a, slots, s);
+  return avg <= 32 ? launch<W, F32, GS, 2, 8, 0>(a, slots, s) : launch<W, F32, GS, 4, 8, 0>(a, slots, s);
 }
 
 }  // namespace few

@@ -1118,13 +1118,13 @@ def gemm_t(fmt, x, w, n, k, w2=None, out_dtype=torch.float32, y=None):
 
 # ------------------------------------------------------- 4-bit weights with group scales; rows sorted by expert
 def _w4_sizes(n, k, group):
-    """(bytes of a packed matrix, bytes of its scale words); the library refuses shapes it does not take."""
-    lib = _lib.load()
-    size, words = lib.qmm_w4_bytes(n, k), lib.qmm_w4_scale_bytes(n, k, group)
-    if size < 0 or words < 0:
+    """(bytes of a packed matrix, bytes of its scale words), as qmm_w4_bytes and qmm_w4_scale_bytes."""
+    blocks, groups = (n + 15) // 16, -(-k // group) if group > 0 else 0
+    if not (0 < n <= 1 << 20 and 0 < k <= 1 << 20 and k % 32 == 0 and groups
+            and (group >= k or (group >= 32 and group & (group - 1) == 0)) and blocks * groups < 1 << 25):
         raise ValueError(f"4-bit weights have K % 32 == 0 and groups of 32, 64, 128, ... values or whole rows, not [{n}, {k}] "
                          f"in groups of {group}")
-    return size, words
+    return blocks * ((k + 127) // 128) * 1024, blocks * groups * 64
 
 
 def w4_pack(codes, scales, zeros=None, group=128):
@@ -1162,16 +1162,20 @@ def _w4_weights(w, ws, n, k, group, E):
                          f"{w.nbytes} and {ws.nbytes}")
 
 
-def _w4_few(rows, E, offsets):
-    """Whether f32 / bf16 rows are multiplied as they are (weights streamed once for up to 64 rows) rather than as f16 tiles."""
-    return rows < GEMM_MIN_TOKENS if offsets is None else rows <= 16 * E
+def _w4_few(rows, n, k, E, f32):
+    """Whether f32 / bf16 rows are multiplied as they are, weights streamed for a few rows at a time, rather than as f16 tiles. bf16
+    rows into bf16: up to 2^30 products (us, few rows against row scale and GEMM: 12288 x 4096 16 rows 15 and 25, 32 rows 26 and 25;
+    4096 x 4096 64 rows 18 and 26; 8 experts 4096 x 4096 64 rows 23 and 27, 32 experts 2880 x 2880 128 rows 39 and 39, 128
+    experts 1536 x 2048 256 rows 47 and 39). Where x or y is f32 (its bits are kept) below 64 rows, or up to four an expert."""
+    return rows < GEMM_MIN_TOKENS or rows <= 4 * E if f32 else rows * n * k <= 1 << 30
 
 
 def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=None):
     """y = x W^T on weights of w4_pack (qmm_w4_mm): one matrix, or with offsets (i32 [E + 1] on the device) the matrix of
-    expert e for rows offsets[e] .. offsets[e + 1] - 1; rows of no expert are left as they were in y. x f32 / bf16 [rows, k]: few
-    rows (below 64, or 16 an expert) are multiplied exactly, more go through row_scale_f16 first; or the f16 operand
-    [rows, k] with its scales f32 [rows, 2] (or None). y [rows, n] f32 or bf16 (out_dtype)."""
+    expert e for rows offsets[e] .. offsets[e + 1] - 1; rows of no expert are left as they were in y. x f32 / bf16 [rows, k],
+    multiplied exactly where the rows are few (with an f32 x or y: below 64, or up to four an expert) and through row_scale_f16
+    and weights rounded to f16 where they are many; or the f16 operand [rows, k] with its scales f32 [rows, 2] (or None).
+    y [rows, n] f32 or bf16 (out_dtype)."""
     s = _here(x, w, ws, offsets, scales, y)
     E = _segments(offsets)
     _w4_weights(w, ws, n, k, group, E)
@@ -1185,7 +1189,7 @@ def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=No
         raise ValueError("scales come with an f16 operand")
     elif x.dtype not in _VALUE:
         raise ValueError(f"x is {x.dtype}")
-    elif not _w4_few(rows, E, offsets):
+    elif not _w4_few(rows, n, k, E, x.dtype == torch.float32 or y.dtype == torch.float32):
         x, scales = row_scale_f16(x)
     _lib.call("qmm_w4_mm", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), x.data_ptr(), _DT[x.dtype],
               None if scales is None else scales.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), _DT[y.dtype], s)

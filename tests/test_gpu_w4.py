@@ -43,13 +43,14 @@ def test_pack(dev, n, k, group, zeros):
     assert torch.equal(ws.cpu().long() & 0xFFFFFFFF, words)
 
 
-def few_case(dev, rows, n, k, group, zeros, x_type, out, offsets=None, E=None, seed=0):
+def few_case(dev, rows, n, k, group, zeros, x_type, out, offsets=None, E=None, seed=0, operand=False):
     g = gen(rows * 1000 + n + k + seed)
     raw = w4_raw(g, n, k, group, zeros, E)
     x = (torch.randn((rows, k), generator=g) * torch.exp2(torch.randint(-6, 7, (rows, 1), generator=g).float())).to(T[x_type])
     w, ws = packed(raw, group, dev)
     y = Guarded((rows, n), T[out], dev)
-    got = ops.w4_mm(x.to(dev), w, ws, n, k, group, offsets=None if offsets is None else offsets.to(dev), y=y.t)
+    xd, scales = ops.row_scale_f16(x.to(dev)) if operand and x_type != "f16" else (x.to(dev), None)   # the operand takes the GEMM
+    got = ops.w4_mm(xd, w, ws, n, k, group, offsets=None if offsets is None else offsets.to(dev), scales=scales, y=y.t)
     assert got.data_ptr() == y.t.data_ptr()
     return x, raw, y
 
@@ -89,12 +90,14 @@ def row_rounding(x, absw, terms):
 
 MANY = [(64, 8, 32, 32, True, "bf16", "bf16"), (65, 200, 96, 32, True, "bf16", "f32"), (100, 129, 288, 64, False, "f32", "f32"),
         (129, 256, 512, 128, True, "bf16", "bf16"), (200, 257, 160, ROW, True, "bf16", "f32"), (257, 520, 1024, 64, True, "bf16", "bf16"),
-        (300, 31, 4096, 128, True, "bf16", "f32"), (1, 40, 256, 128, True, "f16", "f32"), (70, 96, 2048, 256, True, "f16", "bf16")]
+        (300, 31, 4096, 128, True, "bf16", "f32"), (1, 40, 256, 128, True, "f16", "f32"), (70, 96, 2048, 256, True, "f16", "bf16"),
+        # every tile: 64 x 256, 128 x 128, 128 x 256
+        (640, 5000, 160, 32, True, "bf16", "bf16"), (8300, 300, 96, 32, True, "bf16", "f32"), (4090, 2000, 288, 64, True, "bf16", "bf16")]
 
 
 @pytest.mark.parametrize("rows,n,k,group,zeros,x_type,out", MANY)
 def test_many_rows(dev, rows, n, k, group, zeros, x_type, out):
-    x, raw, y = few_case(dev, rows, n, k, group, zeros, x_type, out, seed=1)
+    x, raw, y = few_case(dev, rows, n, k, group, zeros, x_type, out, seed=1, operand=True)
     y.check()
     xd, w = x.double(), raw[3]
     terms = xd.abs() @ w.abs().t()
@@ -114,14 +117,15 @@ def test_f16_operand_with_scales(dev):
 
 
 BY_EXPERT = [([70, 0, 130, 1], 0, 0, 136, 288, 32, "bf16"), ([0, 300, 5], 3, 9, 40, 512, 128, "f32"),
-             ([33] * 9 + [0, 0], 0, 1, 264, 160, 64, "bf16"), ([0, 0, 600, 280], 0, 0, 300, 256, ROW, "bf16")]
+             ([33] * 9 + [0, 0], 0, 1, 264, 160, 64, "bf16"), ([0, 0, 600, 280], 0, 0, 300, 256, ROW, "bf16"),
+             ([500, 0, 1, 1200, 129] * 2, 7, 3, 1000, 160, 32, "bf16")]
 
 
 @pytest.mark.parametrize("counts,first,tail,n,k,group,out", BY_EXPERT)
 def test_many_rows_by_expert(dev, counts, first, tail, n, k, group, out):
     rows, E = first + sum(counts) + tail, len(counts)
     offsets = offsets_of(counts, first)
-    x, raw, y = few_case(dev, rows, n, k, group, True, "bf16", out, offsets, E, seed=2)
+    x, raw, y = few_case(dev, rows, n, k, group, True, "bf16", out, offsets, E, seed=2, operand=True)
     y.check(kept=((0, first), (rows - tail, rows)))
     live = slice(first, rows - tail)
     terms = by_expert(x.double().abs(), raw[3].abs(), offsets)
@@ -131,7 +135,9 @@ def test_many_rows_by_expert(dev, counts, first, tail, n, k, group, out):
 
 
 GRADS = [(1, 8, 32, 32, True, "bf16", "f32"), (77, 100, 288, 32, True, "bf16", "bf16"), (64, 17, 160, 64, True, "f32", "f32"),
-         (129, 200, 512, 128, False, "bf16", "f32"), (200, 64, 1024, ROW, True, "bf16", "bf16"), (257, 320, 96, 64, True, "bf16", "f32")]
+         (129, 200, 512, 128, False, "bf16", "f32"), (200, 64, 1024, ROW, True, "bf16", "bf16"), (257, 320, 96, 64, True, "bf16", "f32"),
+         # every tile: 256 x 256, 256 x 128, 128 x 128
+         (16300, 72, 1024, 32, True, "bf16", "bf16"), (8100, 200, 992, 64, True, "bf16", "bf16"), (2000, 130, 1024, 128, True, "bf16", "f32")]
 
 
 @pytest.mark.parametrize("rows,n,k,group,zeros,dy_type,out", GRADS)
@@ -148,7 +154,7 @@ def test_input_gradient(dev, rows, n, k, group, zeros, dy_type, out):
 
 
 @pytest.mark.parametrize("counts,first,tail,n,k,group", [([70, 0, 130, 1], 0, 0, 136, 288, 32), ([0, 500, 2], 4, 3, 40, 512, 128),
-                                                         ([9] * 12, 0, 0, 72, 160, ROW)])
+                                                         ([9] * 12, 0, 0, 72, 160, ROW), ([900, 0, 2100, 1] * 4, 0, 0, 72, 1024, 32)])
 def test_input_gradient_by_expert(dev, counts, first, tail, n, k, group):
     rows, E = first + sum(counts) + tail, len(counts)
     g = gen(rows + n)
@@ -195,7 +201,7 @@ def test_a_row_does_not_see_its_neighbours(dev):
     raw = w4_raw(gen(2), 48, 256, 64)
     w, ws = packed(raw, 64, dev)
     for rows in (5, 40, 80):
-        x = torch.randn((rows, 256), generator=gen(rows)).bfloat16().to(dev)
+        x = torch.randn((rows, 256), generator=gen(rows)).to(dev)
         clean = ops.w4_mm(x, w, ws, 48, 256, 64)
         x[3, 7], x[4, 100] = float("nan"), float("inf")
         y = ops.w4_mm(x, w, ws, 48, 256, 64)
@@ -220,12 +226,12 @@ def test_offsets_out_of_range_are_clamped(dev):
 
 
 @pytest.mark.parametrize("rows", [3, 100])
-def test_stream_and_graph(dev, rows):
+def test_stream_and_graph(dev, rows):   # f32 rows: the few-row kernel, then row scale and GEMM
     n, k, E = 80, 256, 5
     raw = w4_raw(gen(rows), n, k, 64, True, E)
     w, ws = packed(raw, 64, dev)
     offsets = offsets_of([rows // 3, 0, rows - rows // 3, 0, 0]).to(dev)
-    x = torch.randn((rows, k), generator=gen(9)).bfloat16().to(dev)
+    x = torch.randn((rows, k), generator=gen(9)).to(dev)
     dy = torch.randn((rows, n), generator=gen(10)).bfloat16().to(dev)
     want, dwant = ops.w4_mm(x, w, ws, n, k, 64, offsets=offsets), ops.w4_mm_t(dy, w, ws, n, k, 64, offsets=offsets)
     side = torch.cuda.Stream()
