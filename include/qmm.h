@@ -295,15 +295,22 @@ int64_t qmm_w4_scale_bytes(int64_t n, int64_t k, int64_t group);
  *                               64 of them). A row that holds an infinity gives NaN or infinities. x_scales unused.
  *   x_dtype QMM_F16             the qmm_gemm operand: x16 [rows, k] with x_scales f32 [rows, 2] of qmm_row_scale_f16, or NULL;
  *                               weights enter as f16(s (q - z)) (one rounding; finite for |s| <= 4366), f32 sums.
- * y: [rows, n] of y_dtype, QMM_F32 or QMM_BF16 (rounded once). x, w, ws 16-byte aligned; rows <= 2^24. y overlaps nothing. */
+ * y: [rows, n] of y_dtype, QMM_F32 or QMM_BF16 (rounded once). x, w, ws 16-byte aligned; rows <= 2^24. y overlaps nothing.
+ * workspace: at least qmm_w4_mm_workspace_size bytes, 16-byte aligned (NULL where that is 0): f32 sums of parts of K, added in
+ * order by a second launch, where few outputs have a long sum; calls that overlap need one each. */
 int qmm_w4_mm(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_t *offsets, const void *x, int x_dtype,
-              const float *x_scales, const void *w, const void *ws, void *y, int y_dtype, qmm_stream_t stream);
+              const float *x_scales, const void *w, const void *ws, void *y, int y_dtype, void *workspace,
+              int64_t workspace_bytes, qmm_stream_t stream);
+/* Workspace bytes of qmm_w4_mm and qmm_w4_mm_t, or -1 for sizes that are not taken. */
+int64_t qmm_w4_mm_workspace_size(int64_t rows, int64_t k, int64_t n, int E, int x_dtype);
+int64_t qmm_w4_mm_t_workspace_size(int64_t rows, int64_t k, int64_t n, int E);
 
 /* The transposed product y[t, c] = sum_r x[t, r] W_e[r, c], c < k: the input gradient of qmm_w4_mm with frozen weights. x,
  * scales: the one-part operand of qmm_grad_operand (f16 [rows, n rounded up to 64], padded with zeros). Weights enter as
  * f16(s (q - z)). Other arguments as qmm_w4_mm. */
 int qmm_w4_mm_t(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_t *offsets, const void *x,
-                const float *scales, const void *w, const void *ws, void *y, int y_dtype, qmm_stream_t stream);
+                const float *scales, const void *w, const void *ws, void *y, int y_dtype, void *workspace,
+                int64_t workspace_bytes, qmm_stream_t stream);
 
 /* Products of rows sorted by expert with 16-bit expert weights W [E, n, k], without padding between the experts (the bucketed
  * GEMMs of qmm_moe_grouped pad each to 64 rows and take quantized weights), and their gradients:
@@ -313,13 +320,17 @@ int qmm_w4_mm_t(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const 
  * offsets: i32 [E + 1] on the device, as qmm_w4_mm. dtype QMM_BF16 or QMM_F16 for x, W and dy alike; outputs QMM_F32 or that
  * type (rounded once); f32 sums in an order that follows from the sizes. x [rows, k], dy [rows, n]; n % 8 == 0, k % 8 == 0,
  * both <= 2^20, rows <= 2^24, E <= 1024; tensors 16-byte aligned. Rows of no expert are neither written (y, dx) nor read into
- * a sum (dw). Outputs overlap nothing. */
+ * a sum (dw). Outputs overlap nothing. workspace: as qmm_w4_mm, of the call's own qmm_*_workspace_size (-1 for sizes that are not
+ * taken). */
 int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *x, const void *w, int dtype,
-                  void *y, int y_dtype, qmm_stream_t stream);
+                  void *y, int y_dtype, void *workspace, int64_t workspace_bytes, qmm_stream_t stream);
 int qmm_ragged_mm_t(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy, const void *w, int dtype,
-                    void *dx, int dx_dtype, qmm_stream_t stream);
+                    void *dx, int dx_dtype, void *workspace, int64_t workspace_bytes, qmm_stream_t stream);
 int qmm_ragged_mm_dw(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy, const void *x, int dtype,
-                     void *dw, int dw_dtype, qmm_stream_t stream);
+                     void *dw, int dw_dtype, void *workspace, int64_t workspace_bytes, qmm_stream_t stream);
+int64_t qmm_ragged_mm_workspace_size(int64_t rows, int64_t k, int64_t n, int E);
+int64_t qmm_ragged_mm_t_workspace_size(int64_t rows, int64_t k, int64_t n, int E);
+int64_t qmm_ragged_mm_dw_workspace_size(int64_t rows, int64_t k, int64_t n, int E);
 
 /* MoE router top-k from logits, g_moe_route / g_moe_route_tr after the router matvec
  * (S/gen_moe.py:116-252, :255-500; llama.cpp gating: 1 softmax, 2 sigmoid, 3 softmax over the picked logits):

@@ -29,24 +29,48 @@ int check(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, con
   return QMM_OK;
 }
 
-int tiles(int op, tmm::Args &a, int dtype, int out_dtype, void *out, qmm_stream_t stream) {
+bool takes_few_rows(int64_t rows, int64_t k, int64_t n, int E) {
+  // up to 2^30 products and 64 rows an expert: us, few rows against tiles, 8 experts 4096 x 4096 64 rows 60 and 74, 128 rows 101 and
+  // 75; 128 experts 768 x 2048 512 rows 70 and 86, 1024 rows 100 and 93; 32 experts 2880 x 2880 128 rows 89 and 85
+  return rows * n * k <= (int64_t)1 << 30 && rows <= 64 * (int64_t)E;
+}
+
+int tiles(int op, tmm::Args &a, const tmm::Plan &p, int64_t outputs, int dtype, int out_dtype, void *out, void *workspace,
+          int64_t workspace_bytes, qmm_stream_t stream) {
   a.y = out;
   a.y_type = out_dtype;
   a.wide = 1;
+  if (int st = tmm::in_parts(a, p, outputs, workspace, workspace_bytes)) return st;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  return dtype == QMM_F16 ? ragged_tiles_f16(op, a, s) : ragged_tiles_bf16(op, a, s);
+  return dtype == QMM_F16 ? ragged_tiles_f16(op, a, p.shape, s) : ragged_tiles_bf16(op, a, p.shape, s);
+}
+
+bool sizes_ok(int64_t rows, int64_t k, int64_t n, int E) {
+  return rows >= 0 && rows <= kMaxRows && k > 0 && k <= kMaxSide && k % 8 == 0 && n > 0 && n <= kMaxSide && n % 8 == 0 && E >= 1 &&
+         E <= kMaxRaggedE;
 }
 
 }  // namespace
 
+extern "C" int64_t qmm_ragged_mm_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
+  if (!sizes_ok(rows, k, n, E)) return -1;
+  return rows && !takes_few_rows(rows, k, n, E) ? tmm::part_bytes(tmm::plan_rows(rows, E, n, k), rows * n) : 0;
+}
+extern "C" int64_t qmm_ragged_mm_t_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
+  if (!sizes_ok(rows, k, n, E)) return -1;
+  return rows ? tmm::part_bytes(tmm::plan_rows(rows, E, k, n), rows * k) : 0;
+}
+extern "C" int64_t qmm_ragged_mm_dw_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
+  return sizes_ok(rows, k, n, E) ? tmm::part_bytes(tmm::plan_sum(rows, E, n, k), E * n * k) : -1;
+}
+
 extern "C" int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *x, const void *w,
-                             int dtype, void *y, int y_dtype, qmm_stream_t stream) {
+                             int dtype, void *y, int y_dtype, void *workspace, int64_t workspace_bytes,
+                             qmm_stream_t stream) {
 
   if (int st = check(rows, k, n, E, offsets, x, w, dtype, rows ? y : w, y_dtype)) return st;
   if (rows == 0) return QMM_OK;
-  // up to 2^30 products: us, few rows against tiles, 8 experts 4096 x 4096 64 rows 60 and 74, 128 rows 101 and 75; 128 experts
-  // 768 x 2048 512 rows 70 and 86, 1024 rows 100 and 93; 32 experts 2880 x 2880 128 rows 89 and 85
-  if (rows * n * k <= (int64_t)1 << 30) {
+  if (takes_few_rows(rows, k, n, E)) {
     const few::Args a{offsets, E, (int)rows, (int)n, (int)k, static_cast<const u8 *>(x), static_cast<const u8 *>(w),
                       2 * n * k, nullptr, 0, 0, y, y_dtype == QMM_F32 ? 4 : 2};
     return ragged_few(a, dtype == QMM_F16, reinterpret_cast<hipStream_t>(stream));
@@ -56,11 +80,12 @@ extern "C" int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const in
   a.N = (int)n, a.K = (int)k;
   a.a = static_cast<const u8 *>(x), a.a_row = 2 * k;
   a.b = static_cast<const u8 *>(w), a.b_row = 2 * k, a.b_expert = 2 * n * k;
-  return tiles(kRaggedY, a, dtype, y_dtype, y, stream);
+  return tiles(kRaggedY, a, tmm::plan_rows(rows, E, n, k), rows * n, dtype, y_dtype, y, workspace, workspace_bytes, stream);
 }
 
 extern "C" int qmm_ragged_mm_t(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy, const void *w,
-                               int dtype, void *dx, int dx_dtype, qmm_stream_t stream) {
+                               int dtype, void *dx, int dx_dtype, void *workspace, int64_t workspace_bytes,
+                               qmm_stream_t stream) {
   if (int st = check(rows, k, n, E, offsets, dy, w, dtype, rows ? dx : w, dx_dtype)) return st;
   if (rows == 0) return QMM_OK;
   tmm::Args a{};
@@ -68,16 +93,17 @@ extern "C" int qmm_ragged_mm_t(int64_t rows, int64_t k, int64_t n, int E, const 
   a.N = (int)k, a.K = (int)n;
   a.a = static_cast<const u8 *>(dy), a.a_row = 2 * n;
   a.b = static_cast<const u8 *>(w), a.b_row = 2 * k, a.b_expert = 2 * n * k;
-  return tiles(kRaggedDX, a, dtype, dx_dtype, dx, stream);
+  return tiles(kRaggedDX, a, tmm::plan_rows(rows, E, k, n), rows * k, dtype, dx_dtype, dx, workspace, workspace_bytes, stream);
 }
 
 extern "C" int qmm_ragged_mm_dw(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy,
-                                const void *x, int dtype, void *dw, int dw_dtype, qmm_stream_t stream) {
+                                const void *x, int dtype, void *dw, int dw_dtype, void *workspace,
+                                int64_t workspace_bytes, qmm_stream_t stream) {
   if (int st = check(rows, k, n, E, offsets, dy, x, dtype, dw, dw_dtype)) return st;
   tmm::Args a{};
   a.offsets = offsets, a.E = E, a.rows = (int)rows;
   a.M = (int)n, a.N = (int)k;
   a.a = static_cast<const u8 *>(dy), a.a_row = 2 * n;
   a.b = static_cast<const u8 *>(x), a.b_row = 2 * k;
-  return tiles(kRaggedDW, a, dtype, dw_dtype, dw, stream);
+  return tiles(kRaggedDW, a, tmm::plan_sum(rows, E, n, k), E * n * k, dtype, dw_dtype, dw, workspace, workspace_bytes, stream);
 }

@@ -51,6 +51,8 @@ struct Args {
   int y_type;                  // QMM_F32, QMM_BF16 or QMM_F16
   int wide;                    // output rows are 16-byte aligned
   int tiles_n;
+  int splits;                  // parts of the sum, one a layer of the grid (y); more than one: f32 sums [splits][outputs] into part
+  float *part;
 };
 
 template <int DT>
@@ -179,6 +181,48 @@ __device__ __forceinline__ bool row_tile(const Args &a, int &e, int &lo, int &hi
   nt = gt / gm;
   return true;
 }
+// first step of part i of n
+__device__ __forceinline__ int part_of(int steps, int n, int i) { return (int)((int64_t)steps * i / n); }
+// the outputs of a sum in parts: the layer's f32 sums
+__device__ __forceinline__ void to_part(Args &a, int64_t outputs) {
+  if (a.splits == 1) return;
+  a.y = a.part + blockIdx.y * outputs;
+  a.y_type = QMM_F32;
+  a.scales = nullptr;
+}
+
+// The parts added in order, the rows scaled and rounded: a workgroup a tile of BM rows x 256 columns (by the segments, so that rows
+// of no expert stay as they are) or, without offsets, of all rows.
+constexpr int kJoinRows = 16, kJoinCols = 256;
+static __global__ __launch_bounds__(256) void join_kernel(Args a, int64_t outputs) {
+  int e = 0, lo = 0, hi = a.rows, m0, nt;
+  if (!row_tile<kJoinRows>(a, e, lo, hi, m0, nt)) return;
+  const int m_end = min(m0 + kJoinRows, max(hi - lo, 0)), n = nt * kJoinCols + 4 * (int)(threadIdx.x & 63);
+  const int own = min(4, a.N - n);   // columns of the thread
+  for (int m = m0 + (int)(threadIdx.x >> 6); m < m_end; m += 4) {
+    if (own <= 0) return;
+    const int64_t at = (int64_t)(lo + m) * a.N + n;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < a.splits; ++p) {
+      const float *src = a.part + p * outputs + at;
+      if (a.wide) {
+        v += *reinterpret_cast<const f32x4 *>(src);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += i < own ? src[i] : 0.f;
+      }
+    }
+    const float sc = a.scales ? a.scales[2 * (int64_t)(lo + m) + 1] : 1.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i >= own) break;
+      const float o = v[i] * sc;
+      if (a.y_type == QMM_F32) static_cast<float *>(a.y)[at + i] = o;
+      else if (a.y_type == QMM_BF16) static_cast<__bf16 *>(a.y)[at + i] = (__bf16)o;
+      else static_cast<_Float16 *>(a.y)[at + i] = (_Float16)o;
+    }
+  }
+}
 // row tiles that offsets may give at most
 inline int64_t most_row_tiles(const Args &a, int bm) {
   return a.offsets ? std::min<int64_t>((int64_t)a.rows / bm + a.E, a.rows) : (a.rows + bm - 1) / bm;
@@ -220,6 +264,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   const int seg = max(hi - lo, 0);                        // the segment's rows
   const int m_end = SUM == kSumFixed ? seg : a.M;         // outputs m0 .. min(m0 + BM, m_end) - 1
   const int K = SUM == kSumFixed ? a.K : seg, S = (K + 63) >> 6;
+  const int S0 = part_of(S, a.splits, blockIdx.y), S1 = part_of(S, a.splits, blockIdx.y + 1);   // this layer's steps
 
   // ---- straight into LDS: load i of a wave is 1 KB of the step, lane l's 16 bytes a chunk of row (i NW + wave) ROWS + l / CH
   u32 aoff[LA], boff[LB];
@@ -376,8 +421,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
         if (m < end - first) __builtin_amdgcn_sched_barrier(0);
       }
     };
-    read(0, 0, 0);
-    for (int s = 0; s < S; ++s) {
+    read(0, S0, 0);
+    for (int s = S0; s < S1; ++s) {
 #pragma unroll
       for (int kk = 0; kk < 3; ++kk) {
         read((kk + 1) & 1, s, kk + 1);
@@ -412,18 +457,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 
   // blocks of 32 rows of the wave that hold outputs at all (the last tile of a segment is often nearly empty)
   const int live = n0 + cb0 * 32 < a.N ? min(max((m_end - m0 - rb0 * 32 + 31) >> 5, 0), rows_of) : 0;
-  if (S > 0) {
+  if (S1 > S0) {
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) load_one(0, l);
+    for (int l = 0; l < kLoads; ++l) load_one(S0, l);
     if constexpr (kW4) {
-      load_w4(0);
+      load_w4(S0);
 #pragma unroll
-      for (int i = 0; i < kUnits; ++i) store_w4(0, i);
-      if (S > 1) load_w4(1);
+      for (int i = 0; i < kUnits; ++i) store_w4(S0, i);
+      load_w4(S0 + 1);
     }
     wait_all_barrier();
 #pragma unroll
-    for (int l = 0; l < kFirst; ++l) load_one(1, l);
+    for (int l = 0; l < kFirst; ++l) load_one(S0 + 1, l);
     if (live == NI) walk(std::integral_constant<int, NI>{});
     else if (live == 0) walk(std::integral_constant<int, 0>{});
     else if (NI > 1 && live == 1) walk(std::integral_constant<int, 1>{});
@@ -435,12 +480,85 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   constexpr int kStage = 32 * stage_pitch<NJ>();
   static_assert(kStage * 4 * NW <= 2 * (kA + kB), "the staging areas fit the operands' buffers");
   const int64_t out0 = SUM == kSumFixed ? (int64_t)lo * a.N : (int64_t)e * a.M * a.N;
+  to_part(a, SUM == kSumFixed ? (int64_t)a.rows * a.N : (int64_t)a.E * a.M * a.N);
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     if (i >= live) break;
     store_rows<NJ>(a, reinterpret_cast<float *>(smem) + wave * kStage, acc[i], out0, m0 + (rb0 + i) * 32, m_end, n0 + cb0 * 32,
                    SUM == kSumFixed && a.scales ? a.scales + 2 * (int64_t)lo : nullptr, lane);
   }
+}
+
+// ------------------------------------------------------------------------------------------------------ host
+// A tile shape and in how many parts the sum is taken (more where few tiles would walk a long sum): the least estimated time, that
+// is the workgroups that a CU gets times (turns along the sum times a turn's time + a start and end), or what one workgroup alone
+// takes if that is more, and the parts' way through memory. A shape's figures are measured: us a turn over the workgroups that
+// share a CU on launches that fill the chip, and of one workgroup on a CU.
+struct Shape {
+  int bm, bn;
+  float turn, ends, alone;
+};
+struct Plan {
+  int shape, splits;
+};
+// tiles_of(shape): workgroups without a split; outputs: of the whole call
+template <int COUNT, class T>
+Plan least_time(const Shape (&shapes)[COUNT], int64_t turns, int64_t outputs, T tiles_of) {
+  Plan best{0, 1};
+  float least = 0.f;
+  for (int i = 0; i < COUNT; ++i) {
+    const int64_t tiles = std::max<int64_t>(tiles_of(shapes[i]), 1);
+    for (int p = 1; p <= 16; p *= 2) {
+      if (p > 1 && (turns < 4 * p || tiles * p > 1024 || outputs * p > (16 << 20))) break;
+      const float t = (float)((turns + p - 1) / p);
+      const float busy = (float)((tiles * p + 255) / 256) * (t * shapes[i].turn + shapes[i].ends), one = t * shapes[i].alone + 5.f;
+      const float us = std::max(busy, one) + (p > 1 ? 5.f + (float)(outputs * (2 * p + 1)) * 1e-6f : 0.f);
+      if ((i == 0 && p == 1) || us < least) best = {i, p}, least = us;
+    }
+  }
+  return best;
+}
+// row tiles to expect: a segment's last tile is half empty on average, and hardly an expert is without rows
+inline int64_t expected_row_tiles(int64_t rows, int E, int bm) {
+  if (E == 1) return (rows + bm - 1) / bm;
+  const int64_t hit = std::min<int64_t>(E, rows);
+  return std::max<int64_t>(rows / bm + hit / 2, hit - hit / 10);
+}
+// Us measured and estimated: 16384 rows of 32 experts 2880 x 2880 320, 414, 363, 447 (322, 414, 343, 411); gradients of 2048 x 4096 x
+// 12288 in 4 bits 318, 248, 269, 338 (323, 205, 206, 248).
+constexpr Shape kTiles[] = {{256, 256, 1.65f, 6.f, 1.5f}, {256, 128, 1.04f, 5.f, 1.f}, {128, 128, 0.52f, 3.f, 0.8f}, {64, 128, 0.32f, 2.f, 0.7f}};
+inline Plan plan_rows(int64_t rows, int E, int64_t N, int64_t K) {   // the segments cut A's rows
+  return least_time(kTiles, (K + 63) / 64, rows * N,
+                    [&](const Shape &t) { return expected_row_tiles(rows, E, t.bm) * ((N + t.bn - 1) / t.bn); });
+}
+// The segments cut the sum: E M N outputs, however few rows there are, so that the larger tile, which reads less for them, is taken
+// (us, 16384 rows of 32 experts 2880 x 2880 380 against 462 with 128 x 128, 8000 of 128 768 x 2048 190 against 218) unless the matrix
+// does not fill it.
+inline Plan plan_sum(int64_t rows, int E, int64_t M, int64_t N) {
+  const Shape shapes[] = {std::min(M, N) > 128 ? kTiles[0] : kTiles[2]};
+  const int64_t turns = (E == 1 ? rows : rows / E * 3 / 2) / 64 + 1;
+  Plan p = least_time(shapes, turns, E * M * N, [&](const Shape &t) { return (int64_t)E * ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn); });
+  p.shape = std::min(M, N) > 128 ? 0 : 2;
+  return p;
+}
+inline int64_t part_bytes(const Plan &p, int64_t outputs) { return p.splits > 1 ? p.splits * outputs * 4 : 0; }
+
+// the plan's parts in the caller's workspace
+inline int in_parts(Args &a, const Plan &p, int64_t outputs, void *workspace, int64_t bytes) {
+  a.splits = p.splits;
+  a.part = static_cast<float *>(workspace);
+  if (p.splits == 1) return QMM_OK;
+  if (!workspace || bytes < part_bytes(p, outputs)) return QMM_ERR_WORKSPACE;
+  return aligned(workspace, 16) ? QMM_OK : QMM_ERR_ALIGN;
+}
+inline int launch_join(const Args &in, int64_t rows, int64_t outputs, hipStream_t s) {
+  Args a = in;
+  a.tiles_n = (a.N + kJoinCols - 1) / kJoinCols;
+  a.rows = (int)rows;
+  const int64_t tiles = most_row_tiles(a, kJoinRows) * a.tiles_n;
+  if (tiles > (1 << 22)) return QMM_ERR_SHAPE;
+  join_kernel<<<dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), 0, s>>>(a, outputs);
+  return launch_status();
 }
 
 template <int DT, int SA, int SB, int SUM, int BM, int BN, int WM, int WN, int GS>
@@ -453,38 +571,17 @@ int launch(const Args &in, hipStream_t s) {
   auto *fn = tile_mm_kernel<DT, SA, SB, SUM, BM, BN, WM, WN, GS>;
   static std::atomic<unsigned> raised{0};
   if (int st = raise_dyn_lds(reinterpret_cast<const void *>(fn), lds, raised)) return st;
-  fn<<<dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * WM * WN), lds, s>>>(a);
-  return launch_status();
+  fn<<<dim3((unsigned)((tiles + 7) / 8 * 8), a.splits), dim3(64 * WM * WN), lds, s>>>(a);
+  if (int st = launch_status()) return st;
+  if (a.splits == 1) return QMM_OK;
+  if (SUM == kSumFixed) return launch_join(a, a.rows, (int64_t)a.rows * a.N, s);
+  a.offsets = nullptr;   // every matrix is written
+  a.scales = nullptr;
+  return launch_join(a, (int64_t)a.E * a.M, (int64_t)a.E * a.M * a.N, s);
 }
-
-// Of several tile shapes the one with the least estimated time: the workgroups that a CU gets times (turns along the sum times a
-// turn's time + a start and end). A shape's figures are measured on launches that fill the chip: us a turn over the workgroups that
-// share a CU.
-struct Shape {
-  int bm, bn;
-  float turn, ends;
-};
-template <int COUNT>
-int least_time(const Args &a, const Shape (&shapes)[COUNT], int64_t turns) {
-  const int64_t hit = a.offsets ? std::min(a.E, a.rows) : 1;
-  int best = 0;
-  float least = 0.f;
-  for (int i = 0; i < COUNT; ++i) {
-    const Shape &t = shapes[i];
-    // ragged: a segment's last tile is half empty on average, and hardly an expert is without rows
-    const int64_t m = a.offsets ? std::max<int64_t>(a.rows / t.bm + hit / 2, hit - hit / 10) : (a.rows + t.bm - 1) / t.bm;
-    const int64_t tiles = m * ((a.N + t.bn - 1) / t.bn);
-    const float us = (float)((tiles + 255) / 256) * ((float)turns * t.turn + t.ends);
-    if (i == 0 || us < least) best = i, least = us;
-  }
-  return best;
-}
-// Measured against estimated, us: 16384 rows of 32 experts 2880 x 2880 320, 414, 363, 447 (322, 414, 343, 411 estimated); gradients
-// of 2048 x 4096 x 12288 in 4 bits 318, 248, 269, 338 (323, 205, 206, 248).
 template <int DT, int SA, int SB, int GS>
-int launch_chosen(const Args &a, hipStream_t s) {
-  static const Shape shapes[] = {{256, 256, 1.65f, 6.f}, {256, 128, 1.04f, 5.f}, {128, 128, 0.52f, 3.f}, {64, 128, 0.32f, 2.f}};
-  switch (least_time(a, shapes, (a.K + 63) / 64)) {
+int launch_shape(const Args &a, int shape, hipStream_t s) {
+  switch (shape) {
     case 0: return launch<DT, SA, SB, kSumFixed, 256, 256, 2, 4, GS>(a, s);
     case 1: return launch<DT, SA, SB, kSumFixed, 256, 128, 4, 2, GS>(a, s);
     case 2: return launch<DT, SA, SB, kSumFixed, 128, 128, 2, 2, GS>(a, s);

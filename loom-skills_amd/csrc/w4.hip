@@ -99,7 +99,12 @@ tmm::Args tile_args(int64_t rows, int64_t k, int64_t n, int64_t group, int E, co
   a.y_type = y_dtype;
   a.N = (int)N;
   a.wide = N % 8 == 0 && aligned(y, 16);
+  a.splits = 1;
   return a;
+}
+
+bool sizes_ok(int64_t rows, int64_t k, int64_t n, int E) {
+  return shape_ok(n, k, k) && rows >= 0 && rows <= kMaxRows && E >= 1 && E <= kMaxRaggedE;
 }
 
 }  // namespace
@@ -125,9 +130,18 @@ extern "C" int qmm_w4_pack(int E, int64_t n, int64_t k, int64_t group, const uin
   return launch_status();
 }
 
+extern "C" int64_t qmm_w4_mm_workspace_size(int64_t rows, int64_t k, int64_t n, int E, int x_dtype) {
+  if (!sizes_ok(rows, k, n, E)) return -1;
+  return x_dtype == QMM_F16 && rows ? tmm::part_bytes(w4_gemm_plan(rows, E, n, k), rows * n) : 0;
+}
+extern "C" int64_t qmm_w4_mm_t_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
+  if (!sizes_ok(rows, k, n, E)) return -1;
+  return rows ? tmm::part_bytes(tmm::plan_rows(rows, E, k, n), rows * k) : 0;
+}
+
 extern "C" int qmm_w4_mm(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_t *offsets, const void *x,
                          int x_dtype, const float *x_scales, const void *w, const void *ws, void *y, int y_dtype,
-                         qmm_stream_t stream) {
+                         void *workspace, int64_t workspace_bytes, qmm_stream_t stream) {
   if (x_dtype != QMM_F32 && x_dtype != QMM_BF16 && x_dtype != QMM_F16) return QMM_ERR_DTYPE;
   if (int st = check(rows, k, n, group, E, offsets, x, w, ws, y, y_dtype)) return st;
   if (!aligned(x_scales, 4)) return QMM_ERR_ALIGN;
@@ -137,7 +151,9 @@ extern "C" int qmm_w4_mm(int64_t rows, int64_t k, int64_t n, int64_t group, int 
     tmm::Args a = tile_args(rows, k, n, group, E, offsets, x, x_scales, w, ws, y, y_dtype, n);
     a.a_row = 2 * k;
     a.K = (int)k;
-    return w4_gemm(a, group_steps(k, group), s);
+    const tmm::Plan p = w4_gemm_plan(rows, E, n, k);
+    if (int st = in_parts(a, p, rows * n, workspace, workspace_bytes)) return st;
+    return w4_gemm(a, p.shape, group_steps(k, group), s);
   }
   const few::Args a{offsets, E, (int)rows, (int)n, (int)k, static_cast<const u8 *>(x), static_cast<const u8 *>(w),
                     blocks(n) * tiles(k) * 1024, static_cast<const u32 *>(ws), (int)groups_of(k, group),
@@ -146,7 +162,8 @@ extern "C" int qmm_w4_mm(int64_t rows, int64_t k, int64_t n, int64_t group, int 
 }
 
 extern "C" int qmm_w4_mm_t(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_t *offsets, const void *x,
-                           const float *scales, const void *w, const void *ws, void *y, int y_dtype, qmm_stream_t stream) {
+                           const float *scales, const void *w, const void *ws, void *y, int y_dtype, void *workspace,
+                           int64_t workspace_bytes, qmm_stream_t stream) {
   if (int st = check(rows, k, n, group, E, offsets, x, w, ws, y, y_dtype)) return st;
   if (rows && !scales) return QMM_ERR_NULL;
   if (!aligned(scales, 4)) return QMM_ERR_ALIGN;
@@ -154,5 +171,7 @@ extern "C" int qmm_w4_mm_t(int64_t rows, int64_t k, int64_t n, int64_t group, in
   tmm::Args a = tile_args(rows, k, n, group, E, offsets, x, scales, w, ws, y, y_dtype, k);
   a.K = (int)((n + 63) / 64 * 64);
   a.a_row = 2 * (int64_t)a.K;
-  return w4_gemm_t(a, group_steps(k, group), reinterpret_cast<hipStream_t>(stream));
+  const tmm::Plan p = tmm::plan_rows(rows, E, k, n);
+  if (int st = in_parts(a, p, rows * k, workspace, workspace_bytes)) return st;
+  return w4_gemm_t(a, p.shape, group_steps(k, group), reinterpret_cast<hipStream_t>(stream));
 }

@@ -28,6 +28,7 @@ __global__ __launch_bounds__(256, 2) void w4_gemm_kernel(Args a) {
   int e = 0, lo = 0, hi = a.rows, m0, nt;
   if (!row_tile<kRows>(a, e, lo, hi, m0, nt)) return;
   const int n0 = nt * 128 * NJ + wave * 32 * NJ, rows = min(kRows, max(hi - lo, 0) - m0), T = (a.K + 127) >> 7;
+  const int T0 = part_of(T, a.splits, blockIdx.y), T1 = part_of(T, a.splits, blockIdx.y + 1);   // this layer's turns
 
   // x: load i of a wave is rows 4 (4 i + wave) .. + 3
   const u8 *xp = a.a + (int64_t)(lo + m0) * a.a_row;
@@ -105,12 +106,12 @@ __global__ __launch_bounds__(256, 2) void w4_gemm_kernel(Args a) {
       wait_all_barrier();
     };
     Turn w0, w1;
-    load_x(0);
-    load_w(0, w0);
+    load_x(T0);
+    load_w(T0, w0);
     wait_all_barrier();
-    for (int t = 0; t < T; t += 2) {   // an odd last turn multiplies zeros
+    for (int t = T0; t < T1; t += 2) {
       turn(t, w0, w1);
-      turn(t + 1, w1, w0);
+      if (t + 1 < T1) turn(t + 1, w1, w0);
     }
   };
   const int live = n0 < a.N ? (rows + 31) >> 5 : 0;
@@ -120,6 +121,7 @@ __global__ __launch_bounds__(256, 2) void w4_gemm_kernel(Args a) {
   else if (NI > 2 && live == 2) walk(std::integral_constant<int, NI < 2 ? NI : 2>{});
   else if (NI > 2) walk(std::integral_constant<int, NI < 3 ? NI : 3>{});
 
+  to_part(a, (int64_t)a.rows * a.N);
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     if (i >= live) break;
@@ -138,8 +140,9 @@ int launch_one(const Args &in, hipStream_t s) {
   auto *fn = w4_gemm_kernel<NI, NJ, GS>;
   static std::atomic<unsigned> raised{0};
   if (int st = raise_dyn_lds(reinterpret_cast<const void *>(fn), lds, raised)) return st;
-  fn<<<dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), lds, s>>>(a);
-  return launch_status();
+  fn<<<dim3((unsigned)((tiles + 7) / 8 * 8), a.splits), dim3(256), lds, s>>>(a);
+  if (int st = launch_status()) return st;
+  return a.splits == 1 ? QMM_OK : launch_join(a, a.rows, (int64_t)a.rows * a.N, s);
 }
 template <int NI, int NJ>
 int launch_gs(const Args &a, int gs, hipStream_t s) {
@@ -151,9 +154,14 @@ int launch_gs(const Args &a, int gs, hipStream_t s) {
 // us a turn of 128 values, measured at 8192 x 8192 x 4096: 64 x 128 559 us in all, 64 x 256 525, 128 x 128 525, 128 x 256 469. The
 // order it gives is the measured one at 333 x 12288 x 4096 (52, 65, 58, 65 us), 2048 x 4096 x 12288 (223, 218, 203, 199) and 8000 rows
 // of 128 experts 1536 x 2048 (99, 102, 118, 110).
-int w4_gemm(const Args &a, int gs, hipStream_t s) {
-  static const Shape shapes[] = {{64, 128, 0.53f, 1.f}, {64, 256, 1.02f, 1.5f}, {128, 128, 1.02f, 1.5f}, {128, 256, 1.83f, 2.5f}};
-  switch (least_time(a, shapes, (a.K + 127) / 128)) {
+Plan w4_gemm_plan(int64_t rows, int E, int64_t N, int64_t K) {
+  static const Shape shapes[] = {{64, 128, 0.53f, 1.f, 0.55f}, {64, 256, 1.02f, 1.5f, 1.05f}, {128, 128, 1.02f, 1.5f, 1.05f},
+                                 {128, 256, 1.83f, 2.5f, 1.9f}};
+  return least_time(shapes, (K + 127) / 128, rows * N,
+                    [&](const Shape &t) { return expected_row_tiles(rows, E, t.bm) * ((N + t.bn - 1) / t.bn); });
+}
+int w4_gemm(const Args &a, int shape, int gs, hipStream_t s) {
+  switch (shape) {
     case 0: return launch_gs<2, 1>(a, gs, s);
     case 1: return launch_gs<2, 2>(a, gs, s);
     case 2: return launch_gs<4, 1>(a, gs, s);

@@ -4,9 +4,9 @@
 namespace qmm {
 using namespace tmm;
 
-int w4_gemm_t(const Args &a, int gs, hipStream_t s) {
-  if (gs == 1) return launch_chosen<QMM_F16, kRow, kW4Col, 1>(a, s);
-  return gs == 2 ? launch_chosen<QMM_F16, kRow, kW4Col, 2>(a, s) : launch_chosen<QMM_F16, kRow, kW4Col, 4>(a, s);
+int w4_gemm_t(const Args &a, int shape, int gs, hipStream_t s) {
+  if (gs == 1) return launch_shape<QMM_F16, kRow, kW4Col, 1>(a, shape, s);
+  return gs == 2 ? launch_shape<QMM_F16, kRow, kW4Col, 2>(a, shape, s) : launch_shape<QMM_F16, kRow, kW4Col, 4>(a, shape, s);
 }
 
 }  // namespace qmm

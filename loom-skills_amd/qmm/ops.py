@@ -1170,6 +1170,14 @@ def _w4_few(rows, n, k, E, f32):
     return rows < GEMM_MIN_TOKENS or rows <= 4 * E if f32 else rows * n * k <= 1 << 30
 
 
+def _workspace(name, dev, *sizes):
+    """(a workspace or None, its bytes) of a call that may take its sums in parts."""
+    need = getattr(_lib.load(), name)(*sizes)
+    if need < 0:
+        raise ValueError(f"{name[4:-15]} does not take rows, K, N, experts {sizes[:4]}")
+    return (torch.empty(need, dtype=torch.uint8, device=dev), need) if need else (None, 0)
+
+
 def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=None):
     """y = x W^T on weights of w4_pack (qmm_w4_mm): one matrix, or with offsets (i32 [E + 1] on the device) the matrix of
     expert e for rows offsets[e] .. offsets[e + 1] - 1; rows of no expert are left as they were in y. x f32 / bf16 [rows, k],
@@ -1191,8 +1199,10 @@ def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=No
         raise ValueError(f"x is {x.dtype}")
     elif not _w4_few(rows, n, k, E, x.dtype == torch.float32 or y.dtype == torch.float32):
         x, scales = row_scale_f16(x)
+    work, need = _workspace("qmm_w4_mm_workspace_size", x.device, rows, k, n, E, DTYPE["f16"]) if x.dtype == torch.float16 else (None, 0)
     _lib.call("qmm_w4_mm", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), x.data_ptr(), _DT[x.dtype],
-              None if scales is None else scales.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), _DT[y.dtype], s)
+              None if scales is None else scales.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), _DT[y.dtype],
+              None if work is None else work.data_ptr(), need, s)
     return y
 
 
@@ -1211,9 +1221,11 @@ def w4_mm_t(dy, w, ws, n, k, group, offsets=None, y=None, out_dtype=None):
         return y
     x16 = torch.empty((rows, 1, -(-n // 64) * 64), dtype=torch.float16, device=dy.device)
     scales = torch.empty((rows, 2), dtype=torch.float32, device=dy.device)
+    work, need = _workspace("qmm_w4_mm_t_workspace_size", dy.device, rows, k, n, E)
     _lib.call("qmm_grad_operand", rows, 1, n, dy.data_ptr(), _DT[dy.dtype], x16.data_ptr(), scales.data_ptr(), s)
     _lib.call("qmm_w4_mm_t", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), x16.data_ptr(),
-              scales.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), _DT[y.dtype], s)
+              scales.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), _DT[y.dtype], None if work is None else work.data_ptr(),
+              need, s)
     return y
 
 
@@ -1249,8 +1261,9 @@ def ragged_mm(x, offsets, w, y=None, out_dtype=None):
     rows = x.shape[0]
     _shaped(x, (rows, k), (w.dtype,), "x")
     y = _ragged_out(y, (rows, n), out_dtype, x, (x, offsets, w), "y")
+    work, need = _workspace("qmm_ragged_mm_workspace_size", x.device, rows, k, n, E)
     _lib.call("qmm_ragged_mm", rows, k, n, E, offsets.data_ptr(), x.data_ptr(), w.data_ptr(), _DT[w.dtype], y.data_ptr(),
-              _DT[y.dtype], s)
+              _DT[y.dtype], None if work is None else work.data_ptr(), need, s)
     return y
 
 
@@ -1264,8 +1277,9 @@ def ragged_mm_t(dy, offsets, w, dx=None, out_dtype=None):
     rows = dy.shape[0]
     _shaped(dy, (rows, n), (w.dtype,), "dy")
     dx = _ragged_out(dx, (rows, k), out_dtype, dy, (dy, offsets, w), "dx")
+    work, need = _workspace("qmm_ragged_mm_t_workspace_size", dy.device, rows, k, n, E)
     _lib.call("qmm_ragged_mm_t", rows, k, n, E, offsets.data_ptr(), dy.data_ptr(), w.data_ptr(), _DT[w.dtype], dx.data_ptr(),
-              _DT[dx.dtype], s)
+              _DT[dx.dtype], None if work is None else work.data_ptr(), need, s)
     return dx
 
 
@@ -1281,8 +1295,9 @@ def ragged_mm_dw(dy, x, offsets, dw=None, out_dtype=None):
     n = dy.shape[1]
     _shaped(dy, (rows, n), (x.dtype,), "dy")
     dw = _ragged_out(dw, (E, n, k), out_dtype, x, (x, dy, offsets), "dw")
+    work, need = _workspace("qmm_ragged_mm_dw_workspace_size", x.device, rows, k, n, E)
     _lib.call("qmm_ragged_mm_dw", rows, k, n, E, offsets.data_ptr(), dy.data_ptr(), x.data_ptr(), _DT[x.dtype], dw.data_ptr(),
-              _DT[dw.dtype], s)
+              _DT[dw.dtype], None if work is None else work.data_ptr(), need, s)
     return dw
 
 

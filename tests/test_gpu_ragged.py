@@ -24,6 +24,10 @@ CASES = [  # counts, rows before, rows behind, n, k, type, output
     ([1100, 0, 903], 0, 0, 1032, 520, "bf16", "bf16"),
     ([4000, 4101], 0, 5, 1000, 200, "f16", "f32"),
     ([8000, 1, 0, 8300], 2, 0, 1000, 136, "bf16", "bf16"),
+    # long sums of few outputs in parts: the forward, the input's gradient, the weights'
+    ([640, 0, 300], 3, 5, 72, 16384, "bf16", "bf16"),
+    ([100, 0, 61], 2, 1, 8200, 64, "f16", "f32"),
+    ([7000, 0, 3], 0, 4, 64, 72, "bf16", "bf16"),
 ]
 
 

@@ -92,7 +92,9 @@ MANY = [(64, 8, 32, 32, True, "bf16", "bf16"), (65, 200, 96, 32, True, "bf16", "
         (129, 256, 512, 128, True, "bf16", "bf16"), (200, 257, 160, ROW, True, "bf16", "f32"), (257, 520, 1024, 64, True, "bf16", "bf16"),
         (300, 31, 4096, 128, True, "bf16", "f32"), (1, 40, 256, 128, True, "f16", "f32"), (70, 96, 2048, 256, True, "f16", "bf16"),
         # every tile: 64 x 256, 128 x 128, 128 x 256
-        (640, 5000, 160, 32, True, "bf16", "bf16"), (8300, 300, 96, 32, True, "bf16", "f32"), (4090, 2000, 288, 64, True, "bf16", "bf16")]
+        (640, 5000, 160, 32, True, "bf16", "bf16"), (8300, 300, 96, 32, True, "bf16", "f32"), (4090, 2000, 288, 64, True, "bf16", "bf16"),
+        # long sums of few outputs, in parts
+        (90, 72, 8192, 128, True, "bf16", "f32"), (70, 33, 9088, 32, True, "bf16", "bf16"), (200, 300, 2080, 64, True, "bf16", "f32")]
 
 
 @pytest.mark.parametrize("rows,n,k,group,zeros,x_type,out", MANY)
@@ -118,7 +120,7 @@ def test_f16_operand_with_scales(dev):
 
 BY_EXPERT = [([70, 0, 130, 1], 0, 0, 136, 288, 32, "bf16"), ([0, 300, 5], 3, 9, 40, 512, 128, "f32"),
              ([33] * 9 + [0, 0], 0, 1, 264, 160, 64, "bf16"), ([0, 0, 600, 280], 0, 0, 300, 256, ROW, "bf16"),
-             ([500, 0, 1, 1200, 129] * 2, 7, 3, 1000, 160, 32, "bf16")]
+             ([500, 0, 1, 1200, 129] * 2, 7, 3, 1000, 160, 32, "bf16"), ([70, 0, 33], 3, 2, 41, 8192, 128, "f32")]
 
 
 @pytest.mark.parametrize("counts,first,tail,n,k,group,out", BY_EXPERT)
@@ -137,7 +139,9 @@ def test_many_rows_by_expert(dev, counts, first, tail, n, k, group, out):
 GRADS = [(1, 8, 32, 32, True, "bf16", "f32"), (77, 100, 288, 32, True, "bf16", "bf16"), (64, 17, 160, 64, True, "f32", "f32"),
          (129, 200, 512, 128, False, "bf16", "f32"), (200, 64, 1024, ROW, True, "bf16", "bf16"), (257, 320, 96, 64, True, "bf16", "f32"),
          # every tile: 256 x 256, 256 x 128, 128 x 128
-         (16300, 72, 1024, 32, True, "bf16", "bf16"), (8100, 200, 992, 64, True, "bf16", "bf16"), (2000, 130, 1024, 128, True, "bf16", "f32")]
+         (16300, 72, 1024, 32, True, "bf16", "bf16"), (8100, 200, 992, 64, True, "bf16", "bf16"), (2000, 130, 1024, 128, True, "bf16", "f32"),
+         # long sums in parts
+         (77, 8200, 96, 32, True, "bf16", "f32"), (130, 3000, 160, 64, True, "f32", "bf16")]
 
 
 @pytest.mark.parametrize("rows,n,k,group,zeros,dy_type,out", GRADS)
@@ -154,7 +158,7 @@ def test_input_gradient(dev, rows, n, k, group, zeros, dy_type, out):
 
 
 @pytest.mark.parametrize("counts,first,tail,n,k,group", [([70, 0, 130, 1], 0, 0, 136, 288, 32), ([0, 500, 2], 4, 3, 40, 512, 128),
-                                                         ([9] * 12, 0, 0, 72, 160, ROW), ([900, 0, 2100, 1] * 4, 0, 0, 72, 1024, 32)])
+                                                         ([9] * 12, 0, 0, 72, 160, ROW), ([900, 0, 2100, 1] * 4, 0, 0, 72, 1024, 32), ([70, 0, 33], 4, 3, 6000, 64, 64)])
 def test_input_gradient_by_expert(dev, counts, first, tail, n, k, group):
     rows, E = first + sum(counts) + tail, len(counts)
     g = gen(rows + n)

@@ -37,11 +37,11 @@ def test_w4_pack_statuses(lib):   # noqa: F811
 def test_w4_mm_statuses(lib):   # noqa: F811
     st = header_enum("qmm_status")
 
-    def mm(rows=4, k=64, n=8, group=32, E=1, off=None, x=at(), xd=BF16, s=None, w=at(), ws=at(), y=at(), yd=F32):
-        return lib.qmm_w4_mm(rows, k, n, group, E, off, x, xd, s, w, ws, y, yd, None)
+    def mm(rows=4, k=64, n=8, group=32, E=1, off=None, x=at(), xd=BF16, s=None, w=at(), ws=at(), y=at(), yd=F32, work=None, wb=0):
+        return lib.qmm_w4_mm(rows, k, n, group, E, off, x, xd, s, w, ws, y, yd, work, wb, None)
 
-    def back(rows=4, k=64, n=8, group=32, E=1, off=None, x=at(), s=at(), w=at(), ws=at(), y=at(), yd=F32):
-        return lib.qmm_w4_mm_t(rows, k, n, group, E, off, x, s, w, ws, y, yd, None)
+    def back(rows=4, k=64, n=8, group=32, E=1, off=None, x=at(), s=at(), w=at(), ws=at(), y=at(), yd=F32, work=None, wb=0):
+        return lib.qmm_w4_mm_t(rows, k, n, group, E, off, x, s, w, ws, y, yd, work, wb, None)
 
     for call in (mm, back):
         for bad in (dict(rows=-1), dict(rows=(1 << 24) + 1), dict(k=40), dict(n=0), dict(group=24), dict(k=(1 << 20) + 32)):
@@ -56,6 +56,18 @@ def test_w4_mm_statuses(lib):   # noqa: F811
             assert call(**bad) == st["QMM_ERR_ALIGN"], bad
         assert call(rows=0, x=None, w=None, ws=None, y=None) == 0
     assert back(s=None) == st["QMM_ERR_NULL"]
+    # few outputs with a long sum: its parts need a workspace
+    need = lib.qmm_w4_mm_workspace_size(80, 8192, 64, 1, F16)
+    back_need = lib.qmm_w4_mm_t_workspace_size(80, 64, 8192, 1)
+    assert need >= 2 * 80 * 64 * 4 and back_need >= 2 * 80 * 64 * 4
+    assert lib.qmm_w4_mm_workspace_size(80, 8192, 64, 1, BF16) == 0 and lib.qmm_w4_mm_workspace_size(0, 8192, 64, 1, F16) == 0
+    assert lib.qmm_w4_mm_workspace_size(80, 40, 64, 1, F16) == -1 and lib.qmm_w4_mm_t_workspace_size(80, 64, 64, 0) == -1
+    for bad in (dict(), dict(work=at(), wb=need - 1), dict(work=None, wb=need)):
+        assert mm(rows=80, k=8192, n=64, xd=F16, **bad) == st["QMM_ERR_WORKSPACE"], bad
+    assert mm(rows=80, k=8192, n=64, xd=F16, work=ODD, wb=need) == st["QMM_ERR_ALIGN"]
+    for bad in (dict(), dict(work=at(), wb=back_need - 1)):
+        assert back(rows=80, k=64, n=8192, **bad) == st["QMM_ERR_WORKSPACE"], bad
+    assert back(rows=80, k=64, n=8192, work=ODD, wb=back_need) == st["QMM_ERR_ALIGN"]
     for xd in (Q8, MXFP8, -1):
         assert mm(xd=xd) == st["QMM_ERR_DTYPE"]
 
@@ -64,7 +76,7 @@ def test_ragged_statuses(lib):   # noqa: F811
     st = header_enum("qmm_status")
 
     def of(fn):
-        return lambda rows=4, k=64, n=8, E=2, off=at(), a=at(), b=at(), d=BF16, y=at(), yd=F32: fn(rows, k, n, E, off, a, b, d, y, yd, None)
+        return lambda rows=4, k=64, n=8, E=2, off=at(), a=at(), b=at(), d=BF16, y=at(), yd=F32, work=None, wb=0: fn(rows, k, n, E, off, a, b, d, y, yd, work, wb, None)
 
     for fn in (lib.qmm_ragged_mm, lib.qmm_ragged_mm_t, lib.qmm_ragged_mm_dw):
         call = of(fn)
@@ -78,6 +90,14 @@ def test_ragged_statuses(lib):   # noqa: F811
             assert call(**bad) == st["QMM_ERR_NULL"], bad
         for bad in (dict(a=ODD), dict(b=ODD), dict(y=ODD), dict(off=at(0x10002))):
             assert call(**bad) == st["QMM_ERR_ALIGN"], bad
+    for fn, size, sizes in ((lib.qmm_ragged_mm, lib.qmm_ragged_mm_workspace_size, dict(rows=256, k=65536, n=72, E=1)),
+                            (lib.qmm_ragged_mm_t, lib.qmm_ragged_mm_t_workspace_size, dict(rows=80, k=64, n=8192, E=1)),
+                            (lib.qmm_ragged_mm_dw, lib.qmm_ragged_mm_dw_workspace_size, dict(rows=8192, k=64, n=64, E=1))):
+        need = size(*sizes.values())
+        assert need > 0 and size(-1, 64, 64, 1) == -1 and size(80, 60, 64, 1) == -1
+        for bad in (dict(), dict(work=at(), wb=need - 1)):
+            assert of(fn)(**sizes, **bad) == st["QMM_ERR_WORKSPACE"], bad
+        assert of(fn)(**sizes, work=ODD, wb=need) == st["QMM_ERR_ALIGN"]
     assert of(lib.qmm_ragged_mm)(rows=0, a=None, y=None) == 0
     assert of(lib.qmm_ragged_mm_t)(rows=0, a=None, y=None) == 0
 
