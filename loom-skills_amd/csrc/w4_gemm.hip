@@ -42,11 +42,11 @@ __global__ __launch_bounds__(256, 2) void w4_gemm_kernel(Args a) {
     off[i] = (u32)(row * a_row + 16 * ch);
     col[i] = 8 * ch;
   }
-  auto load_x = [&](int t) __attribute__((always_inline)) {   // past the last turn: zeros
+  auto load_x = [&](int t, int buf) __attribute__((always_inline)) {   // past K: zeros
 #pragma unroll
     for (int i = 0; i < LX; ++i)
       lds_load16(resource(xp + (int64_t)t * 256, x_bytes - t * 256), 128 * t + col[i] < a.K ? off[i] : kPast,
-                 __builtin_amdgcn_readfirstlane(lds0 + (u32)((t & 1) * kTurn + (4 * i + wave) * 1024)));
+                 __builtin_amdgcn_readfirstlane(lds0 + (u32)(buf * kTurn + (4 * i + wave) * 1024)));
   };
 
   // the lane's columns' codes and scales; columns past the last read its row block's neighbours and are not stored
@@ -83,11 +83,11 @@ __global__ __launch_bounds__(256, 2) void w4_gemm_kernel(Args a) {
 
   auto walk = [&](auto blocks) __attribute__((always_inline)) {
     constexpr int NA = decltype(blocks)::value;
-    auto turn = [&](int t, const Turn &w, Turn &next) __attribute__((always_inline)) {
-      load_x(t + 1);
+    auto turn = [&](int t, int buf, const Turn &w, Turn &next) __attribute__((always_inline)) {
+      load_x(t + 1, buf ^ 1);
       load_w(t + 1, next);
       __builtin_amdgcn_sched_barrier(0);
-      const u8 *x = smem + (t & 1) * kTurn;
+      const u8 *x = smem + buf * kTurn;
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
         u32x4 fa[NA > 0 ? NA : 1], fb[NJ];
@@ -106,13 +106,15 @@ __global__ __launch_bounds__(256, 2) void w4_gemm_kernel(Args a) {
       wait_all_barrier();
     };
     Turn w0, w1;
-    load_x(T0);
+    load_x(T0, 0);
     load_w(T0, w0);
     wait_all_barrier();
-    for (int t = T0; t < T1; t += 2) {
-      turn(t, w0, w1);
-      if (t + 1 < T1) turn(t + 1, w1, w0);
+    int t = T0;
+    for (; t + 1 < T1; t += 2) {
+      turn(t, 0, w0, w1);
+      turn(t + 1, 1, w1, w0);
     }
+    if (t < T1) turn(t, 0, w0, w1);
   };
   const int live = n0 < a.N ? (rows + 31) >> 5 : 0;
   if (live == NI) walk(std::integral_constant<int, NI>{});
