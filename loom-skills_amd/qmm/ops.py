@@ -1242,8 +1242,10 @@ def _ragged_weights(offsets, w, what="w"):
 def _ragged_out(y, shape, out_dtype, x, reads, what):
     """An output of a ragged product: f32 or the operands' type (that type when neither y nor out_dtype says)."""
     if y is None:
-        y = torch.empty(shape, dtype=x.dtype if out_dtype is None else out_dtype, device=x.device)
-    elif out_dtype is not None and out_dtype != y.dtype:
+        if out_dtype is not None and out_dtype != x.dtype and out_dtype != torch.float32:
+            raise ValueError(f"out_dtype is float32 or {x.dtype}, not {out_dtype}")
+        return x.new_empty(shape, dtype=out_dtype or x.dtype)
+    if out_dtype is not None and out_dtype != y.dtype:
         raise ValueError(f"{what} is {y.dtype}, out_dtype {out_dtype}")
     _shaped(y, shape, (torch.float32, x.dtype), what)
     _apart(y, what, reads)
@@ -1261,7 +1263,9 @@ def ragged_mm(x, offsets, w, y=None, out_dtype=None):
     rows = x.shape[0]
     _shaped(x, (rows, k), (w.dtype,), "x")
     y = _ragged_out(y, (rows, n), out_dtype, x, (x, offsets, w), "y")
-    work, need = _workspace("qmm_ragged_mm_workspace_size", x.device, rows, k, n, E)
+    work, need = None, 0
+    if rows * n * k > 1 << 30 or rows > 64 * E:   # the few-row kernel takes the others without one
+        work, need = _workspace("qmm_ragged_mm_workspace_size", x.device, rows, k, n, E)
     _lib.call("qmm_ragged_mm", rows, k, n, E, offsets.data_ptr(), x.data_ptr(), w.data_ptr(), _DT[w.dtype], y.data_ptr(),
               _DT[y.dtype], None if work is None else work.data_ptr(), need, s)
     return y
