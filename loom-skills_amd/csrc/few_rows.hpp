@@ -78,7 +78,9 @@ __device__ __forceinline__ Parts split(u32x4 a, u32x4 b) {
 
 // W: the weights; F32: rows x are f32 (w4 only), else 16-bit; GS: 32-value steps a scale covers within a 128-value tile; TT:
 // tiles of 16 tokens at a time; KS: waves that share a 16-row block of W, each with every KS-th 128-value tile (a workgroup has
-// 8 / KS blocks); TL: rows of x a wave keeps in LDS. Grid: (row blocks, experts with rows, token chunks of a dense call).
+// 8 / KS blocks); TL: rows of x a wave keeps in LDS. Grid: (row blocks, experts with rows, layers that share a segment's chunks of
+// tokens: all chunks of a dense call; by expert as many as leave few workgroups without one, for a router that sends most rows to
+// one expert).
 //
 // x: up to TL rows are brought into the wave's own LDS, a batch of U tiles at a time and 8 values a lane (f32 rows split into
 // their parts there, once instead of once a lane), rows of U x 16 chunks, chunk i of row t at i ^ t; a fragment read past the last
@@ -268,16 +270,17 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 ? 2 : F32 || TL > 2 || (TL > 1 
 template <int W, bool F32, int GS, int TT, int KS, int TL>
 int launch(const Args &a, int slots, hipStream_t s) {
   constexpr int kRows = TL > 0 ? TL : 16 * TT;
-  const unsigned chunks = a.offsets ? 1u : (unsigned)min((a.rows + kRows - 1) / kRows, 65535);
-  const int per = 16 * kWaves / KS;
-  few_rows_kernel<W, F32, GS, TT, KS, TL><<<dim3((unsigned)((a.n + per - 1) / per), slots, chunks), dim3(64 * kWaves), 0, s>>>(a);
+  const int per = 16 * kWaves / KS, blocks = (a.n + per - 1) / per;
+  const int most = (a.rows + kRows - 1) / kRows;   // chunks of a segment that holds all rows
+  const int chunks = a.offsets ? max(1, min(most / 4, 2048 / (blocks * slots))) : min(most, 65535);
+  few_rows_kernel<W, F32, GS, TT, KS, TL><<<dim3((unsigned)blocks, slots, (unsigned)chunks), dim3(64 * kWaves), 0, s>>>(a);
   return launch_status();
 }
-// us in a graph on inputs out of cache. x in LDS (TL) against fragments from memory: one dense row, w4 12288 x 4096 7.6 against 9.7,
-// 4096 x 12288 8.6 and 12.7, f32 4096 x 4096 6.0 and 8.2; two or four dense rows no difference. By expert with a row each:
-// 16-bit 8 rows 1536 x 2048 11.9 and 13.8; w4 the same 7.2 and 5.9 (two tiles a wave: nothing to save), 104 rows 28 and 30.
-// Two waves a row block instead of eight where the blocks fill the chip: 104 rows of 128 experts w4 1536 x 2048 28 against 47; with
-// more rows a segment (1500) 122 against 105.
+// us in a graph. x in LDS (TL) against fragments from memory, on inputs out of cache: one dense row, w4 12288 x 4096 7.6 against 9.7,
+// 4096 x 12288 8.6 and 12.7, f32 4096 x 4096 6.0 and 8.2; two or four dense rows no difference. By expert with a row each: 16-bit 8
+// rows 1536 x 2048 11.9 and 13.8, but 32 rows of 32 experts 2880 x 2880 56 and 40 (experts hit more often are walked two rows at a
+// time). w4 with two waves a row block where the blocks fill the chip: 104 rows of 128 experts 1536 x 2048 28 against 47 with
+// eight, 30 without LDS; with more rows a segment (1500) 122 against 105.
 template <int W, bool F32, int GS>
 int launch_tt(const Args &a, hipStream_t s) {
   const int slots = a.offsets ? min(a.E, a.rows) : 1;
@@ -287,7 +290,7 @@ int launch_tt(const Args &a, hipStream_t s) {
     if constexpr (W == kW4) {
       if ((int64_t)((a.n + 15) / 16) * slots >= 2048) return launch<W, F32, GS, 1, 2, 4>(a, slots, s);
     } else {
-      return launch<W, F32, GS, 1, 8, 2>(a, slots, s);
+      if (a.rows <= 8) return launch<W, F32, GS, 1, 8, 2>(a, slots, s);
     }
   }
   if (avg <= 16) return launch<W, F32, GS, 1, 8, 0>(a, slots, s);

@@ -30,9 +30,11 @@ int check(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, con
 }
 
 bool takes_few_rows(int64_t rows, int64_t k, int64_t n, int E) {
-  // up to 2^30 products and 64 rows an expert: us, few rows against tiles, 8 experts 4096 x 4096 64 rows 60 and 74, 128 rows 101 and
-  // 75; 128 experts 768 x 2048 512 rows 70 and 86, 1024 rows 100 and 93; 32 experts 2880 x 2880 128 rows 89 and 85
-  return rows * n * k <= (int64_t)1 << 30 && rows <= 64 * (int64_t)E;
+  // Up to 64 rows, or 32 an expert of up to eight, in up to 2^30 products. us, few rows against tiles: one expert 4096 x 4096 32 rows
+  // 14 and 33, 64 rows 21 and 26; 8 experts 1024 x 2048 128 rows 15 and 24, 256 rows 20 and 25, 512 rows 28 and 22; 32 experts 2880 x
+  // 2880 64 rows 70 and 71, 128 rows 87 and 81; 128 experts 768 x 2048 64 rows 24 and 25, 512 rows 57 and 50. With every row one
+  // expert's, whose rows are walked in turn: 64 experts 512 x 512 256 rows 22 and 8, 4096 rows 201 and 9.
+  return rows * n * k <= (int64_t)1 << 30 && (rows <= 64 || (rows <= 32 * (int64_t)E && E <= 8));
 }
 
 int tiles(int op, tmm::Args &a, const tmm::Plan &p, int64_t outputs, int dtype, int out_dtype, void *out, void *workspace,
@@ -67,7 +69,6 @@ extern "C" int64_t qmm_ragged_mm_dw_workspace_size(int64_t rows, int64_t k, int6
 extern "C" int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *x, const void *w,
                              int dtype, void *y, int y_dtype, void *workspace, int64_t workspace_bytes,
                              qmm_stream_t stream) {
-
   if (int st = check(rows, k, n, E, offsets, x, w, dtype, rows ? y : w, y_dtype)) return st;
   if (rows == 0) return QMM_OK;
   if (takes_few_rows(rows, k, n, E)) {

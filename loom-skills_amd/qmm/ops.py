@@ -1164,10 +1164,13 @@ def _w4_weights(w, ws, n, k, group, E):
 
 def _w4_few(rows, n, k, E, f32):
     """Whether f32 / bf16 rows are multiplied as they are, weights streamed for a few rows at a time, rather than as f16 tiles. bf16
-    rows into bf16: up to 2^30 products (us, few rows against row scale and GEMM: 12288 x 4096 16 rows 15 and 25, 32 rows 26 and 25;
-    4096 x 4096 64 rows 18 and 26; 8 experts 4096 x 4096 64 rows 23 and 27, 32 experts 2880 x 2880 128 rows 39 and 39, 128
-    experts 1536 x 2048 256 rows 47 and 39). Where x or y is f32 (its bits are kept) below 64 rows, or up to four an expert."""
-    return rows < GEMM_MIN_TOKENS or rows <= 4 * E if f32 else rows * n * k <= 1 << 30
+    rows into bf16: up to 64 rows of up to 2^30 products, or 2^29 products of one matrix, 2^27 by expert (us, few rows against row
+    scale and GEMM: 12288 x 4096 16 rows 16 and 25, 32 rows 26 and 25; 1024 x 1024 1024 rows 18 and 14; 64 x 256 8192 rows 5 and
+    11; 8 experts 4096 x 4096 64 rows 23 and 27, 1024 x 2048 512 rows 27 and 19; 64 experts 512 x 1024 2048 rows 29 and 17, every
+    row one expert's 162 and 16). Where x or y is f32 (its bits are kept) below 64 rows, or up to four an expert."""
+    if f32:
+        return rows < GEMM_MIN_TOKENS or rows <= 4 * E
+    return rows * n * k <= (1 << 30 if rows <= 64 else 1 << 29 if E == 1 else 1 << 27)
 
 
 def _workspace(name, dev, *sizes):
@@ -1264,7 +1267,7 @@ def ragged_mm(x, offsets, w, y=None, out_dtype=None):
     _shaped(x, (rows, k), (w.dtype,), "x")
     y = _ragged_out(y, (rows, n), out_dtype, x, (x, offsets, w), "y")
     work, need = None, 0
-    if rows * n * k > 1 << 30 or rows > 64 * E:   # the few-row kernel takes the others without one
+    if rows > 64 or rows * n * k > 1 << 30:   # the few-row kernel takes the others without one
         work, need = _workspace("qmm_ragged_mm_workspace_size", x.device, rows, k, n, E)
     _lib.call("qmm_ragged_mm", rows, k, n, E, offsets.data_ptr(), x.data_ptr(), w.data_ptr(), _DT[w.dtype], y.data_ptr(),
               _DT[y.dtype], None if work is None else work.data_ptr(), need, s)

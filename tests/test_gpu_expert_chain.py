@@ -1,0 +1,235 @@
+"""Expert layers of the 4-bit and ragged products as a user's program runs them: routed, sorted, multiplied, combined, and their
+gradients, against the same layer in 64 bits; the products on other streams, at the limits of the experts' number, on rows that all
+go to one expert; INTEGRATION.md's example as it stands."""
+import os
+import re
+
+import pytest
+import torch
+
+from qmm import ops
+from ragged_case import U, Guarded, by_expert, gen, held, offsets_of, w4_raw
+from test_gpu_w4 import packed
+
+pytestmark = pytest.mark.gpu
+DOC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")
+
+
+def routed(ids, E):
+    """(rows of the assignments sorted by expert, offsets) on the device, as the example sorts them."""
+    order = torch.sort(ids.view(-1), stable=True)
+    return order.indices, torch.searchsorted(order.values, torch.arange(E + 1, device=ids.device, dtype=ids.dtype)).int()
+
+
+def rel(got, want):
+    return float((got.cpu().double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("T,E,KU", [(1, 8, 2), (13, 128, 8), (300, 16, 4)])
+def test_four_bit_experts(dev, T, E, KU):
+    """gate and up in one product, down in another, silu between. The up product's operand is f16 or exact, the activation is rounded
+    to bf16 once (2^-8 / sqrt 3 of a value at most, rms) and the two products' weights and outputs to f16 and f32: rel-L2 below
+    2^-8 / sqrt 3 + 4 2^-11 together, 4.3e-3."""
+    H, F, g = 256, 160, gen(T)
+    gu, dn = w4_raw(g, 2 * F, H, 64, True, E), w4_raw(g, H, F, 32, False, E)
+    x, logits = torch.randn((T, H), generator=g).bfloat16(), torch.randn((T, E), generator=g)
+    gu_w, dn_w = packed(gu, 64, dev), packed(dn, 32, dev)
+    ids, wts = ops.moe_topk(logits.to(dev), KU, gating=1, norm=True)
+    rows, offsets = routed(ids, E)
+    a = ops.w4_mm(x.to(dev)[rows // KU], *gu_w, 2 * F, H, 64, offsets=offsets)
+    a = (torch.nn.functional.silu(a[:, :F]) * a[:, F:]).bfloat16()
+    y = ops.w4_mm(a, *dn_w, H, F, 32, offsets=offsets)
+    out = torch.zeros((T, H), device=dev).index_add_(0, rows // KU, y * wts.view(-1)[rows][:, None])
+    want, xd = torch.zeros((T, H), dtype=torch.float64), x.double()
+    for t in range(T):
+        for e, p in zip(ids[t].tolist(), wts[t].tolist()):
+            u = gu[3][e] @ xd[t]
+            want[t] += p * (dn[3][e] @ (torch.nn.functional.silu(u[:F]) * u[F:]))
+    assert rel(out, want) < 4.3e-3
+
+
+@pytest.mark.parametrize("T,E,KU", [(5, 4, 2), (200, 12, 3)])
+def test_training_step_of_experts(dev, T, E, KU):
+    """The layer's gradients with respect to x and both weights against autograd in 64 bits at the same bf16 values. Every product's
+    output is rounded to bf16 once (at most 2^-8 of a value) and meets two more such roundings on the way back: rel-L2 below 3 2^-8."""
+    H, F, g = 96, 136, gen(T)
+    x, ids = torch.randn((T, H), generator=g).bfloat16(), torch.stack([torch.randperm(E, generator=g)[:KU] for _ in range(T)]).int()
+    up, dn = (torch.randn((E, *s), generator=g).div(s[1] ** 0.5).bfloat16() for s in ((F, H), (H, F)))
+    dy = torch.randn((T, H), generator=g).bfloat16()
+    rows, offsets = routed(ids.to(dev), E)
+    xs, upd, dnd = x.to(dev)[rows // KU], up.to(dev), dn.to(dev)
+    h = ops.ragged_mm(xs, offsets, upd)
+    a = torch.relu(h)
+    y = torch.zeros((T, H), device=dev).index_add_(0, rows // KU, ops.ragged_mm(a, offsets, dnd, out_dtype=torch.float32))
+    da, ddn = ops.ragged_mm_backward(dy.to(dev)[rows // KU], a, offsets, dnd, dw_dtype=torch.float32)
+    dxs, dup = ops.ragged_mm_backward(da * (h > 0), xs, offsets, upd, dw_dtype=torch.float32)
+    dx = torch.zeros((T, H), device=dev).index_add_(0, rows // KU, dxs.float())
+
+    xd, upl, dnl = x.double().requires_grad_(), up.double().requires_grad_(), dn.double().requires_grad_()
+    r, o = rows.cpu(), offsets.cpu().tolist()
+    parts = []
+    for e in range(E):
+        he = xd[r[o[e]:o[e + 1]] // KU] @ upl[e].t()
+        parts.append((he * (h[o[e]:o[e + 1]].cpu() > 0)) @ dnl[e].t())   # the kernel's own signs: a rounding may move one
+    want = torch.zeros((T, H), dtype=torch.float64).index_add(0, r // KU, torch.cat(parts))
+    want.backward(dy.double())
+    for name, got, ref in (("y", y, want.detach()), ("dx", dx, xd.grad), ("up", dup, upl.grad), ("down", ddn, dnl.grad)):
+        assert rel(got, ref) < 3 * 2.0 ** -8, name
+
+
+def test_example(dev):
+    """The document's block as it stands. Few rows and f32 results: only f32 sums and, for dw, the products' own order."""
+    block = [b for b in re.findall(r"^```python\n(.*?)^```", open(DOC).read(), flags=re.S | re.M) if "ops.w4_pack(" in b]
+    assert len(block) == 1
+    T, E, KU, n, k, g = 9, 4, 2, 48, 256, gen(1)
+    dense, experts = w4_raw(g, n, k, 128), w4_raw(g, n, k, 128, True, E)
+    w_experts, ws_experts = packed(experts, 128, dev)
+    x, w16 = torch.randn((T, k), generator=g).bfloat16(), torch.randn((E, n, k), generator=g).bfloat16()
+    dys = torch.randn((T * KU, n), generator=g).bfloat16()
+    ids = torch.stack([torch.randperm(E, generator=g)[:KU] for _ in range(T)]).int()
+    names = dict(ops=ops, torch=torch, codes=dense[0].to(dev), scales=dense[1].to(dev), zeros=dense[2].to(dev), x=x.to(dev), n=n, k=k, E=E,
+                 KU=KU, ids=ids.to(dev), w_experts=w_experts, ws_experts=ws_experts, w16=w16.to(dev), dys=dys.to(dev))
+    exec(block[0], names)
+    held(names["y"], x.double() @ dense[3].t(), (k + 8) * U * (x.double().abs() @ dense[4].t()))
+    offsets, xs = names["offsets"].cpu(), names["xs"].cpu().double()
+    assert offsets.tolist() == [int((ids < e).sum()) for e in range(E + 1)]
+    held(names["ys"], by_expert(xs, w16.double(), offsets), k * U * by_expert(xs.abs(), w16.double().abs(), offsets))
+    held(names["dxs"], by_expert(dys.double(), w16.double(), offsets, t=True), n * U * by_expert(dys.double().abs(), w16.double().abs(), offsets, t=True))
+    o = offsets.tolist()
+    want = torch.stack([dys[a:b].double().t() @ xs[a:b] for a, b in zip(o, o[1:])])
+    held(names["dw"], want, T * KU * U * torch.stack([dys[a:b].double().abs().t() @ xs[a:b].abs() for a, b in zip(o, o[1:])]))
+
+
+def test_calls_on_two_streams(dev):
+    """Calls that overlap, sums in parts and in one: each has its own workspace."""
+    g = gen(7)
+    raw = w4_raw(g, 72, 8192, 128)
+    w, ws = packed(raw, 128, dev)
+    x = [torch.randn((90, 8192), generator=g).bfloat16().to(dev) for _ in range(2)]
+    r, rw = torch.randn((7000, 64), generator=g).bfloat16().to(dev), torch.randn((7000, 72), generator=g).bfloat16().to(dev)
+    offsets = offsets_of([7000]).to(dev)
+    run = lambda i: (ops.w4_mm(x[i], w, ws, 72, 8192, 128), ops.ragged_mm_dw(rw, r, offsets, out_dtype=torch.float32))
+    want = [run(0), run(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(o, want[i]))
+
+
+def test_two_graphs(dev):
+    """Two captured calls whose sums are taken in parts, replayed in turn and again after eager work."""
+    g = gen(8)
+    raw = w4_raw(g, 64, 8192, 64)
+    w, ws = packed(raw, 64, dev)
+    x = [torch.randn((80, 8192), generator=g).bfloat16().to(dev) for _ in range(2)]
+    want = [ops.w4_mm(v, w, ws, 64, 8192, 64) for v in x]
+    graphs, outs = [], []
+    for v in x:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.w4_mm(v, w, ws, 64, 8192, 64))
+        graphs.append(graph)
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        for graph in graphs:
+            graph.replay()
+        assert torch.equal(ops.w4_mm(x[0], w, ws, 64, 8192, 64), want[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_most_experts(dev):
+    """1024 experts, most of them empty: 16 a lane of the search for a tile's expert."""
+    g, E, n, k = gen(3), 1024, 16, 32
+    counts = [int(c) for c in torch.randint(0, 3, (E,), generator=g)]
+    counts[777], counts[1023] = 300, 70
+    rows, offsets = sum(counts) + 4, offsets_of(counts, 1)
+    x, dy = torch.randn((rows, k), generator=g).bfloat16(), torch.randn((rows, n), generator=g).bfloat16()
+    raw, w16 = w4_raw(g, n, k, 32, True, E), torch.randn((E, n, k), generator=g).bfloat16()
+    w, ws = packed(raw, 32, dev)
+    live = slice(1, rows - 3)
+    x[0], x[rows - 3:], dy[0], dy[rows - 3:] = (float("nan"),) * 4
+    y, y16, yr, dx, dxr = (Guarded((rows, c), torch.float32, dev) for c in (n, n, n, k, k))
+    xd, od = x.to(dev), offsets.to(dev)
+    ops.w4_mm(xd, w, ws, n, k, 32, offsets=od, y=y.t)                       # few rows an expert
+    x16, scales = ops.row_scale_f16(xd.nan_to_num())
+    ops.w4_mm(x16, w, ws, n, k, 32, offsets=od, scales=scales, y=y16.t)
+    ops.ragged_mm(xd, od, w16.to(dev), y=yr.t)
+    ops.w4_mm_t(dy.nan_to_num().to(dev), w, ws, n, k, 32, offsets=od, y=dx.t)
+    ops.ragged_mm_t(dy.to(dev), od, w16.to(dev), dx=dxr.t)
+    dw = ops.ragged_mm_dw(dy.to(dev), xd, od, out_dtype=torch.float32)
+    for v in (y, y16, yr, dx, dxr):
+        v.check(kept=((0, 1), (rows - 3, rows)))
+    xa, da = x.double(), dy.double()
+    want, size = by_expert(xa, raw[3], offsets)[live], by_expert(xa.abs(), raw[4], offsets)[live]
+    held(y.t[live], want, (k + 8) * U * size)
+    held(y16.t[live], want, (2.0 ** -11 + k * U) * size + 1e-9)   # 2^-38 max |row| sum |w| is below 1e-9 here
+    held(yr.t[live], by_expert(xa, w16.double(), offsets)[live], k * U * by_expert(xa.abs(), w16.double().abs(), offsets)[live])
+    size = by_expert(da.abs(), raw[3].abs(), offsets, t=True)[live]
+    held(dx.t[live], by_expert(da, raw[3], offsets, t=True)[live], (2.0 ** -11 + n * U) * size + 1e-9)
+    held(dxr.t[live], by_expert(da, w16.double(), offsets, t=True)[live], n * U * by_expert(da.abs(), w16.double().abs(), offsets, t=True)[live])
+    o = offsets.tolist()
+    held(dw, torch.stack([da[a:b].t() @ xa[a:b] for a, b in zip(o, o[1:])]),
+         300 * U * torch.stack([da[a:b].abs().t() @ xa[a:b].abs() for a, b in zip(o, o[1:])]))
+
+
+@pytest.mark.parametrize("rows,E,n,k", [(60, 40, 72, 160), (500, 3, 16, 64), (250, 200, 24, 96), (31, 8, 400, 32)])
+def test_every_row_one_experts(dev, rows, E, n, k):
+    """A segment of all rows among empty ones: the few-row kernels walk it in layers of the grid, or one after the other."""
+    g = gen(rows)
+    offsets = torch.tensor([0] * (E // 2 + 1) + [rows] * (E - E // 2), dtype=torch.int32)
+    raw, w16 = w4_raw(g, n, k, 32, True, E), torch.randn((E, n, k), generator=g).bfloat16()
+    w, ws = packed(raw, 32, dev)
+    x = torch.randn((rows, k), generator=g).bfloat16()
+    for out in (torch.float32, torch.bfloat16):
+        y, yr = Guarded((rows, n), out, dev), Guarded((rows, n), out, dev)
+        ops.w4_mm(x.to(dev), w, ws, n, k, 32, offsets=offsets.to(dev), y=y.t)
+        ops.ragged_mm(x.to(dev), offsets.to(dev), w16.to(dev), y=yr.t)
+        y.check(), yr.check()
+        size = by_expert(x.double().abs(), raw[4], offsets)
+        held(y.t, by_expert(x.double(), raw[3], offsets), (2.0 ** -11 + (k + 8) * U) * size + 1e-8)   # 2^-38 max |row| sum |w| is below 1e-8
+        held(yr.t, by_expert(x.double(), w16.double(), offsets), k * U * by_expert(x.double().abs(), w16.double().abs(), offsets))
+
+
+def test_an_expert_does_not_see_its_neighbours(dev):
+    """NaN and infinities of one expert's rows stay in its outputs and its weights' gradient."""
+    g, n, k, E = gen(6), 72, 128, 3
+    offsets = offsets_of([70, 65, 90])
+    x, dy, w16 = (torch.randn(s, generator=g).bfloat16().to(dev) for s in ((225, k), (225, n), (E, n, k)))
+    raw = w4_raw(g, n, k, 32, True, E)
+    w, ws = packed(raw, 32, dev)
+    od = offsets.to(dev)
+    run = lambda: (ops.ragged_mm(x, od, w16), ops.ragged_mm_t(dy, od, w16), ops.w4_mm(x, w, ws, n, k, 32, offsets=od), ops.w4_mm_t(dy, w, ws, n, k, 32, offsets=od))
+    clean, dw = run(), ops.ragged_mm_dw(dy, x, od)
+    x[70:135], dy[70:135, ::2], dy[70:135, 1::2] = float("nan"), float("inf"), float("nan")
+    for got, want in zip(run(), clean):
+        assert torch.equal(got[:70], want[:70]) and torch.equal(got[135:], want[135:]) and not got[70:135].isfinite().any()
+    got = ops.ragged_mm_dw(dy, x, od)
+    assert torch.equal(got[0], dw[0]) and torch.equal(got[2], dw[2]) and got[1].isnan().all()
+
+
+def test_outputs_at_odd_addresses(dev):
+    """y that starts at an element's multiple, not at sixteen bytes: the tiles' narrow stores."""
+    g, n, k = gen(5), 64, 96
+    raw = w4_raw(g, n, k, 32)
+    w, ws = packed(raw, 32, dev)
+    for rows, x_type in ((5, torch.float32), (130, torch.bfloat16)):
+        x = torch.randn((rows, k), generator=g).to(x_type).to(dev)
+        xa = x if rows < 64 else ops.row_scale_f16(x)[0]
+        scales = None if rows < 64 else ops.row_scale_f16(x)[1]
+        want = ops.w4_mm(xa, w, ws, n, k, 32, scales=scales)
+        y = torch.full((rows * n + 2,), 3.0, device=dev)
+        ops.w4_mm(xa, w, ws, n, k, 32, scales=scales, y=y[1:-1].view(rows, n))
+        assert torch.equal(y[1:-1].view(rows, n), want) and y[0] == 3 and y[-1] == 3
+    dy = torch.randn((33, n), generator=g).to(dev)
+    dx = torch.full((33 * k + 2,), 3.0, device=dev)
+    ops.w4_mm_t(dy, w, ws, n, k, 32, y=dx[1:-1].view(33, k))
+    assert torch.equal(dx[1:-1].view(33, k), ops.w4_mm_t(dy, w, ws, n, k, 32)) and dx[0] == 3 and dx[-1] == 3
