@@ -191,36 +191,38 @@ __device__ __forceinline__ void to_part(Args &a, int64_t outputs) {
   a.scales = nullptr;
 }
 
-// The parts added in order, the rows scaled and rounded: a workgroup a tile of BM rows x 256 columns (by the segments, so that rows
-// of no expert stay as they are) or, without offsets, of all rows.
-constexpr int kJoinRows = 16, kJoinCols = 256;
+// The P parts added in order, the rows scaled and rounded: a workgroup a tile of 16 rows x 64 columns (by the segments, so that rows
+// of no expert stay as they are) or, without offsets, of all rows; a thread four columns of a row, its loads all in flight.
+constexpr int kJoinRows = 16, kJoinCols = 64;
+template <int P>
 static __global__ __launch_bounds__(256) void join_kernel(Args a, int64_t outputs) {
   int e = 0, lo = 0, hi = a.rows, m0, nt;
   if (!row_tile<kJoinRows>(a, e, lo, hi, m0, nt)) return;
-  const int m_end = min(m0 + kJoinRows, max(hi - lo, 0)), n = nt * kJoinCols + 4 * (int)(threadIdx.x & 63);
+  const int m = m0 + (int)(threadIdx.x >> 4), n = nt * kJoinCols + 4 * (int)(threadIdx.x & 15);
   const int own = min(4, a.N - n);   // columns of the thread
-  for (int m = m0 + (int)(threadIdx.x >> 6); m < m_end; m += 4) {
-    if (own <= 0) return;
-    const int64_t at = (int64_t)(lo + m) * a.N + n;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < a.splits; ++p) {
-      const float *src = a.part + p * outputs + at;
-      if (a.wide) {
-        v += *reinterpret_cast<const f32x4 *>(src);
-      } else {
+  if (m >= hi - lo || own <= 0) return;
+  const int64_t at = (int64_t)(lo + m) * a.N + n;
+  f32x4 part[P], v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += i < own ? src[i] : 0.f;
-      }
-    }
-    const float sc = a.scales ? a.scales[2 * (int64_t)(lo + m) + 1] : 1.f;
+  for (int p = 0; p < P; ++p) {
+    const float *src = a.part + p * outputs + at;
+    if (a.wide) {
+      part[p] = *reinterpret_cast<const f32x4 *>(src);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i >= own) break;
-      const float o = v[i] * sc;
-      if (a.y_type == QMM_F32) static_cast<float *>(a.y)[at + i] = o;
-      else if (a.y_type == QMM_BF16) static_cast<__bf16 *>(a.y)[at + i] = (__bf16)o;
-      else static_cast<_Float16 *>(a.y)[at + i] = (_Float16)o;
+      for (int i = 0; i < 4; ++i) part[p][i] = src[min(i, own - 1)];
     }
+  }
+#pragma unroll
+  for (int p = 0; p < P; ++p) v += part[p];
+  const float sc = a.scales ? a.scales[2 * (int64_t)(lo + m) + 1] : 1.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i >= own) break;
+    const float o = v[i] * sc;
+    if (a.y_type == QMM_F32) static_cast<float *>(a.y)[at + i] = o;
+    else if (a.y_type == QMM_BF16) static_cast<__bf16 *>(a.y)[at + i] = (__bf16)o;
+    else static_cast<_Float16 *>(a.y)[at + i] = (_Float16)o;
   }
 }
 // row tiles that offsets may give at most
@@ -557,7 +559,13 @@ inline int launch_join(const Args &in, int64_t rows, int64_t outputs, hipStream_
   a.rows = (int)rows;
   const int64_t tiles = most_row_tiles(a, kJoinRows) * a.tiles_n;
   if (tiles > (1 << 22)) return QMM_ERR_SHAPE;
-  join_kernel<<<dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), 0, s>>>(a, outputs);
+  const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
+  switch (a.splits) {
+    case 2: join_kernel<2><<<grid, dim3(256), 0, s>>>(a, outputs); break;
+    case 4: join_kernel<4><<<grid, dim3(256), 0, s>>>(a, outputs); break;
+    case 8: join_kernel<8><<<grid, dim3(256), 0, s>>>(a, outputs); break;
+    default: join_kernel<16><<<grid, dim3(256), 0, s>>>(a, outputs); break;
+  }
   return launch_status();
 }
 

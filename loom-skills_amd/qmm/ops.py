@@ -52,6 +52,7 @@ fastest), the last two one-time weight preparations.
 Every function validates its arguments on the host (the C ABI returns a status that becomes ``QmmError``) and
 launches asynchronously on torch's current stream. Weights are uint8 tensors holding the raw GGUF block bytes.
 """
+import functools
 import weakref
 
 import torch
@@ -1117,6 +1118,7 @@ def gemm_t(fmt, x, w, n, k, w2=None, out_dtype=torch.float32, y=None):
 
 
 # ------------------------------------------------------- 4-bit weights with group scales; rows sorted by expert
+@functools.lru_cache(maxsize=1024)
 def _w4_sizes(n, k, group):
     """(bytes of a packed matrix, bytes of its scale words), as qmm_w4_bytes and qmm_w4_scale_bytes."""
     blocks, groups = (n + 15) // 16, -(-k // group) if group > 0 else 0
@@ -1173,12 +1175,28 @@ def _w4_few(rows, n, k, E, f32):
     return rows * n * k <= (1 << 30 if rows <= 64 else 1 << 29 if E == 1 else 1 << 27)
 
 
-def _workspace(name, dev, *sizes):
-    """(a workspace or None, its bytes) of a call that may take its sums in parts."""
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, *sizes):
+    """The workspace of a call of these sizes, which may take its sums in parts."""
     need = getattr(_lib.load(), name)(*sizes)
     if need < 0:
         raise ValueError(f"{name[4:-15]} does not take rows, K, N, experts {sizes[:4]}")
+    return need
+
+
+def _workspace(name, dev, *sizes):
+    """(a workspace or None, its bytes)."""
+    need = _workspace_bytes(name, *sizes)
     return (torch.empty(need, dtype=torch.uint8, device=dev), need) if need else (None, 0)
+
+
+def _operand_and_workspace(dev, rows, width, need):
+    """One allocation for an f16 operand [rows, width] (width % 32 == 0), a workspace of need bytes and the operand's scales
+    [rows, 2]: (the tensor that holds them, their addresses)."""
+    size = 2 * rows * width
+    t = torch.empty(size + need + 8 * rows, dtype=torch.uint8, device=dev)
+    p = t.data_ptr()
+    return t, p, p + size, p + size + need
 
 
 def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=None):
@@ -1188,24 +1206,30 @@ def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=No
     and weights rounded to f16 where they are many; or the f16 operand [rows, k] with its scales f32 [rows, 2] (or None).
     y [rows, n] f32 or bf16 (out_dtype)."""
     s = _here(x, w, ws, offsets, scales, y)
-    E = _segments(offsets)
+    E = 1 if offsets is None else _segments(offsets)
     _w4_weights(w, ws, n, k, group, E)
-    if x.dim() != 2 or x.shape[1] != k:
-        raise ValueError(f"x is {tuple(x.shape)}, expected [rows, {k}]")
-    rows = x.shape[0]
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != k:
+        raise ValueError(f"x is {tuple(shape)}, expected [rows, {k}]")
+    rows, dtype = shape[0], x.dtype
     y = _rows_out(y, (rows, n), out_dtype, x, (x, w, ws, offsets, scales))
-    if x.dtype == torch.float16:
+    xp, code, sp, work, need = x.data_ptr(), _DT.get(dtype), None, None, 0
+    if dtype == torch.float16:
         _shaped(scales, (rows, 2), (torch.float32,), "scales")
+        sp = None if scales is None else scales.data_ptr()
+        hold, need = _workspace("qmm_w4_mm_workspace_size", x.device, rows, k, n, E, code)
+        work = None if hold is None else hold.data_ptr()
     elif scales is not None:
         raise ValueError("scales come with an f16 operand")
-    elif x.dtype not in _VALUE:
-        raise ValueError(f"x is {x.dtype}")
-    elif not _w4_few(rows, n, k, E, x.dtype == torch.float32 or y.dtype == torch.float32):
-        x, scales = row_scale_f16(x)
-    work, need = _workspace("qmm_w4_mm_workspace_size", x.device, rows, k, n, E, DTYPE["f16"]) if x.dtype == torch.float16 else (None, 0)
-    _lib.call("qmm_w4_mm", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), x.data_ptr(), _DT[x.dtype],
-              None if scales is None else scales.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), _DT[y.dtype],
-              None if work is None else work.data_ptr(), need, s)
+    elif dtype not in _VALUE:
+        raise ValueError(f"x is {dtype}")
+    elif not _w4_few(rows, n, k, E, dtype == torch.float32 or y.dtype == torch.float32):
+        need = _workspace_bytes("qmm_w4_mm_workspace_size", rows, k, n, E, DTYPE["f16"])
+        hold, x16, work, sp = _operand_and_workspace(x.device, rows, k, need)
+        _lib.call("qmm_row_scale_f16", rows, k, xp, code, sp, x16, None, s)
+        xp, code = x16, DTYPE["f16"]
+    _lib.call("qmm_w4_mm", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), xp, code, sp, w.data_ptr(),
+              ws.data_ptr(), y.data_ptr(), _DT[y.dtype], work, need, s)
     return y
 
 
@@ -1222,13 +1246,11 @@ def w4_mm_t(dy, w, ws, n, k, group, offsets=None, y=None, out_dtype=None):
     y = _rows_out(y, (rows, k), out_dtype, dy, (dy, w, ws, offsets))
     if rows == 0:
         return y
-    x16 = torch.empty((rows, 1, -(-n // 64) * 64), dtype=torch.float16, device=dy.device)
-    scales = torch.empty((rows, 2), dtype=torch.float32, device=dy.device)
-    work, need = _workspace("qmm_w4_mm_t_workspace_size", dy.device, rows, k, n, E)
-    _lib.call("qmm_grad_operand", rows, 1, n, dy.data_ptr(), _DT[dy.dtype], x16.data_ptr(), scales.data_ptr(), s)
-    _lib.call("qmm_w4_mm_t", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), x16.data_ptr(),
-              scales.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), _DT[y.dtype], None if work is None else work.data_ptr(),
-              need, s)
+    need = _workspace_bytes("qmm_w4_mm_t_workspace_size", rows, k, n, E)
+    hold, x16, work, scales = _operand_and_workspace(dy.device, rows, -(-n // 64) * 64, need)
+    _lib.call("qmm_grad_operand", rows, 1, n, dy.data_ptr(), _DT[dy.dtype], x16, scales, s)
+    _lib.call("qmm_w4_mm_t", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), x16, scales, w.data_ptr(),
+              ws.data_ptr(), y.data_ptr(), _DT[y.dtype], work, need, s)
     return y
 
 
