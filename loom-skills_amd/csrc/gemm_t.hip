@@ -374,7 +374,43 @@ __global__ __launch_bounds__(NT) void grad_operand_kernel(int64_t rows, int part
     out[p * (n64 / 8) + n / 8 + (int)threadIdx.x % pad] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
   }
 }
-// any n and alignment: the row is read twice, the second time from L2 (2048 rows of 2 x 12288 bf16: 77 us, 33 above)
+// rows of any length up to 256 J values: a row in the registers of a workgroup, its loads all in flight (us, 448 rows of 5012 bf16
+// values 13 in turn, 8 this way)
+template <int J>
+__global__ __launch_bounds__(256) void grad_operand_odd_kernel(int64_t rows, int parts, int n, int n64, const void *__restrict__ x, int bf,
+                                                               _Float16 *__restrict__ x16, float *__restrict__ scales) {
+  const int64_t row = item_index();
+  if (row >= rows) return;
+  const int total = parts * n;
+  const int64_t in0 = row * total, out0 = row * parts * n64;
+  float v[J], m = 0.f;
+  if (bf) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) v[j] = load_val(x, 1, in0 + min((int)threadIdx.x + 256 * j, total - 1));
+  } else {
+#pragma unroll
+    for (int j = 0; j < J; ++j) v[j] = load_val(x, 0, in0 + min((int)threadIdx.x + 256 * j, total - 1));
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) m = fmaxf(m, fabsf(v[j]));   // past the row its last value again
+  const int e = grad_exponent(block_max<256>(m));
+  const float sc = pow2(-e);
+  if (threadIdx.x == 0) {
+    scales[2 * row] = sc;
+    scales[2 * row + 1] = pow2(e);
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int c = (int)threadIdx.x + 256 * j;   // two parts at most
+    if (c < total) x16[out0 + c + (c >= n ? n64 - n : 0)] = (_Float16)(v[j] * sc);
+  }
+  const int pad = n64 - n;   // fewer than 64 values a part
+  if ((int)threadIdx.x < parts * pad) {
+    const int p = (int)threadIdx.x / pad;
+    x16[out0 + p * n64 + n + (int)threadIdx.x % pad] = (_Float16)0.f;
+  }
+}
+// any n and alignment: the row is read twice, the second time from L2 (2048 rows of 2 x 12288 bf16: 77 us, 33 as above with whole chunks)
 __global__ __launch_bounds__(256) void grad_operand_any_kernel(int64_t rows, int parts, int n, int n64, const void *__restrict__ x, int bf,
                                                                _Float16 *__restrict__ x16, float *__restrict__ scales) {
   const int64_t row = item_index(), in0 = row * parts * n, out0 = row * parts * n64;
@@ -462,7 +498,11 @@ extern "C" int qmm_grad_operand(int64_t rows, int parts, int64_t n, const void *
                                                static_cast<_Float16 *>(x16), scales);
     return launch_status();
   };
-  if (n % 8 || !aligned(x, 16) || !aligned(scales, 8) || chunks > 8192) return go(grad_operand_any_kernel, 256);
+  if (n % 8 || !aligned(x, 16) || !aligned(scales, 8) || chunks > 8192) {
+    if (parts * n <= 256) return go(grad_operand_odd_kernel<1>, 256);
+    if (parts * n <= 2048) return go(grad_operand_odd_kernel<8>, 256);
+    return parts * n <= 8192 ? go(grad_operand_odd_kernel<32>, 256) : go(grad_operand_any_kernel, 256);
+  }
   if (chunks <= 256) return go(grad_operand_kernel<256, 1>, 256);
   if (chunks <= 1024) return go(grad_operand_kernel<512, 2>, 512);
   if (chunks <= 2048) return go(grad_operand_kernel<1024, 2>, 1024);

@@ -233,3 +233,24 @@ def test_outputs_at_odd_addresses(dev):
     dx = torch.full((33 * k + 2,), 3.0, device=dev)
     ops.w4_mm_t(dy, w, ws, n, k, 32, y=dx[1:-1].view(33, k))
     assert torch.equal(dx[1:-1].view(33, k), ops.w4_mm_t(dy, w, ws, n, k, 32)) and dx[0] == 3 and dx[-1] == 3
+
+
+@pytest.mark.parametrize("parts,n", [(1, 78), (1, 257), (2, 127), (1, 2047), (2, 1023), (2, 1025), (1, 5012), (2, 4095), (1, 8191), (1, 8193)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_operand_of_odd_rows(dev, parts, n, dtype):
+    """Rows that are no multiple of eight values long, at the lengths where they change kernels."""
+    from qmm import _lib
+    T, N = 5, -(-n // 64) * 64
+    x = (torch.randn((T, parts, n), generator=gen(n)) * 1e-3).to(dtype).to(dev)
+    x[1, parts - 1, n - 1] = 5.0
+    x[2, 0, 0] = float("nan")
+    x[3] = 0
+    buf = torch.full((T * parts * N + 64,), 9.0, dtype=torch.float16, device=dev)
+    x16, s = buf[:-64].view(T, parts, N), torch.empty((T, 2), device=dev)
+    _lib.call("qmm_grad_operand", T, parts, n, x.data_ptr(), ops._dt(x), x16.data_ptr(), s.data_ptr(), ops._stream())
+    rest = [0, 1, 3, 4]
+    assert (x16[..., n:] == 0).all() and (buf[-64:] == 9).all()
+    assert torch.equal(x16[rest][..., :n], (x.float() * s[:, :1, None]).half()[rest])
+    assert x16[2, 0, 0].isnan() and x16[2, :, :n].isnan().sum() == 1 and s[1].tolist() == [2.0 ** 11, 2.0 ** -11]
+    m = x.float().abs().amax((1, 2))[[0, 4]] * s[[0, 4], 0]
+    assert ((m >= 2.0 ** 13) & (m < 2.0 ** 14)).all() and s[3, 0] == 1
