@@ -77,44 +77,49 @@ __device__ __forceinline__ Parts split(u32x4 a, u32x4 b) {
 }
 
 // W: the weights; F32: rows x are f32 (w4 only), else 16-bit; GS: 32-value steps a scale covers within a 128-value tile; TT:
-// tiles of 16 tokens at a time; KS: waves that share a 16-row block of W, each with every KS-th 128-value tile (a workgroup has
-// 8 / KS blocks); TL: rows of x a wave keeps in LDS. Grid: (row blocks, experts with rows, layers that share a segment's chunks of
-// tokens: all chunks of a dense call; by expert as many as leave few workgroups without one, for a router that sends most rows to
-// one expert).
+// tiles of 16 tokens at a time; KS: waves that share 16-row blocks of W, each with every KS-th 128-value tile; RB: blocks of a wave
+// (a workgroup has 8 RB / KS); TL: rows of x a wave keeps in LDS. Grid: (row blocks, experts with rows, layers that share a
+// segment's chunks of tokens: all chunks of a dense call; by expert as many as leave few workgroups without one, for a router that
+// sends most rows to one expert).
 //
 // x: up to TL rows are brought into the wave's own LDS, a batch of U tiles at a time and 8 values a lane (f32 rows split into
 // their parts there, once instead of once a lane), rows of U x 16 chunks, chunk i of row t at i ^ t; a fragment read past the last
 // row reads that one again, its outputs are not stored. With one row a load then brings 1 KB where the fragments' own loads would
 // use four lanes. More rows are read as fragments from memory.
-template <int W, bool F32, int GS, int TT, int KS, int TL>
-__global__ __launch_bounds__(64 * kWaves, TT > 1 ? 2 : F32 || TL > 2 || (TL > 1 && W == kW4) ? 4 : 6) void few_rows_kernel(Args a) {
+template <int W, bool F32, int GS, int TT, int KS, int TL, int RB>
+__global__ __launch_bounds__(64 * kWaves, TT > 1 || RB > 2 ? 2 : F32 || RB > 1 || TL > 2 || (TL > 1 && W == kW4) ? 4 : 6) void few_rows_kernel(Args a) {
   constexpr int kParts = F32 ? 3 : 1, kLoads = F32 ? 2 : 1, kES = F32 ? 4 : 2;
-  constexpr int U = W == kW4 && !F32 ? 4 : 2;   // tiles of a wave whose weights are in flight
-  constexpr int kBlocks = kWaves / KS;
+  constexpr int U = W == kW4 && !F32 && RB < 4 ? 4 : 2;   // tiles of a wave whose weights are in flight
+  constexpr int kBlocks = kWaves / KS * RB;   // of a workgroup
   static_assert(TL == 0 || (TT == 1 && TL <= 16), "staged rows are one tile of tokens");
-  __shared__ __align__(16) float red[KS > 1 ? kWaves : 1][TT][64][4];
+  __shared__ __align__(16) float red[kWaves][RB * TT][64][4];
   __shared__ __align__(16) u8 xs[TL > 0 ? kWaves : 1][TL > 0 ? kParts : 1][TL > 0 ? TL : 1][U * 256];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, h = lane >> 4, part = wave % KS;
   const int KT = (a.k + 127) >> 7, nb = (a.n + 15) >> 4;
-  const int rb0 = (int)blockIdx.x * kBlocks, rb = min(rb0 + wave / KS, nb - 1);
+  const int rb0 = (int)blockIdx.x * kBlocks;
   int e = 0, lo = 0, hi = a.rows;
   if (a.offsets && !nth_segment(a.offsets, a.E, a.rows, blockIdx.y, e, lo, hi)) return;
-  const u8 *w = a.w + (int64_t)e * a.w_expert;
-  const u32 *ws = nullptr;
-  __amdgpu_buffer_rsrc_t wr;
-  if constexpr (W == kW4) {
-    w += (int64_t)rb * KT * 1024;
-    ws = a.ws + ((int64_t)e * nb + rb) * a.groups * 16 + c;
-  } else {
-    wr = rsrc(w + (int64_t)rb * 32 * a.k, (u32)(min(16, a.n - 16 * rb) * a.k * 2));
+  const u8 *w[RB];
+  const u32 *ws[RB];
+  __amdgpu_buffer_rsrc_t wr[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    const int rb = min(rb0 + wave / KS * RB + r, nb - 1);   // blocks past the last: that one again, not stored
+    const u8 *we = a.w + (int64_t)e * a.w_expert;
+    if constexpr (W == kW4) {
+      w[r] = we + (int64_t)rb * KT * 1024;
+      ws[r] = a.ws + ((int64_t)e * nb + rb) * a.groups * 16 + c;
+    } else {
+      wr[r] = rsrc(we + (int64_t)rb * 32 * a.k, (u32)(min(16, a.n - 16 * rb) * a.k * 2));
+    }
   }
   const u32 one = W == kWF16 ? 0x3C003C00u : 0x3F803F80u;
   const u32x4 ones = {one, one, one, one};
 
   struct Batch {
-    u32x4 q[U][W == kW4 ? 1 : 4];
-    u32 sc[U][4 / GS];
+    u32x4 q[RB][U][W == kW4 ? 1 : 4];
+    u32 sc[RB][U][4 / GS];
     u32x4 x[TL > 0 ? TL * U / 4 + (TL * U % 4 != 0) : 1][kLoads];   // 8 values a lane
   };
   constexpr int kX = TL * U * 16;   // chunks of 8 values of a batch's staged rows
@@ -123,9 +128,11 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 ? 2 : F32 || TL > 2 || (TL > 1 
   for (int t0 = lo + (int)blockIdx.z * kRows; t0 < hi; t0 += (int)gridDim.z * kRows) {
     const int rows = min(kRows, hi - t0);
     const __amdgpu_buffer_rsrc_t xr = rsrc(a.x + (int64_t)t0 * a.k * kES, (u32)rows * (u32)a.k * kES);
-    f32x4 acc[TT];
+    f32x4 acc[RB][TT];
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) acc[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) acc[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     constexpr bool kLds = TL > 0;
     {
@@ -143,15 +150,18 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 ? 2 : F32 || TL > 2 || (TL > 1 
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int t = min(tb + KS * u, KT - 1);
-          if constexpr (W == kW4) {
-            b.q[u][0] = *reinterpret_cast<const u32x4 *>(w + (int64_t)t * 1024 + 16 * lane);
 #pragma unroll
-            for (int g = 0; g < 4 / GS; ++g) b.sc[u][g] = ws[min((4 * t + GS * g) >> a.gshift, a.groups - 1) * 16];
-          } else {
+          for (int r = 0; r < RB; ++r) {
+            if constexpr (W == kW4) {
+              b.q[r][u][0] = *reinterpret_cast<const u32x4 *>(w[r] + (int64_t)t * 1024 + 16 * lane);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int kk = 128 * t + 32 * j + 8 * h;
-              b.q[u][j] = ld(wr, kk < a.k ? (u32)(c * a.k + kk) * 2u : kPast);
+              for (int g = 0; g < 4 / GS; ++g) b.sc[r][u][g] = ws[r][min((4 * t + GS * g) >> a.gshift, a.groups - 1) * 16];
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int kk = 128 * t + 32 * j + 8 * h;
+                b.q[r][u][j] = ld(wr[r], kk < a.k ? (u32)(c * a.k + kk) * 2u : kPast);
+              }
             }
           }
         }
@@ -193,15 +203,22 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 ? 2 : F32 || TL > 2 || (TL > 1 
           }
 #pragma unroll
           for (int g = 0; g < 4 / GS; ++g) {
-            f32x4 dot[TT], sum[TT];
+            f32x4 dot[RB][TT], sum[TT];
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt) dot[tt] = sum[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int tt = 0; tt < TT; ++tt) {
+              sum[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int r = 0; r < RB; ++r) dot[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
 #pragma unroll
             for (int jj = 0; jj < GS; ++jj) {
               const int j = GS * g + jj;
-              u32x4 wf;
-              if constexpr (W == kW4) wf = codes(b.q[u][0][j]);
-              else wf = b.q[u][j];
+              u32x4 wf[RB];
+#pragma unroll
+              for (int r = 0; r < RB; ++r) {
+                if constexpr (W == kW4) wf[r] = codes(b.q[r][u][0][j]);
+                else wf[r] = b.q[r][u][j];
+              }
 #pragma unroll
               for (int tt = 0; tt < TT; ++tt) {
                 Parts xp;
@@ -217,20 +234,26 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 ? 2 : F32 || TL > 2 || (TL > 1 
 #pragma unroll
                 for (int p = kParts - 1; p >= 0; --p) {
                   if constexpr (W == kW4) {
-                    dot[tt] = mfma<W>(xp.p[p], wf, dot[tt]);
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) dot[r][tt] = mfma<W>(xp.p[p], wf[r], dot[r][tt]);
                     sum[tt] = mfma<W>(xp.p[p], ones, sum[tt]);
                   } else {
-                    acc[tt] = mfma<W>(xp.p[p], wf, acc[tt]);
+#pragma unroll
+                    for (int r = 0; r < RB; ++r) acc[r][tt] = mfma<W>(xp.p[p], wf[r], acc[r][tt]);
                   }
                 }
               }
             }
             if constexpr (W == kW4) {
-              const float s = f16_to_f32(b.sc[u][g]), z = (float)(b.sc[u][g] >> 16 & 15u);
 #pragma unroll
-              for (int tt = 0; tt < TT; ++tt)
+              for (int r = 0; r < RB; ++r) {
+                const float s = f16_to_f32(b.sc[r][u][g]), z = (float)(b.sc[r][u][g] >> 16 & 15u);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[tt][i] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[tt][i], dot[tt][i]), acc[tt][i]);
+                for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    acc[r][tt][i] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[tt][i], dot[r][tt][i]), acc[r][tt][i]);
+              }
             }
           }
         }
@@ -251,7 +274,9 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 ? 2 : F32 || TL > 2 || (TL > 1 
       }
     };
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) *reinterpret_cast<f32x4 *>(red[wave][tt][lane]) = acc[tt];
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) *reinterpret_cast<f32x4 *>(red[wave][r * TT + tt][lane]) = acc[r][tt];
     __syncthreads();
     // output (block v / (256 TT), token, row v % 16): the block's waves' sums in order
     for (int v = tid; v < 256 * TT * kBlocks; v += 64 * kWaves) {
@@ -259,7 +284,7 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 ? 2 : F32 || TL > 2 || (TL > 1 
       if (token >= rows) continue;
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < KS; ++i) s += red[b * KS + i][token >> 4][l][token & 3];
+      for (int i = 0; i < KS; ++i) s += red[b / RB * KS + i][b % RB * TT + (token >> 4)][l][token & 3];
       store(token, 16 * (rb0 + b) + r, s);
     }
     __syncthreads();
@@ -267,34 +292,50 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 ? 2 : F32 || TL > 2 || (TL > 1 
 }
 
 // Rows behind the last segment are not written. All extents are checked by the callers.
-template <int W, bool F32, int GS, int TT, int KS, int TL>
+template <int W, bool F32, int GS, int TT, int KS, int TL, int RB = 1>
 int launch(const Args &a, int slots, hipStream_t s) {
   constexpr int kRows = TL > 0 ? TL : 16 * TT;
-  const int per = 16 * kWaves / KS, blocks = (a.n + per - 1) / per;
+  const int per = 16 * kWaves / KS * RB, blocks = (a.n + per - 1) / per;
   const int most = (a.rows + kRows - 1) / kRows;   // chunks of a segment that holds all rows
   const int chunks = a.offsets ? max(1, min(most / 4, 2048 / (blocks * slots))) : min(most, 65535);
-  few_rows_kernel<W, F32, GS, TT, KS, TL><<<dim3((unsigned)blocks, slots, (unsigned)chunks), dim3(64 * kWaves), 0, s>>>(a);
+  few_rows_kernel<W, F32, GS, TT, KS, TL, RB><<<dim3((unsigned)blocks, slots, (unsigned)chunks), dim3(64 * kWaves), 0, s>>>(a);
   return launch_status();
 }
-// us in a graph. x in LDS (TL) against fragments from memory, on inputs out of cache: one dense row, w4 12288 x 4096 7.6 against 9.7,
+// us in a graph on inputs out of cache. x in LDS (TL) against fragments from memory: one dense row, w4 12288 x 4096 7.6 against 9.7,
 // 4096 x 12288 8.6 and 12.7, f32 4096 x 4096 6.0 and 8.2; two or four dense rows no difference. By expert with a row each: 16-bit 8
 // rows 1536 x 2048 11.9 and 13.8, but 32 rows of 32 experts 2880 x 2880 56 and 40 (experts hit more often are walked two rows at a
 // time). w4 with two waves a row block where the blocks fill the chip: 104 rows of 128 experts 1536 x 2048 28 against 47 with
-// eight, 30 without LDS; with more rows a segment (1500) 122 against 105.
+// eight, 30 without LDS; f32 rows with four, two blocks each, 38 against 47.
+//
+// Row blocks of a wave (RB) share its reads of x, their split into bf16 parts and the groups' sums, which is most of the work from
+// f32 rows or five bf16 rows on: as many as leave each CU a workgroup, one, two and three at 12288 x 4096: 8 rows bf16 12.1, 11.2,
+// 10.1, f32 26.8, 18.5, 16.4; 63 rows bf16 47.6, 39.2, 23.2, f32 89, 71, 44 (four: 45, and 82 against 50 in groups of 64, spilling);
+// at 6144 x 4096 16 rows 10.6, 8.0, 8.5, at 4096 x 4096 6.7, 7.9; 2 rows bf16 9.8, 10.1, 10.0; 300 rows of 128 experts 1536 x 2048
+// bf16 49, 44, 39, f32 109, 74, 60. 16-bit weights (no sums, no split): 64 rows of 32 experts 2880 x 2880 79 and 86.
+template <int W, bool F32, int GS, int RB>
+int launch_rb(const Args &a, int avg, int slots, hipStream_t s) {
+  if (avg <= 16) return launch<W, F32, GS, 1, 8, 0, RB>(a, slots, s);
+  return avg <= 32 ? launch<W, F32, GS, 2, 8, 0, RB>(a, slots, s) : launch<W, F32, GS, 4, 8, 0, RB>(a, slots, s);
+}
 template <int W, bool F32, int GS>
 int launch_tt(const Args &a, hipStream_t s) {
   const int slots = a.offsets ? min(a.E, a.rows) : 1;
   const int avg = (a.rows + slots - 1) / slots;   // tokens at a time: as many as a segment may hold
+  const int64_t blocks = (int64_t)((a.n + 15) / 16) * slots;
   if (a.rows == 1) return launch<W, F32, GS, 1, 8, 1>(a, slots, s);
-  if (avg == 1) {
-    if constexpr (W == kW4) {
-      if ((int64_t)((a.n + 15) / 16) * slots >= 2048) return launch<W, F32, GS, 1, 2, 4>(a, slots, s);
-    } else {
-      if (a.rows <= 8) return launch<W, F32, GS, 1, 8, 2>(a, slots, s);
+  if constexpr (W != kW4) {
+    if (avg == 1 && a.rows <= 8) return launch<W, F32, GS, 1, 8, 2>(a, slots, s);
+  } else {
+    if (avg == 1 && blocks >= 2048) {
+      if constexpr (F32) return launch<W, F32, GS, 1, 4, 4, 2>(a, slots, s);
+      else return launch<W, F32, GS, 1, 2, 4>(a, slots, s);
+    }
+    if (F32 || a.offsets || avg >= 5) {
+      if (blocks > 512) return launch_rb<W, F32, GS, 3>(a, avg, slots, s);
+      if (blocks > 256) return launch_rb<W, F32, GS, 2>(a, avg, slots, s);
     }
   }
-  if (avg <= 16) return launch<W, F32, GS, 1, 8, 0>(a, slots, s);
-  return avg <= 32 ? launch<W, F32, GS, 2, 8, 0>(a, slots, s) : launch<W, F32, GS, 4, 8, 0>(a, slots, s);
+  return launch_rb<W, F32, GS, 1>(a, avg, slots, s);
 }
 
 }  // namespace few

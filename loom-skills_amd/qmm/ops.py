@@ -1166,13 +1166,16 @@ def _w4_weights(w, ws, n, k, group, E):
 
 def _w4_few(rows, n, k, E, f32):
     """Whether f32 / bf16 rows are multiplied as they are, weights streamed for a few rows at a time, rather than as f16 tiles. bf16
-    rows into bf16: up to 64 rows of up to 2^30 products, or 2^29 products of one matrix, 2^27 by expert (us, few rows against row
-    scale and GEMM: 12288 x 4096 16 rows 16 and 25, 32 rows 26 and 25; 1024 x 1024 1024 rows 18 and 14; 64 x 256 8192 rows 5 and
-    11; 8 experts 4096 x 4096 64 rows 23 and 27, 1024 x 2048 512 rows 27 and 19; 64 experts 512 x 1024 2048 rows 29 and 17, every
-    row one expert's 162 and 16). Where x or y is f32 (its bits are kept) below 64 rows, or up to four an expert."""
+    rows into bf16: up to 64 rows of up to 2^18 values and 2^32 products, or 2^29 products of one matrix, 2^27 by expert (us, few rows
+    against row scale and GEMM: 12288 x 4096 32 rows 13 and 18, 64 rows 20 and 22, 128 rows 38 and 28; 4096 x 12288 32 rows 25 and
+    18; 28672 x 8192 32 rows 63 and 42; 2048 x 2048 128 rows 10 and 17; 1024 x 1024 1024 rows 18 and 14; 8 experts 4096 x 4096 64
+    rows 18 and 25; 128 experts 1536 x 2048 256 rows 30 and 32, every row one expert's 52 and 27). Where x or y is f32 (its bits are
+    kept) below 64 rows, or up to four an expert."""
     if f32:
         return rows < GEMM_MIN_TOKENS or rows <= 4 * E
-    return rows * n * k <= (1 << 30 if rows <= 64 else 1 << 29 if E == 1 else 1 << 27)
+    if rows <= 64:
+        return rows * k <= 1 << 18 and rows * n * k <= 1 << 32
+    return rows * n * k <= (1 << 29 if E == 1 else 1 << 27)
 
 
 @functools.lru_cache(maxsize=4096)
