@@ -56,11 +56,11 @@ bool sizes_ok(int64_t rows, int64_t k, int64_t n, int E) {
 
 extern "C" int64_t qmm_ragged_mm_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
   if (!sizes_ok(rows, k, n, E)) return -1;
-  return rows && !takes_few_rows(rows, k, n, E) ? tmm::part_bytes(tmm::plan_rows(rows, E, n, k), rows * n) : 0;
+  return rows && !takes_few_rows(rows, k, n, E) ? tmm::part_bytes(tmm::plan_rows(tmm::kTiles, rows, E, n, k), rows * n) : 0;
 }
 extern "C" int64_t qmm_ragged_mm_t_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
   if (!sizes_ok(rows, k, n, E)) return -1;
-  return rows ? tmm::part_bytes(tmm::plan_rows(rows, E, k, n), rows * k) : 0;
+  return rows ? tmm::part_bytes(tmm::plan_rows(tmm::kTiles, rows, E, k, n), rows * k) : 0;
 }
 extern "C" int64_t qmm_ragged_mm_dw_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
   return sizes_ok(rows, k, n, E) ? tmm::part_bytes(tmm::plan_sum(rows, E, n, k), E * n * k) : -1;
@@ -81,7 +81,7 @@ extern "C" int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const in
   a.N = (int)n, a.K = (int)k;
   a.a = static_cast<const u8 *>(x), a.a_row = 2 * k;
   a.b = static_cast<const u8 *>(w), a.b_row = 2 * k, a.b_expert = 2 * n * k;
-  return tiles(kRaggedY, a, tmm::plan_rows(rows, E, n, k), rows * n, dtype, y_dtype, y, workspace, workspace_bytes, stream);
+  return tiles(kRaggedY, a, tmm::plan_rows(tmm::kTiles, rows, E, n, k), rows * n, dtype, y_dtype, y, workspace, workspace_bytes, stream);
 }
 
 extern "C" int qmm_ragged_mm_t(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy, const void *w,
@@ -94,7 +94,7 @@ extern "C" int qmm_ragged_mm_t(int64_t rows, int64_t k, int64_t n, int E, const 
   a.N = (int)k, a.K = (int)n;
   a.a = static_cast<const u8 *>(dy), a.a_row = 2 * n;
   a.b = static_cast<const u8 *>(w), a.b_row = 2 * k, a.b_expert = 2 * n * k;
-  return tiles(kRaggedDX, a, tmm::plan_rows(rows, E, k, n), rows * k, dtype, dx_dtype, dx, workspace, workspace_bytes, stream);
+  return tiles(kRaggedDX, a, tmm::plan_rows(tmm::kTiles, rows, E, k, n), rows * k, dtype, dx_dtype, dx, workspace, workspace_bytes, stream);
 }
 
 extern "C" int qmm_ragged_mm_dw(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy,

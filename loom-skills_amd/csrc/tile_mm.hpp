@@ -494,8 +494,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 // ------------------------------------------------------------------------------------------------------ host
 // A tile shape and in how many parts the sum is taken (more where few tiles would walk a long sum): the least estimated time, that
 // is the workgroups that a CU gets times (turns along the sum times a turn's time + a start and end), or what one workgroup alone
-// takes if that is more, and the parts' way through memory. A shape's figures are measured: us a turn over the workgroups that
-// share a CU on launches that fill the chip, and of one workgroup on a CU.
+// takes if that is more, and the parts' way through memory. A shape's figures (us a turn over the workgroups that share a CU on
+// launches that fill the chip, their start and end, a turn of one workgroup on a CU) are those with which the choice comes closest
+// to the fastest of all shapes and parts, measured on 474 calls of 1e9 to 2e11 operations: 2 % slower than it on average.
 struct Shape {
   int bm, bn;
   float turn, ends, alone;
@@ -514,7 +515,7 @@ Plan least_time(const Shape (&shapes)[COUNT], int64_t turns, int64_t outputs, T 
       if (p > 1 && (turns < 4 * p || tiles * p > 1024 || outputs * p > (16 << 20))) break;
       const float t = (float)((turns + p - 1) / p);
       const float busy = (float)((tiles * p + 255) / 256) * (t * shapes[i].turn + shapes[i].ends), one = t * shapes[i].alone + 5.f;
-      const float us = std::max(busy, one) + (p > 1 ? 5.f + (float)(outputs * (2 * p + 1)) * 1e-6f : 0.f);
+      const float us = std::max(busy, one) + (p > 1 ? 4.5f + (float)(outputs * (2 * p + 1)) * 1e-6f : 0.f);
       if ((i == 0 && p == 1) || us < least) best = {i, p}, least = us;
     }
   }
@@ -526,21 +527,23 @@ inline int64_t expected_row_tiles(int64_t rows, int E, int bm) {
   const int64_t hit = std::min<int64_t>(E, rows);
   return std::max<int64_t>(rows / bm + hit / 2, hit - hit / 10);
 }
-// Us measured and estimated: 16384 rows of 32 experts 2880 x 2880 320, 414, 363, 447 (322, 414, 343, 411); gradients of 2048 x 4096 x
-// 12288 in 4 bits 318, 248, 269, 338 (323, 205, 206, 248).
-constexpr Shape kTiles[] = {{256, 256, 1.65f, 6.f, 1.5f}, {256, 128, 1.04f, 5.f, 1.f}, {128, 128, 0.52f, 3.f, 0.8f}, {64, 128, 0.32f, 2.f, 0.7f}};
-inline Plan plan_rows(int64_t rows, int E, int64_t N, int64_t K) {   // the segments cut A's rows
-  return least_time(kTiles, (K + 63) / 64, rows * N,
+// 16-bit weights (the first three) and 4-bit ones. us, 16384 rows of 32 experts 2880 x 2880 320, 363, 447; gradients of 2048 x 4096 x
+// 12288 in 4 bits 301, 247, 315, 227.
+constexpr Shape kTiles[] = {{256, 256, 1.4f, 6.5f, 1.35f}, {128, 128, 0.49f, 3.8f, 0.94f}, {64, 128, 0.36f, 1.1f, 0.55f}};
+constexpr Shape kTilesW4[] = {{256, 256, 1.93f, 8.3f, 1.5f}, {128, 128, 0.54f, 3.4f, 0.8f}, {64, 128, 0.36f, 1.2f, 0.5f}, {256, 128, 1.03f, 5.f, 1.f}};
+template <int COUNT>
+Plan plan_rows(const Shape (&shapes)[COUNT], int64_t rows, int E, int64_t N, int64_t K) {   // the segments cut A's rows
+  return least_time(shapes, (K + 63) / 64, rows * N,
                     [&](const Shape &t) { return expected_row_tiles(rows, E, t.bm) * ((N + t.bn - 1) / t.bn); });
 }
 // The segments cut the sum: E M N outputs, however few rows there are, so that the larger tile, which reads less for them, is taken
 // (us, 16384 rows of 32 experts 2880 x 2880 380 against 462 with 128 x 128, 8000 of 128 768 x 2048 190 against 218) unless the matrix
 // does not fill it.
 inline Plan plan_sum(int64_t rows, int E, int64_t M, int64_t N) {
-  const Shape shapes[] = {std::min(M, N) > 128 ? kTiles[0] : kTiles[2]};
+  const Shape shapes[] = {std::min(M, N) > 128 ? kTiles[0] : kTiles[1]};
   const int64_t turns = (E == 1 ? rows : rows / E * 3 / 2) / 64 + 1;
   Plan p = least_time(shapes, turns, E * M * N, [&](const Shape &t) { return (int64_t)E * ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn); });
-  p.shape = std::min(M, N) > 128 ? 0 : 2;
+  p.shape = std::min(M, N) > 128 ? 0 : 1;
   return p;
 }
 inline int64_t part_bytes(const Plan &p, int64_t outputs) { return p.splits > 1 ? p.splits * outputs * 4 : 0; }
@@ -589,10 +592,11 @@ int launch(const Args &in, hipStream_t s) {
 }
 template <int DT, int SA, int SB, int GS>
 int launch_shape(const Args &a, int shape, hipStream_t s) {
+  if constexpr (SB == kW4Col)
+    if (shape == 3) return launch<DT, SA, SB, kSumFixed, 256, 128, 4, 2, GS>(a, s);
   switch (shape) {
     case 0: return launch<DT, SA, SB, kSumFixed, 256, 256, 2, 4, GS>(a, s);
-    case 1: return launch<DT, SA, SB, kSumFixed, 256, 128, 4, 2, GS>(a, s);
-    case 2: return launch<DT, SA, SB, kSumFixed, 128, 128, 2, 2, GS>(a, s);
+    case 1: return launch<DT, SA, SB, kSumFixed, 128, 128, 2, 2, GS>(a, s);
     default: return launch<DT, SA, SB, kSumFixed, 64, 128, 1, 4, GS>(a, s);
   }
 }

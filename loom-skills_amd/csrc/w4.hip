@@ -136,7 +136,7 @@ extern "C" int64_t qmm_w4_mm_workspace_size(int64_t rows, int64_t k, int64_t n, 
 }
 extern "C" int64_t qmm_w4_mm_t_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
   if (!sizes_ok(rows, k, n, E)) return -1;
-  return rows ? tmm::part_bytes(tmm::plan_rows(rows, E, k, n), rows * k) : 0;
+  return rows ? tmm::part_bytes(tmm::plan_rows(tmm::kTilesW4, rows, E, k, n), rows * k) : 0;
 }
 
 extern "C" int qmm_w4_mm(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_t *offsets, const void *x,
@@ -171,7 +171,7 @@ extern "C" int qmm_w4_mm_t(int64_t rows, int64_t k, int64_t n, int64_t group, in
   tmm::Args a = tile_args(rows, k, n, group, E, offsets, x, scales, w, ws, y, y_dtype, k);
   a.K = (int)((n + 63) / 64 * 64);
   a.a_row = 2 * (int64_t)a.K;
-  const tmm::Plan p = tmm::plan_rows(rows, E, k, n);
+  const tmm::Plan p = tmm::plan_rows(tmm::kTilesW4, rows, E, k, n);
   if (int st = in_parts(a, p, rows * k, workspace, workspace_bytes)) return st;
   return w4_gemm_t(a, p.shape, group_steps(k, group), reinterpret_cast<hipStream_t>(stream));
 }

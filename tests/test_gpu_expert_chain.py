@@ -254,3 +254,37 @@ def test_gradient_operand_of_odd_rows(dev, parts, n, dtype):
     assert x16[2, 0, 0].isnan() and x16[2, :, :n].isnan().sum() == 1 and s[1].tolist() == [2.0 ** 11, 2.0 ** -11]
     m = x.float().abs().amax((1, 2))[[0, 4]] * s[[0, 4], 0]
     assert ((m >= 2.0 ** 13) & (m < 2.0 ** 14)).all() and s[3, 0] == 1
+
+
+# 256 x 256 and 128 x 128 tiles, whole sums and sums in parts (64 x 128 is what the small cases elsewhere take)
+@pytest.mark.parametrize("counts,N,K", [([9000, 1, 0, 8300], 520, 40), ([4000, 0, 4500, 1, 8800], 264, 416), ([4142], 160, 6304),
+                                        ([5000, 7001, 600], 32, 4352), ([4000, 0, 42], 136, 6624)])
+@pytest.mark.parametrize("back", [False, True])
+def test_larger_tiles(dev, counts, N, K, back):
+    """N outputs a row, K values in their sums, forward and backward."""
+    g, rows, E = gen(N + K), sum(counts) + 5, len(counts)
+    offsets = offsets_of(counts, 2)
+    x, w = torch.randn((rows, K), generator=g).bfloat16().to(dev), torch.randn((E, K, N) if back else (E, N, K), generator=g).bfloat16().to(dev)
+    x[:2], x[-3:] = float("nan"), float("nan")
+    y = Guarded((rows, N), torch.float32, dev)
+    (ops.ragged_mm_t(x, offsets.to(dev), w, dx=y.t) if back else ops.ragged_mm(x, offsets.to(dev), w, y=y.t))
+    y.check(kept=((0, 2), (rows - 3, rows)))
+    want, size = by_expert(x.double(), w.double(), offsets.to(dev), t=back)[2:-3], by_expert(x.double().abs(), w.double().abs(), offsets.to(dev), t=back)[2:-3]
+    held(y.t[2:-3], want, K * U * size, "tiles")
+
+
+@pytest.mark.parametrize("counts,n,k", [([1700], 33, 7232), ([9000, 0, 10700], 40, 544), ([1570], 328, 4960), ([16418], 4340, 32),
+                                        ([12000, 814], 2708, 32), ([16429], 36, 320)])
+def test_larger_tiles_of_the_transposed_product(dev, counts, n, k):
+    g, rows, E = gen(n + k), sum(counts) + 1, len(counts)
+    offsets = offsets_of(counts, 1)
+    raw = w4_raw(g, n, k, 64, True, E)
+    w, ws = packed(raw, 64, dev)
+    dy = torch.randn((rows, n), generator=g).bfloat16().to(dev)
+    y = Guarded((rows, k), torch.float32, dev)
+    ops.w4_mm_t(dy, w, ws, n, k, 64, offsets=offsets.to(dev), y=y.t)
+    y.check(kept=((0, 1),))
+    wd = raw[3].to(dev)
+    want, size = by_expert(dy.double(), wd, offsets.to(dev), t=True)[1:], by_expert(dy.double().abs(), wd.abs(), offsets.to(dev), t=True)[1:]
+    lost = 2.0 ** -38 * dy.double().abs().amax(-1, keepdim=True)[1:].cpu() * by_expert(torch.ones_like(dy, dtype=torch.float64), wd.abs(), offsets.to(dev), t=True)[1:]
+    held(y.t[1:], want, (2.0 ** -11 + n * U) * size + lost, "transposed tiles")
