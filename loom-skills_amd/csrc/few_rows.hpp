@@ -9,6 +9,9 @@
 // is one register. w4 codes 0 .. 15 are exact in bf16, a bf16 row is its own operand and an f32 value the sum of three bf16
 // values (its leading 8 bits, the next 8, the rest: three MFMAs), so every product is exact and every sum f32; the groups' sums
 // of x come from an MFMA with ones.
+//
+// Memory bounds a row or two (12288 x 4096 7.6 us for 26.8 MB, 3.5 TB/s), the f32 rows' split and the fragments' reads more rows (16 f32
+// rows 17 us, 63 44 us): eight waves share a row block along K because a wave's chain of loads is what a small call waits for.
 #pragma once
 #include <type_traits>
 

@@ -16,6 +16,12 @@
 // (buffer_load ... lds), rows past a segment's end and values past a row's end as zeros. The fragments of the next 16 values
 // are read while the MFMAs of these run, and the barrier of a step stands before its last 16 values' MFMAs, so that the next
 // step's first reads run under them.
+//
+// The MFMAs bound a full round of 256 x 256 tiles (a step of 64 values 1.65 us on every CU: 1.30 PFLOP/s, at the clock the power limit
+// holds; a library product of 8192^3 reaches 1.55), a launch the rounds it takes and each tile's start and end (6 us: the operands'
+// first loads, 128 KB of outputs): 16384 rows of 32 experts 2880 x 2880 forward 310 us, 0.88 PFLOP/s, in four rounds, the last a
+// little over half full; their weights' gradient 384 us with eight steps a tile. Many experts of few rows are bound by memory: 8000
+// rows of 128 experts 768 x 2048, dW writes 0.8 GB in 191 us.
 #pragma once
 #include <algorithm>
 #include <type_traits>
