@@ -29,12 +29,12 @@ int check(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, con
   return QMM_OK;
 }
 
-bool takes_few_rows(int64_t rows, int64_t k, int64_t n, int E) {
-  // Up to 64 rows, or 32 an expert of up to eight, in up to 2^30 products. us, few rows against tiles: one expert 4096 x 4096 32 rows
-  // 14 and 33, 64 rows 21 and 26; 8 experts 1024 x 2048 128 rows 15 and 24, 256 rows 20 and 25, 512 rows 28 and 22; 32 experts 2880 x
-  // 2880 64 rows 70 and 71, 128 rows 87 and 81; 128 experts 768 x 2048 64 rows 24 and 25, 512 rows 57 and 50. With every row one
-  // expert's, whose rows are walked in turn: 64 experts 512 x 512 256 rows 22 and 8, 4096 rows 201 and 9.
-  return rows * n * k <= (int64_t)1 << 30 && (rows <= 64 || (rows <= 32 * (int64_t)E && E <= 8));
+bool takes_few_rows(int64_t rows, int64_t k, int64_t n) {
+  // Up to 64 rows of 2^17 values in up to 2^30 products. us, few rows against tiles: one matrix 4096 x 4096 16 rows 10 and 12, 32 rows
+  // 14 and 13, 64 rows 21 and 15; 1024 x 4096 64 rows 20 and 10; 4096 x 1024 32 rows 5 and 9; 8 experts 1024 x 2048 64 rows 9 and 10,
+  // 128 rows 15 and 11; 32 experts 2880 x 2880 32 rows 40 and 44, 128 rows 87 and 82; 128 experts 768 x 2048 64 rows 24 and 25, 512
+  // rows 57 and 51. With every row one expert's, whose rows are walked in turn: 64 experts 512 x 512 256 rows 22 and 7.
+  return rows <= 64 && rows * k <= 1 << 17 && rows * n * k <= (int64_t)1 << 30;
 }
 
 int tiles(int op, tmm::Args &a, const tmm::Plan &p, int64_t outputs, int dtype, int out_dtype, void *out, void *workspace,
@@ -56,7 +56,7 @@ bool sizes_ok(int64_t rows, int64_t k, int64_t n, int E) {
 
 extern "C" int64_t qmm_ragged_mm_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
   if (!sizes_ok(rows, k, n, E)) return -1;
-  return rows && !takes_few_rows(rows, k, n, E) ? tmm::part_bytes(tmm::plan_rows(tmm::kTiles, rows, E, n, k), rows * n) : 0;
+  return rows && !takes_few_rows(rows, k, n) ? tmm::part_bytes(tmm::plan_rows(tmm::kTiles, rows, E, n, k), rows * n) : 0;
 }
 extern "C" int64_t qmm_ragged_mm_t_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
   if (!sizes_ok(rows, k, n, E)) return -1;
@@ -71,7 +71,7 @@ extern "C" int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const in
                              qmm_stream_t stream) {
   if (int st = check(rows, k, n, E, offsets, x, w, dtype, rows ? y : w, y_dtype)) return st;
   if (rows == 0) return QMM_OK;
-  if (takes_few_rows(rows, k, n, E)) {
+  if (takes_few_rows(rows, k, n)) {
     const few::Args a{offsets, E, (int)rows, (int)n, (int)k, static_cast<const u8 *>(x), static_cast<const u8 *>(w),
                       2 * n * k, nullptr, 0, 0, y, y_dtype == QMM_F32 ? 4 : 2};
     return ragged_few(a, dtype == QMM_F16, reinterpret_cast<hipStream_t>(stream));

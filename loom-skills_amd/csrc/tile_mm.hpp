@@ -7,7 +7,7 @@
 // with W_e as 16-bit rows or as 4-bit codes with group scales, dequantized to f16 on their way into LDS: f16(s (q - z)), the
 // one rounding (q - z is exact).
 //
-// A workgroup owns BM x BN outputs, WM x WN waves of (BM / WM) x (BN / WN), and walks the sum 64 values at a time through two
+// A workgroup owns BM x BN outputs, WM x WN waves of (BM / WM) x (BN / WN), and walks the sum 64 values at a time through ST
 // LDS buffers. An operand whose memory rows run along the sum (kRow) keeps them: LDS rows of 64 values, 16-byte chunk i at
 // i ^ (row / 2 % 8), so that the 16 rows a fragment read covers at a time lie in all banks. One whose memory rows run along the
 // outputs (kCol) keeps those too, 64 LDS rows of BM or BN values, and is transposed by ds_read_b64_tr_b16 (16 lanes read a
@@ -81,6 +81,12 @@ __device__ __forceinline__ void lds_load16(u32x4 rsrc, u32 voff, u32 lds) {
 __device__ __forceinline__ void wait_all_barrier() {
   __builtin_amdgcn_s_waitcnt(0x0070);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+// the same but for the wave's last N loads
+template <int N>
+__device__ __forceinline__ void wait_but_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 // bytes past 0 (every extent here is below 2^31: at most 256 rows of 2^21 bytes)
 __device__ __forceinline__ u32x4 resource(const u8 *p, int bytes) {
@@ -236,8 +242,9 @@ inline int64_t most_row_tiles(const Args &a, int bm) {
   return a.offsets ? std::min<int64_t>((int64_t)a.rows / bm + a.E, a.rows) : (a.rows + bm - 1) / bm;
 }
 
-// DT: QMM_BF16 or QMM_F16; SA, SB: the operands' sources; GS: 32-value steps a w4 scale covers (1, 2; 4: more)
-template <int DT, int SA, int SB, int SUM, int BM, int BN, int WM, int WN, int GS>
+// DT: QMM_BF16 or QMM_F16; SA, SB: the operands' sources; GS: 32-value steps a w4 scale covers (1, 2; 4: more); ST: steps in LDS,
+// whose loads go out ST - 1 steps ahead
+template <int DT, int SA, int SB, int SUM, int BM, int BN, int WM, int WN, int GS, int ST>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   constexpr int NW = WM * WN, NT = 64 * NW, NI = BM / WM / 32, NJ = BN / WN / 32;
   constexpr int kA = BM * 128, kB = BN * 128;             // LDS bytes of a step's operands
@@ -245,7 +252,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   constexpr bool kW4 = SB == kW4Col;
   static_assert(SA == kRow || BM >= 128, "a transposed operand is at least 128 wide");
   static_assert(SB == kRow || BN >= 128, "a transposed operand is at least 128 wide");
-  extern __shared__ __align__(1024) u8 smem[];            // A [2], B [2]
+  static_assert(ST == 2 || (ST == 4 && !kW4), "a power of two; the wait's count is of direct loads alone");
+  extern __shared__ __align__(1024) u8 smem[];            // A [ST], B [ST]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   int e = 0, lo = 0, hi = a.rows, m0, nt;
@@ -312,14 +320,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   const int a_bytes = SA == kRow ? min(BM, m_end - m0) * a_row : 0, b_bytes = SB == kRow ? min(BN, a.N - n0) * b_row : 0;
   // past the last step (s >= S) the loads give zeros: kRow by the values' check, kCol by the rows left
   auto load_a = [&](int s, int i) __attribute__((always_inline)) {
-    const u32 dst = __builtin_amdgcn_readfirstlane(lds0 + (u32)((s & 1) * kA + (i * NW + wave) * 1024));
+    const u32 dst = __builtin_amdgcn_readfirstlane(lds0 + (u32)((s & (ST - 1)) * kA + (i * NW + wave) * 1024));
     if constexpr (SA == kRow)
       lds_load16(resource(ap + (int64_t)s * 128, a_bytes - s * 128), 64 * s + acol[i] < K ? aoff[i] : kPast, dst);
     else
       lds_load16(resource(ap + (int64_t)s * 64 * a_row, min(64, K - 64 * s) * a_row - m0 * 2), aoff[i], dst);
   };
   auto load_b = [&](int s, int i) __attribute__((always_inline)) {
-    const u32 dst = __builtin_amdgcn_readfirstlane(lds0 + (u32)(2 * kA + (s & 1) * kB + (i * NW + wave) * 1024));
+    const u32 dst = __builtin_amdgcn_readfirstlane(lds0 + (u32)(ST * kA + (s & (ST - 1)) * kB + (i * NW + wave) * 1024));
     if constexpr (SB == kRow)
       lds_load16(resource(bp + (int64_t)s * 128, b_bytes - s * 128), 64 * s + bcol[i] < K ? boff[i] : kPast, dst);
     else if constexpr (SB == kCol)
@@ -376,12 +384,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
     return v;
   };
   auto read_a = [&](int s, int i, int kk) __attribute__((always_inline)) {
-    const u32 at = (u32)((s & 1) * kA);
+    const u32 at = (u32)((s & (ST - 1)) * kA);
     if constexpr (SA == kRow) return read_row(at, rb0 + i, kk);
     else return read_col(at, BM * 2, rb0 + i, kk);
   };
   auto read_b = [&](int s, int j, int kk) __attribute__((always_inline)) {
-    const u32 at = (u32)(2 * kA + (s & 1) * kB);
+    const u32 at = (u32)(ST * kA + (s & (ST - 1)) * kB);
     if constexpr (SB == kRow) return read_row(at, cb0 + j, kk);
     else return read_col(at, BN * 2, cb0 + j, kk);
   };
@@ -441,7 +449,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
         } else if constexpr (kW4) {
           if (kk == 2) store_w4(s + 1, 0);
         }
-        if (kk == 0) multiply_loading(0, s + 1, kFirst, kLoads);
+        if (kk == 0) multiply_loading(0, s + ST - 1, kFirst, kLoads);
         else multiply(kk & 1);
         if constexpr (kW4) {
           if (kk > 0) {
@@ -454,11 +462,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      wait_all_barrier();
+      if constexpr (ST == 2) wait_all_barrier();
+      else wait_but_barrier<(ST - 2) * kLoads>();   // the next step's loads have landed
       read(0, s + 1, 0);   // past the last step: what the buffer holds, not used
       if constexpr (kW4) load_w4(s + 2);
       __builtin_amdgcn_sched_barrier(0);
-      multiply_loading(1, s + 2, 0, kFirst);   // past the last step: zeros
+      multiply_loading(1, s + ST, 0, kFirst);   // past the last step: zeros
     }
     wait_all_barrier();   // the buffers are the outputs' staging areas next
   };
@@ -467,16 +476,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   const int live = n0 + cb0 * 32 < a.N ? min(max((m_end - m0 - rb0 * 32 + 31) >> 5, 0), rows_of) : 0;
   if (S1 > S0) {
 #pragma unroll
-    for (int l = 0; l < kLoads; ++l) load_one(S0, l);
+    for (int t = 0; t < ST - 1; ++t)
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l) load_one(S0 + t, l);
     if constexpr (kW4) {
       load_w4(S0);
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) store_w4(S0, i);
       load_w4(S0 + 1);
     }
-    wait_all_barrier();
+    if constexpr (ST == 2) wait_all_barrier();
+    else wait_but_barrier<(ST - 2) * kLoads>();
 #pragma unroll
-    for (int l = 0; l < kFirst; ++l) load_one(S0 + 1, l);
+    for (int l = 0; l < kFirst; ++l) load_one(S0 + ST - 1, l);
     if (live == NI) walk(std::integral_constant<int, NI>{});
     else if (live == 0) walk(std::integral_constant<int, 0>{});
     else if (NI > 1 && live == 1) walk(std::integral_constant<int, 1>{});
@@ -486,7 +498,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 
   // ---- outputs (every wave is past its last read of the operands)
   constexpr int kStage = 32 * stage_pitch<NJ>();
-  static_assert(kStage * 4 * NW <= 2 * (kA + kB), "the staging areas fit the operands' buffers");
+  static_assert(kStage * 4 * NW <= ST * (kA + kB), "the staging areas fit the operands' buffers");
   const int64_t out0 = SUM == kSumFixed ? (int64_t)lo * a.N : (int64_t)e * a.M * a.N;
   to_part(a, SUM == kSumFixed ? (int64_t)a.rows * a.N : (int64_t)a.E * a.M * a.N);
 #pragma unroll
@@ -502,7 +514,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 // is the workgroups that a CU gets times (turns along the sum times a turn's time + a start and end), or what one workgroup alone
 // takes if that is more, and the parts' way through memory. A shape's figures (us a turn over the workgroups that share a CU on
 // launches that fill the chip, their start and end, a turn of one workgroup on a CU) are those with which the choice comes closest
-// to the fastest of all shapes and parts, measured on 474 calls of 1e9 to 2e11 operations: 2 % slower than it on average.
+// to the fastest of all shapes and parts, measured on 600 calls of 2e8 to 2e11 operations: 2 to 3.5 % slower than it on average.
 struct Shape {
   int bm, bn;
   float turn, ends, alone;
@@ -520,23 +532,27 @@ Plan least_time(const Shape (&shapes)[COUNT], int64_t turns, int64_t outputs, T 
     for (int p = 1; p <= 16; p *= 2) {
       if (p > 1 && (turns < 4 * p || tiles * p > 1024 || outputs * p > (16 << 20))) break;
       const float t = (float)((turns + p - 1) / p);
-      const float busy = (float)((tiles * p + 255) / 256) * (t * shapes[i].turn + shapes[i].ends), one = t * shapes[i].alone + 5.f;
-      const float us = std::max(busy, one) + (p > 1 ? 4.5f + (float)(outputs * (2 * p + 1)) * 1e-6f : 0.f);
+      const float busy = (float)((tiles * p + 255) / 256) * (t * shapes[i].turn + shapes[i].ends), one = t * shapes[i].alone + 5.5f;
+      const float us = std::max(busy, one) + (p > 1 ? 4.5f + (float)(outputs * (2 * p + 1)) * 0.8e-6f : 0.f);
       if ((i == 0 && p == 1) || us < least) best = {i, p}, least = us;
     }
   }
   return best;
 }
-// row tiles to expect: a segment's last tile is half empty on average, and hardly an expert is without rows
+// row tiles to expect: a segment's last tile is half empty on average and segments differ, hardly an expert is without rows
 inline int64_t expected_row_tiles(int64_t rows, int E, int bm) {
   if (E == 1) return (rows + bm - 1) / bm;
   const int64_t hit = std::min<int64_t>(E, rows);
-  return std::max<int64_t>(rows / bm + hit / 2, hit - hit / 10);
+  return std::max<int64_t>(rows / bm + hit * 3 / 5, hit);
 }
-// 16-bit weights (the first three) and 4-bit ones. us, 16384 rows of 32 experts 2880 x 2880 320, 363, 447; gradients of 2048 x 4096 x
-// 12288 in 4 bits 301, 247, 315, 227.
-constexpr Shape kTiles[] = {{256, 256, 1.4f, 6.5f, 1.35f}, {128, 128, 0.49f, 3.8f, 0.94f}, {64, 128, 0.36f, 1.1f, 0.55f}};
-constexpr Shape kTilesW4[] = {{256, 256, 1.93f, 8.3f, 1.5f}, {128, 128, 0.54f, 3.4f, 0.8f}, {64, 128, 0.36f, 1.2f, 0.5f}, {256, 128, 1.03f, 5.f, 1.f}};
+// 16-bit weights: the last two have four steps in LDS instead of two, one workgroup a CU, for launches that leave CUs without a
+// second one to hide a step's loads behind (us, 512 rows of 4 experts 2880 x 2880 32 -> 20, 2000 rows 2048 x 2048 30 -> 24; 8000 rows of
+// 128 experts 768 x 2048 95 either way, dx 105 -> 122); 16384 rows of 32 experts 2880 x 2880 320, 363, 447 with the first three.
+// 4-bit ones: gradients of 2048 x 4096 x 12288 301, 247, 315, 227.
+constexpr Shape kTiles[] = {{256, 256, 1.4f, 7.f, 1.4f}, {128, 128, 0.47f, 3.2f, 0.9f}, {64, 128, 0.4f, 1.f, 0.7f},
+                            {64, 128, 0.38f, 4.4f, 0.36f}, {128, 128, 0.55f, 5.3f, 0.5f}};
+constexpr Shape kTilesW4[] = {{256, 256, 1.93f, 8.3f, 1.5f}, {128, 128, 0.54f, 3.4f, 0.8f}, {64, 128, 0.36f, 1.2f, 0.5f},
+                              {256, 128, 1.03f, 5.f, 1.f}};
 template <int COUNT>
 Plan plan_rows(const Shape (&shapes)[COUNT], int64_t rows, int E, int64_t N, int64_t K) {   // the segments cut A's rows
   return least_time(shapes, (K + 63) / 64, rows * N,
@@ -578,14 +594,14 @@ inline int launch_join(const Args &in, int64_t rows, int64_t outputs, hipStream_
   return launch_status();
 }
 
-template <int DT, int SA, int SB, int SUM, int BM, int BN, int WM, int WN, int GS>
+template <int DT, int SA, int SB, int SUM, int BM, int BN, int WM, int WN, int GS, int ST = 2>
 int launch(const Args &in, hipStream_t s) {
   Args a = in;
   a.tiles_n = (a.N + BN - 1) / BN;
   const int64_t tiles = SUM == kSumRagged ? ((int64_t)((a.M + BM - 1) / BM) * a.tiles_n + 7) / 8 * 8 * a.E : most_row_tiles(a, BM) * a.tiles_n;
   if (tiles > (1 << 22)) return QMM_ERR_SHAPE;   // HIP refuses 2^32 threads along a grid's dimension
-  constexpr int lds = 2 * (BM + BN) * 128;
-  auto *fn = tile_mm_kernel<DT, SA, SB, SUM, BM, BN, WM, WN, GS>;
+  constexpr int lds = ST * (BM + BN) * 128;
+  auto *fn = tile_mm_kernel<DT, SA, SB, SUM, BM, BN, WM, WN, GS, ST>;
   static std::atomic<unsigned> raised{0};
   if (int st = raise_dyn_lds(reinterpret_cast<const void *>(fn), lds, raised)) return st;
   fn<<<dim3((unsigned)((tiles + 7) / 8 * 8), a.splits), dim3(64 * WM * WN), lds, s>>>(a);
@@ -598,8 +614,12 @@ int launch(const Args &in, hipStream_t s) {
 }
 template <int DT, int SA, int SB, int GS>
 int launch_shape(const Args &a, int shape, hipStream_t s) {
-  if constexpr (SB == kW4Col)
+  if constexpr (SB == kW4Col) {
     if (shape == 3) return launch<DT, SA, SB, kSumFixed, 256, 128, 4, 2, GS>(a, s);
+  } else {
+    if (shape == 3) return launch<DT, SA, SB, kSumFixed, 64, 128, 1, 4, GS, 4>(a, s);
+    if (shape == 4) return launch<DT, SA, SB, kSumFixed, 128, 128, 2, 4, GS, 4>(a, s);
+  }
   switch (shape) {
     case 0: return launch<DT, SA, SB, kSumFixed, 256, 256, 2, 4, GS>(a, s);
     case 1: return launch<DT, SA, SB, kSumFixed, 128, 128, 2, 2, GS>(a, s);

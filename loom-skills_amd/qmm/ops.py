@@ -1291,9 +1291,7 @@ def ragged_mm(x, offsets, w, y=None, out_dtype=None):
     rows = x.shape[0]
     _shaped(x, (rows, k), (w.dtype,), "x")
     y = _ragged_out(y, (rows, n), out_dtype, x, (x, offsets, w), "y")
-    work, need = None, 0
-    if rows > 64 or rows * n * k > 1 << 30:   # the few-row kernel takes the others without one
-        work, need = _workspace("qmm_ragged_mm_workspace_size", x.device, rows, k, n, E)
+    work, need = _workspace("qmm_ragged_mm_workspace_size", x.device, rows, k, n, E)
     _lib.call("qmm_ragged_mm", rows, k, n, E, offsets.data_ptr(), x.data_ptr(), w.data_ptr(), _DT[w.dtype], y.data_ptr(),
               _DT[y.dtype], None if work is None else work.data_ptr(), need, s)
     return y

@@ -1,6 +1,6 @@
 """Expert layers of the 4-bit and ragged products as a user's program runs them: routed, sorted, multiplied, combined, and their
 gradients, against the same layer in 64 bits; the products on other streams, at the limits of the experts' number, on rows that all
-go to one expert; INTEGRATION.md's example as it stands."""
+go to one expert; the integration document's example as it stands."""
 import os
 import re
 
@@ -256,9 +256,11 @@ def test_gradient_operand_of_odd_rows(dev, parts, n, dtype):
     assert ((m >= 2.0 ** 13) & (m < 2.0 ** 14)).all() and s[3, 0] == 1
 
 
-# 256 x 256 and 128 x 128 tiles, whole sums and sums in parts (64 x 128 is what the small cases elsewhere take)
+# every tile and depth of LDS, whole sums and sums in parts
 @pytest.mark.parametrize("counts,N,K", [([9000, 1, 0, 8300], 520, 40), ([4000, 0, 4500, 1, 8800], 264, 416), ([4142], 160, 6304),
-                                        ([5000, 7001, 600], 32, 4352), ([4000, 0, 42], 136, 6624)])
+                                        ([5000, 7001, 600], 32, 4352), ([4000, 0, 42], 136, 6624), ([11000, 0, 8801], 528, 40),
+                                        ([30, 0, 45, 0, 0], 6648, 40), ([4182], 32, 2016), ([75, 0, 4], 40, 1160), ([9001, 0, 7600], 32, 40),
+                                        ([2054], 32, 2120), ([131, 0, 250], 2048, 1000)])
 @pytest.mark.parametrize("back", [False, True])
 def test_larger_tiles(dev, counts, N, K, back):
     """N outputs a row, K values in their sums, forward and backward."""
