@@ -16,6 +16,7 @@ int ragged_tiles(int op, const tmm::Args &a, int shape, hipStream_t s) {
   if (op == kRaggedY) return launch_shape<DT, kRow, kRow, 4>(a, shape, s);
   if (op == kRaggedDX) return launch_shape<DT, kRow, kCol, 4>(a, shape, s);
   if (shape == 0) return launch<DT, kCol, kCol, kSumRagged, 256, 256, 2, 4, 4>(a, s);
+  if (shape == 2) return launch<DT, kCol, kCol, kSumRagged, 128, 128, 2, 4, 4, 4>(a, s);
   return launch<DT, kCol, kCol, kSumRagged, 128, 128, 2, 2, 4>(a, s);
 }
 

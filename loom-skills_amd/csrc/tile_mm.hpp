@@ -522,17 +522,18 @@ struct Shape {
 struct Plan {
   int shape, splits;
 };
-// tiles_of(shape): workgroups without a split; outputs: of the whole call
+// turns: of a workgroup (the longest); mean: of them all, for what a CU's workgroups take together; tiles_of(shape): workgroups without
+// a split; outputs: of the whole call
 template <int COUNT, class T>
-Plan least_time(const Shape (&shapes)[COUNT], int64_t turns, int64_t outputs, T tiles_of) {
+Plan least_time(const Shape (&shapes)[COUNT], int64_t turns, float mean, int64_t outputs, T tiles_of) {
   Plan best{0, 1};
   float least = 0.f;
   for (int i = 0; i < COUNT; ++i) {
     const int64_t tiles = std::max<int64_t>(tiles_of(shapes[i]), 1);
     for (int p = 1; p <= 16; p *= 2) {
       if (p > 1 && (turns < 4 * p || tiles * p > 1024 || outputs * p > (16 << 20))) break;
-      const float t = (float)((turns + p - 1) / p);
-      const float busy = (float)((tiles * p + 255) / 256) * (t * shapes[i].turn + shapes[i].ends), one = t * shapes[i].alone + 5.5f;
+      const float t = (float)((turns + p - 1) / p), each = mean < (float)turns ? mean / p : t;
+      const float busy = (float)((tiles * p + 255) / 256) * (each * shapes[i].turn + shapes[i].ends), one = t * shapes[i].alone + 5.5f;
       const float us = std::max(busy, one) + (p > 1 ? 4.5f + (float)(outputs * (2 * p + 1)) * 0.8e-6f : 0.f);
       if ((i == 0 && p == 1) || us < least) best = {i, p}, least = us;
     }
@@ -555,18 +556,17 @@ constexpr Shape kTilesW4[] = {{256, 256, 1.93f, 8.3f, 1.5f}, {128, 128, 0.54f, 3
                               {256, 128, 1.03f, 5.f, 1.f}};
 template <int COUNT>
 Plan plan_rows(const Shape (&shapes)[COUNT], int64_t rows, int E, int64_t N, int64_t K) {   // the segments cut A's rows
-  return least_time(shapes, (K + 63) / 64, rows * N,
+  return least_time(shapes, (K + 63) / 64, (float)((K + 63) / 64), rows * N,
                     [&](const Shape &t) { return expected_row_tiles(rows, E, t.bm) * ((N + t.bn - 1) / t.bn); });
 }
-// The segments cut the sum: E M N outputs, however few rows there are, so that the larger tile, which reads less for them, is taken
-// (us, 16384 rows of 32 experts 2880 x 2880 380 against 462 with 128 x 128, 8000 of 128 768 x 2048 190 against 218) unless the matrix
-// does not fill it.
+// The segments cut the sum: E M N outputs, however few rows there are; the longest segment is taken as 1.4 times the average. us with
+// the shapes in turn: 16384 rows of 32 experts 2880 x 2880 380 and 462, 8000 of 128 768 x 2048 145, 159, 222, 15314 of 16 1216 x 264
+// 85, 60, 48, 2000 of two 2048 x 1024 44, 28, 21, 500 of four 1024 x 1024 12, 7, 7, 15313 of three 248 x 824 in four parts 44, 31, 26.
+constexpr Shape kTilesSum[] = {{256, 256, 1.35f, 6.8f, 1.35f}, {128, 128, 0.46f, 2.2f, 1.1f}, {128, 128, 0.52f, 5.3f, 0.57f}};
 inline Plan plan_sum(int64_t rows, int E, int64_t M, int64_t N) {
-  const Shape shapes[] = {std::min(M, N) > 128 ? kTiles[0] : kTiles[1]};
-  const int64_t turns = (E == 1 ? rows : rows / E * 3 / 2) / 64 + 1;
-  Plan p = least_time(shapes, turns, E * M * N, [&](const Shape &t) { return (int64_t)E * ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn); });
-  p.shape = std::min(M, N) > 128 ? 0 : 1;
-  return p;
+  const float mean = E == 1 ? (float)(rows / 64 + 1) : (float)rows / (64.f * (float)E) + 1.f;
+  return least_time(kTilesSum, (E == 1 ? rows : rows * 7 / (5 * E)) / 64 + 1, mean, E * M * N,
+                    [&](const Shape &t) { return (int64_t)E * ((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn); });
 }
 inline int64_t part_bytes(const Plan &p, int64_t outputs) { return p.splits > 1 ? p.splits * outputs * 4 : 0; }
 

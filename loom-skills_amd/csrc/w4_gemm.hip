@@ -159,7 +159,7 @@ int launch_gs(const Args &a, int gs, hipStream_t s) {
 Plan w4_gemm_plan(int64_t rows, int E, int64_t N, int64_t K) {
   static const Shape shapes[] = {{64, 128, 0.5f, 1.f, 0.55f}, {64, 256, 1.06f, 1.5f, 1.05f}, {128, 128, 1.06f, 1.5f, 1.05f},
                                  {128, 256, 1.83f, 2.5f, 1.9f}};
-  return least_time(shapes, (K + 127) / 128, rows * N,
+  return least_time(shapes, (K + 127) / 128, (float)((K + 127) / 128), rows * N,
                     [&](const Shape &t) { return expected_row_tiles(rows, E, t.bm) * ((N + t.bn - 1) / t.bn); });
 }
 int w4_gemm(const Args &a, int shape, int gs, hipStream_t s) {

@@ -290,3 +290,20 @@ def test_larger_tiles_of_the_transposed_product(dev, counts, n, k):
     want, size = by_expert(dy.double(), wd, offsets.to(dev), t=True)[1:], by_expert(dy.double().abs(), wd.abs(), offsets.to(dev), t=True)[1:]
     lost = 2.0 ** -38 * dy.double().abs().amax(-1, keepdim=True)[1:].cpu() * by_expert(torch.ones_like(dy, dtype=torch.float64), wd.abs(), offsets.to(dev), t=True)[1:]
     held(y.t[1:], want, (2.0 ** -11 + n * U) * size + lost, "transposed tiles")
+
+
+@pytest.mark.parametrize("counts,n,k", [([10, 0, 14, 5, 1], 520, 3992), ([8750], 144, 2192), ([9000, 0, 7000, 1, 103], 136, 1208),
+                                        ([5000, 796], 16, 2072), ([30], 2952, 1304), ([968], 16, 16), ([70, 1300], 72, 264)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_larger_tiles_of_the_weight_gradient(dev, counts, n, k, dtype):
+    g, rows, E = gen(n + k), sum(counts) + 5, len(counts)
+    offsets = offsets_of(counts, 2)
+    x, dy = torch.randn((rows, k), generator=g).to(dtype).to(dev), (0.1 * torch.randn((rows, n), generator=g)).to(dtype).to(dev)
+    x[:2], x[-3:], dy[:2], dy[-3:] = (float("nan"),) * 4
+    dw = Guarded((E, n, k), torch.float32, dev)
+    ops.ragged_mm_dw(dy, x, offsets.to(dev), dw=dw.t)
+    dw.check()
+    at = offsets.tolist()
+    for e, (a, b) in enumerate(zip(at, at[1:])):
+        xd, dd = x[a:b].double(), dy[a:b].double().t().contiguous()
+        held(dw.t[e], torch.mm(dd, xd).cpu(), (b - a + 16) * U * torch.mm(dd.abs(), xd.abs()).cpu(), f"expert {e}")
