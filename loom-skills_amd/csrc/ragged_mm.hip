@@ -41,7 +41,6 @@ int tiles(int op, tmm::Args &a, const tmm::Plan &p, int64_t outputs, int dtype, 
           int64_t workspace_bytes, qmm_stream_t stream) {
   a.y = out;
   a.y_type = out_dtype;
-  a.wide = 1;
   if (int st = tmm::in_parts(a, p, outputs, workspace, workspace_bytes)) return st;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return dtype == QMM_F16 ? ragged_tiles_f16(op, a, p.shape, s) : ragged_tiles_bf16(op, a, p.shape, s);

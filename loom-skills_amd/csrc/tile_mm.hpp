@@ -55,7 +55,6 @@ struct Args {
   const float *scales;         // [rows, 2] or NULL: output row t times scales[t, 1]
   void *y;
   int y_type;                  // QMM_F32, QMM_BF16 or QMM_F16
-  int wide;                    // output rows are 16-byte aligned
   int tiles_n;
   int splits;                  // parts of the sum, one a layer of the grid (y); more than one: f32 sums [splits][outputs] into part
   float *part;
@@ -125,47 +124,45 @@ __device__ __forceinline__ void store_rows(const Args &a, float *stage, const f3
     for (int r = 0; r < 16; ++r) stage[((r & 3) + 8 * (r >> 2) + 4 * h) * kPitch + 32 * j + c] = acc[j][r];
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_wave_barrier();
-  auto row_scale = [&](int m) __attribute__((always_inline)) { return scales ? scales[2 * (int64_t)m + 1] : 1.f; };
-  if (a.wide) {
-    constexpr int LR = NJ * 4, RP = 64 / LR;   // lanes a row (8 values each), rows a pass
-#pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += RP) {
-      const int r = r0 + lane / LR, col = (lane % LR) * 8;
-      const int m = mb + r, n = nb + col;
+  constexpr int LR = NJ * 4, RP = 64 / LR;   // lanes a row (8 values each), rows a pass
+  const int n = nb + (lane % LR) * 8;
+  auto store = [&](auto *y) __attribute__((always_inline)) {
+    using T = std::remove_reference_t<decltype(*y)>;
+    auto pass = [&](int r0, auto whole) __attribute__((always_inline)) {
+      const int r = r0 + lane / LR, m = mb + r;
       if (m < m_end && n < a.N) {
-        const f32x4 v0 = *reinterpret_cast<const f32x4 *>(stage + r * kPitch + col);
-        const f32x4 v1 = *reinterpret_cast<const f32x4 *>(stage + r * kPitch + col + 4);
-        const float sc = row_scale(m);
-        const int64_t at = out0 + (int64_t)m * a.N + n;
-        if (a.y_type == QMM_F32) {
-          f32x4 *o = reinterpret_cast<f32x4 *>(static_cast<float *>(a.y) + at);
-          o[0] = v0 * sc;
-          o[1] = v1 * sc;
-        } else if (a.y_type == QMM_BF16) {
-          bf16x8 b;
+        const f32x4 *const from = reinterpret_cast<const f32x4 *>(stage + r * kPitch + (lane % LR) * 8);
+        const float sc = scales ? scales[2 * (int64_t)m + 1] : 1.f;
+        const f32x4 v0 = from[0] * sc, v1 = from[1] * sc;
+        T *const to = y + out0 + (int64_t)m * a.N + n;
+        if (decltype(whole)::value || n + 8 <= a.N) {   // 16-byte stores at any address: the GPU's memory takes them
+          if constexpr (sizeof(T) == 4) {
+            __builtin_memcpy(to, &v0, 16);
+            __builtin_memcpy(to + 4, &v1, 16);
+          } else {
+            typedef __attribute__((ext_vector_type(8))) T T8;
+            T8 o;
 #pragma unroll
-          for (int x = 0; x < 8; ++x) b[x] = (__bf16)((x < 4 ? v0[x] : v1[x - 4]) * sc);
-          *reinterpret_cast<bf16x8 *>(static_cast<__bf16 *>(a.y) + at) = b;
+            for (int x = 0; x < 8; ++x) o[x] = (T)(x < 4 ? v0[x] : v1[x - 4]);
+            __builtin_memcpy(to, &o, 16);
+          }
         } else {
-          f16x8 b;
-#pragma unroll
-          for (int x = 0; x < 8; ++x) b[x] = (_Float16)((x < 4 ? v0[x] : v1[x - 4]) * sc);
-          *reinterpret_cast<f16x8 *>(static_cast<_Float16 *>(a.y) + at) = b;
+#pragma unroll 1
+          for (int x = 0; n + x < a.N; ++x) to[x] = (T)(stage[r * kPitch + (lane % LR) * 8 + x] * sc);
         }
       }
+    };
+    if (nb + 32 * NJ <= a.N) {
+#pragma unroll
+      for (int r0 = 0; r0 < 32; r0 += RP) pass(r0, std::true_type{});
+    } else {
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += RP) pass(r0, std::false_type{});
     }
-  } else {
-    for (int v = lane; v < 32 * 32 * NJ; v += 64) {
-      const int r = v / (32 * NJ), m = mb + r, n = nb + v % (32 * NJ);
-      if (m < m_end && n < a.N) {
-        const float o = stage[r * kPitch + v % (32 * NJ)] * row_scale(m);
-        const int64_t at = out0 + (int64_t)m * a.N + n;
-        if (a.y_type == QMM_F32) static_cast<float *>(a.y)[at] = o;
-        else if (a.y_type == QMM_BF16) static_cast<__bf16 *>(a.y)[at] = (__bf16)o;
-        else static_cast<_Float16 *>(a.y)[at] = (_Float16)o;
-      }
-    }
-  }
+  };
+  if (a.y_type == QMM_F32) store(static_cast<float *>(a.y));
+  else if (a.y_type == QMM_BF16) store(static_cast<__bf16 *>(a.y));
+  else store(static_cast<_Float16 *>(a.y));
 }
 
 template <int SRC>
@@ -204,7 +201,8 @@ __device__ __forceinline__ void to_part(Args &a, int64_t outputs) {
 }
 
 // The P parts added in order, the rows scaled and rounded: a workgroup a tile of 16 rows x 64 columns (by the segments, so that rows
-// of no expert stay as they are) or, without offsets, of all rows; a thread four columns of a row, its loads all in flight.
+// of no expert stay as they are) or, without offsets, of all rows; a thread four columns of a row, its loads all in
+// flight.
 constexpr int kJoinRows = 16, kJoinCols = 64;
 template <int P>
 static __global__ __launch_bounds__(256) void join_kernel(Args a, int64_t outputs) {
@@ -218,8 +216,8 @@ static __global__ __launch_bounds__(256) void join_kernel(Args a, int64_t output
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const float *src = a.part + p * outputs + at;
-    if (a.wide) {
-      part[p] = *reinterpret_cast<const f32x4 *>(src);
+    if (own == 4) {
+      __builtin_memcpy(&part[p], src, 16);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) part[p][i] = src[min(i, own - 1)];
@@ -227,15 +225,21 @@ static __global__ __launch_bounds__(256) void join_kernel(Args a, int64_t output
   }
 #pragma unroll
   for (int p = 0; p < P; ++p) v += part[p];
-  const float sc = a.scales ? a.scales[2 * (int64_t)(lo + m) + 1] : 1.f;
+  v *= a.scales ? a.scales[2 * (int64_t)(lo + m) + 1] : 1.f;
+  auto store = [&](auto *y) __attribute__((always_inline)) {
+    using T = std::remove_reference_t<decltype(*y)>;
+    const T o[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    if (own == 4) {
+      __builtin_memcpy(y + at, o, sizeof(o));
+    } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i >= own) break;
-    const float o = v[i] * sc;
-    if (a.y_type == QMM_F32) static_cast<float *>(a.y)[at + i] = o;
-    else if (a.y_type == QMM_BF16) static_cast<__bf16 *>(a.y)[at + i] = (__bf16)o;
-    else static_cast<_Float16 *>(a.y)[at + i] = (_Float16)o;
-  }
+      for (int i = 0; i < 3; ++i)
+        if (i < own) y[at + i] = o[i];
+    }
+  };
+  if (a.y_type == QMM_F32) store(static_cast<float *>(a.y));
+  else if (a.y_type == QMM_BF16) store(static_cast<__bf16 *>(a.y));
+  else store(static_cast<_Float16 *>(a.y));
 }
 // row tiles that offsets may give at most
 inline int64_t most_row_tiles(const Args &a, int bm) {

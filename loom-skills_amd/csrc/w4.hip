@@ -98,7 +98,6 @@ tmm::Args tile_args(int64_t rows, int64_t k, int64_t n, int64_t group, int E, co
   a.y = y;
   a.y_type = y_dtype;
   a.N = (int)N;
-  a.wide = N % 8 == 0 && aligned(y, 16);
   a.splits = 1;
   return a;
 }

@@ -307,3 +307,17 @@ def test_larger_tiles_of_the_weight_gradient(dev, counts, n, k, dtype):
     for e, (a, b) in enumerate(zip(at, at[1:])):
         xd, dd = x[a:b].double(), dy[a:b].double().t().contiguous()
         held(dw.t[e], torch.mm(dd, xd).cpu(), (b - a + 16) * U * torch.mm(dd.abs(), xd.abs()).cpu(), f"expert {e}")
+
+
+@pytest.mark.parametrize("rows,n,k", [(130, 264, 96), (130, 261, 96), (5, 40, 64), (90, 67, 8192)])   # the last: a sum in parts
+@pytest.mark.parametrize("shift", [1, 3, 7])
+def test_bf16_outputs_at_any_address(dev, rows, n, k, shift):
+    raw = w4_raw(gen(n), n, k, 32)
+    w, ws = packed(raw, 32, dev)
+    x = torch.randn((rows, k), generator=gen(rows)).bfloat16().to(dev)
+    x16, scales = ops.row_scale_f16(x) if rows > 64 else (x, None)
+    want = ops.w4_mm(x16, w, ws, n, k, 32, scales=scales, out_dtype=torch.bfloat16)
+    buf = torch.full((rows * n + 16,), 3.0, dtype=torch.bfloat16, device=dev)
+    y = buf[shift:shift + rows * n].view(rows, n)
+    ops.w4_mm(x16, w, ws, n, k, 32, scales=scales, y=y)
+    assert torch.equal(y, want) and (buf[:shift] == 3).all() and (buf[shift + rows * n:] == 3).all()
