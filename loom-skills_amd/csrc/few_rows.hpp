@@ -13,6 +13,7 @@
 // Memory bounds a row or two (12288 x 4096 7.6 us for 26.8 MB, 3.5 TB/s), the f32 rows' split and the fragments' reads more rows (16 f32
 // rows 17 us, 63 44 us): eight waves share a row block along K because a wave's chain of loads is what a small call waits for.
 #pragma once
+#include <algorithm>
 #include <type_traits>
 
 #include "ragged.hpp"
@@ -35,6 +36,8 @@ struct Args {
   int groups, gshift;       // group of 32-value step i: min(i >> gshift, groups - 1)
   void *y;
   int y_bytes;              // 4: f32; 2: bf16 (w4) or the weights' type
+  int parts = 1;            // of K, blocks of the grid's x one after the other; more than one: f32 sums [parts][rows][n] into part
+  float *part = nullptr;
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, u32 bytes) {
@@ -100,7 +103,8 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 || RB > 2 ? 2 : F32 || RB > 1 |
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, h = lane >> 4, part = wave % KS;
   const int KT = (a.k + 127) >> 7, nb = (a.n + 15) >> 4;
-  const int rb0 = (int)blockIdx.x * kBlocks;
+  const int groups = (nb + kBlocks - 1) / kBlocks, piece = (int)blockIdx.x / groups, rb0 = ((int)blockIdx.x - piece * groups) * kBlocks;
+  const int T0 = (int)((int64_t)KT * piece / a.parts), T1 = (int)((int64_t)KT * (piece + 1) / a.parts);   // this piece's tiles
   int e = 0, lo = 0, hi = a.rows;
   if (a.offsets && !nth_segment(a.offsets, a.E, a.rows, blockIdx.y, e, lo, hi)) return;
   const u8 *w[RB];
@@ -152,7 +156,7 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 || RB > 2 ? 2 : F32 || RB > 1 |
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int t = min(tb + KS * u, KT - 1);
+          const int t = min(tb + KS * u, T1 - 1);
 #pragma unroll
           for (int r = 0; r < RB; ++r) {
             if constexpr (W == kW4) {
@@ -191,7 +195,7 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 || RB > 2 ? 2 : F32 || RB > 1 |
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int t = tb + KS * u;
-          if (t >= KT) break;
+          if (t >= T1) break;
           u32x4 xv[TT][4][kLds ? 1 : kLoads];
           if constexpr (!kLds) {
 #pragma unroll
@@ -262,7 +266,7 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 || RB > 2 ? 2 : F32 || RB > 1 |
         }
       };
       Batch b;
-      for (int tb = part; tb < KT; tb += KS * U) {
+      for (int tb = T0 + part; tb < T1; tb += KS * U) {
         load(tb, b);
         use(tb, b);
       }
@@ -271,7 +275,8 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 || RB > 2 ? 2 : F32 || RB > 1 |
     auto store = [&](int token, int row, float v) __attribute__((always_inline)) {   // token of the chunk
       if (token < rows && row < a.n) {
         const int64_t at = (int64_t)(t0 + token) * a.n + row;
-        if (a.y_bytes == 4) static_cast<float *>(a.y)[at] = v;
+        if (a.parts > 1) a.part[(int64_t)piece * a.rows * a.n + at] = v;
+        else if (a.y_bytes == 4) static_cast<float *>(a.y)[at] = v;
         else if constexpr (W == kWF16) static_cast<_Float16 *>(a.y)[at] = (_Float16)v;
         else static_cast<__bf16 *>(a.y)[at] = (__bf16)v;
       }
@@ -301,7 +306,7 @@ int launch(const Args &a, int slots, hipStream_t s) {
   const int per = 16 * kWaves / KS * RB, blocks = (a.n + per - 1) / per;
   const int most = (a.rows + kRows - 1) / kRows;   // chunks of a segment that holds all rows
   const int chunks = a.offsets ? max(1, min(most / 4, 2048 / (blocks * slots))) : min(most, 65535);
-  few_rows_kernel<W, F32, GS, TT, KS, TL, RB><<<dim3((unsigned)blocks, slots, (unsigned)chunks), dim3(64 * kWaves), 0, s>>>(a);
+  few_rows_kernel<W, F32, GS, TT, KS, TL, RB><<<dim3((unsigned)(blocks * a.parts), slots, (unsigned)chunks), dim3(64 * kWaves), 0, s>>>(a);
   return launch_status();
 }
 // us in a graph on inputs out of cache. x in LDS (TL) against fragments from memory: one dense row, w4 12288 x 4096 7.6 against 9.7,
@@ -339,6 +344,18 @@ int launch_tt(const Args &a, hipStream_t s) {
     }
   }
   return launch_rb<W, F32, GS, 1>(a, avg, slots, s);
+}
+
+// In how many parts K is taken, where the row blocks leave most CUs without work and a wave's chain of tiles is long (by us a tile as
+// measured at K = 4096). us without and with: 31 f32 rows 150 x 12128 43 and 11, 63 f32 rows 1024 x 8192 58 and 21, 2048 x 4096 32 and
+// 21, 5 f32 rows 512 x 12288 15.6 and 8.2, 32 bf16 rows 512 x 12288 24 and 10; the host takes 4 more a call.
+inline int parts_of(int64_t rows, int64_t n, int64_t k, int E, bool f32) {
+  const int64_t slots = std::min<int64_t>(E, rows), avg = (rows + slots - 1) / slots, blocks = (n + 15) / 16 * slots;
+  if (avg <= 1 || avg > 64) return 1;
+  const float tiles = (float)k / (128.f * kWaves), us = tiles * (f32 ? 2.4f : 1.1f) * (avg <= 16 ? 1.f : avg <= 32 ? 1.7f : 3.3f);
+  int p = 1;
+  while (p < 16 && blocks * 2 * p <= 256 && tiles >= 2.f * p && us / p > 10.f) p *= 2;
+  return p;
 }
 
 }  // namespace few

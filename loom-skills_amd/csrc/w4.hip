@@ -131,7 +131,9 @@ extern "C" int qmm_w4_pack(int E, int64_t n, int64_t k, int64_t group, const uin
 
 extern "C" int64_t qmm_w4_mm_workspace_size(int64_t rows, int64_t k, int64_t n, int E, int x_dtype) {
   if (!sizes_ok(rows, k, n, E)) return -1;
-  return x_dtype == QMM_F16 && rows ? tmm::part_bytes(w4_gemm_plan(rows, E, n, k), rows * n) : 0;
+  if (!rows) return 0;
+  if (x_dtype == QMM_F16) return tmm::part_bytes(w4_gemm_plan(rows, E, n, k), rows * n);
+  return tmm::part_bytes({0, few::parts_of(rows, n, k, E, x_dtype == QMM_F32)}, rows * n);
 }
 extern "C" int64_t qmm_w4_mm_t_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
   if (!sizes_ok(rows, k, n, E)) return -1;
@@ -154,10 +156,16 @@ extern "C" int qmm_w4_mm(int64_t rows, int64_t k, int64_t n, int64_t group, int 
     if (int st = in_parts(a, p, rows * n, workspace, workspace_bytes)) return st;
     return w4_gemm(a, p.shape, group_steps(k, group), s);
   }
-  const few::Args a{offsets, E, (int)rows, (int)n, (int)k, static_cast<const u8 *>(x), static_cast<const u8 *>(w),
-                    blocks(n) * tiles(k) * 1024, static_cast<const u32 *>(ws), (int)groups_of(k, group),
-                    group_shift(k, group), y, y_dtype == QMM_F32 ? 4 : 2};
-  return w4_few(a, x_dtype == QMM_F32, group_steps(k, group), s);
+  few::Args a{offsets, E, (int)rows, (int)n, (int)k, static_cast<const u8 *>(x), static_cast<const u8 *>(w),
+              blocks(n) * tiles(k) * 1024, static_cast<const u32 *>(ws), (int)groups_of(k, group),
+              group_shift(k, group), y, y_dtype == QMM_F32 ? 4 : 2};
+  tmm::Args join = tile_args(rows, k, n, group, E, offsets, x, nullptr, w, ws, y, y_dtype, n);
+  const tmm::Plan p = {0, few::parts_of(rows, n, k, E, x_dtype == QMM_F32)};
+  if (int st = in_parts(join, p, rows * n, workspace, workspace_bytes)) return st;
+  a.parts = p.splits;
+  a.part = join.part;
+  if (int st = w4_few(a, x_dtype == QMM_F32, group_steps(k, group), s)) return st;
+  return p.splits > 1 ? tmm::launch_join(join, rows, rows * n, s) : QMM_OK;
 }
 
 extern "C" int qmm_w4_mm_t(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_t *offsets, const void *x,

@@ -1231,6 +1231,9 @@ def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=No
         hold, x16, work, sp = _operand_and_workspace(x.device, rows, k, need)
         _lib.call("qmm_row_scale_f16", rows, k, xp, code, sp, x16, None, s)
         xp, code = x16, DTYPE["f16"]
+    elif rows > 1:
+        hold, need = _workspace("qmm_w4_mm_workspace_size", x.device, rows, k, n, E, code)
+        work = None if hold is None else hold.data_ptr()
     _lib.call("qmm_w4_mm", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), xp, code, sp, w.data_ptr(),
               ws.data_ptr(), y.data_ptr(), _DT[y.dtype], work, need, s)
     return y

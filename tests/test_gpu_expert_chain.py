@@ -321,3 +321,24 @@ def test_bf16_outputs_at_any_address(dev, rows, n, k, shift):
     y = buf[shift:shift + rows * n].view(rows, n)
     ops.w4_mm(x16, w, ws, n, k, 32, scales=scales, y=y)
     assert torch.equal(y, want) and (buf[:shift] == 3).all() and (buf[shift + rows * n:] == 3).all()
+
+
+@pytest.mark.parametrize("counts,first,tail,n,k,group,x_type,out", [
+    ([31], 0, 0, 150, 12128, 64, "f32", "bf16"), ([63], 0, 0, 64, 4096, 32, "f32", "f32"), ([32], 0, 0, 33, 12288, 128, "bf16", "f32"),
+    ([5], 0, 0, 17, 12288, 1 << 20, "f32", "f32"), ([20, 0, 11], 2, 3, 40, 12288, 128, "f32", "f32"), ([31, 30], 0, 1, 24, 8192, 64, "f32", "bf16")])
+def test_few_rows_in_parts(dev, counts, first, tail, n, k, group, x_type, out):
+    from qmm import _lib
+    T = {"f32": torch.float32, "bf16": torch.bfloat16}
+    rows, E, g = first + sum(counts) + tail, len(counts), gen(n + k)
+    assert _lib.load().qmm_w4_mm_workspace_size(rows, k, n, E, ops._DT[T[x_type]]) >= 2 * rows * n * 4
+    offsets = offsets_of(counts, first)
+    raw = w4_raw(g, n, k, group, True, E)
+    w, ws = packed(raw, group, dev)
+    x = torch.randn((rows, k), generator=g).to(T[x_type])
+    x[:first], x[rows - tail:] = float("nan"), float("nan")
+    for _ in range(2):
+        y = Guarded((rows, n), T[out], dev)
+        ops.w4_mm(x.to(dev), w, ws, n, k, group, offsets=offsets.to(dev), y=y.t)
+        y.check(kept=((0, first), (rows - tail, rows)))
+        live = slice(first, rows - tail)
+        held(y.t[live], by_expert(x.double(), raw[3], offsets)[live], (k + 8) * U * by_expert(x.double().abs(), raw[4], offsets)[live], "few rows in parts")
