@@ -518,7 +518,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 // is the workgroups that a CU gets times (turns along the sum times a turn's time + a start and end), or what one workgroup alone
 // takes if that is more, and the parts' way through memory. A shape's figures (us a turn over the workgroups that share a CU on
 // launches that fill the chip, their start and end, a turn of one workgroup on a CU) are those with which the choice comes closest
-// to the fastest of all shapes and parts, measured on 600 calls of 2e8 to 2e11 operations: 2 to 3.5 % slower than it on average.
+// to the fastest of all shapes and parts, measured on 800 calls of 1e8 to 2e11 operations: 2 to 3.5 % slower than it on average.
 struct Shape {
   int bm, bn;
   float turn, ends, alone;
