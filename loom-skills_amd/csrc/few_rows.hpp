@@ -84,8 +84,8 @@ __device__ __forceinline__ Parts split(u32x4 a, u32x4 b) {
 
 // W: the weights; F32: rows x are f32 (w4 only), else 16-bit; GS: 32-value steps a scale covers within a 128-value tile; TT:
 // tiles of 16 tokens at a time; KS: waves that share 16-row blocks of W, each with every KS-th 128-value tile; RB: blocks of a wave
-// (a workgroup has 8 RB / KS); TL: rows of x a wave keeps in LDS. Grid: (row blocks, experts with rows, layers that share a
-// segment's chunks of tokens: all chunks of a dense call; by expert as many as leave few workgroups without one, for a router that
+// (a workgroup has 8 RB / KS); TL: rows of x a wave keeps in LDS. Grid: (row blocks of each part of K, experts with rows, layers that
+// share a segment's chunks of tokens: all chunks of a dense call; by expert as many as leave few workgroups without one, for a router that
 // sends most rows to one expert).
 //
 // x: up to TL rows are brought into the wave's own LDS, a batch of U tiles at a time and 8 values a lane (f32 rows split into

@@ -19,7 +19,7 @@ CASES = [  # counts, rows before, rows behind, n, k, type, output
     ([300, 520], 0, 0, 264, 136, "bf16", "f32"),
     ([0, 700, 1, 90], 1, 7, 520, 328, "bf16", "bf16"),
     ([200] * 5, 0, 0, 384, 512, "f16", "f32"),
-    # past 2^30 products the forward takes tiles: 64 x 128, 128 x 128, 256 x 128, 256 x 256
+    # thousands of rows
     ([30, 0, 31, 90, 1, 28] * 17, 3, 2, 600, 616, "bf16", "f32"),
     ([1100, 0, 903], 0, 0, 1032, 520, "bf16", "bf16"),
     ([4000, 4101], 0, 5, 1000, 200, "f16", "f32"),

@@ -70,6 +70,12 @@ def test_w4_mm_statuses(lib):   # noqa: F811
     assert back(rows=80, k=64, n=8192, work=ODD, wb=back_need) == st["QMM_ERR_ALIGN"]
     for xd in (Q8, MXFP8, -1):
         assert mm(xd=xd) == st["QMM_ERR_DTYPE"]
+    # few rows whose row blocks leave CUs without work: K in parts too
+    few = lib.qmm_w4_mm_workspace_size(31, 12288, 64, 1, F32)
+    assert few >= 2 * 31 * 64 * 4 and lib.qmm_w4_mm_workspace_size(1, 12288, 64, 1, F32) == 0
+    for bad in (dict(), dict(work=at(), wb=few - 1)):
+        assert mm(rows=31, k=12288, n=64, xd=F32, **bad) == st["QMM_ERR_WORKSPACE"], bad
+    assert mm(rows=31, k=12288, n=64, xd=F32, work=ODD, wb=few) == st["QMM_ERR_ALIGN"]
 
 
 def test_ragged_statuses(lib):   # noqa: F811
