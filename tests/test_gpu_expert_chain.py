@@ -342,3 +342,62 @@ def test_few_rows_in_parts(dev, counts, first, tail, n, k, group, x_type, out):
         y.check(kept=((0, first), (rows - tail, rows)))
         live = slice(first, rows - tail)
         held(y.t[live], by_expert(x.double(), raw[3], offsets)[live], (k + 8) * U * by_expert(x.double().abs(), raw[4], offsets)[live], "few rows in parts")
+
+
+# 64 x 256, 128 x 128 and 128 x 256 tiles, one turn of K and several with an odd end
+@pytest.mark.parametrize("counts,n,k", [([11761], 781, 32), ([16389], 523, 32), ([19801], 519, 32), ([9000, 7, 7402], 551, 32),
+                                        ([9000, 0, 7803], 645, 32), ([12655], 389, 416), ([19008], 259, 416), ([1540], 7828, 416)])
+def test_larger_tiles_of_the_four_bit_product(dev, counts, n, k):
+    g, rows, E = gen(n + k), sum(counts) + 5, len(counts)
+    offsets = offsets_of(counts, 2)
+    raw = w4_raw(g, n, k, 64, True, E)
+    w, ws = packed(raw, 64, dev)
+    x = torch.randn((rows, k), generator=g).bfloat16().to(dev)
+    x16, scales = ops.row_scale_f16(x)
+    x16[:2], x16[-3:] = float("nan"), float("inf")
+    y = Guarded((rows, n), torch.float32, dev)
+    ops.w4_mm(x16, w, ws, n, k, 64, offsets=offsets.to(dev), scales=scales, y=y.t)
+    y.check(kept=((0, 2), (rows - 3, rows)))
+    wd, xd, od = raw[3].to(dev), x16.double() * scales.double()[:, 1:], offsets.to(dev)
+    held(y.t[2:-3], by_expert(xd, wd, od)[2:-3], ((2.0 ** -11 + k * U) * by_expert(xd.abs(), wd.abs(), od))[2:-3], "4-bit tiles")
+
+
+# two and three row blocks a wave, the last workgroup with fewer, one to four tiles of tokens
+@pytest.mark.parametrize("rows,n,k,group", [(2, 4200, 160, 32), (9, 4121, 288, 64), (20, 4200, 416, 1 << 20), (40, 4137, 160, 64), (5, 8300, 160, 128),
+                                            (16, 8211, 288, 32), (31, 8300, 96, 64), (63, 8227, 160, 32)])
+@pytest.mark.parametrize("x_type", ["bf16", "f32"])
+def test_few_rows_of_many_columns(dev, rows, n, k, group, x_type):
+    g, t = gen(rows + n), {"bf16": torch.bfloat16, "f32": torch.float32}[x_type]
+    raw = w4_raw(g, n, k, group)
+    w, ws = packed(raw, group, dev)
+    x = torch.randn((rows, k), generator=g).to(t)
+    y = Guarded((rows, n), torch.float32, dev)
+    ops.w4_mm(x.to(dev), w, ws, n, k, group, y=y.t)
+    y.check()
+    held(y.t, x.double() @ raw[3].t(), (k + 8) * U * (x.double().abs() @ raw[4].t()), "few rows, many columns")
+
+
+@pytest.mark.parametrize("E,most,n,k,group", [(256, 1, 170, 160, 32), (256, 1, 170, 288, 128), (40, 3, 136, 160, 64), (100, 4, 150, 96, 32), (60, 40, 200, 128, 64),
+                                              (90, 90, 130, 160, 1 << 20)])
+@pytest.mark.parametrize("x_type", ["bf16", "f32"])
+def test_few_rows_of_many_experts(dev, E, most, n, k, group, x_type):
+    g, t = gen(E + n), {"bf16": torch.bfloat16, "f32": torch.float32}[x_type]
+    counts = [int(c) for c in torch.randint(0, most + 1, (E,), generator=g)]
+    if most == 1:
+        counts = [1 if i % 8 else 0 for i in range(E)]
+        counts[3], counts[9] = 0, 2
+    rows, offsets = sum(counts) + 3, offsets_of(counts, 1)
+    raw = w4_raw(g, n, k, group, True, E)
+    w, ws = packed(raw, group, dev)
+    x = torch.randn((rows, k), generator=g).to(t)
+    x[0], x[rows - 2:] = float("inf"), float("nan")
+    y = Guarded((rows, n), torch.float32, dev)
+    from qmm import _lib
+    od, xd = offsets.to(dev), x.to(dev)
+    need = _lib.load().qmm_w4_mm_workspace_size(rows, k, n, E, ops._DT[t])
+    work = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    _lib.call("qmm_w4_mm", rows, k, n, group, E, od.data_ptr(), xd.data_ptr(), ops._DT[t], None, w.data_ptr(), ws.data_ptr(), y.t.data_ptr(),
+              ops._DT[torch.float32], work.data_ptr(), need, ops._stream())   # few rows, whatever the number that the Python call would take
+    y.check(kept=((0, 1), (rows - 2, rows)))
+    live = slice(1, rows - 2)
+    held(y.t[live], by_expert(x.double(), raw[3], offsets)[live], (k + 8) * U * by_expert(x.double().abs(), raw[4], offsets)[live], "few rows, many experts")
