@@ -1283,21 +1283,31 @@ def _ragged_out(y, shape, out_dtype, x, reads, what):
     return y
 
 
+def _ragged_call(name, rows, k, n, E, offsets, p, q, out, s):
+    """One of the three products, its workspace allocated: p, q its inputs of one type, out its output."""
+    work, need = _workspace(name + "_workspace_size", out.device, rows, k, n, E)
+    _lib.call(name, rows, k, n, E, offsets.data_ptr(), p.data_ptr(), q.data_ptr(), _DT[p.dtype], out.data_ptr(), _DT[out.dtype],
+              None if work is None else work.data_ptr(), need, s)
+    return out
+
+
+def _rows_of(t, width, dtype, what):
+    """The number of rows of t [rows, width] of that type."""
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != width or t.dtype != dtype:
+        raise ValueError(f"{what} is {t.dtype} {tuple(shape)}, expected {dtype} [rows, {width}]")
+    return shape[0]
+
+
 def ragged_mm(x, offsets, w, y=None, out_dtype=None):
     """y[t] = W_e x[t] for rows sorted by expert, offsets[e] .. offsets[e + 1] - 1 (i32 [E + 1] on the device) being expert e's
     (qmm_ragged_mm). x [rows, k] and w [E, n, k] bf16 or f16 alike, n % 8 == 0, k % 8 == 0; y [rows, n] of that type or f32
     (out_dtype). Rows of no expert are left as they were in y."""
     s = _here(x, offsets, w, y)
     E, n, k = _ragged_weights(offsets, w)
-    if x.dim() != 2:
-        raise ValueError(f"x is {tuple(x.shape)}, expected [rows, {k}]")
-    rows = x.shape[0]
-    _shaped(x, (rows, k), (w.dtype,), "x")
+    rows = _rows_of(x, k, w.dtype, "x")
     y = _ragged_out(y, (rows, n), out_dtype, x, (x, offsets, w), "y")
-    work, need = _workspace("qmm_ragged_mm_workspace_size", x.device, rows, k, n, E)
-    _lib.call("qmm_ragged_mm", rows, k, n, E, offsets.data_ptr(), x.data_ptr(), w.data_ptr(), _DT[w.dtype], y.data_ptr(),
-              _DT[y.dtype], None if work is None else work.data_ptr(), need, s)
-    return y
+    return _ragged_call("qmm_ragged_mm", rows, k, n, E, offsets, x, w, y, s)
 
 
 def ragged_mm_t(dy, offsets, w, dx=None, out_dtype=None):
@@ -1305,15 +1315,9 @@ def ragged_mm_t(dy, offsets, w, dx=None, out_dtype=None):
     [rows, k] of that type or f32. Rows of no expert are left as they were in dx."""
     s = _here(dy, offsets, w, dx)
     E, n, k = _ragged_weights(offsets, w)
-    if dy.dim() != 2:
-        raise ValueError(f"dy is {tuple(dy.shape)}, expected [rows, {n}]")
-    rows = dy.shape[0]
-    _shaped(dy, (rows, n), (w.dtype,), "dy")
+    rows = _rows_of(dy, n, w.dtype, "dy")
     dx = _ragged_out(dx, (rows, k), out_dtype, dy, (dy, offsets, w), "dx")
-    work, need = _workspace("qmm_ragged_mm_t_workspace_size", dy.device, rows, k, n, E)
-    _lib.call("qmm_ragged_mm_t", rows, k, n, E, offsets.data_ptr(), dy.data_ptr(), w.data_ptr(), _DT[w.dtype], dx.data_ptr(),
-              _DT[dx.dtype], None if work is None else work.data_ptr(), need, s)
-    return dx
+    return _ragged_call("qmm_ragged_mm_t", rows, k, n, E, offsets, dy, w, dx, s)
 
 
 def ragged_mm_dw(dy, x, offsets, dw=None, out_dtype=None):
@@ -1328,15 +1332,19 @@ def ragged_mm_dw(dy, x, offsets, dw=None, out_dtype=None):
     n = dy.shape[1]
     _shaped(dy, (rows, n), (x.dtype,), "dy")
     dw = _ragged_out(dw, (E, n, k), out_dtype, x, (x, dy, offsets), "dw")
-    work, need = _workspace("qmm_ragged_mm_dw_workspace_size", x.device, rows, k, n, E)
-    _lib.call("qmm_ragged_mm_dw", rows, k, n, E, offsets.data_ptr(), dy.data_ptr(), x.data_ptr(), _DT[x.dtype], dw.data_ptr(),
-              _DT[dw.dtype], None if work is None else work.data_ptr(), need, s)
-    return dw
+    return _ragged_call("qmm_ragged_mm_dw", rows, k, n, E, offsets, dy, x, dw, s)
 
 
 def ragged_mm_backward(dy, x, offsets, w, out_dtype=None, dw_dtype=None):
-    """The gradients of ragged_mm at dy: (dx, dw) of out_dtype and dw_dtype (w's type, or f32)."""
-    return ragged_mm_t(dy, offsets, w, out_dtype=out_dtype), ragged_mm_dw(dy, x, offsets, out_dtype=dw_dtype)
+    """The gradients of ragged_mm at dy: (dx, dw) of out_dtype and dw_dtype (w's type, or f32), as ragged_mm_t and ragged_mm_dw."""
+    s = _here(dy, x, offsets, w)
+    E, n, k = shape = _ragged_weights(offsets, w)
+    rows = _rows_of(dy, n, w.dtype, "dy")
+    if _rows_of(x, k, w.dtype, "x") != rows:
+        raise ValueError(f"x has {x.shape[0]} rows, dy {rows}")
+    dx, dw = _ragged_out(None, (rows, k), out_dtype, dy, (), "dx"), _ragged_out(None, shape, dw_dtype, dy, (), "dw")
+    return (_ragged_call("qmm_ragged_mm_t", rows, k, n, E, offsets, dy, w, dx, s),
+            _ragged_call("qmm_ragged_mm_dw", rows, k, n, E, offsets, dy, x, dw, s))
 
 
 def moe_routed(fmt, x, logits, E, KU, H, FE, gating, norm, **kw):

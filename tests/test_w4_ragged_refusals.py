@@ -155,6 +155,10 @@ def test_ragged_surface(ops):   # noqa: F811
         lambda: ops.ragged_mm_t(dy[0], off, w), lambda: ops.ragged_mm_dw(dy[:3], x, off), lambda: ops.ragged_mm_dw(dy.half(), x, off),
         lambda: ops.ragged_mm_dw(dy.float(), x.float(), off), lambda: ops.ragged_mm_dw(dy[0], x, off), lambda: ops.ragged_mm_dw(dy, x, off, dw=torch.zeros(2, 64, 16)),
         lambda: ops.ragged_mm_dw(dy, x, off.float()),
+        lambda: ops.ragged_mm_backward(dy[:3], x, off, w), lambda: ops.ragged_mm_backward(dy, x[:3], off, w), lambda: ops.ragged_mm_backward(dy.half(), x, off, w),
+        lambda: ops.ragged_mm_backward(dy, x.half(), off, w), lambda: ops.ragged_mm_backward(dy, dy, off, w), lambda: ops.ragged_mm_backward(dy, x, off, w.float()),
+        lambda: ops.ragged_mm_backward(dy, x, off[:2], w), lambda: ops.ragged_mm_backward(dy, x, off, w, out_dtype=torch.float16),
+        lambda: ops.ragged_mm_backward(dy, x, off, w, dw_dtype=torch.float16), lambda: ops.ragged_mm_backward(dy[0], x, off, w),
     ]
     for i, call in enumerate(wrong):
         with pytest.raises(ValueError):
