@@ -20,8 +20,8 @@
 // The MFMAs bound a full round of 256 x 256 tiles (a step of 64 values 1.65 us on every CU: 1.30 PFLOP/s, at the clock the power limit
 // holds; a library product of 8192^3 reaches 1.55), a launch the rounds it takes and each tile's start and end (6 us: the operands'
 // first loads, 128 KB of outputs): 16384 rows of 32 experts 2880 x 2880 forward 310 us, 0.88 PFLOP/s, in four rounds, the last a
-// little over half full; their weights' gradient 384 us with eight steps a tile. Many experts of few rows are bound by memory: 8000
-// rows of 128 experts 768 x 2048, dW writes 0.8 GB in 191 us.
+// little over half full; their weights' gradient 355 us with eight steps a tile. Many experts of few rows are bound by memory: 8000
+// rows of 128 experts 768 x 2048, dW writes 0.8 GB in 144 us.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -55,6 +55,7 @@ struct Args {
   const float *scales;         // [rows, 2] or NULL: output row t times scales[t, 1]
   void *y;
   int y_type;                  // QMM_F32, QMM_BF16 or QMM_F16
+  int stream;                  // weight gradient: whole 128-byte lines a row, past what the caches hold
   int tiles_n;
   int splits;                  // parts of the sum, one a layer of the grid (y); more than one: f32 sums [splits][outputs] into part
   float *part;
@@ -112,7 +113,7 @@ __device__ __forceinline__ u32x4 dequant(u32 q, u32 sc) {
 // of a lane are one column of 16 rows, a store covers neighbouring columns. scales: of the segment's rows, or NULL.
 template <int NJ>
 constexpr int stage_pitch() { return NJ * 32 + 8; }   // floats; 4 rows apart is 32 banks apart
-template <int NJ>
+template <int NJ, bool STREAM = false>
 __device__ __forceinline__ void store_rows(const Args &a, float *stage, const f32x16 (&acc)[NJ], int64_t out0, int mb, int m_end, int nb,
                                            const float *scales, int lane) {
   constexpr int kPitch = stage_pitch<NJ>();
@@ -124,40 +125,35 @@ __device__ __forceinline__ void store_rows(const Args &a, float *stage, const f3
     for (int r = 0; r < 16; ++r) stage[((r & 3) + 8 * (r >> 2) + 4 * h) * kPitch + 32 * j + c] = acc[j][r];
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_wave_barrier();
-  constexpr int LR = NJ * 4, RP = 64 / LR;   // lanes a row (8 values each), rows a pass
-  const int n = nb + (lane % LR) * 8;
   auto store = [&](auto *y) __attribute__((always_inline)) {
     using T = std::remove_reference_t<decltype(*y)>;
+    constexpr int V = 16 / sizeof(T), L = 32 * NJ / V;   // values a lane, lanes a row: a store covers neighbouring lines
+    typedef __attribute__((ext_vector_type(V))) T TV;
+    const int col = (lane % L) * V, n = nb + col;
     auto pass = [&](int r0, auto whole) __attribute__((always_inline)) {
-      const int r = r0 + lane / LR, m = mb + r;
+      const int r = r0 + lane / L, m = mb + r;
       if (m < m_end && n < a.N) {
-        const f32x4 *const from = reinterpret_cast<const f32x4 *>(stage + r * kPitch + (lane % LR) * 8);
+        const float *const from = stage + r * kPitch + col;
         const float sc = scales ? scales[2 * (int64_t)m + 1] : 1.f;
-        const f32x4 v0 = from[0] * sc, v1 = from[1] * sc;
         T *const to = y + out0 + (int64_t)m * a.N + n;
-        if (decltype(whole)::value || n + 8 <= a.N) {   // 16-byte stores at any address: the GPU's memory takes them
-          if constexpr (sizeof(T) == 4) {
-            __builtin_memcpy(to, &v0, 16);
-            __builtin_memcpy(to + 4, &v1, 16);
-          } else {
-            typedef __attribute__((ext_vector_type(8))) T T8;
-            T8 o;
+        if (decltype(whole)::value || n + V <= a.N) {
+          TV o;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) o[x] = (T)(x < 4 ? v0[x] : v1[x - 4]);
-            __builtin_memcpy(to, &o, 16);
-          }
+          for (int x = 0; x < V; ++x) o[x] = (T)(from[x] * sc);
+          if constexpr (STREAM) __builtin_nontemporal_store(o, reinterpret_cast<TV *>(to));
+          else __builtin_memcpy(to, &o, 16);   // at any address: the GPU's memory takes them
         } else {
 #pragma unroll 1
-          for (int x = 0; n + x < a.N; ++x) to[x] = (T)(stage[r * kPitch + (lane % LR) * 8 + x] * sc);
+          for (int x = 0; n + x < a.N; ++x) to[x] = (T)(from[x] * sc);
         }
       }
     };
     if (nb + 32 * NJ <= a.N) {
 #pragma unroll
-      for (int r0 = 0; r0 < 32; r0 += RP) pass(r0, std::true_type{});
+      for (int r0 = 0; r0 < 32; r0 += 64 / L) pass(r0, std::true_type{});
     } else {
 #pragma unroll 1
-      for (int r0 = 0; r0 < 32; r0 += RP) pass(r0, std::false_type{});
+      for (int r0 = 0; r0 < 32; r0 += 64 / L) pass(r0, std::false_type{});
     }
   };
   if (a.y_type == QMM_F32) store(static_cast<float *>(a.y));
@@ -508,8 +504,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     if (i >= live) break;
-    store_rows<NJ>(a, reinterpret_cast<float *>(smem) + wave * kStage, acc[i], out0, m0 + (rb0 + i) * 32, m_end, n0 + cb0 * 32,
-                   SUM == kSumFixed && a.scales ? a.scales + 2 * (int64_t)lo : nullptr, lane);
+    float *const stage = reinterpret_cast<float *>(smem) + wave * kStage;
+    const int mb = m0 + (rb0 + i) * 32, nb = n0 + cb0 * 32;
+    if constexpr (SUM == kSumRagged) {
+      if (a.stream) store_rows<NJ, true>(a, stage, acc[i], out0, mb, m_end, nb, nullptr, lane);
+      else store_rows<NJ>(a, stage, acc[i], out0, mb, m_end, nb, nullptr, lane);
+    } else {
+      store_rows<NJ>(a, stage, acc[i], out0, mb, m_end, nb, a.scales ? a.scales + 2 * (int64_t)lo : nullptr, lane);
+    }
   }
 }
 
@@ -564,7 +566,7 @@ Plan plan_rows(const Shape (&shapes)[COUNT], int64_t rows, int E, int64_t N, int
                     [&](const Shape &t) { return expected_row_tiles(rows, E, t.bm) * ((N + t.bn - 1) / t.bn); });
 }
 // The segments cut the sum: E M N outputs, however few rows there are; the longest segment is taken as 1.4 times the average. us with
-// the shapes in turn: 16384 rows of 32 experts 2880 x 2880 380 and 462, 8000 of 128 768 x 2048 145, 159, 222, 15314 of 16 1216 x 264
+// the shapes in turn: 16384 rows of 32 experts 2880 x 2880 380 and 462, 8000 of 128 768 x 2048 into bf16 145, 159, 222, 15314 of 16 1216 x 264
 // 85, 60, 48, 2000 of two 2048 x 1024 44, 28, 21, 500 of four 1024 x 1024 12, 7, 7, 15313 of three 248 x 824 in four parts 44, 31, 26.
 constexpr Shape kTilesSum[] = {{256, 256, 1.35f, 6.8f, 1.35f}, {128, 128, 0.46f, 2.2f, 1.1f}, {128, 128, 0.52f, 5.3f, 0.57f}};
 inline Plan plan_sum(int64_t rows, int E, int64_t M, int64_t N) {

@@ -122,3 +122,25 @@ def test_long_four_bit_weights(dev):
     y = ops.w4_mm_t(x, w, ws, n, k, 128, out_dtype=torch.bfloat16)
     xd, wt = x[-300:].double(), wd.t().contiguous()
     held(y[-300:], torch.mm(xd, wt), (n * U + 2.0 ** -11) * torch.mm(xd.abs(), wt.abs()) + 1e-6)
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,k", [(1032, 2080), (1000, 4160)])   # whole lines a row in f32 (or both types), part of a tile's columns, rows
+def test_weight_gradients_past_the_cache(dev, out, n, k):
+    """Outputs past 256 MB: those of whole 128-byte lines a row are stored past the cache, at any other address as elsewhere."""
+    counts = [70, 0, 3, 130, 64, 1] * 12
+    E, rows = len(counts), sum(counts)
+    offsets = torch.tensor([0] + counts).cumsum(0).to(torch.int32)
+    x, dy = normal((rows, k)), normal((rows, n))
+    buf = torch.full((E * n * k + 512,), 3.0, dtype=out, device=DEV)
+    for first in (256, 264):   # 128-byte lines, and not
+        dw = buf[first:first + E * n * k].view(E, n, k)
+        assert dw.nbytes > 256 << 20
+        ops.ragged_mm_dw(dy, x, offsets.to(DEV), dw=dw)
+        for e in (0, 1, 2, 3, E - 1):
+            a, b = int(offsets[e]), int(offsets[e + 1])
+            dd, xd = dy[a:b].double().t().contiguous(), x[a:b].double()
+            held(dw[e], torch.mm(dd, xd), 130 * U * torch.mm(dd.abs(), xd.abs()))
+        assert not dw[1::6].any()
+        assert (buf[:first] == 3).all() and (buf[first + E * n * k:] == 3).all()
+        buf.fill_(3.0)
