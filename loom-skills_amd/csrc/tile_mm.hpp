@@ -21,7 +21,7 @@
 // holds; a library product of 8192^3 reaches 1.55), a launch the rounds it takes and each tile's start and end (6 us: the operands'
 // first loads, 128 KB of outputs): 16384 rows of 32 experts 2880 x 2880 forward 310 us, 0.88 PFLOP/s, in four rounds, the last a
 // little over half full; their weights' gradient 355 us with eight steps a tile. Many experts of few rows are bound by memory: 8000
-// rows of 128 experts 768 x 2048, dW writes 0.8 GB in 144 us.
+// rows of 128 experts 768 x 2048, dW writes 0.8 GB in 144 us, and what it no longer pushes out of the last-level cache saves dx 25.
 #pragma once
 #include <algorithm>
 #include <type_traits>
