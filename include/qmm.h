@@ -59,6 +59,9 @@ enum qmm_dtype {
   QMM_MXFP8 = 3, /* E4M3 codes + E8M0 per 32 */
   QMM_Q8 = 4     /* planar Q8_1: int8 codes [rows, K], then at byte rows*K f32 (f16-rounded d, code sum) per 32 */
 };
+/* Added to the output type of qmm_w4_mm, qmm_w4_mm_t, qmm_ragged_mm and qmm_ragged_mm_t: rows of no expert are set to zero by the same
+ * launch (they are left as they were without it). */
+#define QMM_ZERO_REST 256
 enum qmm_gemm_mode { QMM_GEMM_STORE = 0, QMM_GEMM_ACC = 1, QMM_GEMM_SWIGLU = 2 };
 /* The expert activations (QMM_ACT_SILU, QMM_ACT_SWIGLU_OAI) and those of qmm_linear and qmm_ffn_gate_up. QMM_ACT_GELU is
  * the tanh form, QMM_ACT_GELU_ERF v Phi(v). */
@@ -290,7 +293,8 @@ int64_t qmm_w4_scale_bytes(int64_t n, int64_t k, int64_t group);
 
 /* The product y[t, r] = sum_c x[t, c] W_e[r, c] on packed 4-bit weights. offsets NULL: one matrix (E = 1) for all rows; else
  * i32 [E + 1] on the device, expert e's rows being offsets[e] .. offsets[e + 1] - 1, as many as it has (offsets are clamped to
- * 0 .. rows, an expert whose end is not past its start has none; rows of no expert are not written, and no row belongs to two).
+ * 0 .. rows, an expert whose end is not past its start has none; no row belongs to two). Rows of no expert are not written, or set
+ * to zero with y_dtype | QMM_ZERO_REST.
  *   x_dtype QMM_F32 / QMM_BF16  x [rows, k]: exact products, f32 sums; for few rows an expert (weights are read once for up to
  *                               64 of them). A row that holds an infinity gives NaN or infinities. x_scales unused.
  *   x_dtype QMM_F16             the qmm_gemm operand: x16 [rows, k] with x_scales f32 [rows, 2] of qmm_row_scale_f16, or NULL;
@@ -319,8 +323,8 @@ int qmm_w4_mm_t(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const 
  *   qmm_ragged_mm_dw  dw[e, r, c] = sum_t dy[t, r] x[t, c]        over expert e's rows, zero for an expert without rows
  * offsets: i32 [E + 1] on the device, as qmm_w4_mm. dtype QMM_BF16 or QMM_F16 for x, W and dy alike; outputs QMM_F32 or that
  * type (rounded once); f32 sums in an order that follows from the sizes. x [rows, k], dy [rows, n]; n % 8 == 0, k % 8 == 0,
- * both <= 2^20, rows <= 2^24, E <= 1024; tensors 16-byte aligned. Rows of no expert are neither written (y, dx) nor read into
- * a sum (dw). Outputs overlap nothing. workspace: as qmm_w4_mm, of the call's own qmm_*_workspace_size (-1 for sizes that are not
+ * both <= 2^20, rows <= 2^24, E <= 1024; tensors 16-byte aligned. Rows of no expert are neither written (y, dx; set to zero with
+ * y_dtype or dx_dtype | QMM_ZERO_REST) nor read into a sum (dw). Outputs overlap nothing. workspace: as qmm_w4_mm, of the call's own qmm_*_workspace_size (-1 for sizes that are not
  * taken). */
 int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *x, const void *w, int dtype,
                   void *y, int y_dtype, void *workspace, int64_t workspace_bytes, qmm_stream_t stream);

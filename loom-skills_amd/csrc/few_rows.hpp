@@ -38,6 +38,7 @@ struct Args {
   int y_bytes;              // 4: f32; 2: bf16 (w4) or the weights' type
   int parts = 1;            // of K, blocks of the grid's x one after the other; more than one: f32 sums [parts][rows][n] into part
   float *part = nullptr;
+  int rest = 0;             // rows of no expert are set to zero, by one more layer of the grid's y
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, u32 bytes) {
@@ -106,6 +107,11 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 || RB > 2 ? 2 : F32 || RB > 1 |
   const int groups = (nb + kBlocks - 1) / kBlocks, piece = (int)blockIdx.x / groups, rb0 = ((int)blockIdx.x - piece * groups) * kBlocks;
   const int T0 = (int)((int64_t)KT * piece / a.parts), T1 = (int)((int64_t)KT * (piece + 1) / a.parts);   // this piece's tiles
   int e = 0, lo = 0, hi = a.rows;
+  if (a.rest && blockIdx.y == gridDim.y - 1) {
+    zero_rest(a.offsets, a.E, a.rows, static_cast<u8 *>(a.y), (int64_t)a.n * a.y_bytes, (int)(blockIdx.z * gridDim.x + blockIdx.x),
+              (int)(gridDim.x * gridDim.z));
+    return;
+  }
   if (a.offsets && !nth_segment(a.offsets, a.E, a.rows, blockIdx.y, e, lo, hi)) return;
   const u8 *w[RB];
   const u32 *ws[RB];
@@ -299,14 +305,14 @@ __global__ __launch_bounds__(64 * kWaves, TT > 1 || RB > 2 ? 2 : F32 || RB > 1 |
   }
 }
 
-// Rows behind the last segment are not written. All extents are checked by the callers.
+// All extents are checked by the callers.
 template <int W, bool F32, int GS, int TT, int KS, int TL, int RB = 1>
 int launch(const Args &a, int slots, hipStream_t s) {
   constexpr int kRows = TL > 0 ? TL : 16 * TT;
   const int per = 16 * kWaves / KS * RB, blocks = (a.n + per - 1) / per;
   const int most = (a.rows + kRows - 1) / kRows;   // chunks of a segment that holds all rows
   const int chunks = a.offsets ? max(1, min(most / 4, 2048 / (blocks * slots))) : min(most, 65535);
-  few_rows_kernel<W, F32, GS, TT, KS, TL, RB><<<dim3((unsigned)(blocks * a.parts), slots, (unsigned)chunks), dim3(64 * kWaves), 0, s>>>(a);
+  few_rows_kernel<W, F32, GS, TT, KS, TL, RB><<<dim3((unsigned)(blocks * a.parts), slots + (a.rest ? 1 : 0), (unsigned)chunks), dim3(64 * kWaves), 0, s>>>(a);
   return launch_status();
 }
 // us in a graph on inputs out of cache. x in LDS (TL) against fragments from memory: one dense row, w4 12288 x 4096 7.6 against 9.7,

@@ -37,10 +37,11 @@ bool takes_few_rows(int64_t rows, int64_t k, int64_t n) {
   return rows <= 64 && rows * k <= 1 << 17 && rows * n * k <= (int64_t)1 << 30;
 }
 
-int tiles(int op, tmm::Args &a, const tmm::Plan &p, int64_t outputs, int dtype, int out_dtype, void *out, void *workspace,
-          int64_t workspace_bytes, qmm_stream_t stream) {
+int tiles(int op, tmm::Args &a, const tmm::Plan &p, int64_t outputs, int dtype, int out_dtype, bool rest, void *out,
+          void *workspace, int64_t workspace_bytes, qmm_stream_t stream) {
   a.y = out;
   a.y_type = out_dtype;
+  if (rest) a.rest = rest_blocks(a.rows, (int64_t)a.N * (out_dtype == QMM_F32 ? 4 : 2));
   if (int st = tmm::in_parts(a, p, outputs, workspace, workspace_bytes)) return st;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return dtype == QMM_F16 ? ragged_tiles_f16(op, a, p.shape, s) : ragged_tiles_bf16(op, a, p.shape, s);
@@ -68,11 +69,13 @@ extern "C" int64_t qmm_ragged_mm_dw_workspace_size(int64_t rows, int64_t k, int6
 extern "C" int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *x, const void *w,
                              int dtype, void *y, int y_dtype, void *workspace, int64_t workspace_bytes,
                              qmm_stream_t stream) {
+  const bool rest = zero_rest_asked(y_dtype);
   if (int st = check(rows, k, n, E, offsets, x, w, dtype, rows ? y : w, y_dtype)) return st;
   if (rows == 0) return QMM_OK;
   if (takes_few_rows(rows, k, n)) {
-    const few::Args a{offsets, E, (int)rows, (int)n, (int)k, static_cast<const u8 *>(x), static_cast<const u8 *>(w),
+    few::Args a{offsets, E, (int)rows, (int)n, (int)k, static_cast<const u8 *>(x), static_cast<const u8 *>(w),
                       2 * n * k, nullptr, 0, 0, y, y_dtype == QMM_F32 ? 4 : 2};
+    a.rest = rest;
     return ragged_few(a, dtype == QMM_F16, reinterpret_cast<hipStream_t>(stream));
   }
   tmm::Args a{};
@@ -80,12 +83,13 @@ extern "C" int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const in
   a.N = (int)n, a.K = (int)k;
   a.a = static_cast<const u8 *>(x), a.a_row = 2 * k;
   a.b = static_cast<const u8 *>(w), a.b_row = 2 * k, a.b_expert = 2 * n * k;
-  return tiles(kRaggedY, a, tmm::plan_rows(tmm::kTiles, rows, E, n, k), rows * n, dtype, y_dtype, y, workspace, workspace_bytes, stream);
+  return tiles(kRaggedY, a, tmm::plan_rows(tmm::kTiles, rows, E, n, k), rows * n, dtype, y_dtype, rest, y, workspace, workspace_bytes, stream);
 }
 
 extern "C" int qmm_ragged_mm_t(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy, const void *w,
                                int dtype, void *dx, int dx_dtype, void *workspace, int64_t workspace_bytes,
                                qmm_stream_t stream) {
+  const bool rest = zero_rest_asked(dx_dtype);
   if (int st = check(rows, k, n, E, offsets, dy, w, dtype, rows ? dx : w, dx_dtype)) return st;
   if (rows == 0) return QMM_OK;
   tmm::Args a{};
@@ -93,7 +97,7 @@ extern "C" int qmm_ragged_mm_t(int64_t rows, int64_t k, int64_t n, int E, const 
   a.N = (int)k, a.K = (int)n;
   a.a = static_cast<const u8 *>(dy), a.a_row = 2 * n;
   a.b = static_cast<const u8 *>(w), a.b_row = 2 * k, a.b_expert = 2 * n * k;
-  return tiles(kRaggedDX, a, tmm::plan_rows(tmm::kTiles, rows, E, k, n), rows * k, dtype, dx_dtype, dx, workspace, workspace_bytes, stream);
+  return tiles(kRaggedDX, a, tmm::plan_rows(tmm::kTiles, rows, E, k, n), rows * k, dtype, dx_dtype, rest, dx, workspace, workspace_bytes, stream);
 }
 
 extern "C" int qmm_ragged_mm_dw(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *dy,
@@ -110,5 +114,5 @@ extern "C" int qmm_ragged_mm_dw(int64_t rows, int64_t k, int64_t n, int E, const
   const int64_t row = k * (dw_dtype == QMM_F32 ? 4 : 2);
   const tmm::Plan plan = tmm::plan_sum(rows, E, n, k);
   a.stream = plan.splits == 1 && row % 128 == 0 && aligned(dw, 128) && E * n * row > (int64_t)256 << 20;
-  return tiles(kRaggedDW, a, plan, E * n * k, dtype, dw_dtype, dw, workspace, workspace_bytes, stream);
+  return tiles(kRaggedDW, a, plan, E * n * k, dtype, dw_dtype, false, dw, workspace, workspace_bytes, stream);
 }

@@ -59,6 +59,7 @@ struct Args {
   int tiles_n;
   int splits;                  // parts of the sum, one a layer of the grid (y); more than one: f32 sums [splits][outputs] into part
   float *part;
+  int rest;                    // kSumFixed: the grid's last workgroups along x, which set the rows of no expert to zero (ragged.hpp); 0: none
 };
 
 template <int DT>
@@ -186,6 +187,14 @@ __device__ __forceinline__ bool row_tile(const Args &a, int &e, int &lo, int &hi
   nt = gt / gm;
   return true;
 }
+// whether the workgroup is one of those for the rows of no expert, which are done then
+__device__ __forceinline__ bool rest_done(const Args &a) {
+  const int part = (int)blockIdx.x - ((int)gridDim.x - a.rest);
+  if (part < 0) return false;
+  if (blockIdx.y == 0)
+    zero_rest(a.offsets, a.E, a.rows, static_cast<u8 *>(a.y), (int64_t)a.N * (a.y_type == QMM_F32 ? 4 : 2), part, a.rest);
+  return true;
+}
 // first step of part i of n
 __device__ __forceinline__ int part_of(int steps, int n, int i) { return (int)((int64_t)steps * i / n); }
 // the outputs of a sum in parts: the layer's f32 sums
@@ -258,6 +267,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 
   int e = 0, lo = 0, hi = a.rows, m0, nt;
   if constexpr (SUM == kSumFixed) {
+    if (rest_done(a)) return;
     if (!row_tile<BM>(a, e, lo, hi, m0, nt)) return;
   } else {
     // every XCD takes an eighth of every expert's tiles, one expert after the other: experts differ in their rows
@@ -610,7 +620,7 @@ int launch(const Args &in, hipStream_t s) {
   auto *fn = tile_mm_kernel<DT, SA, SB, SUM, BM, BN, WM, WN, GS, ST>;
   static std::atomic<unsigned> raised{0};
   if (int st = raise_dyn_lds(reinterpret_cast<const void *>(fn), lds, raised)) return st;
-  fn<<<dim3((unsigned)((tiles + 7) / 8 * 8), a.splits), dim3(64 * WM * WN), lds, s>>>(a);
+  fn<<<dim3((unsigned)((tiles + 7) / 8 * 8 + a.rest), a.splits), dim3(64 * WM * WN), lds, s>>>(a);
   if (int st = launch_status()) return st;
   if (a.splits == 1) return QMM_OK;
   if (SUM == kSumFixed) return launch_join(a, a.rows, (int64_t)a.rows * a.N, s);

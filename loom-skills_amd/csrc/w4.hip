@@ -70,7 +70,8 @@ __global__ void w4_scales_kernel(const u16 *scales, const u8 *zeros, u32 *ws, in
 }
 
 int check(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_t *offsets, const void *x, const void *w,
-          const void *ws, const void *y, int y_dtype) {
+          const void *ws, const void *y, int &y_dtype, int &rest) {
+  rest = zero_rest_asked(y_dtype) && offsets;
   if (!shape_ok(n, k, group) || rows < 0 || rows > kMaxRows) return QMM_ERR_SHAPE;
   if (E < 1 || E > kMaxRaggedE || (!offsets && E != 1)) return QMM_ERR_RANGE;
   if (y_dtype != QMM_F32 && y_dtype != QMM_BF16) return QMM_ERR_DTYPE;
@@ -81,7 +82,7 @@ int check(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_
 }
 
 tmm::Args tile_args(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_t *offsets, const void *x,
-                    const float *scales, const void *w, const void *ws, void *y, int y_dtype, int64_t N) {
+                    const float *scales, const void *w, const void *ws, void *y, int y_dtype, int64_t N, int rest) {
   tmm::Args a{};
   a.offsets = offsets;
   a.E = E;
@@ -99,6 +100,7 @@ tmm::Args tile_args(int64_t rows, int64_t k, int64_t n, int64_t group, int E, co
   a.y_type = y_dtype;
   a.N = (int)N;
   a.splits = 1;
+  a.rest = rest ? rest_blocks(rows, N * (y_dtype == QMM_F32 ? 4 : 2)) : 0;
   return a;
 }
 
@@ -144,12 +146,13 @@ extern "C" int qmm_w4_mm(int64_t rows, int64_t k, int64_t n, int64_t group, int 
                          int x_dtype, const float *x_scales, const void *w, const void *ws, void *y, int y_dtype,
                          void *workspace, int64_t workspace_bytes, qmm_stream_t stream) {
   if (x_dtype != QMM_F32 && x_dtype != QMM_BF16 && x_dtype != QMM_F16) return QMM_ERR_DTYPE;
-  if (int st = check(rows, k, n, group, E, offsets, x, w, ws, y, y_dtype)) return st;
+  int rest;
+  if (int st = check(rows, k, n, group, E, offsets, x, w, ws, y, y_dtype, rest)) return st;
   if (!aligned(x_scales, 4)) return QMM_ERR_ALIGN;
   if (rows == 0) return QMM_OK;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (x_dtype == QMM_F16) {
-    tmm::Args a = tile_args(rows, k, n, group, E, offsets, x, x_scales, w, ws, y, y_dtype, n);
+    tmm::Args a = tile_args(rows, k, n, group, E, offsets, x, x_scales, w, ws, y, y_dtype, n, rest);
     a.a_row = 2 * k;
     a.K = (int)k;
     const tmm::Plan p = w4_gemm_plan(rows, E, n, k);
@@ -159,11 +162,12 @@ extern "C" int qmm_w4_mm(int64_t rows, int64_t k, int64_t n, int64_t group, int 
   few::Args a{offsets, E, (int)rows, (int)n, (int)k, static_cast<const u8 *>(x), static_cast<const u8 *>(w),
               blocks(n) * tiles(k) * 1024, static_cast<const u32 *>(ws), (int)groups_of(k, group),
               group_shift(k, group), y, y_dtype == QMM_F32 ? 4 : 2};
-  tmm::Args join = tile_args(rows, k, n, group, E, offsets, x, nullptr, w, ws, y, y_dtype, n);
+  tmm::Args join = tile_args(rows, k, n, group, E, offsets, x, nullptr, w, ws, y, y_dtype, n, 0);
   const tmm::Plan p = {0, few::parts_of(rows, n, k, E, x_dtype == QMM_F32)};
   if (int st = in_parts(join, p, rows * n, workspace, workspace_bytes)) return st;
   a.parts = p.splits;
   a.part = join.part;
+  a.rest = rest;
   if (int st = w4_few(a, x_dtype == QMM_F32, group_steps(k, group), s)) return st;
   return p.splits > 1 ? tmm::launch_join(join, rows, rows * n, s) : QMM_OK;
 }
@@ -171,11 +175,12 @@ extern "C" int qmm_w4_mm(int64_t rows, int64_t k, int64_t n, int64_t group, int 
 extern "C" int qmm_w4_mm_t(int64_t rows, int64_t k, int64_t n, int64_t group, int E, const int32_t *offsets, const void *x,
                            const float *scales, const void *w, const void *ws, void *y, int y_dtype, void *workspace,
                            int64_t workspace_bytes, qmm_stream_t stream) {
-  if (int st = check(rows, k, n, group, E, offsets, x, w, ws, y, y_dtype)) return st;
+  int rest;
+  if (int st = check(rows, k, n, group, E, offsets, x, w, ws, y, y_dtype, rest)) return st;
   if (rows && !scales) return QMM_ERR_NULL;
   if (!aligned(scales, 4)) return QMM_ERR_ALIGN;
   if (rows == 0) return QMM_OK;
-  tmm::Args a = tile_args(rows, k, n, group, E, offsets, x, scales, w, ws, y, y_dtype, k);
+  tmm::Args a = tile_args(rows, k, n, group, E, offsets, x, scales, w, ws, y, y_dtype, k, rest);
   a.K = (int)((n + 63) / 64 * 64);
   a.a_row = 2 * (int64_t)a.K;
   const tmm::Plan p = tmm::plan_rows(tmm::kTilesW4, rows, E, k, n);

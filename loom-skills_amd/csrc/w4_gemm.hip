@@ -27,6 +27,7 @@ __global__ __launch_bounds__(256, NI * NJ == 2 ? 4 : 2) void w4_gemm_kernel(Args
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
   int e = 0, lo = 0, hi = a.rows, m0, nt;
+  if (rest_done(a)) return;
   if (!row_tile<kRows>(a, e, lo, hi, m0, nt)) return;
   const int n0 = nt * 128 * NJ + wave * 32 * NJ, rows = min(kRows, max(hi - lo, 0) - m0), T = (a.K + 127) >> 7;
   const int T0 = part_of(T, a.splits, blockIdx.y), T1 = part_of(T, a.splits, blockIdx.y + 1);   // this layer's turns
@@ -143,7 +144,7 @@ int launch_one(const Args &in, hipStream_t s) {
   auto *fn = w4_gemm_kernel<NI, NJ, GS>;
   static std::atomic<unsigned> raised{0};
   if (int st = raise_dyn_lds(reinterpret_cast<const void *>(fn), lds, raised)) return st;
-  fn<<<dim3((unsigned)((tiles + 7) / 8 * 8), a.splits), dim3(256), lds, s>>>(a);
+  fn<<<dim3((unsigned)((tiles + 7) / 8 * 8 + a.rest), a.splits), dim3(256), lds, s>>>(a);
   if (int st = launch_status()) return st;
   return a.splits == 1 ? QMM_OK : launch_join(a, a.rows, (int64_t)a.rows * a.N, s);
 }

@@ -1148,6 +1148,10 @@ def w4_pack(codes, scales, zeros=None, group=128):
     return w, ws
 
 
+# QMM_ZERO_REST added to the type of an output that a call makes: rows of no expert, which it would leave as they were, are zero then
+_ZERO_REST = 256
+
+
 def _segments(offsets):
     """The number of experts that offsets [E + 1] separate (None: one matrix for all rows)."""
     if offsets is None:
@@ -1204,7 +1208,7 @@ def _operand_and_workspace(dev, rows, width, need):
 
 def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=None):
     """y = x W^T on weights of w4_pack (qmm_w4_mm): one matrix, or with offsets (i32 [E + 1] on the device) the matrix of
-    expert e for rows offsets[e] .. offsets[e + 1] - 1; rows of no expert are left as they were in y. x f32 / bf16 [rows, k],
+    expert e for rows offsets[e] .. offsets[e + 1] - 1; rows of no expert are zero, or left as they were in a given y. x f32 / bf16 [rows, k],
     multiplied exactly where the rows are few (with an f32 x or y: below 64, or up to four an expert) and through row_scale_f16
     and weights rounded to f16 where they are many; or the f16 operand [rows, k] with its scales f32 [rows, 2] (or None).
     y [rows, n] f32 or bf16 (out_dtype)."""
@@ -1215,6 +1219,7 @@ def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=No
     if len(shape) != 2 or shape[1] != k:
         raise ValueError(f"x is {tuple(shape)}, expected [rows, {k}]")
     rows, dtype = shape[0], x.dtype
+    rest = _ZERO_REST if y is None and offsets is not None else 0
     y = _rows_out(y, (rows, n), out_dtype, x, (x, w, ws, offsets, scales))
     xp, code, sp, work, need = x.data_ptr(), _DT.get(dtype), None, None, 0
     if dtype == torch.float16:
@@ -1235,13 +1240,13 @@ def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=No
         hold, need = _workspace("qmm_w4_mm_workspace_size", x.device, rows, k, n, E, code)
         work = None if hold is None else hold.data_ptr()
     _lib.call("qmm_w4_mm", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), xp, code, sp, w.data_ptr(),
-              ws.data_ptr(), y.data_ptr(), _DT[y.dtype], work, need, s)
+              ws.data_ptr(), y.data_ptr(), _DT[y.dtype] | rest, work, need, s)
     return y
 
 
 def w4_mm_t(dy, w, ws, n, k, group, offsets=None, y=None, out_dtype=None):
     """dx = dy W, the input gradient of w4_mm at dy (f32 / bf16 [rows, n]) with frozen weights (qmm_grad_operand, qmm_w4_mm_t);
-    offsets as w4_mm. dx [rows, k] f32 or bf16 (out_dtype, or y)."""
+    offsets and rows of no expert as w4_mm. dx [rows, k] f32 or bf16 (out_dtype, or y)."""
     s = _here(dy, w, ws, offsets, y)
     E = _segments(offsets)
     _w4_weights(w, ws, n, k, group, E)
@@ -1249,6 +1254,7 @@ def w4_mm_t(dy, w, ws, n, k, group, offsets=None, y=None, out_dtype=None):
         raise ValueError(f"dy is {tuple(dy.shape)}, expected [rows, {n}]")
     rows = dy.shape[0]
     _shaped(dy, (rows, n), _VALUE, "dy")
+    rest = _ZERO_REST if y is None and offsets is not None else 0
     y = _rows_out(y, (rows, k), out_dtype, dy, (dy, w, ws, offsets))
     if rows == 0:
         return y
@@ -1256,7 +1262,7 @@ def w4_mm_t(dy, w, ws, n, k, group, offsets=None, y=None, out_dtype=None):
     hold, x16, work, scales = _operand_and_workspace(dy.device, rows, -(-n // 64) * 64, need)
     _lib.call("qmm_grad_operand", rows, 1, n, dy.data_ptr(), _DT[dy.dtype], x16, scales, s)
     _lib.call("qmm_w4_mm_t", rows, k, n, group, E, None if offsets is None else offsets.data_ptr(), x16, scales, w.data_ptr(),
-              ws.data_ptr(), y.data_ptr(), _DT[y.dtype], work, need, s)
+              ws.data_ptr(), y.data_ptr(), _DT[y.dtype] | rest, work, need, s)
     return y
 
 
@@ -1283,10 +1289,10 @@ def _ragged_out(y, shape, out_dtype, x, reads, what):
     return y
 
 
-def _ragged_call(name, rows, k, n, E, offsets, p, q, out, s):
-    """One of the three products, its workspace allocated: p, q its inputs of one type, out its output."""
+def _ragged_call(name, rows, k, n, E, offsets, p, q, out, s, rest=0):
+    """One of the three products, its workspace allocated: p, q its inputs of one type, out its output, rest added to its type."""
     work, need = _workspace(name + "_workspace_size", out.device, rows, k, n, E)
-    _lib.call(name, rows, k, n, E, offsets.data_ptr(), p.data_ptr(), q.data_ptr(), _DT[p.dtype], out.data_ptr(), _DT[out.dtype],
+    _lib.call(name, rows, k, n, E, offsets.data_ptr(), p.data_ptr(), q.data_ptr(), _DT[p.dtype], out.data_ptr(), _DT[out.dtype] | rest,
               None if work is None else work.data_ptr(), need, s)
     return out
 
@@ -1302,22 +1308,24 @@ def _rows_of(t, width, dtype, what):
 def ragged_mm(x, offsets, w, y=None, out_dtype=None):
     """y[t] = W_e x[t] for rows sorted by expert, offsets[e] .. offsets[e + 1] - 1 (i32 [E + 1] on the device) being expert e's
     (qmm_ragged_mm). x [rows, k] and w [E, n, k] bf16 or f16 alike, n % 8 == 0, k % 8 == 0; y [rows, n] of that type or f32
-    (out_dtype). Rows of no expert are left as they were in y."""
+    (out_dtype). Rows of no expert are zero, or left as they were in a given y."""
     s = _here(x, offsets, w, y)
     E, n, k = _ragged_weights(offsets, w)
     rows = _rows_of(x, k, w.dtype, "x")
+    rest = _ZERO_REST if y is None else 0
     y = _ragged_out(y, (rows, n), out_dtype, x, (x, offsets, w), "y")
-    return _ragged_call("qmm_ragged_mm", rows, k, n, E, offsets, x, w, y, s)
+    return _ragged_call("qmm_ragged_mm", rows, k, n, E, offsets, x, w, y, s, rest)
 
 
 def ragged_mm_t(dy, offsets, w, dx=None, out_dtype=None):
     """dx[t] = W_e^T dy[t], the gradient of ragged_mm with respect to x (qmm_ragged_mm_t): dy [rows, n] of w's type, dx
-    [rows, k] of that type or f32. Rows of no expert are left as they were in dx."""
+    [rows, k] of that type or f32. Rows of no expert are zero, or left as they were in a given dx."""
     s = _here(dy, offsets, w, dx)
     E, n, k = _ragged_weights(offsets, w)
     rows = _rows_of(dy, n, w.dtype, "dy")
+    rest = _ZERO_REST if dx is None else 0
     dx = _ragged_out(dx, (rows, k), out_dtype, dy, (dy, offsets, w), "dx")
-    return _ragged_call("qmm_ragged_mm_t", rows, k, n, E, offsets, dy, w, dx, s)
+    return _ragged_call("qmm_ragged_mm_t", rows, k, n, E, offsets, dy, w, dx, s, rest)
 
 
 def ragged_mm_dw(dy, x, offsets, dw=None, out_dtype=None):
@@ -1336,14 +1344,15 @@ def ragged_mm_dw(dy, x, offsets, dw=None, out_dtype=None):
 
 
 def ragged_mm_backward(dy, x, offsets, w, out_dtype=None, dw_dtype=None):
-    """The gradients of ragged_mm at dy: (dx, dw) of out_dtype and dw_dtype (w's type, or f32), as ragged_mm_t and ragged_mm_dw."""
+    """The gradients of ragged_mm at dy: (dx, dw) of out_dtype and dw_dtype (w's type, or f32), as ragged_mm_t and ragged_mm_dw; dx
+    of a row of no expert is zero."""
     s = _here(dy, x, offsets, w)
     E, n, k = shape = _ragged_weights(offsets, w)
     rows = _rows_of(dy, n, w.dtype, "dy")
     if _rows_of(x, k, w.dtype, "x") != rows:
         raise ValueError(f"x has {x.shape[0]} rows, dy {rows}")
     dx, dw = _ragged_out(None, (rows, k), out_dtype, dy, (), "dx"), _ragged_out(None, shape, dw_dtype, dy, (), "dw")
-    return (_ragged_call("qmm_ragged_mm_t", rows, k, n, E, offsets, dy, w, dx, s),
+    return (_ragged_call("qmm_ragged_mm_t", rows, k, n, E, offsets, dy, w, dx, s, _ZERO_REST),
             _ragged_call("qmm_ragged_mm_dw", rows, k, n, E, offsets, dy, x, dw, s))
 
 

@@ -178,3 +178,21 @@ def test_good_calls_reach_the_library(ops):   # noqa: F811
                  lambda: ops.ragged_mm_dw(torch.zeros(4, 16).bfloat16(), x.bfloat16(), off)):
         with pytest.raises(AssertionError, match="was reached"):
             call()
+
+
+def test_rows_of_no_expert_flag(lib):   # noqa: F811
+    """QMM_ZERO_REST comes with the types that a call takes; the weights' gradient has no such rows."""
+    import re
+    from test_abi import HEADER
+    from qmm import ops
+    rest = int(re.search(r"#define QMM_ZERO_REST (\d+)", open(HEADER).read()).group(1))
+    st = header_enum("qmm_status")
+    assert ops._ZERO_REST == rest
+    for yd, good in ((F32, True), (BF16, True), (F16, False), (Q8, False), (-1, False), (2 * rest, False)):
+        want = 0 if good else st["QMM_ERR_DTYPE"]
+        assert lib.qmm_w4_mm(0, 64, 8, 32, 2, at(), None, BF16, None, None, None, None, yd | rest, None, 0, None) == want
+        assert lib.qmm_w4_mm_t(0, 64, 8, 32, 2, at(), None, None, None, None, None, yd | rest, None, 0, None) == want
+        for fn in (lib.qmm_ragged_mm, lib.qmm_ragged_mm_t):
+            assert fn(0, 64, 8, 2, at(), None, at(), BF16, None, yd | rest, None, 0, None) == want
+    assert lib.qmm_w4_mm(0, 64, 8, 32, 1, None, None, BF16, None, None, None, None, F32 | rest, None, 0, None) == 0
+    assert lib.qmm_ragged_mm_dw(4, 64, 8, 2, at(), at(), at(), BF16, at(), F32 | rest, None, 0, None) == st["QMM_ERR_DTYPE"]
