@@ -296,7 +296,7 @@ int64_t qmm_w4_scale_bytes(int64_t n, int64_t k, int64_t group);
  * 0 .. rows, an expert whose end is not past its start has none; no row belongs to two). Rows of no expert are not written, or set
  * to zero with y_dtype | QMM_ZERO_REST.
  *   x_dtype QMM_F32 / QMM_BF16  x [rows, k]: exact products, f32 sums; for few rows an expert (weights are read once for up to
- *                               64 of them). A row that holds an infinity gives NaN or infinities. x_scales unused.
+ *                               64 of them). Any finite rows; one that holds an infinity gives NaN or infinities. x_scales unused.
  *   x_dtype QMM_F16             the qmm_gemm operand: x16 [rows, k] with x_scales f32 [rows, 2] of qmm_row_scale_f16, or NULL;
  *                               weights enter as f16(s (q - z)) (one rounding; finite for |s| <= 4366), f32 sums.
  * y: [rows, n] of y_dtype, QMM_F32 or QMM_BF16 (rounded once). x, w, ws 16-byte aligned; rows <= 2^24. y overlaps nothing.
