@@ -297,7 +297,8 @@ int64_t qmm_w4_scale_bytes(int64_t n, int64_t k, int64_t group);
  * to zero with y_dtype | QMM_ZERO_REST.
  *   x_dtype QMM_F32 / QMM_BF16  x [rows, k]: exact products, f32 sums; for few rows an expert (weights are read once for up to
  *                               64 of them). Any finite rows; one that holds an infinity gives NaN or infinities. x_scales unused.
- *   x_dtype QMM_F16             the qmm_gemm operand: x16 [rows, k] with x_scales f32 [rows, 2] of qmm_row_scale_f16, or NULL;
+ *   x_dtype QMM_F16             the qmm_gemm operand: x16 [rows, k] with x_scales f32 [rows, 2] of qmm_row_scale_f16 or
+ *                               qmm_row_scale_f16_wide, or NULL;
  *                               weights enter as f16(s (q - z)) (one rounding; finite for |s| <= 4366), f32 sums.
  * y: [rows, n] of y_dtype, QMM_F32 or QMM_BF16 (rounded once). x, w, ws 16-byte aligned; rows <= 2^24. y overlaps nothing.
  * workspace: at least qmm_w4_mm_workspace_size bytes, 16-byte aligned (NULL where that is 0): f32 sums of parts of K, added in
@@ -506,6 +507,10 @@ int qmm_moe_grouped_mxfp8(int fmt, int fused, int act, int E, int KU, int64_t ma
  * (QMM_F32 as the reference, or QMM_BF16). This is the A operand qmm_gemm takes. */
 int qmm_row_scale_f16(int64_t rows, int64_t k, const void *x, int x_dtype, float *scales, void *x16,
                       const int32_t *tile_info, qmm_stream_t stream);
+
+/* qmm_row_scale_f16 with e = clamp(exponent(max|x|) - 13, -126, 114): rows of any finite size are brought to 2^13 .. 2^14 and keep
+ * f16's eleven bits, where the reference's clamp leaves a row below 2^-14 among f16's subnormals and one past 2^116 infinite. */
+int qmm_row_scale_f16_wide(int64_t rows, int64_t k, const void *x, int x_dtype, float *scales, void *x16, qmm_stream_t stream);
 
 /* qmm_row_scale_f16 over listed rows only: for i < n, row rows[i] (skipped when < 0) of x [.., k] is scaled and
  * written where qmm_row_scale_f16 writes it (x16 / scales at that row). With the bucket's pos as the list these are

@@ -32,6 +32,7 @@ SIGNATURES = {
     "qmm_grad_operand": [c_i64, c_int, c_i64, c_vp, c_int, c_vp, c_vp, c_vp],
     "qmm_gemm_t": [c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_i64, c_vp],
     "qmm_gemm_t_workspace_size": [c_int, c_i64, c_i64, c_i64, c_int],
+    "qmm_row_scale_f16_wide": [c_i64, c_i64, c_vp, c_int, c_vp, c_vp, c_vp],
     "qmm_w4_pack": [c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp],
     "qmm_w4_bytes": [c_i64, c_i64],
     "qmm_w4_scale_bytes": [c_i64, c_i64, c_i64],

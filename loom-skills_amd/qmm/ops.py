@@ -1209,8 +1209,8 @@ def _operand_and_workspace(dev, rows, width, need):
 def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=None):
     """y = x W^T on weights of w4_pack (qmm_w4_mm): one matrix, or with offsets (i32 [E + 1] on the device) the matrix of
     expert e for rows offsets[e] .. offsets[e + 1] - 1; rows of no expert are zero, or left as they were in a given y. x f32 / bf16 [rows, k],
-    multiplied exactly where the rows are few (with an f32 x or y: below 64, or up to four an expert) and through row_scale_f16
-    and weights rounded to f16 where they are many; or the f16 operand [rows, k] with its scales f32 [rows, 2] (or None).
+    multiplied exactly where the rows are few (with an f32 x or y: below 64, or up to four an expert) and through a power of two
+    a row to f16 (qmm_row_scale_f16_wide) and weights rounded to f16 where they are many; or the f16 operand [rows, k] with its scales f32 [rows, 2] (or None).
     y [rows, n] f32 or bf16 (out_dtype)."""
     s = _here(x, w, ws, offsets, scales, y)
     E = 1 if offsets is None else _segments(offsets)
@@ -1234,7 +1234,7 @@ def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=No
     elif not _w4_few(rows, n, k, E, dtype == torch.float32 or y.dtype == torch.float32):
         need = _workspace_bytes("qmm_w4_mm_workspace_size", rows, k, n, E, DTYPE["f16"])
         hold, x16, work, sp = _operand_and_workspace(x.device, rows, k, need)
-        _lib.call("qmm_row_scale_f16", rows, k, xp, code, sp, x16, None, s)
+        _lib.call("qmm_row_scale_f16_wide", rows, k, xp, code, sp, x16, s)
         xp, code = x16, DTYPE["f16"]
     elif rows > 1:
         hold, need = _workspace("qmm_w4_mm_workspace_size", x.device, rows, k, n, E, code)
