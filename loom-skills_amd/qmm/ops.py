@@ -1153,11 +1153,9 @@ _ZERO_REST = 256
 
 
 def _segments(offsets):
-    """The number of experts that offsets [E + 1] separate (None: one matrix for all rows)."""
-    if offsets is None:
-        return 1
-    if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.numel() < 2:
-        raise ValueError(f"offsets are i32 [E + 1], not {offsets.dtype} {tuple(offsets.shape)}")
+    """The number of experts that offsets [E + 1] separate."""
+    if offsets is None or offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.numel() < 2:
+        raise ValueError("offsets are i32 [E + 1], not " + ("None" if offsets is None else f"{offsets.dtype} {tuple(offsets.shape)}"))
     return offsets.numel() - 1
 
 
@@ -1248,7 +1246,7 @@ def w4_mm_t(dy, w, ws, n, k, group, offsets=None, y=None, out_dtype=None):
     """dx = dy W, the input gradient of w4_mm at dy (f32 / bf16 [rows, n]) with frozen weights (qmm_grad_operand, qmm_w4_mm_t);
     offsets and rows of no expert as w4_mm. dx [rows, k] f32 or bf16 (out_dtype, or y)."""
     s = _here(dy, w, ws, offsets, y)
-    E = _segments(offsets)
+    E = 1 if offsets is None else _segments(offsets)
     _w4_weights(w, ws, n, k, group, E)
     if dy.dim() != 2:
         raise ValueError(f"dy is {tuple(dy.shape)}, expected [rows, {n}]")

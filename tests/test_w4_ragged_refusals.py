@@ -196,3 +196,12 @@ def test_rows_of_no_expert_flag(lib):   # noqa: F811
             assert fn(0, 64, 8, 2, at(), None, at(), BF16, None, yd | rest, None, 0, None) == want
     assert lib.qmm_w4_mm(0, 64, 8, 32, 1, None, None, BF16, None, None, None, None, F32 | rest, None, 0, None) == 0
     assert lib.qmm_ragged_mm_dw(4, 64, 8, 2, at(), at(), at(), BF16, at(), F32 | rest, None, 0, None) == st["QMM_ERR_DTYPE"]
+
+
+def test_ragged_products_need_offsets(ops):   # noqa: F811
+    """None means one matrix for all rows to the 4-bit products alone."""
+    x, dy, w = torch.zeros(4, 64).bfloat16(), torch.zeros(4, 16).bfloat16(), torch.zeros(1, 16, 64).bfloat16()
+    for call in (lambda: ops.ragged_mm(x, None, w), lambda: ops.ragged_mm_t(dy, None, w), lambda: ops.ragged_mm_dw(dy, x, None),
+                 lambda: ops.ragged_mm_backward(dy, x, None, w)):
+        with pytest.raises(ValueError, match="offsets"):
+            call()
