@@ -22,8 +22,7 @@ int64_t groups_of(int64_t k, int64_t group) { return (k + group - 1) / group; }
 // a group is 32 2^i values, or whole rows
 bool shape_ok(int64_t n, int64_t k, int64_t group) {
   if (n <= 0 || n > kMaxSide || k <= 0 || k > kMaxSide || k % 32) return false;
-  if (group < k && (group < 32 || (group & (group - 1)) != 0)) return false;
-  return blocks(n) * groups_of(k, group) * 64 < (int64_t)1 << 31;   // the scale words have 32-bit offsets
+  return group >= k || (group >= 32 && (group & (group - 1)) == 0);
 }
 // 32-value step i lies in group i >> shift
 int group_shift(int64_t k, int64_t group) {

@@ -1123,9 +1123,9 @@ def _w4_sizes(n, k, group):
     """(bytes of a packed matrix, bytes of its scale words), as qmm_w4_bytes and qmm_w4_scale_bytes."""
     blocks, groups = (n + 15) // 16, -(-k // group) if group > 0 else 0
     if not (0 < n <= 1 << 20 and 0 < k <= 1 << 20 and k % 32 == 0 and groups
-            and (group >= k or (group >= 32 and group & (group - 1) == 0)) and blocks * groups < 1 << 25):
-        raise ValueError(f"4-bit weights have K % 32 == 0 and groups of 32, 64, 128, ... values or whole rows, not [{n}, {k}] "
-                         f"in groups of {group}")
+            and (group >= k or (group >= 32 and group & (group - 1) == 0))):
+        raise ValueError(f"4-bit weights have K % 32 == 0, up to 2^20 rows and values and groups of 32, 64, 128, ... values or whole "
+                         f"rows, not [{n}, {k}] in groups of {group}")
     return blocks * ((k + 127) // 128) * 1024, blocks * groups * 64
 
 

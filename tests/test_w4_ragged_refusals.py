@@ -180,6 +180,16 @@ def test_good_calls_reach_the_library(ops):   # noqa: F811
             call()
 
 
+def test_w4_scale_words_past_31_bits(lib, ops):   # noqa: F811
+    """2^20 rows of 16384 values in groups of 32: 2^31 bytes of scale words."""
+    n, k, group = 1 << 20, 16384, 32
+    assert lib.qmm_w4_scale_bytes(n, k, group) == 1 << 31 and lib.qmm_w4_bytes(n, k) == 1 << 33
+    assert lib.qmm_w4_scale_bytes(1 << 20, 1 << 20, 32) == 1 << 37 and lib.qmm_w4_scale_bytes((1 << 20) + 1, k, group) == -1
+    assert ops._w4_sizes(n, k, group) == (1 << 33, 1 << 31)
+    st = header_enum("qmm_status")
+    assert lib.qmm_w4_pack(1, n, k, group, None, None, None, None, None, None) == st["QMM_ERR_NULL"]
+
+
 def test_rows_of_no_expert_flag(lib):   # noqa: F811
     """QMM_ZERO_REST comes with the types that a call takes; the weights' gradient has no such rows."""
     import re
