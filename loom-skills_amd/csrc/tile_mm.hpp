@@ -59,7 +59,7 @@ struct Args {
   int tiles_n;
   int splits;                  // parts of the sum, one a layer of the grid (y); more than one: f32 sums [splits][outputs] into part
   float *part;
-  int rest;                    // kSumFixed: the grid's last workgroups along x, which set the rows of no expert to zero (ragged.hpp); 0: none
+  int rest;                    // kSumFixed: the layer's last workgroups, which set the rows of no expert to zero (ragged.hpp); 0: none
 };
 
 template <int DT>
@@ -168,6 +168,15 @@ __device__ __forceinline__ int chunk_swizzle(int row) {
   else return ((row & 3) << 2) ^ ((row >> 2) & 3);
 }
 
+// The workgroup among those of a layer of the sum (the grid's y). HIP refuses 2^32 threads along a grid's dimension: what passes 2^21
+// workgroups lies along z.
+__device__ __forceinline__ int workgroup() { return (int)(blockIdx.z * gridDim.x + blockIdx.x); }
+inline dim3 tile_grid(int64_t tiles, int rest, int layers) {
+  const int64_t n = (tiles + 7) / 8 * 8 + rest, x = std::min<int64_t>(n, 1 << 21);
+  return dim3((unsigned)x, (unsigned)layers, (unsigned)((n + x - 1) / x));
+}
+constexpr int64_t kMaxTiles = 1 << 30;   // more have outputs that no card holds
+
 // The workgroup's output tile where the segments cut A's rows: expert, segment, first row in it, column tile; false for a workgroup
 // too many. Workgroup i runs on XCD i % 8, which takes a contiguous range of tiles: an expert's in groups of kGroupM row tiles,
 // rows fastest, so that the tiles that an XCD works on at a time share operands in its L2.
@@ -176,8 +185,8 @@ __device__ __forceinline__ bool row_tile(const Args &a, int &e, int &lo, int &hi
   TileScan sc{(a.rows + BM - 1) / BM, 0, 1};
   if (a.offsets) sc = scan_tiles<BM>(a.offsets, a.E, a.rows);
   const int total = sc.total * a.tiles_n, per = (total + 7) >> 3;
-  const int i = (int)(blockIdx.x >> 3);
-  int t = (int)(blockIdx.x & 7) * per + i, first = 0;
+  const int i = workgroup() >> 3;
+  int t = (workgroup() & 7) * per + i, first = 0;
   if (i >= per || t >= total) return false;
   if (a.offsets) find_tile<BM>(a.offsets, a.E, a.rows, sc, t / a.tiles_n, e, lo, hi, first);
   t -= first * a.tiles_n;
@@ -189,7 +198,7 @@ __device__ __forceinline__ bool row_tile(const Args &a, int &e, int &lo, int &hi
 }
 // whether the workgroup is one of those for the rows of no expert, which are done then
 __device__ __forceinline__ bool rest_done(const Args &a) {
-  const int part = (int)blockIdx.x - ((int)gridDim.x - a.rest);
+  const int part = workgroup() - ((int)(gridDim.x * gridDim.z) - a.rest);
   if (part < 0) return false;
   if (blockIdx.y == 0)
     zero_rest(a.offsets, a.E, a.rows, static_cast<u8 *>(a.y), (int64_t)a.N * (a.y_type == QMM_F32 ? 4 : 2), part, a.rest);
@@ -272,9 +281,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
   } else {
     // every XCD takes an eighth of every expert's tiles, one expert after the other: experts differ in their rows
     const int tiles_m = (a.M + BM - 1) / BM, per_e = tiles_m * a.tiles_n, per = (per_e + 7) >> 3;
-    const int i = (int)(blockIdx.x >> 3);
+    const int i = workgroup() >> 3;
     e = i / per;
-    const int r = (int)(blockIdx.x & 7) * per + i - e * per;
+    const int r = (workgroup() & 7) * per + i - e * per;
     if (e >= a.E || r >= per_e) return;
     m0 = (r % tiles_m) * BM;
     nt = r / tiles_m;
@@ -599,8 +608,8 @@ inline int launch_join(const Args &in, int64_t rows, int64_t outputs, hipStream_
   a.tiles_n = (a.N + kJoinCols - 1) / kJoinCols;
   a.rows = (int)rows;
   const int64_t tiles = most_row_tiles(a, kJoinRows) * a.tiles_n;
-  if (tiles > (1 << 22)) return QMM_ERR_SHAPE;
-  const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
+  if (tiles > kMaxTiles) return QMM_ERR_SHAPE;
+  const dim3 grid = tile_grid(tiles, 0, 1);
   switch (a.splits) {
     case 2: join_kernel<2><<<grid, dim3(256), 0, s>>>(a, outputs); break;
     case 4: join_kernel<4><<<grid, dim3(256), 0, s>>>(a, outputs); break;
@@ -615,12 +624,12 @@ int launch(const Args &in, hipStream_t s) {
   Args a = in;
   a.tiles_n = (a.N + BN - 1) / BN;
   const int64_t tiles = SUM == kSumRagged ? ((int64_t)((a.M + BM - 1) / BM) * a.tiles_n + 7) / 8 * 8 * a.E : most_row_tiles(a, BM) * a.tiles_n;
-  if (tiles > (1 << 22)) return QMM_ERR_SHAPE;   // HIP refuses 2^32 threads along a grid's dimension
+  if (tiles > kMaxTiles) return QMM_ERR_SHAPE;
   constexpr int lds = ST * (BM + BN) * 128;
   auto *fn = tile_mm_kernel<DT, SA, SB, SUM, BM, BN, WM, WN, GS, ST>;
   static std::atomic<unsigned> raised{0};
   if (int st = raise_dyn_lds(reinterpret_cast<const void *>(fn), lds, raised)) return st;
-  fn<<<dim3((unsigned)((tiles + 7) / 8 * 8 + a.rest), a.splits), dim3(64 * WM * WN), lds, s>>>(a);
+  fn<<<tile_grid(tiles, a.rest, a.splits), dim3(64 * WM * WN), lds, s>>>(a);
   if (int st = launch_status()) return st;
   if (a.splits == 1) return QMM_OK;
   if (SUM == kSumFixed) return launch_join(a, a.rows, (int64_t)a.rows * a.N, s);

@@ -139,12 +139,12 @@ int launch_one(const Args &in, hipStream_t s) {
   Args a = in;
   a.tiles_n = (a.N + 128 * NJ - 1) / (128 * NJ);
   const int64_t tiles = most_row_tiles(a, 32 * NI) * a.tiles_n;
-  if (tiles > (1 << 22)) return QMM_ERR_SHAPE;
+  if (tiles > kMaxTiles) return QMM_ERR_SHAPE;
   constexpr int stage = 4 * 32 * stage_pitch<NJ>() * 4, x = 2 * 32 * NI * 256, lds = stage > x ? stage : x;
   auto *fn = w4_gemm_kernel<NI, NJ, GS>;
   static std::atomic<unsigned> raised{0};
   if (int st = raise_dyn_lds(reinterpret_cast<const void *>(fn), lds, raised)) return st;
-  fn<<<dim3((unsigned)((tiles + 7) / 8 * 8 + a.rest), a.splits), dim3(256), lds, s>>>(a);
+  fn<<<tile_grid(tiles, a.rest, a.splits), dim3(256), lds, s>>>(a);
   if (int st = launch_status()) return st;
   return a.splits == 1 ? QMM_OK : launch_join(a, a.rows, (int64_t)a.rows * a.N, s);
 }
