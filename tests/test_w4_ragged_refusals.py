@@ -215,3 +215,9 @@ def test_ragged_products_need_offsets(ops):   # noqa: F811
                  lambda: ops.ragged_mm_backward(dy, x, None, w)):
         with pytest.raises(ValueError, match="offsets"):
             call()
+
+
+def test_exact_products_take_no_operand(ops):   # noqa: F811
+    w, ws = w4()
+    with pytest.raises(ValueError, match="exact"):
+        ops.w4_mm(torch.zeros(80, 64).half(), w, ws, 8, 64, 32, exact=True)
