@@ -353,32 +353,29 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
       lds_load16(resource(bp + (int64_t)s * 64 * b_row, min(64, K - 64 * s) * b_row - n0 * 2), boff[i], dst);
   };
 
-  // ---- w4: unit u of a step is a lane's 16 bytes of a 16-row x 128-value tile. Rows and tiles past the end read the last ones:
-  // their outputs are not stored, and in the sum A is zero there.
-  constexpr int kAll = BN * 2, kUnits = (kAll + NT - 1) / NT;   // units of a step, of a thread
+  // ---- w4: unit tid of a step's 2 BN is a lane's 16 bytes of a 16-row x 128-value tile. Rows and tiles past the end read the last
+  // ones: their outputs are not stored, and in the sum A is zero there.
+  static_assert(!kW4 || 2 * BN <= NT, "a unit a thread");
   constexpr int kScales = 4 / GS;
-  u32 cw[kUnits][4], cs[kUnits][kScales];
+  u32 cw[4], cs[kScales];
   auto load_w4 = [&](int s) __attribute__((always_inline)) {
+    const int l = tid & 63, b = tid >> 6;
+    const int rb = min(4 * s + (b & 3), a.w_blocks - 1), t = min((n0 >> 7) + (b >> 2), a.w_tiles - 1);
+    const u32x4 v = *reinterpret_cast<const u32x4 *>(bp + ((int64_t)rb * a.w_tiles + t) * 1024 + 16 * l);
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const int u = i * NT + tid, l = u & 63, b = u >> 6;
-      const int rb = min(4 * s + (b & 3), a.w_blocks - 1), t = min((n0 >> 7) + (b >> 2), a.w_tiles - 1);
-      const u32x4 v = *reinterpret_cast<const u32x4 *>(bp + ((int64_t)rb * a.w_tiles + t) * 1024 + 16 * l);
+    for (int j = 0; j < 4; ++j) cw[j] = v[j];
+    const u32 *sp = a.ws + ((int64_t)e * a.w_blocks + rb) * a.groups * 16 + (l & 15);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) cw[i][j] = v[j];
-      const u32 *sp = a.ws + ((int64_t)e * a.w_blocks + rb) * a.groups * 16 + (l & 15);
-#pragma unroll
-      for (int g = 0; g < kScales; ++g) cs[i][g] = sp[min((4 * t + GS * g) >> a.gshift, a.groups - 1) * 16];
-    }
+    for (int g = 0; g < kScales; ++g) cs[g] = sp[min((4 * t + GS * g) >> a.gshift, a.groups - 1) * 16];
   };
-  auto store_w4 = [&](int s, int i) __attribute__((always_inline)) {
-    const int u = i * NT + tid, l = u & 63, b = u >> 6;
-    if (kAll % NT && u >= kAll) return;
+  auto store_w4 = [&](int s) __attribute__((always_inline)) {
+    const int l = tid & 63, b = tid >> 6;
+    if (2 * BN < NT && tid >= 2 * BN) return;
     u8 *out = smem + 2 * kA + (s & 1) * kB;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = 16 * (b & 3) + (l & 15), ch = 16 * (b >> 2) + 4 * j + (l >> 4);
-      *reinterpret_cast<u32x4 *>(out + row * (BN * 2) + ((ch ^ chunk_swizzle<SB>(row)) * 16)) = dequant(cw[i][j], cs[i][j / GS]);
+      *reinterpret_cast<u32x4 *>(out + row * (BN * 2) + ((ch ^ chunk_swizzle<SB>(row)) * 16)) = dequant(cw[j], cs[j / GS]);
     }
   };
 
@@ -421,8 +418,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  constexpr int kGap = 128 * ((kUnits + 1) / 2) / (NI * NJ) + 1;   // vector instructions between two MFMAs
-  static_assert(!kW4 || kUnits <= 2, "a unit a phase");
+  constexpr int kGap = 128 / (NI * NJ) + 1;   // w4: vector instructions between two MFMAs
   constexpr int kLoads = LA + (kW4 ? 0 : LB);
   // of a step's loads, those that go out past the barrier; the rest follow a phase later (w4: none, that phase has the weights)
   constexpr int kFirst = kW4 ? kLoads : (kLoads + 1) / 2;
@@ -463,10 +459,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
         read((kk + 1) & 1, s, kk + 1);
         __builtin_amdgcn_sched_barrier(0);
         // the next step's weights, whose buffer the last barrier has freed: late in the step, their loads are one step old then
-        if constexpr (kW4 && kUnits > 1) {
-          if (kk > 0) store_w4(s + 1, kk - 1);
-        } else if constexpr (kW4) {
-          if (kk == 2) store_w4(s + 1, 0);
+        if constexpr (kW4) {
+          if (kk == 2) store_w4(s + 1);
         }
         if (kk == 0) multiply_loading(0, s + ST - 1, kFirst, kLoads);
         else multiply(kk & 1);
@@ -500,8 +494,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
       for (int l = 0; l < kLoads; ++l) load_one(S0 + t, l);
     if constexpr (kW4) {
       load_w4(S0);
-#pragma unroll
-      for (int i = 0; i < kUnits; ++i) store_w4(S0, i);
+      store_w4(S0);
       load_w4(S0 + 1);
     }
     if constexpr (ST == 2) wait_all_barrier();
