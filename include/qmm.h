@@ -337,6 +337,14 @@ int64_t qmm_ragged_mm_workspace_size(int64_t rows, int64_t k, int64_t n, int E);
 int64_t qmm_ragged_mm_t_workspace_size(int64_t rows, int64_t k, int64_t n, int E);
 int64_t qmm_ragged_mm_dw_workspace_size(int64_t rows, int64_t k, int64_t n, int E);
 
+/* The tile that a product of these sizes takes, of outputs BM x BN, the steps that its LDS holds and the parts of its sum:
+ * parts << 40 | steps << 32 | BM << 16 | BN; 0 where there are no rows or the few-row kernel takes them, -1 for sizes or a product
+ * that are not taken. QMM_PRODUCT_W4 is qmm_w4_mm on the f16 operand. */
+enum qmm_product {
+  QMM_PRODUCT_W4 = 0, QMM_PRODUCT_W4_T = 1, QMM_PRODUCT_RAGGED = 2, QMM_PRODUCT_RAGGED_T = 3, QMM_PRODUCT_RAGGED_DW = 4
+};
+int64_t qmm_tile_plan(int product, int64_t rows, int64_t k, int64_t n, int E);
+
 /* MoE router top-k from logits, g_moe_route / g_moe_route_tr after the router matvec
  * (S/gen_moe.py:116-252, :255-500; llama.cpp gating: 1 softmax, 2 sigmoid, 3 softmax over the picked logits):
  *   ids i32 [tokens, KU] = the top-KU experts by score (ties to the lower id), wts f32 [tokens, KU].

@@ -5,6 +5,7 @@
 //   qmm_ragged_mm_t   dx[t] = W_e^T dy[t]
 //   qmm_ragged_mm_dw  dW_e = sum_t dy[t] x[t]^T
 #include "ragged_mm.hpp"
+#include "w4_mm.hpp"
 
 using namespace qmm;
 
@@ -64,6 +65,27 @@ extern "C" int64_t qmm_ragged_mm_t_workspace_size(int64_t rows, int64_t k, int64
 }
 extern "C" int64_t qmm_ragged_mm_dw_workspace_size(int64_t rows, int64_t k, int64_t n, int E) {
   return sizes_ok(rows, k, n, E) ? tmm::part_bytes(tmm::plan_sum(rows, E, n, k), E * n * k) : -1;
+}
+
+extern "C" int64_t qmm_tile_plan(int product, int64_t rows, int64_t k, int64_t n, int E) {
+  const bool four_bit = product == QMM_PRODUCT_W4 || product == QMM_PRODUCT_W4_T;
+  if (four_bit ? qmm_w4_mm_t_workspace_size(rows, k, n, E) < 0 : !sizes_ok(rows, k, n, E)) return -1;
+  if (product == QMM_PRODUCT_RAGGED_DW) {
+    const tmm::Plan p = tmm::plan_sum(rows, E, n, k);
+    return tmm::plan_word(tmm::kTilesSum[p.shape], p);
+  }
+  if (product < 0 || product > QMM_PRODUCT_RAGGED_DW) return -1;
+  if (rows == 0 || (product == QMM_PRODUCT_RAGGED && takes_few_rows(rows, k, n))) return 0;
+  if (product == QMM_PRODUCT_W4) {
+    const tmm::Plan p = w4_gemm_plan(rows, E, n, k);
+    return tmm::plan_word(w4_gemm_shape(p.shape), p);
+  }
+  if (product == QMM_PRODUCT_W4_T) {
+    const tmm::Plan p = tmm::plan_rows(tmm::kTilesW4, rows, E, k, n);
+    return tmm::plan_word(tmm::kTilesW4[p.shape], p);
+  }
+  const tmm::Plan p = product == QMM_PRODUCT_RAGGED ? tmm::plan_rows(tmm::kTiles, rows, E, n, k) : tmm::plan_rows(tmm::kTiles, rows, E, k, n);
+  return tmm::plan_word(tmm::kTiles[p.shape], p);
 }
 
 extern "C" int qmm_ragged_mm(int64_t rows, int64_t k, int64_t n, int E, const int32_t *offsets, const void *x, const void *w,

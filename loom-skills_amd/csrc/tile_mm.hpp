@@ -536,10 +536,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 struct Shape {
   int bm, bn;
   float turn, ends, alone;
+  int depth = 2;   // steps in LDS
 };
 struct Plan {
   int shape, splits;
 };
+// what qmm_tile_plan says of it
+inline int64_t plan_word(const Shape &t, const Plan &p) {
+  return (int64_t)p.splits << 40 | (int64_t)t.depth << 32 | (int64_t)t.bm << 16 | t.bn;
+}
 // turns: of a workgroup (the longest); mean: of them all, for what a CU's workgroups take together; tiles_of(shape): workgroups without
 // a split; outputs: of the whole call
 template <int COUNT, class T>
@@ -569,7 +574,7 @@ inline int64_t expected_row_tiles(int64_t rows, int E, int bm) {
 // 128 experts 768 x 2048 95 either way, dx 105 -> 122); 16384 rows of 32 experts 2880 x 2880 320, 363, 447 with the first three.
 // 4-bit ones: gradients of 2048 x 4096 x 12288 301, 247, 315, 227.
 constexpr Shape kTiles[] = {{256, 256, 1.4f, 7.f, 1.4f}, {128, 128, 0.47f, 3.2f, 0.9f}, {64, 128, 0.4f, 1.f, 0.7f},
-                            {64, 128, 0.38f, 4.4f, 0.36f}, {128, 128, 0.55f, 5.3f, 0.5f}};
+                            {64, 128, 0.38f, 4.4f, 0.36f, 4}, {128, 128, 0.55f, 5.3f, 0.5f, 4}};
 constexpr Shape kTilesW4[] = {{256, 256, 1.93f, 8.3f, 1.5f}, {128, 128, 0.54f, 3.4f, 0.8f}, {64, 128, 0.36f, 1.2f, 0.5f},
                               {256, 128, 1.03f, 5.f, 1.f}};
 template <int COUNT>
@@ -580,7 +585,7 @@ Plan plan_rows(const Shape (&shapes)[COUNT], int64_t rows, int E, int64_t N, int
 // The segments cut the sum: E M N outputs, however few rows there are; the longest segment is taken as 1.4 times the average. us with
 // the shapes in turn: 16384 rows of 32 experts 2880 x 2880 380 and 462, 8000 of 128 768 x 2048 into bf16 145, 159, 222, 15314 of 16 1216 x 264
 // 85, 60, 48, 2000 of two 2048 x 1024 44, 28, 21, 500 of four 1024 x 1024 12, 7, 7, 15313 of three 248 x 824 in four parts 44, 31, 26.
-constexpr Shape kTilesSum[] = {{256, 256, 1.35f, 6.8f, 1.35f}, {128, 128, 0.46f, 2.2f, 1.1f}, {128, 128, 0.52f, 5.3f, 0.57f}};
+constexpr Shape kTilesSum[] = {{256, 256, 1.35f, 6.8f, 1.35f}, {128, 128, 0.46f, 2.2f, 1.1f}, {128, 128, 0.52f, 5.3f, 0.57f, 4}};
 inline Plan plan_sum(int64_t rows, int E, int64_t M, int64_t N) {
   const float mean = E == 1 ? (float)(rows / 64 + 1) : (float)rows / (64.f * (float)E) + 1.f;
   return least_time(kTilesSum, (E == 1 ? rows : rows * 7 / (5 * E)) / 64 + 1, mean, E * M * N,

@@ -158,9 +158,10 @@ int launch_gs(const Args &a, int gs, hipStream_t s) {
 // Figures as those of tile_mm.hpp's shapes, for turns of 128 values: 2 % from the fastest choice on average. us at 8192 x 8192 x 4096 64
 // x 128 559, 64 x 256 525, 128 x 128 525, 128 x 256 469, at 333 x 12288 x 4096 52, 65, 58, 65, at 2048 x 4096 x 12288 223, 218, 203, 199, at
 // 8000 rows of 128 experts 1536 x 2048 96, 100, 118, 110.
+static constexpr Shape shapes[] = {{64, 128, 0.5f, 1.f, 0.55f}, {64, 256, 1.06f, 1.5f, 1.05f}, {128, 128, 1.06f, 1.5f, 1.05f},
+                                   {128, 256, 1.83f, 2.5f, 1.9f}};
+const Shape &w4_gemm_shape(int shape) { return shapes[shape]; }
 Plan w4_gemm_plan(int64_t rows, int E, int64_t N, int64_t K) {
-  static const Shape shapes[] = {{64, 128, 0.5f, 1.f, 0.55f}, {64, 256, 1.06f, 1.5f, 1.05f}, {128, 128, 1.06f, 1.5f, 1.05f},
-                                 {128, 256, 1.83f, 2.5f, 1.9f}};
   return least_time(shapes, (K + 127) / 128, (float)((K + 127) / 128), rows * N,
                     [&](const Shape &t) { return expected_row_tiles(rows, E, t.bm) * ((N + t.bn - 1) / t.bn); });
 }

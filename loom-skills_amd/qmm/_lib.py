@@ -46,6 +46,7 @@ SIGNATURES = {
     "qmm_ragged_mm_t_workspace_size": [c_i64, c_i64, c_i64, c_int],
     "qmm_ragged_mm_dw": [c_i64, c_i64, c_i64, c_int, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_vp, c_i64, c_vp],
     "qmm_ragged_mm_dw_workspace_size": [c_i64, c_i64, c_i64, c_int],
+    "qmm_tile_plan": [c_int, c_i64, c_i64, c_i64, c_int],
     "qmm_moe_topk": [c_vp, c_i64, c_int, c_int, c_int, c_int, c_float, c_vp, c_vp, c_vp, c_vp],
     "qmm_moe_topk_operand": [c_vp, c_i64, c_int, c_int, c_int, c_int, c_float, c_vp, c_vp, c_vp, c_i64, c_vp, c_int,
                              c_int, c_vp, c_vp, c_vp],
@@ -98,7 +99,7 @@ SIGNATURES = {
 RESTYPE = {"qmm_strerror": ctypes.c_char_p, "qmm_row_bytes": c_i64, "qmm_mxfp4t_scale_bytes": c_i64,
            "qmm_w4_bytes": c_i64, "qmm_w4_scale_bytes": c_i64, "qmm_w4_mm_workspace_size": c_i64,
            "qmm_w4_mm_t_workspace_size": c_i64, "qmm_ragged_mm_workspace_size": c_i64, "qmm_ragged_mm_t_workspace_size": c_i64,
-           "qmm_ragged_mm_dw_workspace_size": c_i64,
+           "qmm_ragged_mm_dw_workspace_size": c_i64, "qmm_tile_plan": c_i64,
            "qmm_moe_routed_workspace_size": c_i64, "qmm_gemm_t_workspace_size": c_i64, "qmm_rms_norm_grad_workspace_size": c_i64}
 
 

@@ -256,7 +256,7 @@ def test_gradient_operand_of_odd_rows(dev, parts, n, dtype):
     assert ((m >= 2.0 ** 13) & (m < 2.0 ** 14)).all() and s[3, 0] == 1
 
 
-# every tile and depth of LDS, whole sums and sums in parts
+# larger tiles, deep and not, whole sums and sums in parts (a case of every tile and type: tile_cases.py)
 @pytest.mark.parametrize("counts,N,K", [([9000, 1, 0, 8300], 520, 40), ([4000, 0, 4500, 1, 8800], 264, 416), ([4142], 160, 6304),
                                         ([5000, 7001, 600], 32, 4352), ([4000, 0, 42], 136, 6624), ([11000, 0, 8801], 528, 40),
                                         ([30, 0, 45, 0, 0], 6648, 40), ([4182], 32, 2016), ([75, 0, 4], 40, 1160), ([9001, 0, 7600], 32, 40),

@@ -91,7 +91,7 @@ def row_rounding(x, absw, terms):
 MANY = [(64, 8, 32, 32, True, "bf16", "bf16"), (65, 200, 96, 32, True, "bf16", "f32"), (100, 129, 288, 64, False, "f32", "f32"),
         (129, 256, 512, 128, True, "bf16", "bf16"), (200, 257, 160, ROW, True, "bf16", "f32"), (257, 520, 1024, 64, True, "bf16", "bf16"),
         (300, 31, 4096, 128, True, "bf16", "f32"), (1, 40, 256, 128, True, "f16", "f32"), (70, 96, 2048, 256, True, "f16", "bf16"),
-        # every tile: 64 x 256, 128 x 128, 128 x 256
+        # larger sizes (a case of every tile: tile_cases.py)
         (640, 5000, 160, 32, True, "bf16", "bf16"), (8300, 300, 96, 32, True, "bf16", "f32"), (4090, 2000, 288, 64, True, "bf16", "bf16"),
         # long sums of few outputs, in parts
         (90, 72, 8192, 128, True, "bf16", "f32"), (70, 33, 9088, 32, True, "bf16", "bf16"), (200, 300, 2080, 64, True, "bf16", "f32")]
@@ -138,7 +138,7 @@ def test_many_rows_by_expert(dev, counts, first, tail, n, k, group, out):
 
 GRADS = [(1, 8, 32, 32, True, "bf16", "f32"), (77, 100, 288, 32, True, "bf16", "bf16"), (64, 17, 160, 64, True, "f32", "f32"),
          (129, 200, 512, 128, False, "bf16", "f32"), (200, 64, 1024, ROW, True, "bf16", "bf16"), (257, 320, 96, 64, True, "bf16", "f32"),
-         # every tile: 256 x 256, 256 x 128, 128 x 128
+         # larger sizes (a case of every tile: tile_cases.py)
          (16300, 72, 1024, 32, True, "bf16", "bf16"), (8100, 200, 992, 64, True, "bf16", "bf16"), (2000, 130, 1024, 128, True, "bf16", "f32"),
          # long sums in parts
          (77, 8200, 96, 32, True, "bf16", "f32"), (130, 3000, 160, 64, True, "f32", "bf16")]
