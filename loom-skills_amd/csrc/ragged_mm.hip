@@ -131,8 +131,8 @@ extern "C" int qmm_ragged_mm_dw(int64_t rows, int64_t k, int64_t n, int E, const
   a.M = (int)n, a.N = (int)k;
   a.a = static_cast<const u8 *>(dy), a.a_row = 2 * n;
   a.b = static_cast<const u8 *>(x), a.b_row = 2 * k;
-  // past the last-level cache's 256 MB dW is written by whole lines that are not kept there: us, 8000 rows of 128 experts 768 x 2048 into
-  // f32 192 without and 144, 16384 rows of 32 experts 2880 x 2880 into bf16 373 and 355
+  // past the last-level cache's 256 MB dW is written by whole lines that are not kept there: us on one card in turn, 8000 rows of 128
+  // experts 768 x 2048 into f32 192 without and 144, 16384 rows of 32 experts 2880 x 2880 into bf16 373 and 355
   const int64_t row = k * (dw_dtype == QMM_F32 ? 4 : 2);
   const tmm::Plan plan = tmm::plan_sum(rows, E, n, k);
   a.stream = plan.splits == 1 && row % 128 == 0 && aligned(dw, 128) && E * n * row > (int64_t)256 << 20;

@@ -17,11 +17,12 @@
 // are read while the MFMAs of these run, and the barrier of a step stands before its last 16 values' MFMAs, so that the next
 // step's first reads run under them.
 //
-// The MFMAs bound a full round of 256 x 256 tiles (a step of 64 values 1.65 us on every CU: 1.30 PFLOP/s, at the clock the power limit
-// holds; a library product of 8192^3 reaches 1.55), a launch the rounds it takes and each tile's start and end (6 us: the operands'
-// first loads, 128 KB of outputs): 16384 rows of 32 experts 2880 x 2880 forward 310 us, 0.88 PFLOP/s, in four rounds, the last a
-// little over half full; their weights' gradient 355 us with eight steps a tile. Many experts of few rows are bound by memory: 8000
-// rows of 128 experts 768 x 2048, dW writes 0.8 GB in 144 us, and what it no longer pushes out of the last-level cache saves dx 25.
+// The MFMAs bound a full round of 256 x 256 tiles (a step of 64 values 1.56 us on every CU, by 4096 x 4096 outputs of 4096 and 8192
+// values: 1.38 PFLOP/s, at the clock the power limit holds; a library product of 8192^3 reaches 1.55), a launch the rounds it takes and
+// each tile's start and end (the operands' first loads, 128 KB of outputs; 8 us a further round of 4096 x 4096 outputs). Kernels alone,
+// least and mean of 21 calls: 16384 rows of 32 experts 2880 x 2880 forward 313 and 340 us, 0.87 PFLOP/s, in four rounds, the last a
+// little over half full; their weights' gradient 385 and 402 with eight steps a tile. Many experts of few rows are bound by memory: 8000
+// rows of 128 experts 768 x 2048, dW writes 0.8 GB in 144 us (163 and 176 among calls of dx, which it evicts from the last-level cache).
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -531,7 +532,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_mm_kernel(Args a) {
 // A tile shape and in how many parts the sum is taken (more where few tiles would walk a long sum): the least estimated time, that
 // is the workgroups that a CU gets times (turns along the sum times a turn's time + a start and end), or what one workgroup alone
 // takes if that is more, and the parts' way through memory. A shape's figures (us a turn over the workgroups that share a CU on
-// launches that fill the chip, their start and end, a turn of one workgroup on a CU) are those with which the choice comes closest
+// launches that fill the chip, their start and end, a turn of one workgroup on a CU) are no measurements of their own: they are those with which the choice comes closest
 // to the fastest of all shapes and parts, measured on 800 calls of 1e8 to 2e11 operations: 2 to 3.5 % slower than it on average.
 struct Shape {
   int bm, bn;

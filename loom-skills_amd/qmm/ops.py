@@ -1250,7 +1250,7 @@ def w4_mm(x, w, ws, n, k, group, offsets=None, scales=None, y=None, out_dtype=No
 
 def w4_mm_t(dy, w, ws, n, k, group, offsets=None, y=None, out_dtype=None):
     """dx = dy W, the input gradient of w4_mm at dy (f32 / bf16 [rows, n]) with frozen weights (qmm_grad_operand, qmm_w4_mm_t):
-    rows enter as f16 times a power of two and weights as f16, whatever their number (relative error about 3e-4 in f32);
+    rows enter as f16 times a power of two and weights as f16 (infinite for scales past 4366), whatever their number: 3e-4 of the result;
     offsets and rows of no expert as w4_mm. dx [rows, k] f32 or bf16 (out_dtype, or y)."""
     s = _here(dy, w, ws, offsets, y)
     E = 1 if offsets is None else _segments(offsets)
