@@ -600,11 +600,12 @@ __global__ __launch_bounds__(256) void combine_vec_kernel(int64_t tokens, int64_
   reinterpret_cast<f32x4 *>(y + t * H)[c4] = acc;
 }
 
-// A row's exponent by its largest magnitude m. wide: the rows that qmm_row_scale_f16's clamp leaves small or past f16's range are brought to
+// A row's exponent by its largest magnitude m. WIDE: the rows that qmm_row_scale_f16's clamp leaves small or past f16's range are brought to
 // 2^13 too (subnormal rows as near as 2^126 brings them; NaN values are passed over and stay NaN, infinities stay).
-__device__ __forceinline__ int row_exponent(float m, int wide) {
+template <bool WIDE>
+__device__ __forceinline__ int row_exponent(float m) {
   const int e = (int)((f32_as_u32(m) >> 23) & 255u) - 127 - 13;
-  return wide ? min(max(e, -126), 114) : min(max(e, 0), 100);
+  return WIDE ? min(max(e, -126), 114) : min(max(e, 0), 100);
 }
 __device__ __forceinline__ float load_act(const void *x, int bf, int64_t i) {
   return bf ? bf16_to_f32(static_cast<const u16 *>(x)[i]) : static_cast<const float *>(x)[i];
@@ -622,10 +623,11 @@ __device__ __forceinline__ bool pad_row(const int32_t *info, int64_t r, int64_t 
   return true;
 }
 
+template <bool WIDE>
 __global__ __launch_bounds__(256) void row_scale_kernel(int64_t rows, int64_t k, const void *__restrict__ x, int bf,
                                                         float *__restrict__ scales, _Float16 *__restrict__ x16,
                                                         const int32_t *__restrict__ tile_info,
-                                                        const int32_t *__restrict__ info, int wide) {
+                                                        const int32_t *__restrict__ info) {
   const int64_t r = blockIdx.x;
   if (tile_info && (tile_info[2 * (r / kTile)] < 0 || r % kTile >= tile_info[2 * (r / kTile) + 1])) return;
   if (pad_row(info, r, k, scales, x16)) return;
@@ -637,7 +639,7 @@ __global__ __launch_bounds__(256) void row_scale_kernel(int64_t rows, int64_t k,
   if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = m;
   __syncthreads();
   m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-  const int e = row_exponent(m, wide);
+  const int e = row_exponent<WIDE>(m);
   const float sc = u32_as_f32((u32)(127 - e) << 23), inv = u32_as_f32((u32)(127 + e) << 23);
   for (int64_t c = threadIdx.x; c < k; c += 256) x16[r * k + c] = (_Float16)(load_act(x, bf, r * k + c) * sc);
   if (threadIdx.x == 0) {
@@ -669,12 +671,12 @@ __device__ __forceinline__ void load8(const void *x, int64_t i8, float (&v)[8]) 
 // held in registers between the row maximum and the conversion); the maximum is a wave butterfly, so the row needs no
 // workgroup barrier or LDS. Rows up to 64 x 8 x NCH values; the host takes the workgroup-a-row kernel below
 // for wider rows, the scalar kernel above for misaligned or k % 8 != 0 ones.
-template <bool BF, int NCH>
+template <bool BF, int NCH, bool WIDE>
 __global__ __launch_bounds__(256) void row_scale_wave_kernel(int64_t rows, int64_t k, const void *__restrict__ x,
                                                              float *__restrict__ scales, _Float16 *__restrict__ x16,
                                                              const int32_t *__restrict__ tile_info,
                                                              const int32_t *__restrict__ info,
-                                                             const int32_t *__restrict__ ridx, int wide) {
+                                                             const int32_t *__restrict__ ridx) {
   const int lane = threadIdx.x & 63;
   const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= rows) return;
@@ -711,7 +713,7 @@ __global__ __launch_bounds__(256) void row_scale_wave_kernel(int64_t rows, int64
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-  const int e = row_exponent(m, wide);
+  const int e = row_exponent<WIDE>(m);
   const float sc = u32_as_f32((u32)(127 - e) << 23), inv = u32_as_f32((u32)(127 + e) << 23);
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
@@ -735,11 +737,11 @@ __global__ __launch_bounds__(256) void row_scale_wave_kernel(int64_t rows, int64
 // between the maximum and the conversion, all loaded before any is used), so the row is read once where the scalar
 // kernel read it twice, a value a load (2048 x 12288 f32: 42 -> 23 us; bf16 39.5 -> 15.7).
 constexpr int kRsBlockValues = 32768;   // values of the longest row
-template <bool BF, int NCH>
+template <bool BF, int NCH, bool WIDE>
 __global__ __launch_bounds__(256) void row_scale_block_kernel(int64_t k, const void *__restrict__ x,
                                                               float *__restrict__ scales, _Float16 *__restrict__ x16,
                                                               const int32_t *__restrict__ tile_info,
-                                                              const int32_t *__restrict__ info, int wide) {
+                                                              const int32_t *__restrict__ info) {
   constexpr int V = BF ? 8 : 4;   // values of a piece
   const int64_t r = blockIdx.x;
   if (tile_info && (tile_info[2 * (r / kTile)] < 0 || r % kTile >= tile_info[2 * (r / kTile) + 1])) return;
@@ -767,7 +769,7 @@ __global__ __launch_bounds__(256) void row_scale_block_kernel(int64_t k, const v
   if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = m;
   __syncthreads();
   m = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-  const int e = row_exponent(m, wide);
+  const int e = row_exponent<WIDE>(m);
   const float sc = u32_as_f32((u32)(127 - e) << 23), inv = u32_as_f32((u32)(127 + e) << 23);
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
@@ -1016,9 +1018,10 @@ int qmm_moe_combine_gated(int64_t tokens, int64_t rows, int64_t H, int KU, const
   return combine(tokens, rows, H, KU, ys, pos, wts, 1, sg, y, stream);
 }
 
+}   // extern "C"
+template <bool WIDE = false>
 static int row_scale(int64_t rows, int64_t k, const void *x, int x_dtype, float *scales, void *x16,
-                     const int32_t *tile_info, const int32_t *info, hipStream_t s, const int32_t *ridx = nullptr,
-                     int wide = 0) {
+                     const int32_t *tile_info, const int32_t *info, hipStream_t s, const int32_t *ridx = nullptr) {
   if (!x || !scales || !x16) return QMM_ERR_NULL;
   if (x_dtype != QMM_F32 && x_dtype != QMM_BF16) return QMM_ERR_DTYPE;
   if (rows <= 0 || k <= 0 || rows > (1ll << 24)) return QMM_ERR_SHAPE;
@@ -1031,8 +1034,8 @@ static int row_scale(int64_t rows, int64_t k, const void *x, int x_dtype, float 
     const int64_t per = (k / 8 + 63) / 64;   // chunks a lane
     const bool bf = x_dtype == QMM_BF16;
 #define QMM_RS(N)                                                                                                   \
-  (bf ? (row_scale_wave_kernel<true, N><<<grid, 256, 0, s>>>(rows, k, x, scales, o, tile_info, info, ridx, wide), 0)    \
-      : (row_scale_wave_kernel<false, N><<<grid, 256, 0, s>>>(rows, k, x, scales, o, tile_info, info, ridx, wide), 0))
+  (bf ? (row_scale_wave_kernel<true, N, WIDE><<<grid, 256, 0, s>>>(rows, k, x, scales, o, tile_info, info, ridx), 0)    \
+      : (row_scale_wave_kernel<false, N, WIDE><<<grid, 256, 0, s>>>(rows, k, x, scales, o, tile_info, info, ridx), 0))
     if (per <= 1) QMM_RS(1);
     else if (per <= 2) QMM_RS(2);
     else if (per <= 4) QMM_RS(4);
@@ -1040,7 +1043,7 @@ static int row_scale(int64_t rows, int64_t k, const void *x, int x_dtype, float 
     else QMM_RS(16);
 #undef QMM_RS
   } else if (k % 8 == 0 && k <= kRsBlockValues && aligned(x, 16) && aligned(x16, 16)) {
-#define QMM_RSB(BF, N) row_scale_block_kernel<BF, N><<<(unsigned)rows, 256, 0, s>>>(k, x, scales, o, tile_info, info, wide)
+#define QMM_RSB(BF, N) row_scale_block_kernel<BF, N, WIDE><<<(unsigned)rows, 256, 0, s>>>(k, x, scales, o, tile_info, info)
     if (x_dtype == QMM_BF16) {
       if (k <= 16384) QMM_RSB(true, 8);
       else QMM_RSB(true, 16);
@@ -1051,18 +1054,19 @@ static int row_scale(int64_t rows, int64_t k, const void *x, int x_dtype, float 
     }
 #undef QMM_RSB
   } else {
-    row_scale_kernel<<<(unsigned)rows, 256, 0, s>>>(rows, k, x, x_dtype == QMM_BF16, scales, o, tile_info, info, wide);
+    row_scale_kernel<WIDE><<<(unsigned)rows, 256, 0, s>>>(rows, k, x, x_dtype == QMM_BF16, scales, o, tile_info, info);
   }
   return launch_status();
 }
 
+extern "C" {
 int qmm_row_scale_f16(int64_t rows, int64_t k, const void *x, int x_dtype, float *scales, void *x16,
                       const int32_t *tile_info, qmm_stream_t stream) {
   return row_scale(rows, k, x, x_dtype, scales, x16, tile_info, nullptr, reinterpret_cast<hipStream_t>(stream));
 }
 
 int qmm_row_scale_f16_wide(int64_t rows, int64_t k, const void *x, int x_dtype, float *scales, void *x16, qmm_stream_t stream) {
-  return row_scale(rows, k, x, x_dtype, scales, x16, nullptr, nullptr, reinterpret_cast<hipStream_t>(stream), nullptr, 1);
+  return row_scale<true>(rows, k, x, x_dtype, scales, x16, nullptr, nullptr, reinterpret_cast<hipStream_t>(stream));
 }
 
 int qmm_row_scale_f16_rows(int64_t n, const int32_t *rows, int64_t k, const void *x, int x_dtype, float *scales,
