@@ -118,8 +118,8 @@ inline bool zero_rest_asked(int &dtype) {
 }
 // workgroups for it: they look at the offsets only where every row is an expert's
 inline int rest_blocks(int64_t rows, int64_t row_bytes) {
-  const int64_t n = rows * row_bytes >> 16;   // 64 KB each
-  return n < 1 ? 1 : n > 256 ? 256 : (int)n;
+  const int64_t n = rows * row_bytes >> 18;   // 256 KB each, one an XCD at least
+  return n < 8 ? 8 : n > 64 ? 64 : (int)n & ~7;
 }
 
 }  // namespace qmm

@@ -60,7 +60,7 @@ struct Args {
   int tiles_n;
   int splits;                  // parts of the sum, one a layer of the grid (y); more than one: f32 sums [splits][outputs] into part
   float *part;
-  int rest;                    // kSumFixed: the layer's last workgroups, which set the rows of no expert to zero (ragged.hpp); 0: none
+  int rest;                    // kSumFixed: the layer's first workgroups, a multiple of eight, which set the rows of no expert to zero (ragged.hpp); 0: none
 };
 
 template <int DT>
@@ -171,9 +171,10 @@ __device__ __forceinline__ int chunk_swizzle(int row) {
 
 // The workgroup among those of a layer of the sum (the grid's y). HIP refuses 2^32 threads along a grid's dimension: what passes 2^21
 // workgroups lies along z.
-__device__ __forceinline__ int workgroup() { return (int)(blockIdx.z * gridDim.x + blockIdx.x); }
+constexpr int kGridX = 1 << 21;
+__device__ __forceinline__ int workgroup() { return (int)(blockIdx.z * kGridX + blockIdx.x); }
 inline dim3 tile_grid(int64_t tiles, int rest, int layers) {
-  const int64_t n = (tiles + 7) / 8 * 8 + rest, x = std::min<int64_t>(n, 1 << 21);
+  const int64_t n = (tiles + 7) / 8 * 8 + rest, x = std::min<int64_t>(n, kGridX);
   return dim3((unsigned)x, (unsigned)layers, (unsigned)((n + x - 1) / x));
 }
 constexpr int64_t kMaxTiles = 1 << 30;   // more have outputs that no card holds
@@ -186,8 +187,8 @@ __device__ __forceinline__ bool row_tile(const Args &a, int &e, int &lo, int &hi
   TileScan sc{(a.rows + BM - 1) / BM, 0, 1};
   if (a.offsets) sc = scan_tiles<BM>(a.offsets, a.E, a.rows);
   const int total = sc.total * a.tiles_n, per = (total + 7) >> 3;
-  const int i = workgroup() >> 3;
-  int t = (workgroup() & 7) * per + i, first = 0;
+  const int wg = workgroup() - a.rest, i = wg >> 3;
+  int t = (wg & 7) * per + i, first = 0;
   if (i >= per || t >= total) return false;
   if (a.offsets) find_tile<BM>(a.offsets, a.E, a.rows, sc, t / a.tiles_n, e, lo, hi, first);
   t -= first * a.tiles_n;
@@ -199,8 +200,8 @@ __device__ __forceinline__ bool row_tile(const Args &a, int &e, int &lo, int &hi
 }
 // whether the workgroup is one of those for the rows of no expert, which are done then
 __device__ __forceinline__ bool rest_done(const Args &a) {
-  const int part = workgroup() - ((int)(gridDim.x * gridDim.z) - a.rest);
-  if (part < 0) return false;
+  const int part = workgroup();
+  if (part >= a.rest) return false;
   if (blockIdx.y == 0)
     zero_rest(a.offsets, a.E, a.rows, static_cast<u8 *>(a.y), (int64_t)a.N * (a.y_type == QMM_F32 ? 4 : 2), part, a.rest);
   return true;
@@ -606,6 +607,7 @@ inline int launch_join(const Args &in, int64_t rows, int64_t outputs, hipStream_
   Args a = in;
   a.tiles_n = (a.N + kJoinCols - 1) / kJoinCols;
   a.rows = (int)rows;
+  a.rest = 0;
   const int64_t tiles = most_row_tiles(a, kJoinRows) * a.tiles_n;
   if (tiles > kMaxTiles) return QMM_ERR_SHAPE;
   const dim3 grid = tile_grid(tiles, 0, 1);
