@@ -20,9 +20,9 @@
 // The MFMAs bound a full round of 256 x 256 tiles (a step of 64 values 1.56 us on every CU, by 4096 x 4096 outputs of 4096 and 8192
 // values: 1.38 PFLOP/s, at the clock the power limit holds; a library product of 8192^3 reaches 1.55), a launch the rounds it takes and
 // each tile's start and end (the operands' first loads, 128 KB of outputs; 8 us a further round of 4096 x 4096 outputs). Kernels alone,
-// least and mean of 21 calls: 16384 rows of 32 experts 2880 x 2880 forward 313 and 340 us, 0.87 PFLOP/s, in four rounds, the last a
-// little over half full; their weights' gradient 385 and 402 with eight steps a tile. Many experts of few rows are bound by memory: 8000
-// rows of 128 experts 768 x 2048, dW writes 0.8 GB in 144 us (163 and 176 among calls of dx, which it evicts from the last-level cache).
+// least and mean of 21 calls: 16384 rows of 32 experts 2880 x 2880 forward 315 and 340 us, 0.86 PFLOP/s, in four rounds, the last a
+// little over half full; their weights' gradient 378 and 397 with eight steps a tile. Many experts of few rows are bound by memory: 8000
+// rows of 128 experts 768 x 2048, dW writes 0.8 GB in 144 us (164 and 175 among calls of dx, which it evicts from the last-level cache).
 #pragma once
 #include <algorithm>
 #include <type_traits>
