@@ -76,16 +76,16 @@ __device__ __forceinline__ void find_tile(const int32_t *offsets, int E, int row
 
 // Rows of no expert set to zero (QMM_ZERO_REST): workgroup `part` of `parts` that have no other work, beside those that write the
 // experts' rows. Offsets that never fall leave the rows before the first segment and behind the last, two runs of bytes; others are
-// looked at a row at a time. y: of 2- or 4-byte values at a multiple of their size.
-__device__ __forceinline__ void zero_run(u8 *p, int64_t bytes, int part, int parts) {
+// looked at a row and wave at a time. y: of 2- or 4-byte values at a multiple of their size.
+__device__ __forceinline__ void zero_run(u8 *p, int64_t bytes, int thread, int threads) {
   typedef __attribute__((ext_vector_type(4))) u32 u32x4;
   const u32x4 zero = {0, 0, 0, 0};
-  const int64_t step = (int64_t)parts * blockDim.x, units = bytes >> 4;
-  for (int64_t i = (int64_t)part * blockDim.x + threadIdx.x; i < units; i += step) __builtin_memcpy(p + 16 * i, &zero, 16);
+  const int64_t units = bytes >> 4;
+  for (int64_t i = thread; i < units; i += threads) __builtin_memcpy(p + 16 * i, &zero, 16);
   const int left = (int)(bytes & 15) >> 1;   // a last unit by halves
-  if (part == 0 && (int)threadIdx.x < left) {
+  if (thread < left) {
     const u16 z = 0;
-    __builtin_memcpy(p + 16 * units + 2 * threadIdx.x, &z, 2);
+    __builtin_memcpy(p + 16 * units + 2 * thread, &z, 2);
   }
 }
 __device__ __forceinline__ void zero_rest(const int32_t *offsets, int E, int rows, u8 *y, int64_t row_bytes, int part, int parts) {
@@ -97,17 +97,19 @@ __device__ __forceinline__ void zero_rest(const int32_t *offsets, int E, int row
   }
   if (!__ballot(falls)) {
     const int first = clamp_row(offsets[0], rows), end = clamp_row(offsets[E], rows);
-    zero_run(y, first * row_bytes, part, parts);
-    zero_run(y + end * row_bytes, (rows - end) * row_bytes, part, parts);
+    const int thread = part * (int)blockDim.x + (int)threadIdx.x, threads = parts * (int)blockDim.x;
+    zero_run(y, first * row_bytes, thread, threads);
+    zero_run(y + end * row_bytes, (rows - end) * row_bytes, thread, threads);
     return;
   }
-  for (int row = part; row < rows; row += parts) {
+  const int waves = (int)blockDim.x >> 6;
+  for (int row = part * waves + ((int)threadIdx.x >> 6); row < rows; row += parts * waves) {
     bool in = false;
     for (int c = 0; c < E; c += 64) {
       const int i = min(c + lane, E - 1);
       in |= clamp_row(offsets[i], rows) <= row && row < clamp_row(offsets[i + 1], rows);
     }
-    if (!__ballot(in)) zero_run(y + row * row_bytes, row_bytes, 0, 1);
+    if (!__ballot(in)) zero_run(y + row * row_bytes, row_bytes, lane, 64);
   }
 }
 // Whether an output's type asks for it, which it does not say any more then.
